@@ -203,6 +203,7 @@ def prepare(case, seed):
     if own:
         import ter_amd as T
         s["attn"] = T.PagedAttention(nh, nkv, d, s["longest"], THETA, neox=c["neox"], dtype=dt)
+        s["cache"] = T.PagedCache(kc, vc)
         s["batch"] = T.PagedBatch(s["rows"], s["lens"], pages)
     return s
 
@@ -212,9 +213,9 @@ def run(state):
     kind = s["case"]["kind"]
     if own:
         if kind == "append":
-            q = s["attn"].append(s["q"], s["k"], s["v"], s["kc"], s["vc"], s["batch"])
+            q = s["attn"].append(s["q"], s["k"], s["v"], s["cache"], s["batch"])
             return dict(q=q, k_cache=s["kc"], v_cache=s["vc"])
-        return s["attn"].attend(s["q"], s["kc"], s["vc"], s["batch"], shared=s["shared"] if kind == "shared" else 0)
+        return s["attn"].attend(s["q"], s["cache"], s["batch"], shared=s["shared"] if kind == "shared" else 0)
     if kind == "append":
         return _append(s)
     return _attend(s, s["shared"] if kind == "shared" else 0)
