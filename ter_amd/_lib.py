@@ -1,4 +1,5 @@
-"""ctypes bindings of libter_hip.so (the C-ABI declared in include/ter_hip.h).
+"""ctypes bindings of libter_hip.so (the C-ABI declared in include/ter_hip.h
+and include/ter_hip_paged.h).
 
 The library is always the in-tree build, ter_amd/libter_hip.so (built by
 ter_amd/build.py).  Loading fails loudly when it is missing: there is no
@@ -47,6 +48,10 @@ LAYOUT_T16 = 16
 ARGMAX_STATE_BYTES = 16512
 ROPE_NORM = 0
 ROPE_NEOX = 1
+PAGED_F16, PAGED_BF16 = 0, 1
+PAGED_SEQ_MAX = 1024
+PAGED_ROWS_MAX = 1 << 20
+PAGED_POS_MAX = 1 << 20
 BIN_TERT = 0x54455254
 BIN_LLRT = 0x4C4C5254
 BIN_F16, BIN_F32, BIN_TRITS = 0, 1, 2
@@ -143,6 +148,31 @@ class BinTensor(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """ter_hip_paged_cache_t -- one layer's key and value pages."""
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("page_stride", C.c_int64),
+        ("pos_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+    ]
+
+
+class PagedBatch(C.Structure):
+    """ter_hip_paged_batch_t -- rows, lengths and page tables of a batch of sequences."""
+    _fields_ = [
+        ("row0", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("pages_stride", C.c_int64),
+        ("max_pages", C.c_int32),
+        ("n_seq", C.c_int32),
+    ]
+
+
 class OpCounts(C.Structure):
     _fields_ = [
         ("total_ops", C.c_uint64),
@@ -218,6 +248,19 @@ SIGNATURES = [
     ("ter_hip_read_probe", C.c_int, [_P, C.c_size_t, C.c_int32, _P, _P]),
 ]
 
+# the same for every symbol of include/ter_hip_paged.h
+_PB, _PC = C.POINTER(PagedBatch), C.POINTER(PagedCache)
+PAGED_SIGNATURES = [
+    ("ter_hip_paged_create", C.c_int, [C.POINTER(C.c_void_p), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float,
+                                       C.c_int32, C.c_int32]),
+    ("ter_hip_paged_destroy", None, [_P]),
+    ("ter_hip_paged_append", C.c_int, [_P, _PB, _PC, C.c_int32, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P,
+                                       C.c_int64, _P]),
+    ("ter_hip_paged_attend_ws", C.c_size_t, [_P, _PB, _PC, C.c_int32, C.c_int32]),
+    ("ter_hip_paged_attend", C.c_int, [_P, _PB, _PC, C.c_int32, _P, C.c_int64, _P, C.c_int64, C.c_int32, C.c_float,
+                                       _P, C.c_size_t, _P]),
+]
+
 _lib = None
 
 
@@ -248,7 +291,7 @@ def lib():
         except ImportError:
             pass
         L = C.CDLL(LIB_PATH)
-        for name, res, args in SIGNATURES:
+        for name, res, args in SIGNATURES + PAGED_SIGNATURES:
             f = getattr(L, name)
             f.restype = res
             f.argtypes = args

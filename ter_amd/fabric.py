@@ -555,6 +555,190 @@ class Attention:
             pass
 
 
+class PagedCache:
+    """One layer's keys and values in pages: k, v fp16 or bf16 [n_pages]
+    [page_size][n_kv_heads][head_dim] CUDA tensors of the same shape and
+    strides, head_dim contiguous.  Any other order in memory is a view of it:
+    pages of heads before positions (permute), k and v interleaved in one
+    tensor (kv[:, 0], kv[:, 1]), an s_max-position cache of Attention (view as
+    pages of consecutive positions).  page_size is a multiple of 16."""
+
+    def __init__(self, k, v):
+        torch = _torch()
+        for t, nm in ((k, "k"), (v, "v")):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in (torch.float16, torch.bfloat16):
+                raise TypeError(f"{nm} must be a CUDA float16 or bfloat16 tensor")
+            if t.dim() != 4 or t.numel() == 0 or t.stride(3) != 1:
+                raise ValueError(f"{nm} must be [n_pages][page_size][n_kv_heads][head_dim], head_dim contiguous")
+        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must have one shape, one layout, one type and one device")
+        self.k, self.v = k, v
+        self.page_size = k.shape[1]
+        # (the stride of a dimension of size 1 says nothing)
+        st = [k.stride(i) if k.shape[i] > 1 else k.shape[3] for i in range(3)]
+        self._c = L.PagedCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], k.shape[0], k.shape[1])
+        self._ref = C.byref(self._c)
+        self._key = (k.dtype, k.get_device(), k.shape[2], k.shape[3])
+
+
+class PagedBatch:
+    """A batch of sequences: row0 int32 [n + 1] (the rows of sequence b in q,
+    k, v and out are row0[b] .. row0[b+1] - 1), kv_len int32 [n] (positions of
+    each, those rows included: they are its last ones), pages int32 [n]
+    [max_pages] (its pages in order).  CUDA tensors, read on the device by
+    every launch, so they may change between calls or replays of a graph."""
+
+    def __init__(self, row0, kv_len, pages):
+        torch = _torch()
+        for t, nm, dim in ((row0, "row0", 1), (kv_len, "kv_len", 1), (pages, "pages", 2)):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32:
+                raise TypeError(f"{nm} must be a CUDA int32 tensor")
+            if t.dim() != dim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+                raise ValueError(f"{nm} must have {dim} dimension(s), the last one contiguous")
+        n = kv_len.shape[0]
+        if row0.shape[0] != n + 1 or pages.shape[0] != n:
+            raise ValueError(f"{n} sequences: row0 needs {n + 1} entries and pages {n} rows")
+        if not row0.device == kv_len.device == pages.device:
+            raise ValueError("row0, kv_len and pages must be on one device")
+        self.row0, self.kv_len, self.pages = row0, kv_len, pages
+        self.n_seq = n
+        self._c = L.PagedBatch(row0.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
+                               pages.stride(0) if n > 1 else pages.shape[1], pages.shape[1], n)
+        self._ref = C.byref(self._c)
+        self._dev = kv_len.get_device()
+
+
+class PagedAttention:
+    """Batches of sequences over a paged cache (ter_hip_paged_*): append()
+    rotates new queries and keys and writes keys and values to their pages,
+    attend() is causal attention of ragged rows (prompts, pieces of prompts,
+    single tokens, mixed) over the pages.  One context serves every layer and
+    any number of streams.  Rows of q are [T][n_heads][head_dim] or
+    [T][n_heads * head_dim], possibly parts of wider rows."""
+
+    def __init__(self, n_heads: int, n_kv_heads: int, head_dim: int, max_pos: int, theta: float, neox: bool = True,
+                 dtype=None, device=None):
+        torch = _torch()
+        dtype = dtype or torch.float16
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("dtype must be torch.float16 or torch.bfloat16")
+        self._h = None
+        h = C.c_void_p()
+        with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+            self._dev = torch.cuda.current_device()
+            L.check(L.lib().ter_hip_paged_create(C.byref(h), n_heads, n_kv_heads, head_dim, max_pos, C.c_float(theta),
+                                                 L.ROPE_NEOX if neox else L.ROPE_NORM,
+                                                 L.PAGED_BF16 if dtype == torch.bfloat16 else L.PAGED_F16),
+                    "ter_hip_paged_create")
+        self._h = h
+        self.n_heads, self.n_kv_heads, self.head_dim, self.max_pos = n_heads, n_kv_heads, head_dim, max_pos
+        self.dtype = dtype
+        self._key = (dtype, self._dev, n_kv_heads, head_dim)
+
+    def _rows(self, t, heads: int, n: int, name: str) -> int:
+        """Checks n rows of `heads` heads; returns their stride."""
+        if t.dtype != self.dtype or not t.is_cuda or t.get_device() != self._dev:
+            raise TypeError(f"{name} must be a {self.dtype} tensor on cuda:{self._dev}")
+        d, s, st = self.head_dim, t.shape, t.stride()
+        if len(s) == 3:
+            ok = s[1] == heads and s[2] == d and st[2] == 1 and (heads == 1 or st[1] == d)
+        else:
+            ok = len(s) == 2 and s[1] == heads * d and st[1] == 1
+        if not ok or s[0] != n:
+            raise ValueError(f"{name} must hold {n} rows of [{heads}][{d}], each contiguous")
+        return st[0] if n > 1 else heads * d
+
+    def _check(self, cache: PagedCache, batch: PagedBatch):
+        if cache._key != self._key or batch._dev != self._dev:
+            raise ValueError("the cache or the batch is of another type, shape or device than the context")
+
+    def append(self, q, k, v, cache: PagedCache, batch: PagedBatch, q_out=None, stream=None):
+        """Writes k and v [T][n_kv_heads][head_dim] to their pages, keys
+        rotated, and returns the rotated q (in q_out; q itself is fine).  q
+        None: keys and values only."""
+        self._check(cache, batch)
+        n = k.shape[0]
+        ks, vs = self._rows(k, self.n_kv_heads, n, "k"), self._rows(v, self.n_kv_heads, n, "v")
+        if q is None:
+            if q_out is not None:
+                raise ValueError("q_out without q")
+        else:
+            qs = self._rows(q, self.n_heads, n, "q")
+            if q_out is None:
+                q_out = self._empty(n, stream)
+            os = self._rows(q_out, self.n_heads, n, "q_out")
+        with _Device(self._dev):
+            rc = L.lib().ter_hip_paged_append(self._h, batch._ref, cache._ref, n, *(
+                (None, 0) if q is None else (q.data_ptr(), qs)), k.data_ptr(), ks, v.data_ptr(), vs, *(
+                (None, 0) if q is None else (q_out.data_ptr(), os)), _stream(stream))
+        L.check(rc, "ter_hip_paged_append")
+        return q_out
+
+    def attend(self, q, cache: PagedCache, batch: PagedBatch, shared: int = 0, scale: Optional[float] = None, out=None,
+               stream=None):
+        """softmax(scale q K^T) V of every row of q (rotated) over the positions
+        up to its own; scale defaults to 1 / sqrt(head_dim).  shared: that many
+        first positions are the same pages in every sequence, and are computed
+        once for all of them."""
+        self._check(cache, batch)
+        n = q.shape[0]
+        qs = self._rows(q, self.n_heads, n, "q")
+        if scale is not None and not scale > 0:
+            raise ValueError("scale must be > 0")
+        if out is None:
+            out = self._empty(n, stream)
+        os = self._rows(out, self.n_heads, n, "out")
+        lib = L.lib()
+        need = lib.ter_hip_paged_attend_ws(self._h, batch._ref, cache._ref, n, shared)
+        # a workspace of its own for every call, from the allocator of the
+        # stream (or graph) that runs it
+        ws = self._empty(need, stream, True) if need else None
+        with _Device(self._dev):
+            rc = lib.ter_hip_paged_attend(self._h, batch._ref, cache._ref, n, q.data_ptr(), qs, out.data_ptr(), os,
+                                          shared, scale or 0.0, _ptr(ws), need, _stream(stream))
+        L.check(rc, "ter_hip_paged_attend")
+        return out
+
+    def _empty(self, n: int, stream, raw: bool = False):
+        torch = _torch()
+        shape, dtype = (n, torch.uint8) if raw else ((n, self.n_heads, self.head_dim), self.dtype)
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self._dev)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self._dev)):
+            return torch.empty(shape, dtype=dtype, device=self._dev)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            L.lib().ter_hip_paged_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _Device:
+    """Makes a device current where it is not (launches go to the current one)."""
+
+    __slots__ = ("dev", "was")
+
+    def __init__(self, dev: int):
+        self.dev = dev
+
+    def __enter__(self):
+        torch = _torch()
+        was = torch._C._cuda_getDevice()
+        self.was = was if was != self.dev else None
+        if self.was is not None:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *_):
+        if self.was is not None:
+            _torch().cuda.set_device(self.was)
+
+
 def _held(it: dict) -> list:
     """What a plan built from item `it` must keep alive: the device table
     holds raw pointers into the weight buffer (as it was when the plan was
