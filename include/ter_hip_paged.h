@@ -42,7 +42,7 @@ extern "C" {
 #define TER_HIP_PAGED_BF16 1
 
 #define TER_HIP_PAGED_SEQ_MAX 1024       /* sequences per call                */
-#define TER_HIP_PAGED_ROWS_MAX (1 << 20) /* rows per call                     */
+#define TER_HIP_PAGED_ROWS_MAX (1 << 17) /* rows per call                     */
 #define TER_HIP_PAGED_POS_MAX (1 << 20)  /* positions per sequence            */
 
 /* One layer's pages.  Element (page, slot, head, d) of k (v) is at

@@ -50,7 +50,7 @@ ROPE_NORM = 0
 ROPE_NEOX = 1
 PAGED_F16, PAGED_BF16 = 0, 1
 PAGED_SEQ_MAX = 1024
-PAGED_ROWS_MAX = 1 << 20
+PAGED_ROWS_MAX = 1 << 17
 PAGED_POS_MAX = 1 << 20
 BIN_TERT = 0x54455254
 BIN_LLRT = 0x4C4C5254

@@ -44,10 +44,27 @@ struct PagedAttendArgs {
     const char* q;
     char* out;
     long long q_stride, out_stride;  // bytes
-    float scale;
-    int nh, nkv, group;
-    int shared;
+    float scale2;                    // scale * log2(e)
+    int nh, nkv, group, tokens_log2;
+    int shared;                      // a multiple of 16
+    unsigned page_magic;             // ceil(2^32 / (page_size / 16)); 0 for pages of 16
+    int max_wg, min_per, uncut;      // paged_cut()
+    // the workspace (paged_attend_layout)
+    int* before;                     // [n_seq + 1] units before each sequence
+    float* slots;                    // [2 max_wg][slot_rows][hd], then [2 max_wg][slot_rows][2]
+    float* slot_stats;
+    int slot_rows;
+    float* whole;                    // shared: [2: own positions, prefix][n_rows nh][hd], then [..][2]
+    float* whole_stats;
 };
+
+// How a call is cut, and where its parts lie in the workspace (offsets in
+// bytes; the rows of `whole` are there with a shared prefix only).
+struct PagedAttendLayout {
+    int tokens_log2, max_wg, min_per, uncut, slot_rows;
+    size_t before, slots, slot_stats, whole, whole_stats, bytes;
+};
+PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared);
 
 hipError_t launch_paged_rope_table(float* tab, int hd, int max_pos, double theta, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendArgs& a, int hd, bool neox, bool bf16, hipStream_t st);

@@ -156,8 +156,10 @@ int ter_hip_paged_append(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
 
 size_t ter_hip_paged_attend_ws(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t* batch,
                                const ter_hip_paged_cache_t* cache, int32_t n_rows, int32_t shared) {
-    (void)ctx, (void)batch, (void)cache, (void)n_rows, (void)shared;
-    return 0;
+    PagedBatch b;
+    PagedCache c;
+    if (check_batch(ctx, batch, cache, n_rows, &b, &c) || n_rows == 0 || b.n_seq == 0 || shared < 0) return 0;
+    return paged_attend_layout(ctx->nh, ctx->nkv, ctx->hd, b.n_seq, n_rows, b.capacity, shared / 16 * 16).bytes;
 }
 
 int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t* batch,
@@ -169,24 +171,43 @@ int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
     if (rc) return rc;
     if (shared < 0 || shared > a.b.capacity)
         return fail(TER_HIP_ERR_SHAPE, "shared=%d of %d positions", shared, a.b.capacity);
-    if (!(scale >= 0.f) || std::isinf(scale)) return fail(TER_HIP_ERR_SHAPE, "scale must be > 0 and finite, or 0");
+    if (!(scale >= 0.f) || scale > 1e38f) return fail(TER_HIP_ERR_SHAPE, "scale must be > 0 and finite, or 0");
     if (n_rows == 0 || batch->n_seq == 0) return TER_HIP_OK;
     if ((rc = check_rows("q", q, q_stride, (int64_t)ctx->nh * ctx->hd))) return rc;
     if ((rc = check_rows("out", out, out_stride, (int64_t)ctx->nh * ctx->hd))) return rc;
-    const size_t need = ter_hip_paged_attend_ws(ctx, batch, cache, n_rows, shared);
-    if (need && !ws) return fail(TER_HIP_ERR_NULL, "null workspace");
-    if (ws_bytes < need) return fail(TER_HIP_ERR_SHAPE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+    shared = shared / 16 * 16;
+    const PagedAttendLayout p =
+        paged_attend_layout(ctx->nh, ctx->nkv, ctx->hd, batch->n_seq, n_rows, a.b.capacity, shared);
+    // units are counted in 31 bits (a sequence's rows may lie behind its whole table)
+    const int64_t tiles = ((int64_t)n_rows >> p.tokens_log2) + batch->n_seq;
+    if (tiles * ctx->nkv * (((int64_t)a.b.capacity + n_rows) / 64 + 2 + shared / 64) > 0x7FFFFFFFll)
+        return fail(TER_HIP_ERR_SHAPE, "%d rows over %d positions are too many for one call", n_rows, a.b.capacity);
+    if (!ws) return fail(TER_HIP_ERR_NULL, "null workspace");
+    if (ws_bytes < p.bytes) return fail(TER_HIP_ERR_SHAPE, "workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
     if (!aligned(ws, 16)) return fail(TER_HIP_ERR_ALIGN, "workspace misaligned");
     if ((rc = check_device(ctx))) return rc;
     a.q = static_cast<const char*>(q);
     a.out = static_cast<char*>(out);
     a.q_stride = q_stride * 2;
     a.out_stride = out_stride * 2;
-    a.scale = scale > 0.f ? scale : (float)(1.0 / std::sqrt((double)ctx->hd));
+    a.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / std::sqrt((double)ctx->hd)) * 1.4426950408889634);
     a.nh = ctx->nh;
     a.nkv = ctx->nkv;
     a.group = ctx->nh / ctx->nkv;
-    a.shared = shared / 16 * 16;
+    a.tokens_log2 = p.tokens_log2;
+    a.shared = shared;
+    const unsigned d = (unsigned)a.c.page_size / 16;  // x / d = x * magic >> 32 for x < 2^17, d <= 4096
+    a.page_magic = d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d);
+    a.max_wg = p.max_wg;
+    a.min_per = p.min_per;
+    a.uncut = p.uncut;
+    a.slot_rows = p.slot_rows;
+    char* w = static_cast<char*>(ws);
+    a.before = reinterpret_cast<int*>(w + p.before);
+    a.slots = reinterpret_cast<float*>(w + p.slots);
+    a.slot_stats = reinterpret_cast<float*>(w + p.slot_stats);
+    a.whole = reinterpret_cast<float*>(w + p.whole);
+    a.whole_stats = reinterpret_cast<float*>(w + p.whole_stats);
     const hipError_t e = launch_paged_attend(a, ctx->hd, ctx->bf16, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "paged attention launch");
     return TER_HIP_OK;

@@ -1,79 +1,833 @@
 // paged_attend.hip -- causal attention of the new rows of a batch of sequences
-// over a paged cache.  The simple form: one wave per row and query head, 64
-// positions at a time (lane = position for the scores, lane = output elements
-// for the sums), with the running maximum and sum of a softmax in one pass.
+// over a paged cache: prompts, pieces of prompts and single tokens in one
+// launch, and a prefix that all sequences share multiplied once.
+//
+// For a row with query q that sees positions s < lim:
+//   x_s = scale log2(e) q . K_s,  out = sum_s 2^(x_s + o) V_s / sum_s 2^(x_s + o)
+// for any offset o.  One pass over the positions holds the running sums in
+// binary32 with an o near minus the largest x so far; where that grows by
+// enough, sums are multiplied by 2^(new o - old o).  Partial results (sums and
+// their o) of different ranges of positions are joined the same way.
 #include "common.h"
 #include "paged.h"
+#include "paged_plan.h"
 
 namespace terhip {
 namespace {
 
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+#define TER_LDS __attribute__((address_space(3)))
+
+// Uniform reads: of tables in memory through the scalar cache (nothing in the
+// launch writes them), of LDS into a scalar register.
+struct ConstInts {
+    const int32_t* p;
+    __device__ int operator[](long long i) const {
+        return *(const __attribute__((address_space(4))) int32_t*)(size_t)(p + i);
+    }
+};
+struct LdsInts {
+    const int* p;
+    __device__ int operator[](int i) const { return __builtin_amdgcn_readfirstlane(p[i]); }
+};
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    // Weights below 2^-14 lose bits in fp16: with this added to the exponent
+    // the largest weight is 2^8 .. 2^15 (paged_tile's kSlack) and those 2^-22
+    // of it are still exact to 11 bits.
+    static constexpr float kOffset = 8.f;
+    static __device__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+    static __device__ v4 read_tr(const TER_LDS char* p) {
+        typedef __fp16 h4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((TER_LDS h4*)p));
+    }
+    static constexpr unsigned kExp = 0x7C00u;  // exponent bits: all set in infinities and NaN
+};
+template <>
+struct Elem<__bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    static constexpr float kOffset = 0.f;
+    static __device__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+    }
+    static __device__ v4 read_tr(const TER_LDS char* p) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((TER_LDS v4*)p);
+    }
+    static constexpr unsigned kExp = 0x7F80u;
+};
+
+// 16 bytes a lane from memory straight to LDS at lds_off + 16 * lane.  Inline
+// asm without outputs: the compiler's own wait insertion would make every LDS
+// read wait for the loads of the next tile; the waits are explicit instead.
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned lds_off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds_off), "v"(voff), "s"(rsrc)
+                 : "memory");
+}
+// Waits until at most N loads are in flight, and for this wave's LDS reads.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier_only() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// One key tile in LDS: 64 rows of K, then 64 of V, HD * 2 bytes each, their
+// 16-byte pieces permuted within the row so that the operand reads below hit
+// all banks: piece p of row r is at p ^ swizzle(r).
+template <int HD>
+struct Tile {
+    static constexpr int ROW = HD * 2;
+    static constexpr int V = kPagedKeys * ROW;
+    static constexpr int BYTES = 2 * V;
+    static constexpr int RPI = 1024 / ROW;   // rows a load instruction fills
+    static constexpr int NI = 16 / RPI;      // instructions for a wave's 16 rows of K or V
+    static constexpr int PIECES = ROW / 16;
+    // K operands: 16 or 32 rows, one piece of each
+    static __device__ int swizzle_k(int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; }
+    // V operands: 64 bytes of each of four rows (transposing reads)
+    static __device__ int swizzle_v(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+};
+
+// An MFMA's result may be read by another kind of instruction only some wait
+// states later (up to 20), which hardware does not enforce and the compiler
+// fills.  It has left out the wait where the reader is the first instruction
+// behind a branch (an element of the scores read as it was before), so every
+// such result passes through here first.
+template <class V>
+__device__ __forceinline__ void settle(V& x) {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x));
+}
+template <class V>
+__device__ __forceinline__ void settle(V& x, V& y) {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x), "+v"(y));
+}
+
+// A segment's work as one workgroup sees it (all uniform).
+struct Work {
+    int kv, kv_end;      // first position of the segment's key tile 0; positions from kv_end on are zeros
+    int tok0, n_tok;     // first token row (packed), tokens of the row tile
+    int rows;            // n_tok * group
+    int seq;             // -1: the prefix, rows of any sequence
+    int row0, base;      // of the sequence
+    int kvh;
+    int j0, j1;          // key tiles
+    int dst;             // 0: out; 1: a slot; 2: whole rows
+    const int32_t* table;
+    float* slot;
+    float* slot_stats;
+};
+
 template <typename T, int HD>
-__global__ __launch_bounds__(64) void paged_attend_kernel(PagedAttendArgs a) {
-    constexpr int D = HD / 64;
-    const int t = blockIdx.x, h = blockIdx.y, g = h / a.group, lane = threadIdx.x;
-    const int b = paged_seq_of_row(a.b.row0, a.b.n_seq, t);
-    if (b < 0) return;
-    const int r0 = max(a.b.row0[b], 0), r1 = min(a.b.row0[b + 1], a.b.n_rows);
-    const long long pos = (long long)max(a.b.kv_len[b], 0) - (r1 - r0) + (t - r0);
-    const int lim = (int)min(max(pos + 1, 0ll), (long long)a.b.capacity);
-    const int32_t* table = a.b.pages + (long long)b * a.b.pages_stride;
-    const T* q = reinterpret_cast<const T*>(a.q + (long long)t * a.q_stride) + h * HD;
-    float m = -__builtin_inff(), l = 0.f, o[D];
-    for (int j = 0; j < D; ++j) o[j] = 0.f;
-    for (int s0 = 0; s0 < lim; s0 += 64) {
-        const int s = s0 + lane, n = min(64, lim - s0);
-        long long at = -1;
-        float score = -__builtin_inff();
-        if (s < lim) {
-            const int slot = s / a.c.page_size, page = table[slot];
-            float dot = 0.f;
-            if (page >= 0 && page < a.c.n_pages) {
-                at = page * a.c.page_stride + (long long)(s - slot * a.c.page_size) * a.c.pos_stride +
-                     (long long)g * a.c.head_stride;
-                const T* k = reinterpret_cast<const T*>(a.c.k + at);
-                for (int d = 0; d < HD; ++d) dot = __builtin_fmaf((float)q[d], (float)k[d], dot);
+struct Kernel {
+    typedef Elem<T> E;
+    typedef typename E::v8 v8;
+    typedef typename E::v4 v4;
+    typedef typename E::v2 v2;
+    typedef Tile<HD> L;
+    static constexpr int RING = 2 * L::BYTES;
+    // An offset stays while the largest weight is at most 2^kSlack above its start
+    static constexpr float kSlack = 7.f;
+
+    // ---- loads: wave w takes rows 16 w .. 16 w + 15 of K and V
+    struct Loader {
+        unsigned ko[L::NI], vo[L::NI];  // byte offsets of this lane's piece in the 16 rows
+        unsigned lds;
+        int w;
+        __device__ void init(const PagedAttendArgs& a, unsigned lds_off, int wave, int lane) {
+            w = wave;
+            lds = lds_off + wave * 16 * L::ROW;
+            const int r0 = lane / L::PIECES, p = lane % L::PIECES;
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) {
+                const int r = i * L::RPI + r0;
+                ko[i] = r * a.c.pos_stride + (p ^ L::swizzle_k(r)) * 16;
+                vo[i] = r * a.c.pos_stride + (p ^ L::swizzle_v(r)) * 16;
             }
-            score = dot * a.scale;
         }
-        float mx = score;
-        for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-        const float mn = fmaxf(m, mx), ref = mn == -__builtin_inff() ? 0.f : mn;
-        const float al = __expf(m - ref), p = s < lim ? __expf(score - ref) : 0.f;
-        l *= al;
-        for (int j = 0; j < D; ++j) o[j] *= al;
-        float sum = p;
-        for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
-        l += sum;
-        m = mn;
-        for (int i = 0; i < n; ++i) {
-            const float pi = __shfl(p, i);
-            const long long ai = __shfl(at, i);
-            if (ai < 0) continue;
-            const T* v = reinterpret_cast<const T*>(a.c.v + ai);
-            for (int j = 0; j < D; ++j) o[j] = __builtin_fmaf(pi, (float)v[lane * D + j], o[j]);
+        // The page of this wave's rows of key tile j (-1: none), and the load of them.
+        __device__ int page(const PagedAttendArgs& a, const Work& s, int j) const {
+            const int pos = s.kv + j * kPagedKeys + 16 * w;
+            if (pos >= s.kv_end) return -1;
+            const unsigned x = (unsigned)pos >> 4;
+            const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
+            return ConstInts{s.table}[i];
+        }
+        __device__ void issue(const PagedAttendArgs& a, const Work& s, int j, int page, int stage) const {
+            const int pos = s.kv + j * kPagedKeys + 16 * w;
+            const unsigned x = (unsigned)pos >> 4;
+            const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
+            const int slot = pos - (int)i * a.c.page_size;
+            int n = min(s.kv_end - pos, 16);
+            if (page < 0 || page >= a.c.n_pages) n = 0;
+            const unsigned bytes = n > 0 ? (unsigned)(n - 1) * a.c.pos_stride + L::ROW : 0u;
+            const long long at = n > 0 ? page * a.c.page_stride + (long long)slot * a.c.pos_stride +
+                                             (long long)s.kvh * a.c.head_stride
+                                       : 0;
+            const unsigned long long kb = (unsigned long long)(a.c.k + at), vb = (unsigned long long)(a.c.v + at);
+            const u32x4 kr = {(unsigned)kb, (unsigned)(kb >> 32) & 0xFFFFu, bytes, 0x00020000u};
+            const u32x4 vr = {(unsigned)vb, (unsigned)(vb >> 32) & 0xFFFFu, bytes, 0x00020000u};
+            const unsigned d = lds + stage * L::BYTES;
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) load_to_lds(kr, ko[i], d + i * 1024);
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) load_to_lds(vr, vo[i], d + L::V + i * 1024);
+        }
+    };
+
+    // Positions (from the segment's first one on) that packed token row t of a segment sees.
+    static __device__ int limit_of(const PagedAttendArgs& a, const Work& s, int t, const int* row0) {
+        int base = s.base, r0 = s.row0;
+        if (s.seq < 0) {
+            int lo = 0, hi = a.b.n_seq;  // row0[lo] <= t < row0[hi] (LDS copy)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (row0[mid] <= t)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            if (row0[0] > t || row0[a.b.n_seq] <= t) return 0;
+            const PagedSeq q = paged_seq(row0[lo], row0[lo + 1], gptr(a.b.kv_len)[lo], a.b.n_rows, a.b.capacity);
+            base = q.base;
+            r0 = q.r0;
+        }
+        return min(max(base + t - r0 + 1, 0), s.kv_end) - s.kv;
+    }
+
+    // Pointers of one row's partial sums.
+    static __device__ float* sums_of(const PagedAttendArgs& a, const Work& s, int r, int t, int h) {
+        return s.dst == 1 ? s.slot + (long long)r * HD
+                          : a.whole + ((long long)(s.seq < 0 ? a.b.n_rows : 0) + t) * a.nh * HD + (long long)h * HD;
+    }
+    static __device__ float* stats_of(const PagedAttendArgs& a, const Work& s, int r, int t, int h) {
+        return s.dst == 1 ? s.slot_stats + 2 * r
+                          : a.whole_stats + (((long long)(s.seq < 0 ? a.b.n_rows : 0) + t) * a.nh + h) * 2;
+    }
+
+    // ---- up to 128 rows: wave w takes rows 32 w .. 32 w + 31 against the 64
+    // keys of a tile.  S^T = K Q^T, so a lane's scores are all of query row
+    // lane % 32: its statistics need no exchange but one with lane ^ 32, and S^T
+    // in the accumulator layout is, up to the order of the keys, the operand of
+    // O^T = V^T P^T.  That order is the same for V's operand: transposing
+    // reads of four keys each.
+    static __device__ __forceinline__ void rows128(const PagedAttendArgs& a, const Work& s, const Loader& ld,
+                                                   const TER_LDS char* ring, const int* row0, int w, int lane) {
+        const int half = lane >> 5, col = lane & 31;
+        const int r = 32 * w + col, tok = r / a.group, t = s.tok0 + tok;
+        const int h = s.kvh * a.group + (r - tok * a.group);
+        const bool live = r < s.rows;
+        const int lim = live ? limit_of(a, s, t, row0) : 0;
+        v8 q[HD / 16];
+        {
+            const char* p = a.q + (live ? (long long)t * a.q_stride + (long long)h * L::ROW : 0) + half * 16;
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) q[c] = *gptr(reinterpret_cast<const v8*>(p + c * 32));
+        }
+        // the fewest and most positions that a row of this wave sees
+        int lo = live ? lim : 0x7FFFFFFF, hi = lim;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            lo = min(lo, __shfl_xor(lo, m));
+            hi = max(hi, __shfl_xor(hi, m));
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+
+        f32x16 o[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+        float l = 0.f, top = -__builtin_inff(), off = 0.f;
+
+        // LDS offsets: K pieces of row col (+ 32 by offset); V rows of the
+        // lane's transposing read
+        int ka[HD / 16], va[HD / 32];
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) ka[c] = col * L::ROW + (((2 * c + half) ^ L::swizzle_k(col)) * 16);
+        const int vr = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+            va[d] = L::V + vr * L::ROW +
+                    (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
+
+        int pg = ld.page(a, s, s.j0);
+        ld.issue(a, s, s.j0, pg, 0);
+        pg = s.j0 + 1 < s.j1 ? ld.page(a, s, s.j0 + 1) : -1;
+        int stage = 0;
+        for (int j = s.j0; j < s.j1; ++j, stage ^= 1) {
+            wait_loads<0>();
+            barrier_only();
+            if (j + 1 < s.j1) {
+                ld.issue(a, s, j + 1, pg, stage ^ 1);
+                if (j + 2 < s.j1) pg = ld.page(a, s, j + 2);
+            }
+            const int at = j * kPagedKeys;
+            if (at >= hi) continue;  // no row of this wave sees the tile
+            const TER_LDS char* tile = ring + stage * L::BYTES;
+            f32x16 x[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c)
+                    x[b] = E::mma32(*(const TER_LDS v8*)(tile + ka[c] + b * 32 * L::ROW), q[c], x[b]);
+            }
+            settle(x[0], x[1]);
+            const bool masked = at + kPagedKeys > lo;
+            if (masked) {
+                const int n = lim - at - 4 * half;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (32 * b + 8 * (i >> 2) + (i & 3) >= n) x[b][i] = -__builtin_inff();
+            }
+            float mx = x[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, x[i >> 4][i & 15]);
+            mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
+            if (__ballot(mx > top + kSlack)) {
+                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
+                const float al = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
+                top = nt;
+                off = no;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= al;
+            }
+            v8 p[4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, off));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, off));
+                    l += e0;
+                    l += e1;
+                    p[2 * b + (i >> 3)][i & 7] = (T)e0;
+                    p[2 * b + (i >> 3)][(i & 7) + 1] = (T)e1;
+                }
+            if (!masked) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) {
+                        const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
+                        const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
+                        o[d] = E::mma32(__builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7), p[c], o[d]);
+                    }
+            } else {
+                // Values that some row does not see may be infinite or NaN,
+                // and a zero weight times those is NaN: such elements are
+                // taken out here and added below to the rows that see them.
+                unsigned odd = 0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) {
+                        const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
+                        const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
+                        u32x4 y = __builtin_bit_cast(u32x4, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool b0 = (y[i] & E::kExp) == E::kExp, b1 = (y[i] >> 16 & E::kExp) == E::kExp;
+                            odd |= b0 || b1;
+                            y[i] &= (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
+                        }
+                        o[d] = E::mma32(__builtin_bit_cast(v8, y), p[c], o[d]);
+                    }
+                if (__ballot(odd != 0)) {
+                    for (int k = 0; k < kPagedKeys; ++k) {
+                        const bool sees = at + k < lim;
+                        const TER_LDS char* v = tile + L::V + k * L::ROW + 8 * half;
+#pragma unroll
+                        for (int d = 0; d < HD / 32; ++d) {
+                            // (elements 32 d .. 32 d + 31 of the row: four pieces in a row, swizzled or not)
+                            const TER_LDS char* vd = v + ((4 * d) ^ L::swizzle_v(k)) * 16;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const u32x2 y = *(const TER_LDS u32x2*)(vd + 4 * i);
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) {
+                                    const unsigned short z = (unsigned short)(y[m >> 1] >> (16 * (m & 1)));
+                                    if (sees && (z & E::kExp) == E::kExp) o[d][i + m] += (float)__builtin_bit_cast(T, z);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        l += lane_xor32(l);
+        if (!live) return;
+        if (s.dst == 0) {
+            const float inv = lim > 0 ? 1.f / l : 0.f;
+            char* p = a.out + (long long)t * a.out_stride + (long long)h * L::ROW + half * 8;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const v4 y = {(T)(o[d][i] * inv), (T)(o[d][i + 1] * inv), (T)(o[d][i + 2] * inv),
+                                  (T)(o[d][i + 3] * inv)};
+                    *gptr(reinterpret_cast<v4*>(p + 64 * d + 4 * i)) = y;
+                }
+            return;
+        }
+        float* p = sums_of(a, s, r, t, h) + half * 4;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *gptr(reinterpret_cast<f32x4*>(p + 32 * d + 2 * i)) =
+                    f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (half == 0)
+            *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, t, h))) = f32x2{lim > s.j0 * kPagedKeys ? off : __builtin_inff(), l};
+    }
+
+    // ---- up to 16 rows: wave w takes keys 16 w .. 16 w + 15 of every tile, so
+    // it waits for no other wave; the waves' sums meet in LDS at the end.
+    static __device__ __forceinline__ void rows16(const PagedAttendArgs& a, const Work& s, const Loader& ld,
+                                                  TER_LDS char* ring, const int* row0, int w, int lane) {
+        const int quad = lane >> 4, col = lane & 15;
+        const int tok = col / a.group, t = s.tok0 + tok, h = s.kvh * a.group + (col - tok * a.group);
+        const bool live = col < s.rows;
+        const int lim = live ? limit_of(a, s, t, row0) : 0;
+        int pg = ld.page(a, s, s.j0);
+        ld.issue(a, s, s.j0, pg, 0);
+        if (s.j0 + 1 < s.j1) {
+            pg = ld.page(a, s, s.j0 + 1);
+            ld.issue(a, s, s.j0 + 1, pg, 1);
+            if (s.j0 + 2 < s.j1) pg = ld.page(a, s, s.j0 + 2);
+        }
+        v8 q[HD / 32];
+        {
+            const char* p = a.q + (live ? (long long)t * a.q_stride + (long long)h * L::ROW : 0) + quad * 16;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) q[c] = *gptr(reinterpret_cast<const v8*>(p + c * 64));
+        }
+        int lo = live ? lim : 0x7FFFFFFF;
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) lo = min(lo, __shfl_xor(lo, m));
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        f32x4 o[HD / 16];
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float l = 0.f, top = -__builtin_inff(), off = 0.f;
+        const int kr = 16 * w + col, vr = 16 * w + 4 * quad + (col >> 2);
+        int ka[HD / 32], va[HD / 16];
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) ka[c] = kr * L::ROW + (((4 * c + quad) ^ L::swizzle_k(kr)) * 16);
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+            va[d] = L::V + vr * L::ROW + (((2 * d + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
+        int stage = 0;
+        for (int j = s.j0; j < s.j1; ++j, stage ^= 1) {
+            // the next tile's loads may still be in flight
+            if (j + 1 < s.j1)
+                wait_loads<2 * L::NI>();
+            else
+                wait_loads<0>();
+            const int at = j * kPagedKeys + 16 * w;
+            const TER_LDS char* tile = ring + stage * L::BYTES;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) x = E::mma16(*(const TER_LDS v8*)(tile + ka[c]), q[c], x);
+            settle(x);
+            const bool masked = at + 16 > lo;
+            if (masked) {
+                const int n = lim - at - 4 * quad;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= n) x[i] = -__builtin_inff();
+            }
+            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            mx = fmaxf(mx, lane_xor16(mx));
+            mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
+            if (__ballot(mx > top + kSlack)) {
+                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
+                const float al = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
+                top = nt;
+                off = no;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) o[d] *= al;
+            }
+            v4 p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.scale2, off));
+                l += e;
+                p[i] = (T)e;
+            }
+            if (!masked) {
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(E::read_tr(tile + va[d]), p, o[d]);
+            } else {
+                unsigned odd = 0;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    u32x2 y = __builtin_bit_cast(u32x2, E::read_tr(tile + va[d]));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const bool b0 = (y[i] & E::kExp) == E::kExp, b1 = (y[i] >> 16 & E::kExp) == E::kExp;
+                        odd |= b0 || b1;
+                        y[i] &= (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
+                    }
+                    o[d] = E::mma16k16(__builtin_bit_cast(v4, y), p, o[d]);
+                }
+                if (__ballot(odd != 0)) {
+                    for (int k = 0; k < 16; ++k) {
+                        const bool sees = at + k < lim;
+                        const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW;
+#pragma unroll
+                        for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int e = 16 * d + 4 * quad + i;
+                                const unsigned short y = *(const TER_LDS unsigned short*)(
+                                    v + (((e >> 3) ^ L::swizzle_v(16 * w + k)) * 16) + (e & 7) * 2);
+                                if (sees && (y & E::kExp) == E::kExp) o[d][i] += (float)__builtin_bit_cast(T, y);
+                            }
+                    }
+                }
+            }
+            if (j + 2 < s.j1) {
+                wait_lds();  // this tile's reads are done
+                ld.issue(a, s, j + 2, pg, stage);
+                if (j + 3 < s.j1) pg = ld.page(a, s, j + 3);
+            }
+        }
+        l += lane_xor16(l);
+        l += lane_xor32(l);
+        // the waves' sums: [wave][row][HD], then [wave][row][2]
+        __syncthreads();
+        TER_LDS float* sums = (TER_LDS float*)ring;
+        TER_LDS float* stats = sums + kWaves * 16 * HD;
+        if (live) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+                *(TER_LDS f32x4*)(sums + (w * 16 + col) * HD + 16 * d + 4 * quad) = o[d];
+            if (quad == 0) {
+                stats[(w * 16 + col) * 2] = lim > s.j0 * kPagedKeys + 16 * w ? off : __builtin_inff();
+                stats[(w * 16 + col) * 2 + 1] = l;
+            }
+        }
+        __syncthreads();
+        for (int i = w * 64 + lane; i < s.rows * (HD / 4); i += kThreads) {
+            const int r = i / (HD / 4), e = (i - r * (HD / 4)) * 4;
+            float f[kWaves], least = __builtin_inff(), tl = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) least = fminf(least, stats[(k * 16 + r) * 2]);
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) {
+                const float ok = stats[(k * 16 + r) * 2];
+                f[k] = ok == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(least - ok);
+                if (f[k] != 0.f || stats[(k * 16 + r) * 2 + 1] != stats[(k * 16 + r) * 2 + 1]) {  // (NaN stays)
+                    tl += f[k] * stats[(k * 16 + r) * 2 + 1];
+                    y += f[k] * *(TER_LDS f32x4*)(sums + (k * 16 + r) * HD + e);
+                }
+            }
+            const int rt = s.tok0 + r / a.group, rh = s.kvh * a.group + r % a.group;
+            if (s.dst == 0) {
+                const float inv = least == __builtin_inff() ? 0.f : 1.f / tl;
+                const v4 z = {(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
+                *gptr(reinterpret_cast<v4*>(a.out + (long long)rt * a.out_stride + (long long)rh * L::ROW + e * 2)) = z;
+            } else {
+                *gptr(reinterpret_cast<f32x4*>(sums_of(a, s, r, rt, rh) + e)) = y;
+                if (e == 0) *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, rt, rh))) = f32x2{least, tl};
+            }
         }
     }
-    T* out = reinterpret_cast<T*>(a.out + (long long)t * a.out_stride) + h * HD + lane * D;
-    for (int j = 0; j < D; ++j) out[j] = (T)(lim > 0 ? o[j] / l : 0.f);
+};
+
+// Units before each sequence (paged_plan.h), [n_seq + 1] in LDS; `row0` a copy
+// of the row boundaries beside it.
+__device__ __forceinline__ int count_units(const PagedAttendArgs& a, const PagedLine& l, int* before, int* row0, int* tmp) {
+    const int n = a.b.n_seq, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int each = (n + kThreads - 1) / kThreads;
+    int sum = 0;
+    for (int i = tid * each; i < min(n, (tid + 1) * each); ++i) {
+        const int r0 = gptr(a.b.row0)[i], r1 = gptr(a.b.row0)[i + 1];
+        row0[i] = r0;
+        if (i == n - 1) row0[n] = r1;
+        const int u = paged_units(paged_seq(r0, r1, gptr(a.b.kv_len)[i], a.b.n_rows, a.b.capacity), l.q, l.kv0) * a.nkv;
+        before[i] = sum;
+        sum += u;
+    }
+    int inc = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(inc, d);
+        if (lane >= d) inc += v;
+    }
+    if (lane == 63) tmp[w] = inc;
+    __syncthreads();
+    int add = l.prefix_units + inc - sum, total = l.prefix_units;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        if (k < w) add += tmp[k];
+        total += tmp[k];
+    }
+    for (int i = tid * each; i < min(n, (tid + 1) * each); ++i) before[i] += add;
+    if (tid == 0) before[n] = total;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(total);
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendArgs a) {
+    typedef Kernel<T, HD> K;
+    extern __shared__ __align__(1024) unsigned char lds[];
+    int* before = reinterpret_cast<int*>(lds + K::RING);
+    int* row0 = before + a.b.n_seq + 1;
+    int* tmp = row0 + a.b.n_seq + 1;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TER_LDS char* ring = (TER_LDS char*)lds;
+
+    PagedLine l = paged_line(a.tokens_log2, a.shared, a.b.n_rows, a.nkv);
+    const int total = count_units(a, l, before, row0, tmp);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = before[i];
+    paged_cut(l, total, a.max_wg, a.min_per, a.uncut);
+    // neighbouring ranges on one XCD (blocks go round the 8 XCDs): they read the same keys
+    const int chunk = (l.n_wg + 7) / 8, g = (int)(blockIdx.x % 8) * chunk + (int)(blockIdx.x / 8);
+    if ((int)(blockIdx.x / 8) >= chunk || g >= l.n_wg) return;
+
+    const ConstInts rows{a.b.row0}, lens{a.b.kv_len};
+    auto segment = [&](int u) {
+        return paged_segment(l, u, rows, lens, a.b.n_seq, a.b.n_rows, a.b.capacity, a.nkv, LdsInts{before});
+    };
+    auto cut = [&](int i) {
+        const long long u = (long long)i * l.per;
+        return u >= total ? total : paged_snap(l, segment((int)u), (int)u);
+    };
+    typename K::Loader ld;
+    ld.init(a, (unsigned)(size_t)ring, w, lane);
+    const int u1 = cut(g + 1);
+    for (int u = cut(g); u < u1;) {
+        const PagedSegment sg = segment(u);
+        const int end = min(u1, sg.start + sg.n);
+        Work s;
+        s.seq = sg.seq;
+        s.kvh = sg.kvh;
+        s.j0 = u - sg.start;
+        s.j1 = end - sg.start;
+        const bool whole = s.j0 == 0 && s.j1 == sg.n;
+        if (sg.seq < 0) {
+            s.tok0 = sg.tile << l.q;
+            s.n_tok = min(a.b.n_rows - s.tok0, 1 << l.q);
+            s.kv = 0;
+            s.kv_end = a.shared;
+            s.row0 = s.base = 0;
+            s.table = a.b.pages;
+        } else {
+            const PagedSeq q = paged_seq(rows[sg.seq], rows[sg.seq + 1], lens[sg.seq], a.b.n_rows, a.b.capacity);
+            const int i = sg.tile << l.q;
+            s.tok0 = q.r0 + i;
+            s.n_tok = min(q.n - i, 1 << l.q);
+            s.kv = a.shared;
+            s.kv_end = max(paged_limit(q, i + s.n_tok - 1, a.b.capacity), a.shared);
+            s.row0 = q.r0;
+            s.base = q.base;
+            s.table = a.b.pages + (long long)sg.seq * a.b.pages_stride;
+        }
+        s.rows = s.n_tok * a.group;
+        s.dst = !whole ? 1 : a.shared ? 2 : 0;
+        const int slot = 2 * g + (s.j0 == 0 ? 1 : 0);
+        s.slot = a.slots + (long long)slot * a.slot_rows * HD;
+        s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
+        __syncthreads();  // the ring is free
+        if (s.rows > 16)
+            K::rows128(a, s, ld, ring, row0, w, lane);
+        else
+            K::rows16(a, s, ld, ring, row0, w, lane);
+        u = end;
+    }
+}
+
+// Joins the partial results of segments that were cut (and, with a shared
+// prefix, of the prefix with each row's own positions).  A workgroup is one row
+// tile of a sequence and KV head, every gridDim.z-th row of it; HD / 4 threads
+// take the elements, kThreads / (HD / 4) groups of them every so manieth part.
+template <typename T, int HD>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttendArgs a) {
+    constexpr int TPR = HD / 4, GROUPS = kThreads / TPR;
+    __shared__ __align__(16) float sums[GROUPS][HD];
+    __shared__ float stats[GROUPS][2];
+    typedef typename Elem<T>::v4 v4;
+    const int q = a.tokens_log2, kvh = blockIdx.y, x = blockIdx.x;
+    const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
+    // row tiles of sequence b: from (r0 >> q) + b on (there are no more than that leaves room for)
+    int lo = 0, hi = a.b.n_seq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((paged_seq(rows[mid], rows[mid + 1], 0, a.b.n_rows, 0).r0 >> q) + mid <= x)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const PagedSeq s = paged_seq(rows[lo], rows[lo + 1], lens[lo], a.b.n_rows, a.b.capacity);
+    const int tile = x - (s.r0 >> q) - lo;
+    if (tile < 0 || tile >= paged_row_tiles(s, q)) return;
+    PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
+    paged_cut(l, before[a.b.n_seq], a.max_wg, a.min_per, a.uncut);
+    const int b0 = before[lo], each = (before[lo + 1] - b0) / a.nkv;
+    const int start = b0 + kvh * each + (int)paged_key_tiles_before(s, tile, q, l.kv0);
+    const PagedParts own = paged_parts(l, start, paged_key_tiles(s, tile, q, l.kv0));
+    const int n_own = own.last - own.first + 1;
+    if (!a.shared && n_own == 1) return;  // written where it was computed
+
+    const int n_rows = min(s.n - (tile << q), 1 << q) * a.group;
+    const int grp = threadIdx.x / TPR, e = (threadIdx.x % TPR) * 4;
+    for (int r = blockIdx.z; r < n_rows; r += gridDim.z) {
+        const int tok = r / a.group, t = s.r0 + (tile << q) + tok, h = kvh * a.group + r - tok * a.group;
+        PagedParts pre{0, -1};
+        int pr = 0;
+        if (a.shared) {
+            pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_tiles, l.prefix_tiles);
+            pr = (t & ((1 << q) - 1)) * a.group + r - tok * a.group;
+        }
+        const int n_pre = pre.last - pre.first + 1, n = n_own + n_pre;
+        auto place = [&](int i, const float*& sum, const float*& stat) {
+            const bool is_pre = i >= n_own;
+            const PagedParts& p = is_pre ? pre : own;
+            if ((is_pre ? n_pre : n_own) == 1) {
+                const long long at = ((long long)(is_pre ? a.b.n_rows : 0) + t) * a.nh + h;
+                sum = a.whole + at * HD;
+                stat = a.whole_stats + at * 2;
+            } else {
+                const long long at = (long long)paged_slot(p, p.first + i - (is_pre ? n_own : 0)) * a.slot_rows +
+                                     (is_pre ? pr : r);
+                sum = a.slots + at * HD;
+                stat = a.slot_stats + at * 2;
+            }
+        };
+        float off = __builtin_inff(), tl = 0.f;
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        for (int i = grp; i < n; i += GROUPS) {
+            const float *ps, *pt;
+            place(i, ps, pt);
+            const f32x2 st = *gptr(reinterpret_cast<const f32x2*>(pt));
+            const f32x4 v = *gptr(reinterpret_cast<const f32x4*>(ps + e));
+            if (st[0] == __builtin_inff()) continue;
+            const float no = fminf(off, st[0]);
+            const float f0 = off == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
+            const float f1 = __builtin_amdgcn_exp2f(no - st[0]);
+            tl = tl * f0 + st[1] * f1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = y[k] * f0 + v[k] * f1;
+            off = no;
+        }
+        __syncthreads();
+        *reinterpret_cast<f32x4*>(&sums[grp][e]) = y;
+        if (e == 0) {
+            stats[grp][0] = off;
+            stats[grp][1] = tl;
+        }
+        __syncthreads();
+        if (grp == 0) {
+            float least = __builtin_inff(), total = 0.f;
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) least = fminf(least, stats[k][0]);
+            f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) {
+                const float f = stats[k][0] == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(least - stats[k][0]);
+                if (f != 0.f || stats[k][1] != stats[k][1]) {  // (NaN stays)
+                    total += f * stats[k][1];
+                    z += f * *reinterpret_cast<const f32x4*>(&sums[k][e]);
+                }
+            }
+            const float inv = least == __builtin_inff() ? 0.f : 1.f / total;
+            const v4 out = {(T)(z[0] * inv), (T)(z[1] * inv), (T)(z[2] * inv), (T)(z[3] * inv)};
+            *gptr(reinterpret_cast<v4*>(a.out + (long long)t * a.out_stride + (long long)h * HD * 2 + e * 2)) = out;
+        }
+    }
+}
+
+template <typename T, int HD>
+hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
+    static LdsLimit limit;
+    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves) * 4;
+    const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
+    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves) * 4, {fn});
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.max_wg), dim3(kThreads), lds, st, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (!a.shared && a.uncut * kPagedKeys > a.b.capacity + a.b.n_rows) return hipSuccess;  // nothing is cut
+    const int tiles = (a.b.n_rows >> a.tokens_log2) + a.b.n_seq;
+    const int z = min(a.slot_rows, tiles * a.nkv >= 1024 ? 4 : 32);
+    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(tiles, a.nkv, z), dim3(kThreads), 0, st, a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
+PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared) {
+    PagedAttendLayout p{};
+    const int group = nh / nkv;
+    p.tokens_log2 = paged_tokens_log2(group);
+    int dev = 0;
+    int cus = hipGetDevice(&dev) == hipSuccess ? device_cu_count(dev) : 256;
+    p.max_wg = (2 * cus + 7) / 8 * 8;
+    p.min_per = 2;
+    p.uncut = capacity + n_rows <= 512 ? 9 : 1;
+    p.slot_rows = min(kPagedRows, (int)min((long long)n_rows * group, (long long)(1 << p.tokens_log2) * group));
+    auto take = [&](size_t n) {
+        const size_t at = p.bytes;
+        p.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    const size_t slots = 2 * (size_t)p.max_wg * p.slot_rows, whole = shared ? 2 * (size_t)n_rows * nh : 0;
+    p.before = take((size_t)(n_seq + 1) * 4);
+    p.slot_stats = take(slots * 2 * 4);
+    p.whole_stats = take(whole * 2 * 4);
+    p.slots = take(slots * hd * 4);
+    p.whole = take(whole * hd * 4);
+    return p;
+}
+
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int hd, bool bf16, hipStream_t st) {
-    const dim3 grid(a.b.n_rows, a.nh), block(64);
-    if (hd == 128) {
-        if (bf16)
-            hipLaunchKernelGGL((paged_attend_kernel<__bf16, 128>), grid, block, 0, st, a);
-        else
-            hipLaunchKernelGGL((paged_attend_kernel<_Float16, 128>), grid, block, 0, st, a);
-    } else {
-        if (bf16)
-            hipLaunchKernelGGL((paged_attend_kernel<__bf16, 64>), grid, block, 0, st, a);
-        else
-            hipLaunchKernelGGL((paged_attend_kernel<_Float16, 64>), grid, block, 0, st, a);
-    }
-    return hipGetLastError();
+    if (hd == 128) return bf16 ? launch<__bf16, 128>(a, st) : launch<_Float16, 128>(a, st);
+    return bf16 ? launch<__bf16, 64>(a, st) : launch<_Float16, 64>(a, st);
 }
 
 }  // namespace terhip

@@ -1,0 +1,188 @@
+// paged_plan.h -- how the attention over a paged cache is cut into work, for
+// the device and (tests) the host: integer arithmetic only.
+//
+// The query rows of one KV head and one sequence (its tokens times the query
+// heads of the group) are cut into row tiles of 2^q tokens, the positions that
+// a tile's last row sees into key tiles of 64.  A segment is one row tile with
+// all its key tiles, a unit one key tile of one segment.  All units of a launch
+// form one line,
+//   [ shared prefix: KV head, row tile over all rows ][ sequence, KV head, row tile ],
+// which is cut into equal ranges, one for each workgroup, whatever the lengths
+// are: a long sequence is spread over many workgroups, many short ones share
+// one.  A cut close to a segment's edge is moved there.  A segment that is cut
+// leaves one partial result in each range that holds a part of it; they
+// are joined by a second kernel.  Lengths are known on the device only, so each
+// workgroup finds its range itself: unit counts of row tiles have a closed form,
+// so it needs one prefix sum over the sequences.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define TER_HD __host__ __device__ __forceinline__
+#else
+#define TER_HD inline
+#endif
+
+namespace terhip {
+
+constexpr int kPagedKeys = 64;   // positions of a key tile
+constexpr int kPagedRows = 128;  // rows of a row tile
+
+TER_HD int paged_min(int a, int b) { return a < b ? a : b; }
+TER_HD int paged_max(int a, int b) { return a > b ? a : b; }
+
+// log2 of the tokens of a row tile: the largest power of two of them that has
+// at most 128 rows.
+TER_HD int paged_tokens_log2(int group) {
+    int q = 0;
+    while ((2 << q) * group <= kPagedRows) ++q;
+    return q;
+}
+
+struct PagedSeq {
+    int r0, n;  // first row, rows
+    int base;   // positions before the rows (negative: rows that see nothing), at most cap
+};
+TER_HD PagedSeq paged_seq(int row0, int row1, int kv_len, int n_rows, int cap) {
+    PagedSeq s;
+    s.r0 = paged_min(paged_max(row0, 0), n_rows);
+    s.n = paged_min(paged_max(row1, s.r0), n_rows) - s.r0;
+    s.base = paged_min(paged_max(kv_len, 0) - s.n, cap);
+    return s;
+}
+// Positions that row i of a sequence sees.
+TER_HD int paged_limit(const PagedSeq& s, int i, int cap) { return paged_min(paged_max(s.base + i + 1, 0), cap); }
+
+TER_HD int paged_row_tiles(const PagedSeq& s, int q) { return (s.n + (1 << q) - 1) >> q; }
+// Key tiles of row tile rt of a sequence from position kv0 on, at least one (a
+// row that sees nothing has an output too).
+TER_HD int paged_key_tiles(const PagedSeq& s, int rt, int q, int kv0) {
+    const int a = s.base - kv0 + paged_min(s.n, (rt + 1) << q);
+    return a <= kPagedKeys ? 1 : (a + kPagedKeys - 1) / kPagedKeys;
+}
+// Key tiles of row tiles 0 .. n - 1, all of them full.
+TER_HD long long paged_key_tiles_before(const PagedSeq& s, int n, int q, int kv0) {
+    const int c = s.base - kv0, room = kPagedKeys - c;
+    const int ones = paged_min(n, room >= (1 << q) ? room >> q : 0);  // tiles of at most 64 positions
+    if (ones == n) return n;
+    const long long m = n - ones;
+    if (q >= 6)  // ceil((c + 2^q i) / 64), i = ones + 1 .. n
+        return ones + m * ((c + 63) >> 6) + ((m * (ones + 1 + n) / 2) << (q - 6));
+    // ceil(x / R) for x = e + ones + 1 .. e + n, R row tiles to a key tile
+    const int lr = 6 - q, e = (c + (1 << q) - 1) >> q;
+    const long long x1 = e + n, x0 = e + ones, a1 = x1 >> lr, a0 = x0 >> lr, r = (1 << lr) - 1;
+    return ones + (((a1 * (a1 + 1) / 2) << lr) + (x1 & r) * (a1 + 1)) -
+           (((a0 * (a0 + 1) / 2) << lr) + (x0 & r) * (a0 + 1));
+}
+// Units of a sequence, for one KV head.
+TER_HD int paged_units(const PagedSeq& s, int q, int kv0) {
+    const int t = paged_row_tiles(s, q);
+    return t ? (int)paged_key_tiles_before(s, t - 1, q, kv0) + paged_key_tiles(s, t - 1, q, kv0) : 0;
+}
+// The row tile that holds unit r of a sequence and KV head.
+TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
+    int lo = 0, hi = paged_row_tiles(s, q) - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (paged_key_tiles_before(s, mid, q, kv0) <= r)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+// One launch's line of units.  The ranges: workgroup g of n_wg takes the units
+// from cut g to cut g + 1, cut g being near g * per.
+struct PagedLine {
+    int q, kv0;                // row tile, first position behind the prefix
+    int prefix_tiles;          // key tiles of the prefix
+    int prefix_rows;           // row tiles over all rows
+    int prefix_units;          // of all KV heads
+    int total;
+    int per, near;             // units a range, cuts closer than `near` to an edge move there
+    int n_wg;
+};
+TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
+    PagedLine l{};
+    l.q = q;
+    l.kv0 = shared;
+    l.prefix_tiles = (shared + kPagedKeys - 1) / kPagedKeys;
+    l.prefix_rows = (n_rows + (1 << q) - 1) >> q;
+    l.prefix_units = l.prefix_tiles * l.prefix_rows * nkv;
+    return l;
+}
+// total: prefix units and those of the sequences.  max_wg: workgroups of the
+// launch.  min_per: fewer units than that are not worth a workgroup.  uncut:
+// segments of fewer units are never cut.
+TER_HD void paged_cut(PagedLine& l, int total, int max_wg, int min_per, int uncut) {
+    l.total = total;
+    l.per = paged_max(min_per, (total + max_wg - 1) / max_wg);
+    l.near = paged_max(paged_max(1, l.per / 8), (uncut + 1) / 2);
+    l.n_wg = (total + l.per - 1) / l.per;
+}
+
+struct PagedSegment {
+    int start, n;   // first unit, units
+    int seq;        // -1: the prefix
+    int kvh, tile;  // KV head, row tile
+};
+
+// The segment of unit u (0 <= u < total).  before: units before each sequence
+// (prefix units included), [n_seq + 1].
+template <class Ints, class Before>
+TER_HD PagedSegment paged_segment(const PagedLine& l, int u, Ints row0, Ints kv_len, int n_seq, int n_rows, int cap,
+                                  int nkv, Before before) {
+    PagedSegment g;
+    if (u < l.prefix_units) {
+        const int i = u / l.prefix_tiles;
+        g.seq = -1;
+        g.kvh = i / l.prefix_rows;
+        g.tile = i - g.kvh * l.prefix_rows;
+        g.start = i * l.prefix_tiles;
+        g.n = l.prefix_tiles;
+        return g;
+    }
+    int lo = 0, hi = n_seq - 1;  // the last sequence that begins at u or before (empty ones before it end there too)
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[mid] <= u)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const PagedSeq s = paged_seq(row0[lo], row0[lo + 1], kv_len[lo], n_rows, cap);
+    const int b0 = before[lo], each = (before[lo + 1] - b0) / nkv, at = u - b0;
+    g.seq = lo;
+    g.kvh = at / each;
+    const int r = at - g.kvh * each;
+    g.tile = paged_row_tile_of(s, r, l.q, l.kv0);
+    g.start = b0 + g.kvh * each + (int)paged_key_tiles_before(s, g.tile, l.q, l.kv0);
+    g.n = paged_key_tiles(s, g.tile, l.q, l.kv0);
+    return g;
+}
+
+// Where a cut at unit u of segment g goes.
+TER_HD int paged_snap(const PagedLine& l, const PagedSegment& g, int u) {
+    const int off = u - g.start;
+    return off < l.near ? g.start : g.n - off < l.near ? g.start + g.n : u;
+}
+
+// The ranges that hold parts of a segment: first .. last, one if it is not cut.
+// Range g writes its part to slot 2 g + 1 if the part begins the segment (it is
+// then the last of the range), else to slot 2 g.
+struct PagedParts {
+    int first, last;
+};
+TER_HD PagedParts paged_parts(const PagedLine& l, int start, int n) {
+    PagedParts p;
+    const int a = start + l.near, z = start + n - l.near;  // cuts from a to z stay inside
+    const int c0 = (a + l.per - 1) / l.per, c1 = z < 0 ? -1 : z / l.per;
+    p.first = c0 - 1;
+    p.last = paged_max(c0 - 1, c1);
+    return p;
+}
+TER_HD int paged_slot(const PagedParts& p, int i) { return i == p.first ? 2 * i + 1 : 2 * i; }
+
+}  // namespace terhip

@@ -202,3 +202,16 @@ def test_python_refuses_host_tensors():
         T.PagedBatch(i, i[:2], torch.zeros(2, 2, dtype=torch.int32))
     with pytest.raises(TypeError):
         T.PagedAttention(4, 2, 64, 16, 1e4, dtype=torch.float32)
+
+
+def test_cutting_of_the_work(tmp_path):
+    """tests/c/paged_plan.cpp: every unit of work in one range, partial results
+    where the joining kernel looks for them, closed forms against counting."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not installed")
+    exe = str(tmp_path / "paged_plan")
+    subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", os.path.join(ROOT, "tests", "c", "paged_plan.cpp"), "-o", exe],
+                   check=True)
+    r = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout
