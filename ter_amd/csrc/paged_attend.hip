@@ -286,30 +286,35 @@ struct Kernel {
         int pg = ld.page(a, s, s.j0);
         ld.issue(a, s, s.j0, pg, 0);
         pg = s.j0 + 1 < s.j1 ? ld.page(a, s, s.j0 + 1) : -1;
-        int stage = 0;
-        for (int j = s.j0; j < s.j1; ++j, stage ^= 1) {
+        int stage = 0, j = s.j0;
+        auto next = [&]() {  // tile j is in LDS, tile j + 1 on its way
             wait_loads<0>();
             barrier_only();
             if (j + 1 < s.j1) {
                 ld.issue(a, s, j + 1, pg, stage ^ 1);
                 if (j + 2 < s.j1) pg = ld.page(a, s, j + 2);
             }
-            const int at = j * kPagedKeys;
-            if (at >= hi) continue;  // no row of this wave sees the tile
+        };
+        auto step = [&](auto masked) {
+            constexpr bool kMasked = decltype(masked)::value;
             const TER_LDS char* tile = ring + stage * L::BYTES;
             f32x16 x[2];
+            v8 k[HD / 16];
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) k[c] = *(const TER_LDS v8*)(tile + ka[c]);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
 #pragma unroll
-                for (int c = 0; c < HD / 16; ++c)
-                    x[b] = E::mma32(*(const TER_LDS v8*)(tile + ka[c] + b * 32 * L::ROW), q[c], x[b]);
+                for (int c = 0; c < HD / 16; ++c) {
+                    x[b] = E::mma32(k[c], q[c], x[b]);
+                    if (b == 0) k[c] = *(const TER_LDS v8*)(tile + ka[c] + 32 * L::ROW);
+                }
             }
             settle(x[0], x[1]);
-            const bool masked = at + kPagedKeys > lo;
-            if (masked) {
-                const int n = lim - at - 4 * half;
+            if (kMasked) {
+                const int n = lim - j * kPagedKeys - 4 * half;
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -343,56 +348,58 @@ struct Kernel {
                     p[2 * b + (i >> 3)][i & 7] = (T)e0;
                     p[2 * b + (i >> 3)][(i & 7) + 1] = (T)e1;
                 }
-            if (!masked) {
+            // Values that some row does not see may be infinite or NaN, and a
+            // zero weight times those is NaN: in masked tiles such elements are
+            // taken out here and added below to the rows that see them.
+            unsigned odd = 0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) {
-                        const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
-                        const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
-                        o[d] = E::mma32(__builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7), p[c], o[d]);
-                    }
-            } else {
-                // Values that some row does not see may be infinite or NaN,
-                // and a zero weight times those is NaN: such elements are
-                // taken out here and added below to the rows that see them.
-                unsigned odd = 0;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) {
-                        const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
-                        const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
-                        u32x4 y = __builtin_bit_cast(u32x4, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int d = 0; d < HD / 32; ++d) {
+                    const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
+                    const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
+                    u32x4 y = __builtin_bit_cast(u32x4, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    if (kMasked) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const bool b0 = (y[i] & E::kExp) == E::kExp, b1 = (y[i] >> 16 & E::kExp) == E::kExp;
                             odd |= b0 || b1;
                             y[i] &= (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
                         }
-                        o[d] = E::mma32(__builtin_bit_cast(v8, y), p[c], o[d]);
                     }
-                if (__ballot(odd != 0)) {
-                    for (int k = 0; k < kPagedKeys; ++k) {
-                        const bool sees = at + k < lim;
-                        const TER_LDS char* v = tile + L::V + k * L::ROW + 8 * half;
+                    o[d] = E::mma32(__builtin_bit_cast(v8, y), p[c], o[d]);
+                }
+            if (kMasked && __ballot(odd != 0)) {
+                for (int i = 0; i < HD / 32; ++i) settle(o[i]);
+                for (int k = 0; k < kPagedKeys; ++k) {
+                    const bool sees = j * kPagedKeys + k < lim;
+                    const TER_LDS char* v = tile + L::V + k * L::ROW + 8 * half;
 #pragma unroll
-                        for (int d = 0; d < HD / 32; ++d) {
-                            // (elements 32 d .. 32 d + 31 of the row: four pieces in a row, swizzled or not)
-                            const TER_LDS char* vd = v + ((4 * d) ^ L::swizzle_v(k)) * 16;
+                    for (int d = 0; d < HD / 32; ++d) {
+                        // (elements 32 d .. 32 d + 31 of the row: four pieces in a row, swizzled or not)
+                        const TER_LDS char* vd = v + ((4 * d) ^ L::swizzle_v(k)) * 16;
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const u32x2 y = *(const TER_LDS u32x2*)(vd + 4 * i);
+                        for (int i = 0; i < 16; i += 4) {
+                            const u32x2 y = *(const TER_LDS u32x2*)(vd + 4 * i);
 #pragma unroll
-                                for (int m = 0; m < 4; ++m) {
-                                    const unsigned short z = (unsigned short)(y[m >> 1] >> (16 * (m & 1)));
-                                    if (sees && (z & E::kExp) == E::kExp) o[d][i + m] += (float)__builtin_bit_cast(T, z);
-                                }
+                            for (int m = 0; m < 4; ++m) {
+                                const unsigned short z = (unsigned short)(y[m >> 1] >> (16 * (m & 1)));
+                                if (sees && (z & E::kExp) == E::kExp) o[d][i + m] += (float)__builtin_bit_cast(T, z);
                             }
                         }
                     }
                 }
             }
+        };
+        // tiles that every row of this wave sees whole, then the others
+        const int full = min(s.j1, max(s.j0, lo / kPagedKeys));
+        for (; j < full; ++j, stage ^= 1) {
+            next();
+            step(std::false_type{});
+        }
+        for (; j < s.j1; ++j, stage ^= 1) {
+            next();
+            if (j * kPagedKeys < hi) step(std::true_type{});
         }
         l += lane_xor32(l);
         if (!live) return;
