@@ -120,6 +120,32 @@ struct Tile {
     static __device__ int swizzle_v(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 };
 
+// The sign bits of the halves of y that hold infinities or NaN (all exponent
+// bits set: adding the lowest one carries into the sign), and y without them.
+template <typename T>
+__device__ __forceinline__ unsigned odd_halves(unsigned y) {
+    constexpr unsigned E1 = Elem<T>::kExp, E2 = E1 | E1 << 16, one = E1 & (0u - E1);
+    return ((y & E2) + (one | one << 16)) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ unsigned without_odd(unsigned y) {
+    const unsigned s = odd_halves<T>(y);
+    return y & ~((s - (s >> 15)) | s);
+}
+
+// Adds the odd ones of four values to four sums, where the row sees them.
+template <typename T, class V>
+__device__ __forceinline__ void add_odd(V& sums, int i, u32x2 y, bool sees) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const unsigned short u = (unsigned short)(y[m >> 1] >> (16 * (m & 1)));
+        if (sees && (u & Elem<T>::kExp) == Elem<T>::kExp) sums[i + m] += (float)__builtin_bit_cast(T, u);
+    }
+}
+// What sums are multiplied by when their offset changes by x <= 0: never zero,
+// which would turn infinite ones into NaN.
+__device__ __forceinline__ float shrink(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 1.17549435e-38f); }
+
 // An MFMA's result may be read by another kind of instruction only some wait
 // states later (up to 20), which hardware does not enforce and the compiler
 // fills.  It has left out the wait where the reader is the first instruction
@@ -243,7 +269,10 @@ struct Kernel {
     // O^T = V^T P^T.  That order is the same for V's operand: transposing
     // reads of four keys each.
     static __device__ __forceinline__ void rows128(const PagedAttendArgs& a, const Work& s, const Loader& ld,
-                                                   const TER_LDS char* ring, const int* row0, int w, int lane) {
+                                                   TER_LDS char* ring, const int* row0, int* shared, int& tick,
+                                                   int w, int lane) {
+        int* const lows = shared;                 // [kWaves]
+        int* const flag = shared + kWaves;        // [2] the tick at which a tile of a stage held odd values
         const int half = lane >> 5, col = lane & 31;
         const int r = 32 * w + col, tok = r / a.group, t = s.tok0 + tok;
         const int h = s.kvh * a.group + (r - tok * a.group);
@@ -255,12 +284,19 @@ struct Kernel {
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) q[c] = *gptr(reinterpret_cast<const v8*>(p + c * 32));
         }
-        // the fewest and most positions that a row of this wave sees
+        // the fewest positions that a row sees, the most that one of this wave does
         int lo = live ? lim : 0x7FFFFFFF, hi = lim;
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1) {
             lo = min(lo, __shfl_xor(lo, m));
             hi = max(hi, __shfl_xor(hi, m));
+        }
+        if (s.seq >= 0) {
+            lo = paged_limit({0, 0, s.base}, s.tok0 - s.row0, s.kv_end) - s.kv;
+        } else {
+            if (lane == 0) lows[w] = lo;
+            __syncthreads();
+            lo = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
@@ -287,119 +323,191 @@ struct Kernel {
         ld.issue(a, s, s.j0, pg, 0);
         pg = s.j0 + 1 < s.j1 ? ld.page(a, s, s.j0 + 1) : -1;
         int stage = 0, j = s.j0;
-        auto next = [&]() {  // tile j is in LDS, tile j + 1 on its way
+        auto arrive = [&]() {  // tile j is in LDS
             wait_loads<0>();
             barrier_only();
+        };
+        // The same for a tile that some row does not see whole.  Values there
+        // may be infinite or NaN, and a zero weight times those is NaN: they
+        // are added to the sums of the rows that see them and set to zero in
+        // LDS.  Each wave looks at the rows that it loaded.
+        auto arrive_masked = [&]() {
+            wait_loads<0>();
+            TER_LDS char* const vt = ring + stage * L::BYTES + L::V;
+            TER_LDS u32x4* const mine = (TER_LDS u32x4*)(vt + w * 16 * L::ROW + lane * 16);
+            unsigned odd = 0;
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) {
+                const u32x4 y = mine[64 * i];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
+            }
+            ++tick;
+            if (odd) flag[stage] = tick;
+            wait_lds();
+            barrier_only();
+            if (__builtin_amdgcn_readfirstlane(flag[stage]) != tick) return;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) settle(o[d]);
+#pragma clang loop unroll(disable)
+            for (int k = 0; k < kPagedKeys; ++k) {
+                const bool sees = j * kPagedKeys + k < lim;
+                const TER_LDS char* v = vt + k * L::ROW + 8 * half;
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d) {
+                    // (elements 32 d .. 32 d + 31 of the row: four pieces in a row, swizzled or not)
+                    const TER_LDS char* vd = v + ((4 * d) ^ L::swizzle_v(k)) * 16;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) add_odd<T>(o[d], i, *(const TER_LDS u32x2*)(vd + 4 * i), sees);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < L::NI; ++i) {
+                u32x4 y = mine[64 * i];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) y[m] = without_odd<T>(y[m]);
+                mine[64 * i] = y;
+            }
+            __syncthreads();
+        };
+        auto fetch = [&]() {  // tile j + 1 on its way
             if (j + 1 < s.j1) {
                 ld.issue(a, s, j + 1, pg, stage ^ 1);
                 if (j + 2 < s.j1) pg = ld.page(a, s, j + 2);
             }
         };
+        // One tile, its two halves of 32 keys staggered: while the matrix
+        // cores form the second half's scores the vector units turn the first
+        // half's into weights, and so on with the value products.  (A wave
+        // issues in order, so the two kinds have to alternate in its code:
+        // the scheduling groups below.)
         auto step = [&](auto masked) {
             constexpr bool kMasked = decltype(masked)::value;
             const TER_LDS char* tile = ring + stage * L::BYTES;
             f32x16 x[2];
-            v8 k[HD / 16];
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) k[c] = *(const TER_LDS v8*)(tile + ka[c]);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
-#pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    x[b] = E::mma32(k[c], q[c], x[b]);
-                    if (b == 0) k[c] = *(const TER_LDS v8*)(tile + ka[c] + 32 * L::ROW);
-                }
-            }
-            settle(x[0], x[1]);
-            if (kMasked) {
-                const int n = lim - j * kPagedKeys - 4 * half;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
+            v8 k[HD / 16], p[2][2], y[2][HD / 32];
+            float al = 1.f;
+            auto read_k = [&](int b, int c) { k[c] = *(const TER_LDS v8*)(tile + ka[c] + b * 32 * L::ROW); };
+            auto scores = [&](int b, int c) { x[b] = E::mma32(k[c], q[c], x[b]); };
+            auto read_v = [&](int c, int d) {
+                const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
+                const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
+                y[c & 1][d] = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            auto value = [&](int c, int d) {
+                o[d] = E::mma32(y[c & 1][d], p[c >> 1][c & 1], o[d]);
+            };
+            // The offset for half b; al is what sums so far are to be multiplied by.
+            auto decide = [&](int b) {
+                settle(x[b]);
+                if (kMasked) {
+                    const int n = lim - j * kPagedKeys - 32 * b - 4 * half;
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (32 * b + 8 * (i >> 2) + (i & 3) >= n) x[b][i] = -__builtin_inff();
-            }
-            float mx = x[0][0];
+                        if (8 * (i >> 2) + (i & 3) >= n) x[b][i] = -__builtin_inff();
+                }
+                float mx = x[b][0];
 #pragma unroll
-            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, x[i >> 4][i & 15]);
-            mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
-            if (__ballot(mx > top + kSlack)) {
-                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
-                const float al = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
-                top = nt;
-                off = no;
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[b][i]);
+                mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
+                if (__ballot(mx > top + kSlack)) {
+                    const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
+                    al = top == -__builtin_inff() ? 1.f : shrink(no - off);
+                    top = nt;
+                    off = no;
+                    return true;
+                }
+                return false;
+            };
+            auto rescale = [&]() {
                 l *= al;
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= al;
+            };
+            auto weight = [&](int b, int i) {  // elements i, i + 1
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, off));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, off));
+                l += e0;
+                l += e1;
+                p[b][i >> 3][i & 7] = (T)e0;
+                p[b][i >> 3][(i & 7) + 1] = (T)e1;
+            };
+
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) read_k(0, c);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[0][i] = x[1][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                scores(0, c);
+                read_k(1, c);
             }
-            v8 p[4];
+            if (decide(0)) rescale();
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int c = 0; c < HD / 16; ++c) scores(1, c);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, off));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, off));
-                    l += e0;
-                    l += e1;
-                    p[2 * b + (i >> 3)][i & 7] = (T)e0;
-                    p[2 * b + (i >> 3)][(i & 7) + 1] = (T)e1;
-                }
-            // Values that some row does not see may be infinite or NaN, and a
-            // zero weight times those is NaN: in masked tiles such elements are
-            // taken out here and added below to the rows that see them.
-            unsigned odd = 0;
+            for (int d = 0; d < HD / 32; ++d) read_v(0, d);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int i = 0; i < 16; i += 2) weight(0, i);
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // a matrix product
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                // an LDS read
+                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (HD / 16), 0);  // vector work
+            }
+            // (weights are formed here, not where they are used)
+            asm volatile("" : "+v"(p[0][0]), "+v"(p[0][1]), "+v"(l));
+            __builtin_amdgcn_sched_barrier(0);
+            const bool grown = decide(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) read_v(1, d);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d) {
-                    const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
-                    const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
-                    u32x4 y = __builtin_bit_cast(u32x4, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
-                    if (kMasked) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool b0 = (y[i] & E::kExp) == E::kExp, b1 = (y[i] >> 16 & E::kExp) == E::kExp;
-                            odd |= b0 || b1;
-                            y[i] &= (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
-                        }
-                    }
-                    o[d] = E::mma32(__builtin_bit_cast(v8, y), p[c], o[d]);
+                    value(c, d);
+                    read_v(2 + c, d);
                 }
-            if (kMasked && __ballot(odd != 0)) {
-                for (int i = 0; i < HD / 32; ++i) settle(o[i]);
-                for (int k = 0; k < kPagedKeys; ++k) {
-                    const bool sees = j * kPagedKeys + k < lim;
-                    const TER_LDS char* v = tile + L::V + k * L::ROW + 8 * half;
+            const float sum = l;
+            l = 0.f;
 #pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) {
-                        // (elements 32 d .. 32 d + 31 of the row: four pieces in a row, swizzled or not)
-                        const TER_LDS char* vd = v + ((4 * d) ^ L::swizzle_v(k)) * 16;
+            for (int i = 0; i < 16; i += 2) weight(1, i);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const u32x2 y = *(const TER_LDS u32x2*)(vd + 4 * i);
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) {
-                                const unsigned short z = (unsigned short)(y[m >> 1] >> (16 * (m & 1)));
-                                if (sees && (z & E::kExp) == E::kExp) o[d][i + m] += (float)__builtin_bit_cast(T, z);
-                            }
-                        }
-                    }
-                }
+            for (int c = 0; c < HD / 16; ++c) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (HD / 16), 0);
             }
+            asm volatile("" : "+v"(p[1][0]), "+v"(p[1][1]), "+v"(l));
+            __builtin_amdgcn_sched_barrier(0);
+            const float more = l;
+            l = sum;
+            if (grown) rescale();
+            l += more;
+#pragma unroll
+            for (int c = 2; c < 4; ++c)
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d) value(c, d);
         };
-        // tiles that every row of this wave sees whole, then the others
+        // tiles that every row sees whole, then the others
         const int full = min(s.j1, max(s.j0, lo / kPagedKeys));
         for (; j < full; ++j, stage ^= 1) {
-            next();
+            arrive();
             step(std::false_type{});
         }
         for (; j < s.j1; ++j, stage ^= 1) {
-            next();
-            if (j * kPagedKeys < hi) step(std::true_type{});
+            arrive_masked();
+            if (j * kPagedKeys < hi)
+                step(std::true_type{});
+            else
+                fetch();  // no row of this wave sees it
         }
         l += lane_xor32(l);
         if (!live) return;
@@ -471,13 +579,43 @@ struct Kernel {
             else
                 wait_loads<0>();
             const int at = j * kPagedKeys + 16 * w;
-            const TER_LDS char* tile = ring + stage * L::BYTES;
+            TER_LDS char* tile = ring + stage * L::BYTES;
+            if (at + 16 > lo) {  // (as in rows128, by each wave for its own keys)
+                TER_LDS u32x4* const mine = (TER_LDS u32x4*)(tile + L::V + w * 16 * L::ROW + lane * 16);
+                unsigned odd = 0;
+#pragma unroll
+                for (int i = 0; i < L::NI; ++i) {
+                    const u32x4 y = mine[64 * i];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
+                }
+                if (__ballot(odd != 0)) {
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) settle(o[d]);
+#pragma clang loop unroll(disable)
+                    for (int k = 0; k < 16; ++k) {
+                        const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW + (quad & 1) * 8;
+#pragma unroll
+                        for (int d = 0; d < HD / 16; ++d)
+                            add_odd<T>(o[d], 0,
+                                       *(const TER_LDS u32x2*)(v + ((2 * d + (quad >> 1)) ^ L::swizzle_v(16 * w + k)) * 16),
+                                       at + k < lim);
+                    }
+#pragma unroll
+                    for (int i = 0; i < L::NI; ++i) {
+                        u32x4 y = mine[64 * i];
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) y[m] = without_odd<T>(y[m]);
+                        mine[64 * i] = y;
+                    }
+                    wait_lds();
+                }
+            }
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) x = E::mma16(*(const TER_LDS v8*)(tile + ka[c]), q[c], x);
             settle(x);
-            const bool masked = at + 16 > lo;
-            if (masked) {
+            if (at + 16 > lo) {
                 const int n = lim - at - 4 * quad;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -488,7 +626,7 @@ struct Kernel {
             mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
             if (__ballot(mx > top + kSlack)) {
                 const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
-                const float al = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
+                const float al = top == -__builtin_inff() ? 1.f : shrink(no - off);
                 top = nt;
                 off = no;
                 l *= al;
@@ -502,38 +640,8 @@ struct Kernel {
                 l += e;
                 p[i] = (T)e;
             }
-            if (!masked) {
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(E::read_tr(tile + va[d]), p, o[d]);
-            } else {
-                unsigned odd = 0;
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    u32x2 y = __builtin_bit_cast(u32x2, E::read_tr(tile + va[d]));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const bool b0 = (y[i] & E::kExp) == E::kExp, b1 = (y[i] >> 16 & E::kExp) == E::kExp;
-                        odd |= b0 || b1;
-                        y[i] &= (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
-                    }
-                    o[d] = E::mma16k16(__builtin_bit_cast(v4, y), p, o[d]);
-                }
-                if (__ballot(odd != 0)) {
-                    for (int k = 0; k < 16; ++k) {
-                        const bool sees = at + k < lim;
-                        const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW;
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int e = 16 * d + 4 * quad + i;
-                                const unsigned short y = *(const TER_LDS unsigned short*)(
-                                    v + (((e >> 3) ^ L::swizzle_v(16 * w + k)) * 16) + (e & 7) * 2);
-                                if (sees && (y & E::kExp) == E::kExp) o[d][i] += (float)__builtin_bit_cast(T, y);
-                            }
-                    }
-                }
-            }
+            for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(E::read_tr(tile + va[d]), p, o[d]);
             if (j + 2 < s.j1) {
                 wait_lds();  // this tile's reads are done
                 ld.issue(a, s, j + 2, pg, stage);
@@ -645,6 +753,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
         const long long u = (long long)i * l.per;
         return u >= total ? total : paged_snap(l, segment((int)u), (int)u);
     };
+    int tick = 0;
+    if (threadIdx.x < 2) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
     const int u1 = cut(g + 1);
@@ -682,7 +792,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
         s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
         __syncthreads();  // the ring is free
         if (s.rows > 16)
-            K::rows128(a, s, ld, ring, row0, w, lane);
+            K::rows128(a, s, ld, ring, row0, tmp, tick, w, lane);
         else
             K::rows16(a, s, ld, ring, row0, w, lane);
         u = end;
@@ -792,9 +902,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttendArgs a)
 template <typename T, int HD>
 hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
-    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves) * 4;
+    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves + 2) * 4;
     const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
-    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves) * 4, {fn});
+    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves + 2) * 4, {fn});
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.max_wg), dim3(kThreads), lds, st, a);
     e = hipGetLastError();
