@@ -50,7 +50,9 @@ struct PagedAttendArgs {
     unsigned page_magic;             // ceil(2^32 / (page_size / 16)); 0 for pages of 16
     int max_wg, min_per, uncut;      // paged_cut()
     // the workspace (paged_attend_layout)
-    int* before;                     // [n_seq + 1] units before each sequence
+    int* cuts;                       // [max_wg][8] where a range begins inside a segment: rows of the row tile
+                                     //   (0: it does not), first token row, KV head, first and last range of it
+    int* before;                     // shared: [n_seq + 1] units before each sequence
     float* slots;                    // [2 max_wg][slot_rows][hd], then [2 max_wg][slot_rows][2]
     float* slot_stats;
     int slot_rows;
@@ -62,7 +64,7 @@ struct PagedAttendArgs {
 // bytes; the rows of `whole` are there with a shared prefix only).
 struct PagedAttendLayout {
     int tokens_log2, max_wg, min_per, uncut, slot_rows;
-    size_t before, slots, slot_stats, whole, whole_stats, bytes;
+    size_t cuts, before, slots, slot_stats, whole, whole_stats, bytes;
 };
 PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared);
 

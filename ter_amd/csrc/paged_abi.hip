@@ -203,6 +203,7 @@ int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
     a.uncut = p.uncut;
     a.slot_rows = p.slot_rows;
     char* w = static_cast<char*>(ws);
+    a.cuts = reinterpret_cast<int*>(w + p.cuts);
     a.before = reinterpret_cast<int*>(w + p.before);
     a.slots = reinterpret_cast<float*>(w + p.slots);
     a.slot_stats = reinterpret_cast<float*>(w + p.slot_stats);

@@ -19,6 +19,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -738,12 +739,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
 
     PagedLine l = paged_line(a.tokens_log2, a.shared, a.b.n_rows, a.nkv);
     const int total = count_units(a, l, before, row0, tmp);
-    if (blockIdx.x == 0)
+    if (a.shared && blockIdx.x == 0)
         for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = before[i];
     paged_cut(l, total, a.max_wg, a.min_per, a.uncut);
     // neighbouring ranges on one XCD (blocks go round the 8 XCDs): they read the same keys
-    const int chunk = (l.n_wg + 7) / 8, g = (int)(blockIdx.x % 8) * chunk + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= chunk || g >= l.n_wg) return;
+    // (blocks beyond the last range have the numbers behind it: each number once)
+    const int chunk = (l.n_wg + 7) / 8, x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8);
+    const int g = y < chunk ? x * chunk + y : 8 * chunk + x * (a.max_wg / 8 - chunk) + y - chunk;
+    if (g >= l.n_wg) {
+        if (threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
+        return;
+    }
 
     const ConstInts rows{a.b.row0}, lens{a.b.kv_len};
     auto segment = [&](int u) {
@@ -757,8 +763,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
     if (threadIdx.x < 2) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
-    const int u1 = cut(g + 1);
-    for (int u = cut(g); u < u1;) {
+    const int u0 = cut(g), u1 = cut(g + 1);
+    if (u0 >= u1 && threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
+    for (int u = u0; u < u1;) {
         const PagedSegment sg = segment(u);
         const int end = min(u1, sg.start + sg.n);
         Work s;
@@ -786,6 +793,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
             s.table = a.b.pages + (long long)sg.seq * a.b.pages_stride;
         }
         s.rows = s.n_tok * a.group;
+        if (u == u0 && threadIdx.x == 0) {  // what the joining kernel has to know of this cut
+            const PagedParts p = paged_parts(l, sg.start, sg.n);
+            *gptr(reinterpret_cast<i32x4*>(a.cuts + 8 * g)) = i32x4{u == sg.start ? 0 : s.rows, s.tok0, s.kvh, p.first};
+            gptr(a.cuts)[8 * g + 4] = p.last;
+        }
         s.dst = !whole ? 1 : a.shared ? 2 : 0;
         const int slot = 2 * g + (s.j0 == 0 ? 1 : 0);
         s.slot = a.slots + (long long)slot * a.slot_rows * HD;
@@ -799,103 +811,140 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
     }
 }
 
-// Joins the partial results of segments that were cut (and, with a shared
-// prefix, of the prefix with each row's own positions).  A workgroup is one row
-// tile of a sequence and KV head, every gridDim.z-th row of it; HD / 4 threads
-// take the elements, kThreads / (HD / 4) groups of them every so manieth part.
+// ---- joining.  A row takes HD / 4 threads, S groups of them every S-th partial
+// result of the row.
 template <typename T, int HD>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttendArgs a) {
-    constexpr int TPR = HD / 4, GROUPS = kThreads / TPR;
-    __shared__ __align__(16) float sums[GROUPS][HD];
-    __shared__ float stats[GROUPS][2];
+struct Join {
+    static constexpr int TPR = HD / 4, GROUPS = kThreads / TPR;
     typedef typename Elem<T>::v4 v4;
-    const int q = a.tokens_log2, kvh = blockIdx.y, x = blockIdx.x;
-    const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
-    // row tiles of sequence b: from (r0 >> q) + b on (there are no more than that leaves room for)
-    int lo = 0, hi = a.b.n_seq - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((paged_seq(rows[mid], rows[mid + 1], 0, a.b.n_rows, 0).r0 >> q) + mid <= x)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    const PagedSeq s = paged_seq(rows[lo], rows[lo + 1], lens[lo], a.b.n_rows, a.b.capacity);
-    const int tile = x - (s.r0 >> q) - lo;
-    if (tile < 0 || tile >= paged_row_tiles(s, q)) return;
-    PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
-    paged_cut(l, before[a.b.n_seq], a.max_wg, a.min_per, a.uncut);
-    const int b0 = before[lo], each = (before[lo + 1] - b0) / a.nkv;
-    const int start = b0 + kvh * each + (int)paged_key_tiles_before(s, tile, q, l.kv0);
-    const PagedParts own = paged_parts(l, start, paged_key_tiles(s, tile, q, l.kv0));
-    const int n_own = own.last - own.first + 1;
-    if (!a.shared && n_own == 1) return;  // written where it was computed
-
-    const int n_rows = min(s.n - (tile << q), 1 << q) * a.group;
-    const int grp = threadIdx.x / TPR, e = (threadIdx.x % TPR) * 4;
-    for (int r = blockIdx.z; r < n_rows; r += gridDim.z) {
-        const int tok = r / a.group, t = s.r0 + (tile << q) + tok, h = kvh * a.group + r - tok * a.group;
-        PagedParts pre{0, -1};
-        int pr = 0;
-        if (a.shared) {
-            pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_tiles, l.prefix_tiles);
-            pr = (t & ((1 << q) - 1)) * a.group + r - tok * a.group;
-        }
-        const int n_pre = pre.last - pre.first + 1, n = n_own + n_pre;
-        auto place = [&](int i, const float*& sum, const float*& stat) {
-            const bool is_pre = i >= n_own;
-            const PagedParts& p = is_pre ? pre : own;
-            if ((is_pre ? n_pre : n_own) == 1) {
-                const long long at = ((long long)(is_pre ? a.b.n_rows : 0) + t) * a.nh + h;
-                sum = a.whole + at * HD;
-                stat = a.whole_stats + at * 2;
-            } else {
-                const long long at = (long long)paged_slot(p, p.first + i - (is_pre ? n_own : 0)) * a.slot_rows +
-                                     (is_pre ? pr : r);
-                sum = a.slots + at * HD;
-                stat = a.slot_stats + at * 2;
-            }
-        };
-        float off = __builtin_inff(), tl = 0.f;
+    struct Lds {
+        float sums[GROUPS][HD], stats[GROUPS][2];
+    };
+    struct Sum {
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
-        for (int i = grp; i < n; i += GROUPS) {
-            const float *ps, *pt;
-            place(i, ps, pt);
-            const f32x2 st = *gptr(reinterpret_cast<const f32x2*>(pt));
-            const f32x4 v = *gptr(reinterpret_cast<const f32x4*>(ps + e));
-            if (st[0] == __builtin_inff()) continue;
-            const float no = fminf(off, st[0]);
+        float l = 0.f, off = __builtin_inff();
+        __device__ void add(f32x4 v, float lv, float o) {
+            if (o == __builtin_inff()) return;  // nothing seen there
+            const float no = fminf(off, o);
             const float f0 = off == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
-            const float f1 = __builtin_amdgcn_exp2f(no - st[0]);
-            tl = tl * f0 + st[1] * f1;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = y[k] * f0 + v[k] * f1;
+            const float f1 = __builtin_amdgcn_exp2f(no - o);
+            l = l * f0 + lv * f1;
+            y = y * f0 + v * f1;
             off = no;
         }
-        __syncthreads();
-        *reinterpret_cast<f32x4*>(&sums[grp][e]) = y;
-        if (e == 0) {
-            stats[grp][0] = off;
-            stats[grp][1] = tl;
-        }
-        __syncthreads();
-        if (grp == 0) {
-            float least = __builtin_inff(), total = 0.f;
+    };
+    // Partial result i of n of a row: place(i, sums, stats).  All threads call
+    // it; those of a row's first group return with the whole, `live` rows write it.
+    template <class Place>
+    static __device__ void row(Lds& lds, int S, int n, bool live, Place place, char* out) {
+        const int grp = threadIdx.x / TPR, e = (threadIdx.x % TPR) * 4, sub = grp & (S - 1);
+        Sum t;
+        if (live) {
+            constexpr int U = 4;  // partial results in flight
+            for (int i0 = sub; i0 < n; i0 += U * S) {
+                f32x4 v[U];
+                f32x2 st[U];
 #pragma unroll
-            for (int k = 0; k < GROUPS; ++k) least = fminf(least, stats[k][0]);
-            f32x4 z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < GROUPS; ++k) {
-                const float f = stats[k][0] == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(least - stats[k][0]);
-                if (f != 0.f || stats[k][1] != stats[k][1]) {  // (NaN stays)
-                    total += f * stats[k][1];
-                    z += f * *reinterpret_cast<const f32x4*>(&sums[k][e]);
+                for (int u = 0; u < U; ++u) {
+                    const float *ps, *pt;
+                    place(min(i0 + u * S, n - 1), ps, pt);
+                    v[u] = *gptr(reinterpret_cast<const f32x4*>(ps + e));
+                    st[u] = *gptr(reinterpret_cast<const f32x2*>(pt));
                 }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i0 + u * S < n) t.add(v[u], st[u][1], st[u][0]);
             }
-            const float inv = least == __builtin_inff() ? 0.f : 1.f / total;
-            const v4 out = {(T)(z[0] * inv), (T)(z[1] * inv), (T)(z[2] * inv), (T)(z[3] * inv)};
-            *gptr(reinterpret_cast<v4*>(a.out + (long long)t * a.out_stride + (long long)h * HD * 2 + e * 2)) = out;
         }
+        if (S > 1) {
+            __syncthreads();
+            *reinterpret_cast<f32x4*>(&lds.sums[grp][e]) = t.y;
+            if (e == 0) {
+                lds.stats[grp][0] = t.off;
+                lds.stats[grp][1] = t.l;
+            }
+            __syncthreads();
+            if (sub == 0)
+                for (int k = 1; k < S; ++k)
+                    t.add(*reinterpret_cast<const f32x4*>(&lds.sums[grp + k][e]), lds.stats[grp + k][1],
+                          lds.stats[grp + k][0]);
+        }
+        if (live && sub == 0) {
+            const float inv = t.off == __builtin_inff() ? 0.f : 1.f / t.l;
+            const v4 z = {(T)(t.y[0] * inv), (T)(t.y[1] * inv), (T)(t.y[2] * inv), (T)(t.y[3] * inv)};
+            *gptr(reinterpret_cast<v4*>(out + e * 2)) = z;
+        }
+    }
+};
+
+// Without a shared prefix: the rows of each segment that was cut, spread over
+// the workgroups of its cuts (a.cuts, written by the ranges that begin there).
+template <typename T, int HD>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttendArgs a) {
+    typedef Join<T, HD> J;
+    __shared__ typename J::Lds lds;
+    const ConstInts cut{a.cuts + 8 * blockIdx.x};
+    const int rows = cut[0], g = blockIdx.x;
+    if (rows == 0) return;
+    const int tok0 = cut[1], kvh = cut[2], first = cut[3], n = cut[4] - first + 1;
+    int S = 1;
+    while (S < J::GROUPS && 4 * S < n) S *= 2;
+    const int per = J::GROUPS / S, grp = threadIdx.x / J::TPR;
+    const int worker = (g - first - 1) * gridDim.y + blockIdx.y, workers = (n - 1) * gridDim.y;
+    for (int r0 = worker * per; r0 < rows; r0 += workers * per) {
+        const int r = r0 + grp / S, tok = r / a.group, t = tok0 + tok, h = kvh * a.group + r - tok * a.group;
+        J::row(
+            lds, S, n, r < rows,
+            [&](int i, const float*& sums, const float*& stats) {
+                const long long at = (long long)(2 * (first + i) + (i == 0 ? 1 : 0)) * a.slot_rows + r;
+                sums = a.slots + at * HD;
+                stats = a.slot_stats + at * 2;
+            },
+            a.out + (long long)t * a.out_stride + (long long)h * HD * 2);
+    }
+}
+
+// With a shared prefix: each row's own positions and the prefix, either of
+// which may have been cut.  A workgroup is one token row of one KV head.
+template <typename T, int HD>
+__global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttendArgs a) {
+    typedef Join<T, HD> J;
+    __shared__ typename J::Lds lds;
+    const int t = blockIdx.x, kvh = blockIdx.y, q = a.tokens_log2;
+    const int b = paged_seq_of_row(a.b.row0, a.b.n_seq, t);
+    if (b < 0) return;
+    const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
+    const PagedSeq s = paged_seq(rows[b], rows[b + 1], lens[b], a.b.n_rows, a.b.capacity);
+    PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
+    paged_cut(l, before[a.b.n_seq], a.max_wg, a.min_per, a.uncut);
+    const int tile = (t - s.r0) >> q, b0 = before[b], each = (before[b + 1] - b0) / a.nkv;
+    const PagedParts own = paged_parts(l, b0 + kvh * each + (int)paged_key_tiles_before(s, tile, q, l.kv0),
+                                       paged_key_tiles(s, tile, q, l.kv0));
+    const PagedParts pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_tiles, l.prefix_tiles);
+    const int n_own = own.last - own.first + 1, n_pre = pre.last - pre.first + 1;
+    const int own_row = ((t - s.r0) & ((1 << q) - 1)) * a.group, pre_row = (t & ((1 << q) - 1)) * a.group;
+    int S = J::GROUPS;
+    while (S > 1 && (J::GROUPS / S < a.group || 2 * S > n_own + n_pre)) S /= 2;
+    const int per = J::GROUPS / S, grp = threadIdx.x / J::TPR;
+    for (int i0 = 0; i0 < a.group; i0 += per) {
+        const int i = i0 + grp / S, h = kvh * a.group + i;
+        J::row(
+            lds, S, n_own + n_pre, i < a.group,
+            [&](int k, const float*& sums, const float*& stats) {
+                const bool is_pre = k >= n_own;
+                const PagedParts& p = is_pre ? pre : own;
+                if (p.first == p.last) {
+                    const long long at = ((long long)(is_pre ? a.b.n_rows : 0) + t) * a.nh + h;
+                    sums = a.whole + at * HD;
+                    stats = a.whole_stats + at * 2;
+                } else {
+                    const long long at = (long long)paged_slot(p, p.first + k - (is_pre ? n_own : 0)) * a.slot_rows +
+                                         (is_pre ? pre_row : own_row) + i;
+                    sums = a.slots + at * HD;
+                    stats = a.slot_stats + at * 2;
+                }
+            },
+            a.out + (long long)t * a.out_stride + (long long)h * HD * 2);
     }
 }
 
@@ -910,9 +959,10 @@ hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (!a.shared && a.uncut * kPagedKeys > a.b.capacity + a.b.n_rows) return hipSuccess;  // nothing is cut
-    const int tiles = (a.b.n_rows >> a.tokens_log2) + a.b.n_seq;
-    const int z = min(a.slot_rows, tiles * a.nkv >= 1024 ? 4 : 32);
-    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(tiles, a.nkv, z), dim3(kThreads), 0, st, a);
+    if (a.shared)
+        hipLaunchKernelGGL((paged_join_shared_kernel<T, HD>), dim3(a.b.n_rows, a.nkv), dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(a.max_wg, 4), dim3(kThreads), 0, st, a);
     return hipGetLastError();
 }
 
@@ -934,7 +984,8 @@ PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_
         return at;
     };
     const size_t slots = 2 * (size_t)p.max_wg * p.slot_rows, whole = shared ? 2 * (size_t)n_rows * nh : 0;
-    p.before = take((size_t)(n_seq + 1) * 4);
+    p.cuts = take((size_t)p.max_wg * 32);
+    p.before = take(shared ? (size_t)(n_seq + 1) * 4 : 0);
     p.slot_stats = take(slots * 2 * 4);
     p.whole_stats = take(whole * 2 * 4);
     p.slots = take(slots * hd * 4);
