@@ -180,7 +180,7 @@ int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
         paged_attend_layout(ctx->nh, ctx->nkv, ctx->hd, batch->n_seq, n_rows, a.b.capacity, shared);
     // units are counted in 31 bits (a sequence's rows may lie behind its whole table)
     const int64_t tiles = ((int64_t)n_rows >> p.tokens_log2) + batch->n_seq;
-    if (tiles * ctx->nkv * (((int64_t)a.b.capacity + n_rows) / 64 + 2 + shared / 64) > 0x7FFFFFFFll)
+    if (tiles * ctx->nkv * (((int64_t)a.b.capacity + n_rows) / 64 + 10 + shared / 64) > 0x7FFFFFFFll)
         return fail(TER_HIP_ERR_SHAPE, "%d rows over %d positions are too many for one call", n_rows, a.b.capacity);
     if (!ws) return fail(TER_HIP_ERR_NULL, "null workspace");
     if (ws_bytes < p.bytes) return fail(TER_HIP_ERR_SHAPE, "workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);

@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
+constexpr int kSolo = 8;  // key tiles up to which a segment of few rows may be one wave's
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -203,26 +204,27 @@ struct Kernel {
                 vo[i] = r * a.c.pos_stride + (p ^ L::swizzle_v(r)) * 16;
             }
         }
-        // The page of this wave's rows of key tile j (-1: none), and the load of them.
-        __device__ int page(const PagedAttendArgs& a, const Work& s, int j) const {
-            const int pos = s.kv + j * kPagedKeys + 16 * w;
+        // The page of 16 positions from `at` on (counted from the segment's
+        // first one; -1: none), and the load of them into this wave's rows.
+        __device__ int page(const PagedAttendArgs& a, const Work& s, int at) const {
+            const int pos = s.kv + at;
             if (pos >= s.kv_end) return -1;
             const unsigned x = (unsigned)pos >> 4;
             const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
             return ConstInts{s.table}[i];
         }
-        __device__ void issue(const PagedAttendArgs& a, const Work& s, int j, int page, int stage) const {
-            const int pos = s.kv + j * kPagedKeys + 16 * w;
+        __device__ void issue(const PagedAttendArgs& a, const Work& s, int at, int page, int stage) const {
+            const int pos = s.kv + at;
             const unsigned x = (unsigned)pos >> 4;
             const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
             const int slot = pos - (int)i * a.c.page_size;
             int n = min(s.kv_end - pos, 16);
             if (page < 0 || page >= a.c.n_pages) n = 0;
             const unsigned bytes = n > 0 ? (unsigned)(n - 1) * a.c.pos_stride + L::ROW : 0u;
-            const long long at = n > 0 ? page * a.c.page_stride + (long long)slot * a.c.pos_stride +
-                                             (long long)s.kvh * a.c.head_stride
-                                       : 0;
-            const unsigned long long kb = (unsigned long long)(a.c.k + at), vb = (unsigned long long)(a.c.v + at);
+            const long long o = n > 0 ? page * a.c.page_stride + (long long)slot * a.c.pos_stride +
+                                            (long long)s.kvh * a.c.head_stride
+                                      : 0;
+            const unsigned long long kb = (unsigned long long)(a.c.k + o), vb = (unsigned long long)(a.c.v + o);
             const u32x4 kr = {(unsigned)kb, (unsigned)(kb >> 32) & 0xFFFFu, bytes, 0x00020000u};
             const u32x4 vr = {(unsigned)vb, (unsigned)(vb >> 32) & 0xFFFFu, bytes, 0x00020000u};
             const unsigned d = lds + stage * L::BYTES;
@@ -320,9 +322,10 @@ struct Kernel {
             va[d] = L::V + vr * L::ROW +
                     (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
 
-        int pg = ld.page(a, s, s.j0);
-        ld.issue(a, s, s.j0, pg, 0);
-        pg = s.j0 + 1 < s.j1 ? ld.page(a, s, s.j0 + 1) : -1;
+        const auto mine = [&](int j) { return j * kPagedKeys + 16 * w; };
+        int pg = ld.page(a, s, mine(s.j0));
+        ld.issue(a, s, mine(s.j0), pg, 0);
+        pg = s.j0 + 1 < s.j1 ? ld.page(a, s, mine(s.j0 + 1)) : -1;
         int stage = 0, j = s.j0;
         auto arrive = [&]() {  // tile j is in LDS
             wait_loads<0>();
@@ -335,11 +338,11 @@ struct Kernel {
         auto arrive_masked = [&]() {
             wait_loads<0>();
             TER_LDS char* const vt = ring + stage * L::BYTES + L::V;
-            TER_LDS u32x4* const mine = (TER_LDS u32x4*)(vt + w * 16 * L::ROW + lane * 16);
+            TER_LDS u32x4* const own = (TER_LDS u32x4*)(vt + w * 16 * L::ROW + lane * 16);
             unsigned odd = 0;
 #pragma unroll
             for (int i = 0; i < L::NI; ++i) {
-                const u32x4 y = mine[64 * i];
+                const u32x4 y = own[64 * i];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
             }
@@ -365,17 +368,17 @@ struct Kernel {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < L::NI; ++i) {
-                u32x4 y = mine[64 * i];
+                u32x4 y = own[64 * i];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) y[m] = without_odd<T>(y[m]);
-                mine[64 * i] = y;
+                own[64 * i] = y;
             }
             __syncthreads();
         };
         auto fetch = [&]() {  // tile j + 1 on its way
             if (j + 1 < s.j1) {
-                ld.issue(a, s, j + 1, pg, stage ^ 1);
-                if (j + 2 < s.j1) pg = ld.page(a, s, j + 2);
+                ld.issue(a, s, mine(j + 1), pg, stage ^ 1);
+                if (j + 2 < s.j1) pg = ld.page(a, s, mine(j + 2));
             }
         };
         // One tile, its two halves of 32 keys staggered: while the matrix
@@ -536,20 +539,24 @@ struct Kernel {
             *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, t, h))) = f32x2{lim > s.j0 * kPagedKeys ? off : __builtin_inff(), l};
     }
 
-    // ---- up to 16 rows: wave w takes keys 16 w .. 16 w + 15 of every tile, so
-    // it waits for no other wave; the waves' sums meet in LDS at the end.
+    // ---- up to 16 rows, 16 keys at a time.  kSolo: by one wave.  Else wave w
+    // takes keys 16 w .. 16 w + 15 of every tile; no wave waits for another
+    // before their sums meet in LDS at the end.
+    template <bool kSolo>
     static __device__ __forceinline__ void rows16(const PagedAttendArgs& a, const Work& s, const Loader& ld,
                                                   TER_LDS char* ring, const int* row0, int w, int lane) {
         const int quad = lane >> 4, col = lane & 15;
         const int tok = col / a.group, t = s.tok0 + tok, h = s.kvh * a.group + (col - tok * a.group);
         const bool live = col < s.rows;
         const int lim = live ? limit_of(a, s, t, row0) : 0;
-        int pg = ld.page(a, s, s.j0);
-        ld.issue(a, s, s.j0, pg, 0);
-        if (s.j0 + 1 < s.j1) {
-            pg = ld.page(a, s, s.j0 + 1);
-            ld.issue(a, s, s.j0 + 1, pg, 1);
-            if (s.j0 + 2 < s.j1) pg = ld.page(a, s, s.j0 + 2);
+        const int first = s.j0 * kPagedKeys + (kSolo ? 0 : 16 * w), stride = kSolo ? 16 : kPagedKeys;
+        const int n = kSolo ? max(1, (min(s.j1 * kPagedKeys, s.kv_end - s.kv) - first + 15) / 16) : s.j1 - s.j0;
+        int pg = ld.page(a, s, first);
+        ld.issue(a, s, first, pg, 0);
+        if (1 < n) {
+            pg = ld.page(a, s, first + stride);
+            ld.issue(a, s, first + stride, pg, 1);
+            if (2 < n) pg = ld.page(a, s, first + 2 * stride);
         }
         v8 q[HD / 32];
         {
@@ -573,13 +580,13 @@ struct Kernel {
         for (int d = 0; d < HD / 16; ++d)
             va[d] = L::V + vr * L::ROW + (((2 * d + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
         int stage = 0;
-        for (int j = s.j0; j < s.j1; ++j, stage ^= 1) {
-            // the next tile's loads may still be in flight
-            if (j + 1 < s.j1)
+        for (int i = 0; i < n; ++i, stage ^= 1) {
+            // the next keys' loads may still be in flight
+            if (i + 1 < n)
                 wait_loads<2 * L::NI>();
             else
                 wait_loads<0>();
-            const int at = j * kPagedKeys + 16 * w;
+            const int at = first + i * stride;
             TER_LDS char* tile = ring + stage * L::BYTES;
             if (at + 16 > lo) {  // (as in rows128, by each wave for its own keys)
                 TER_LDS u32x4* const mine = (TER_LDS u32x4*)(tile + L::V + w * 16 * L::ROW + lane * 16);
@@ -617,10 +624,10 @@ struct Kernel {
             for (int c = 0; c < HD / 32; ++c) x = E::mma16(*(const TER_LDS v8*)(tile + ka[c]), q[c], x);
             settle(x);
             if (at + 16 > lo) {
-                const int n = lim - at - 4 * quad;
+                const int see = lim - at - 4 * quad;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= n) x[i] = -__builtin_inff();
+                for (int k = 0; k < 4; ++k)
+                    if (k >= see) x[k] = -__builtin_inff();
             }
             float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             mx = fmaxf(mx, lane_xor16(mx));
@@ -643,14 +650,33 @@ struct Kernel {
             }
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(E::read_tr(tile + va[d]), p, o[d]);
-            if (j + 2 < s.j1) {
-                wait_lds();  // this tile's reads are done
-                ld.issue(a, s, j + 2, pg, stage);
-                if (j + 3 < s.j1) pg = ld.page(a, s, j + 3);
+            if (i + 2 < n) {
+                wait_lds();  // these keys' reads are done
+                ld.issue(a, s, at + 2 * stride, pg, stage);
+                if (i + 3 < n) pg = ld.page(a, s, at + 3 * stride);
             }
         }
         l += lane_xor16(l);
         l += lane_xor32(l);
+        if (kSolo) {
+            if (!live) return;
+            if (s.dst == 0) {
+                const float inv = lim > 0 ? 1.f / l : 0.f;
+                char* p = a.out + (long long)t * a.out_stride + (long long)h * L::ROW + quad * 8;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    const v4 y = {(T)(o[d][0] * inv), (T)(o[d][1] * inv), (T)(o[d][2] * inv), (T)(o[d][3] * inv)};
+                    *gptr(reinterpret_cast<v4*>(p + 32 * d)) = y;
+                }
+            } else {
+                float* p = sums_of(a, s, col, t, h) + 4 * quad;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) *gptr(reinterpret_cast<f32x4*>(p + 16 * d)) = o[d];
+                if (quad == 0)
+                    *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, col, t, h))) = f32x2{lim > first ? off : __builtin_inff(), l};
+            }
+            return;
+        }
         // the waves' sums: [wave][row][HD], then [wave][row][2]
         __syncthreads();
         TER_LDS float* sums = (TER_LDS float*)ring;
@@ -660,7 +686,7 @@ struct Kernel {
             for (int d = 0; d < HD / 16; ++d)
                 *(TER_LDS f32x4*)(sums + (w * 16 + col) * HD + 16 * d + 4 * quad) = o[d];
             if (quad == 0) {
-                stats[(w * 16 + col) * 2] = lim > s.j0 * kPagedKeys + 16 * w ? off : __builtin_inff();
+                stats[(w * 16 + col) * 2] = lim > first ? off : __builtin_inff();
                 stats[(w * 16 + col) * 2 + 1] = l;
             }
         }
@@ -764,16 +790,21 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
     const int u0 = cut(g), u1 = cut(g + 1);
-    if (u0 >= u1 && threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
-    for (int u = u0; u < u1;) {
-        const PagedSegment sg = segment(u);
+    if (u0 >= u1) {
+        if (threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
+        return;
+    }
+    PagedSegment sg = segment(u0);
+    PagedSeq q{};
+    int turn = -1;  // of a run of short segments: the wave whose turn it is
+    for (int u = u0;;) {
         const int end = min(u1, sg.start + sg.n);
         Work s;
         s.seq = sg.seq;
         s.kvh = sg.kvh;
-        s.j0 = u - sg.start;
-        s.j1 = end - sg.start;
-        const bool whole = s.j0 == 0 && s.j1 == sg.n;
+        s.j0 = max(u - sg.start - kPagedLead, 0);
+        s.j1 = end - sg.start - kPagedLead;
+        const bool whole = u == sg.start && end == sg.start + sg.n;
         if (sg.seq < 0) {
             s.tok0 = sg.tile << l.q;
             s.n_tok = min(a.b.n_rows - s.tok0, 1 << l.q);
@@ -782,7 +813,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
             s.row0 = s.base = 0;
             s.table = a.b.pages;
         } else {
-            const PagedSeq q = paged_seq(rows[sg.seq], rows[sg.seq + 1], lens[sg.seq], a.b.n_rows, a.b.capacity);
+            q = paged_seq(rows[sg.seq], rows[sg.seq + 1], lens[sg.seq], a.b.n_rows, a.b.capacity);
             const int i = sg.tile << l.q;
             s.tok0 = q.r0 + i;
             s.n_tok = min(q.n - i, 1 << l.q);
@@ -793,21 +824,31 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
             s.table = a.b.pages + (long long)sg.seq * a.b.pages_stride;
         }
         s.rows = s.n_tok * a.group;
+        s.dst = !whole ? 1 : a.shared ? 2 : 0;
+        const int slot = 2 * g + (u == sg.start ? 1 : 0);
+        s.slot = a.slots + (long long)slot * a.slot_rows * HD;
+        s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
         if (u == u0 && threadIdx.x == 0) {  // what the joining kernel has to know of this cut
             const PagedParts p = paged_parts(l, sg.start, sg.n);
             *gptr(reinterpret_cast<i32x4*>(a.cuts + 8 * g)) = i32x4{u == sg.start ? 0 : s.rows, s.tok0, s.kvh, p.first};
             gptr(a.cuts)[8 * g + 4] = p.last;
         }
-        s.dst = !whole ? 1 : a.shared ? 2 : 0;
-        const int slot = 2 * g + (s.j0 == 0 ? 1 : 0);
-        s.slot = a.slots + (long long)slot * a.slot_rows * HD;
-        s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
-        __syncthreads();  // the ring is free
-        if (s.rows > 16)
-            K::rows128(a, s, ld, ring, row0, tmp, tick, w, lane);
-        else
-            K::rows16(a, s, ld, ring, row0, w, lane);
+        if (s.rows <= 16 && s.j1 - s.j0 <= kSolo && (u > u0 || end < u1)) {
+            // short ones beside others: the waves take turns, each by itself
+            if (turn < 0) __syncthreads();
+            turn = (turn + 1) & (kWaves - 1);
+            if (turn == w) K::template rows16<true>(a, s, ld, ring, row0, w, lane);
+        } else {
+            turn = -1;
+            __syncthreads();  // the ring is free
+            if (s.rows > 16)
+                K::rows128(a, s, ld, ring, row0, tmp, tick, w, lane);
+            else
+                K::template rows16<false>(a, s, ld, ring, row0, w, lane);
+        }
         u = end;
+        if (u >= u1) break;
+        if (!paged_advance(l, sg, q, a.nkv)) sg = segment(u);
     }
 }
 
@@ -918,9 +959,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
     PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
     paged_cut(l, before[a.b.n_seq], a.max_wg, a.min_per, a.uncut);
     const int tile = (t - s.r0) >> q, b0 = before[b], each = (before[b + 1] - b0) / a.nkv;
-    const PagedParts own = paged_parts(l, b0 + kvh * each + (int)paged_key_tiles_before(s, tile, q, l.kv0),
-                                       paged_key_tiles(s, tile, q, l.kv0));
-    const PagedParts pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_tiles, l.prefix_tiles);
+    const PagedParts own = paged_parts(l, b0 + kvh * each + paged_length_before(s, tile, q, l.kv0),
+                                       paged_length(s, tile, q, l.kv0));
+    const PagedParts pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_length, l.prefix_length);
     const int n_own = own.last - own.first + 1, n_pre = pre.last - pre.first + 1;
     const int own_row = ((t - s.r0) & ((1 << q) - 1)) * a.group, pre_row = (t & ((1 << q) - 1)) * a.group;
     int S = J::GROUPS;

@@ -7,7 +7,10 @@
 // all its key tiles, a unit one key tile of one segment.  All units of a launch
 // form one line,
 //   [ shared prefix: KV head, row tile over all rows ][ sequence, KV head, row tile ],
-// which is cut into equal ranges, one for each workgroup, whatever the lengths
+// where every segment begins with kPagedLead units of no work: what its start
+// and end cost beside its key tiles (queries and first tiles from memory,
+// results to it) is about as much.  The line
+// is cut into equal ranges, one for each workgroup, whatever the lengths
 // are: a long sequence is spread over many workgroups, many short ones share
 // one.  A cut close to a segment's edge is moved there.  A segment that is cut
 // leaves one partial result in each range that holds a part of it; they
@@ -28,6 +31,7 @@ namespace terhip {
 
 constexpr int kPagedKeys = 64;   // positions of a key tile
 constexpr int kPagedRows = 128;  // rows of a row tile
+constexpr int kPagedLead = 3;
 
 TER_HD int paged_min(int a, int b) { return a < b ? a : b; }
 TER_HD int paged_max(int a, int b) { return a > b ? a : b; }
@@ -75,17 +79,23 @@ TER_HD long long paged_key_tiles_before(const PagedSeq& s, int n, int q, int kv0
     return ones + (((a1 * (a1 + 1) / 2) << lr) + (x1 & r) * (a1 + 1)) -
            (((a0 * (a0 + 1) / 2) << lr) + (x0 & r) * (a0 + 1));
 }
-// Units of a sequence, for one KV head.
+// Units of a segment, of the row tiles before it, of a sequence for one KV head.
+TER_HD int paged_length(const PagedSeq& s, int rt, int q, int kv0) {
+    return kPagedLead + paged_key_tiles(s, rt, q, kv0);
+}
+TER_HD int paged_length_before(const PagedSeq& s, int n, int q, int kv0) {
+    return n * kPagedLead + (int)paged_key_tiles_before(s, n, q, kv0);
+}
 TER_HD int paged_units(const PagedSeq& s, int q, int kv0) {
     const int t = paged_row_tiles(s, q);
-    return t ? (int)paged_key_tiles_before(s, t - 1, q, kv0) + paged_key_tiles(s, t - 1, q, kv0) : 0;
+    return t ? paged_length_before(s, t - 1, q, kv0) + paged_length(s, t - 1, q, kv0) : 0;
 }
 // The row tile that holds unit r of a sequence and KV head.
 TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
     int lo = 0, hi = paged_row_tiles(s, q) - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (paged_key_tiles_before(s, mid, q, kv0) <= r)
+        if (paged_length_before(s, mid, q, kv0) <= r)
             lo = mid;
         else
             hi = mid - 1;
@@ -97,7 +107,7 @@ TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
 // from cut g to cut g + 1, cut g being near g * per.
 struct PagedLine {
     int q, kv0;                // row tile, first position behind the prefix
-    int prefix_tiles;          // key tiles of the prefix
+    int prefix_length;         // units of a row tile on the prefix
     int prefix_rows;           // row tiles over all rows
     int prefix_units;          // of all KV heads
     int total;
@@ -108,14 +118,14 @@ TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
     PagedLine l{};
     l.q = q;
     l.kv0 = shared;
-    l.prefix_tiles = (shared + kPagedKeys - 1) / kPagedKeys;
+    l.prefix_length = shared ? kPagedLead + (shared + kPagedKeys - 1) / kPagedKeys : 0;
     l.prefix_rows = (n_rows + (1 << q) - 1) >> q;
-    l.prefix_units = l.prefix_tiles * l.prefix_rows * nkv;
+    l.prefix_units = l.prefix_length * l.prefix_rows * nkv;
     return l;
 }
 // total: prefix units and those of the sequences.  max_wg: workgroups of the
 // launch.  min_per: fewer units than that are not worth a workgroup.  uncut:
-// segments of fewer units are never cut.
+// segments of fewer key tiles are never cut.
 TER_HD void paged_cut(PagedLine& l, int total, int max_wg, int min_per, int uncut) {
     l.total = total;
     l.per = paged_max(min_per, (total + max_wg - 1) / max_wg);
@@ -136,12 +146,12 @@ TER_HD PagedSegment paged_segment(const PagedLine& l, int u, Ints row0, Ints kv_
                                   int nkv, Before before) {
     PagedSegment g;
     if (u < l.prefix_units) {
-        const int i = u / l.prefix_tiles;
+        const int i = u / l.prefix_length;
         g.seq = -1;
         g.kvh = i / l.prefix_rows;
         g.tile = i - g.kvh * l.prefix_rows;
-        g.start = i * l.prefix_tiles;
-        g.n = l.prefix_tiles;
+        g.start = i * l.prefix_length;
+        g.n = l.prefix_length;
         return g;
     }
     int lo = 0, hi = n_seq - 1;  // the last sequence that begins at u or before (empty ones before it end there too)
@@ -158,15 +168,29 @@ TER_HD PagedSegment paged_segment(const PagedLine& l, int u, Ints row0, Ints kv_
     g.kvh = at / each;
     const int r = at - g.kvh * each;
     g.tile = paged_row_tile_of(s, r, l.q, l.kv0);
-    g.start = b0 + g.kvh * each + (int)paged_key_tiles_before(s, g.tile, l.q, l.kv0);
-    g.n = paged_key_tiles(s, g.tile, l.q, l.kv0);
+    g.start = b0 + g.kvh * each + paged_length_before(s, g.tile, l.q, l.kv0);
+    g.n = paged_length(s, g.tile, l.q, l.kv0);
     return g;
+}
+// To the segment behind g where that is of the same sequence s (or of the
+// prefix); false: it is not.
+TER_HD bool paged_advance(const PagedLine& l, PagedSegment& g, const PagedSeq& s, int nkv) {
+    const int tiles = g.seq < 0 ? l.prefix_rows : paged_row_tiles(s, l.q);
+    if (g.tile + 1 < tiles)
+        ++g.tile;
+    else if (g.kvh + 1 < nkv)
+        ++g.kvh, g.tile = 0;
+    else
+        return false;
+    g.start += g.n;
+    if (g.seq >= 0) g.n = paged_length(s, g.tile, l.q, l.kv0);
+    return true;
 }
 
 // Where a cut at unit u of segment g goes.
 TER_HD int paged_snap(const PagedLine& l, const PagedSegment& g, int u) {
     const int off = u - g.start;
-    return off < l.near ? g.start : g.n - off < l.near ? g.start + g.n : u;
+    return off < kPagedLead + l.near ? g.start : g.n - off < l.near ? g.start + g.n : u;
 }
 
 // The ranges that hold parts of a segment: first .. last, one if it is not cut.
@@ -177,7 +201,7 @@ struct PagedParts {
 };
 TER_HD PagedParts paged_parts(const PagedLine& l, int start, int n) {
     PagedParts p;
-    const int a = start + l.near, z = start + n - l.near;  // cuts from a to z stay inside
+    const int a = start + kPagedLead + l.near, z = start + n - l.near;  // cuts from a to z stay inside
     const int c0 = (a + l.per - 1) / l.per, c1 = z < 0 ? -1 : z / l.per;
     p.first = c0 - 1;
     p.last = paged_max(c0 - 1, c1);

@@ -44,7 +44,7 @@ int main() {
         std::vector<PagedSegment> segs;
         for (int h = 0; h < nkv && shared; ++h)
             for (int t = 0; t < (n_rows + (1 << q) - 1) >> q; ++t)
-                segs.push_back({0, (shared + 63) / 64, -1, h, t});
+                segs.push_back({0, kPagedLead + (shared + 63) / 64, -1, h, t});
         for (int b = 0; b < n_seq; ++b) {
             const PagedSeq s = paged_seq(row0[b], row0[b + 1], len[b], n_rows, cap);
             CHECK(s.r0 >= 0 && s.n >= 0 && s.r0 + s.n <= n_rows);
@@ -56,12 +56,13 @@ int main() {
                 const int n = paged_key_tiles(s, tiles, q, shared);
                 CHECK(n >= 1 && n * 64 >= see);
                 if (s.base + last + 1 <= cap) CHECK(n == paged_max(1, (see + 63) / 64));
-                CHECK(paged_key_tiles_before(s, tiles, q, shared) == units);
-                units += n;
+                CHECK(paged_length_before(s, tiles, q, shared) == units);
+                CHECK(paged_length(s, tiles, q, shared) == n + kPagedLead);
+                units += n + kPagedLead;
             }
             CHECK(tiles == paged_row_tiles(s, q) && units == paged_units(s, q, shared));
             for (int h = 0; h < nkv; ++h)
-                for (int t = 0; t < tiles; ++t) segs.push_back({0, paged_key_tiles(s, t, q, shared), b, h, t});
+                for (int t = 0; t < tiles; ++t) segs.push_back({0, paged_length(s, t, q, shared), b, h, t});
             before.push_back(before.back() + units * nkv);
         }
         int total = 0;
@@ -87,6 +88,15 @@ int main() {
             const PagedSegment g = find(u);
             CHECK(g.start == segs[k].start && g.n == segs[k].n && g.seq == segs[k].seq && g.kvh == segs[k].kvh &&
                   g.tile == segs[k].tile);
+            PagedSegment next = g;
+            const PagedSeq s = g.seq < 0 ? PagedSeq{} : paged_seq(row0[g.seq], row0[g.seq + 1], len[g.seq], n_rows, cap);
+            if (paged_advance(l, next, s, nkv)) {
+                const PagedSegment& m = segs[k + 1];
+                CHECK(next.start == m.start && next.n == m.n && next.seq == m.seq && next.kvh == m.kvh &&
+                      next.tile == m.tile);
+            } else {
+                CHECK(k + 1 == segs.size() || segs[k + 1].seq != g.seq);
+            }
         }
         for (int w = 0; w < l.n_wg; ++w) {
             const int u0 = cut(w), u1 = cut(w + 1);
@@ -95,6 +105,8 @@ int main() {
                 const PagedSegment g = find(u);
                 const int e = paged_min(u1, g.start + g.n);
                 for (int i = u; i < e; ++i) ++done[i];
+                CHECK(u == g.start || u > g.start + kPagedLead);
+                CHECK(e > g.start + kPagedLead);
                 if (u > g.start || e < g.start + g.n) {
                     const int slot = u == g.start ? 2 * w + 1 : 2 * w;
                     CHECK(used.insert(slot).second);
