@@ -579,6 +579,9 @@ struct Kernel {
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d)
             va[d] = L::V + vr * L::ROW + (((2 * d + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
+        // The queries, which the compiler waits for, have to be here before the
+        // loop: inside it that wait would be one for all loads in flight.
+        wait_loads<0>();
         int stage = 0;
         for (int i = 0; i < n; ++i, stage ^= 1) {
             // the next keys' loads may still be in flight
@@ -620,8 +623,15 @@ struct Kernel {
                 }
             }
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            v8 k[HD / 32];
+            v4 y[HD / 16];
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) x = E::mma16(*(const TER_LDS v8*)(tile + ka[c]), q[c], x);
+            for (int c = 0; c < HD / 32; ++c) k[c] = *(const TER_LDS v8*)(tile + ka[c]);
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) y[d] = E::read_tr(tile + va[d]);
+            __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) x = E::mma16(k[c], q[c], x);
             settle(x);
             if (at + 16 > lo) {
                 const int see = lim - at - 4 * quad;
@@ -649,7 +659,7 @@ struct Kernel {
                 p[i] = (T)e;
             }
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(E::read_tr(tile + va[d]), p, o[d]);
+            for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(y[d], p, o[d]);
             if (i + 2 < n) {
                 wait_lds();  // these keys' reads are done
                 ld.issue(a, s, at + 2 * stride, pg, stage);
