@@ -184,7 +184,13 @@ struct Kernel {
     typedef typename E::v4 v4;
     typedef typename E::v2 v2;
     typedef Tile<HD> L;
-    static constexpr int RING = 2 * L::BYTES;
+    // Stages of the ring, and workgroups of a CU (by LDS and registers): 64 KB
+    // each and two of them at head_dim 128; 48 KB and three at 64, where a
+    // stage is half as large and more of them have to be in flight.
+    static constexpr int NST = HD == 128 ? 2 : 3;
+    static constexpr int PER_CU = HD == 128 ? 2 : 3;
+    static constexpr int RING = NST * L::BYTES;
+    static __device__ __forceinline__ int after(int stage) { return stage + 1 == NST ? 0 : stage + 1; }
     // An offset stays while the largest weight is at most 2^kSlack above its start
     static constexpr float kSlack = 7.f;
 
@@ -275,7 +281,7 @@ struct Kernel {
                                                    TER_LDS char* ring, const int* row0, int* shared, int& tick,
                                                    int w, int lane) {
         int* const lows = shared;                 // [kWaves]
-        int* const flag = shared + kWaves;        // [2] the tick at which a tile of a stage held odd values
+        int* const flag = shared + kWaves;        // [NST] the tick at which a tile of a stage held odd values
         const int half = lane >> 5, col = lane & 31;
         const int r = 32 * w + col, tok = r / a.group, t = s.tok0 + tok;
         const int h = s.kvh * a.group + (r - tok * a.group);
@@ -323,12 +329,26 @@ struct Kernel {
                     (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
 
         const auto mine = [&](int j) { return j * kPagedKeys + 16 * w; };
-        int pg = ld.page(a, s, mine(s.j0));
-        ld.issue(a, s, mine(s.j0), pg, 0);
-        pg = s.j0 + 1 < s.j1 ? ld.page(a, s, mine(s.j0 + 1)) : -1;
+        // NST - 1 tiles ahead of the one in work
+        int pg = ld.page(a, s, mine(s.j0)), put = 0, todo = s.j0;
+        auto fetch = [&]() {
+            if (todo < s.j1) {
+                ld.issue(a, s, mine(todo), pg, put);
+                if (++todo < s.j1) pg = ld.page(a, s, mine(todo));
+                put = after(put);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NST - 1; ++i) fetch();
         int stage = 0, j = s.j0;
-        auto arrive = [&]() {  // tile j is in LDS
-            wait_loads<0>();
+        auto landed = [&]() {  // this wave's rows of tile j are in LDS
+            if (NST > 2 && j + 1 < s.j1)
+                wait_loads<2 * L::NI>();
+            else
+                wait_loads<0>();
+        };
+        auto arrive = [&]() {
+            landed();
             barrier_only();
         };
         // The same for a tile that some row does not see whole.  Values there
@@ -336,7 +356,7 @@ struct Kernel {
         // are added to the sums of the rows that see them and set to zero in
         // LDS.  Each wave looks at the rows that it loaded.
         auto arrive_masked = [&]() {
-            wait_loads<0>();
+            landed();
             TER_LDS char* const vt = ring + stage * L::BYTES + L::V;
             TER_LDS u32x4* const own = (TER_LDS u32x4*)(vt + w * 16 * L::ROW + lane * 16);
             unsigned odd = 0;
@@ -374,12 +394,6 @@ struct Kernel {
                 own[64 * i] = y;
             }
             __syncthreads();
-        };
-        auto fetch = [&]() {  // tile j + 1 on its way
-            if (j + 1 < s.j1) {
-                ld.issue(a, s, mine(j + 1), pg, stage ^ 1);
-                if (j + 2 < s.j1) pg = ld.page(a, s, mine(j + 2));
-            }
         };
         // One tile, its two halves of 32 keys staggered: while the matrix
         // cores form the second half's scores the vector units turn the first
@@ -502,11 +516,11 @@ struct Kernel {
         };
         // tiles that every row sees whole, then the others
         const int full = min(s.j1, max(s.j0, lo / kPagedKeys));
-        for (; j < full; ++j, stage ^= 1) {
+        for (; j < full; ++j, stage = after(stage)) {
             arrive();
             step(std::false_type{});
         }
-        for (; j < s.j1; ++j, stage ^= 1) {
+        for (; j < s.j1; ++j, stage = after(stage)) {
             arrive_masked();
             if (j * kPagedKeys < hi)
                 step(std::true_type{});
@@ -551,13 +565,16 @@ struct Kernel {
         const int lim = live ? limit_of(a, s, t, row0) : 0;
         const int first = s.j0 * kPagedKeys + (kSolo ? 0 : 16 * w), stride = kSolo ? 16 : kPagedKeys;
         const int n = kSolo ? max(1, (min(s.j1 * kPagedKeys, s.kv_end - s.kv) - first + 15) / 16) : s.j1 - s.j0;
-        int pg = ld.page(a, s, first);
-        ld.issue(a, s, first, pg, 0);
-        if (1 < n) {
-            pg = ld.page(a, s, first + stride);
-            ld.issue(a, s, first + stride, pg, 1);
-            if (2 < n) pg = ld.page(a, s, first + 2 * stride);
-        }
+        int pg = ld.page(a, s, first), put = 0, todo = 0;
+        auto fetch = [&]() {
+            if (todo < n) {
+                ld.issue(a, s, first + todo * stride, pg, put);
+                if (++todo < n) pg = ld.page(a, s, first + todo * stride);
+                put = after(put);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NST; ++i) fetch();
         v8 q[HD / 32];
         {
             const char* p = a.q + (live ? (long long)t * a.q_stride + (long long)h * L::ROW : 0) + quad * 16;
@@ -583,9 +600,11 @@ struct Kernel {
         // loop: inside it that wait would be one for all loads in flight.
         wait_loads<0>();
         int stage = 0;
-        for (int i = 0; i < n; ++i, stage ^= 1) {
+        for (int i = 0; i < n; ++i, stage = after(stage)) {
             // the next keys' loads may still be in flight
-            if (i + 1 < n)
+            if (NST > 2 && i + 2 < n)
+                wait_loads<4 * L::NI>();
+            else if (i + 1 < n)
                 wait_loads<2 * L::NI>();
             else
                 wait_loads<0>();
@@ -660,11 +679,8 @@ struct Kernel {
             }
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(y[d], p, o[d]);
-            if (i + 2 < n) {
-                wait_lds();  // these keys' reads are done
-                ld.issue(a, s, at + 2 * stride, pg, stage);
-                if (i + 3 < n) pg = ld.page(a, s, at + 3 * stride);
-            }
+            wait_lds();  // these keys' reads are done: their place is free
+            fetch();
         }
         l += lane_xor16(l);
         l += lane_xor32(l);
@@ -764,7 +780,7 @@ __device__ __forceinline__ int count_units(const PagedAttendArgs& a, const Paged
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendArgs a) {
+__global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a) {
     typedef Kernel<T, HD> K;
     extern __shared__ __align__(1024) unsigned char lds[];
     int* before = reinterpret_cast<int*>(lds + K::RING);
@@ -792,11 +808,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attend_kernel(PagedAttendAr
         return paged_segment(l, u, rows, lens, a.b.n_seq, a.b.n_rows, a.b.capacity, a.nkv, LdsInts{before});
     };
     auto cut = [&](int i) {
-        const long long u = (long long)i * l.per;
-        return u >= total ? total : paged_snap(l, segment((int)u), (int)u);
+        const int u = paged_cut_at(l, i);
+        return u >= total ? total : paged_snap(l, segment(u), u);
     };
     int tick = 0;
-    if (threadIdx.x < 2) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
+    if (threadIdx.x < K::NST) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
     const int u0 = cut(g), u1 = cut(g + 1);
@@ -1002,9 +1018,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
 template <typename T, int HD>
 hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
-    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves + 2) * 4;
+    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves + 3) * 4;
     const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
-    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves + 2) * 4, {fn});
+    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves + 3) * 4, {fn});
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.max_wg), dim3(kThreads), lds, st, a);
     e = hipGetLastError();
@@ -1025,7 +1041,7 @@ PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_
     p.tokens_log2 = paged_tokens_log2(group);
     int dev = 0;
     int cus = hipGetDevice(&dev) == hipSuccess ? device_cu_count(dev) : 256;
-    p.max_wg = (2 * cus + 7) / 8 * 8;
+    p.max_wg = ((hd == 128 ? Kernel<_Float16, 128>::PER_CU : Kernel<_Float16, 64>::PER_CU) * cus + 7) / 8 * 8;
     p.min_per = 2;
     p.uncut = capacity + n_rows <= 512 ? 9 : 1;
     p.slot_rows = min(kPagedRows, (int)min((long long)n_rows * group, (long long)(1 << p.tokens_log2) * group));

@@ -104,15 +104,14 @@ TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
 }
 
 // One launch's line of units.  The ranges: workgroup g of n_wg takes the units
-// from cut g to cut g + 1, cut g being near g * per.
+// from cut g to cut g + 1, cut g being at or near total * g / n_wg.
 struct PagedLine {
     int q, kv0;                // row tile, first position behind the prefix
     int prefix_length;         // units of a row tile on the prefix
     int prefix_rows;           // row tiles over all rows
     int prefix_units;          // of all KV heads
     int total;
-    int per, near;             // units a range, cuts closer than `near` to an edge move there
-    int n_wg;
+    int n_wg, near;            // ranges; cuts closer than `near` to an edge move there
 };
 TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
     PagedLine l{};
@@ -128,9 +127,13 @@ TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
 // segments of fewer key tiles are never cut.
 TER_HD void paged_cut(PagedLine& l, int total, int max_wg, int min_per, int uncut) {
     l.total = total;
-    l.per = paged_max(min_per, (total + max_wg - 1) / max_wg);
-    l.near = paged_max(paged_max(1, l.per / 8), (uncut + 1) / 2);
-    l.n_wg = (total + l.per - 1) / l.per;
+    l.n_wg = paged_min(max_wg, (total + min_per - 1) / min_per);
+    l.near = paged_max(paged_max(1, l.n_wg ? total / l.n_wg / 8 : 0), (uncut + 1) / 2);
+}
+TER_HD int paged_cut_at(const PagedLine& l, int g) { return (int)((long long)l.total * g / l.n_wg); }
+// The first cut at unit u or behind it.
+TER_HD int paged_cut_from(const PagedLine& l, int u) {
+    return u <= 0 ? 0 : (int)(((long long)u * l.n_wg + l.total - 1) / l.total);
 }
 
 struct PagedSegment {
@@ -201,8 +204,8 @@ struct PagedParts {
 };
 TER_HD PagedParts paged_parts(const PagedLine& l, int start, int n) {
     PagedParts p;
-    const int a = start + kPagedLead + l.near, z = start + n - l.near;  // cuts from a to z stay inside
-    const int c0 = (a + l.per - 1) / l.per, c1 = z < 0 ? -1 : z / l.per;
+    // cuts from start + lead + near to start + n - near stay inside
+    const int c0 = paged_cut_from(l, start + kPagedLead + l.near), c1 = paged_cut_from(l, start + n - l.near + 1) - 1;
     p.first = c0 - 1;
     p.last = paged_max(c0 - 1, c1);
     return p;

@@ -78,8 +78,8 @@ int main() {
             return paged_segment(l, u, row0.data(), len.data(), n_seq, n_rows, cap, nkv, before.data());
         };
         auto cut = [&](int g) {
-            const long long u = (long long)g * l.per;
-            return u >= total ? total : paged_snap(l, find((int)u), (int)u);
+            const int u = paged_cut_at(l, g);
+            return u >= total ? total : paged_snap(l, find(u), u);
         };
         size_t k = 0;
         for (int u = 0; u < total; ++u) {
