@@ -35,9 +35,31 @@ struct ConstInts {
         return *(const __attribute__((address_space(4))) int32_t*)(size_t)(p + i);
     }
 };
-struct LdsInts {
-    const int* p;
-    __device__ int operator[](int i) const { return __builtin_amdgcn_readfirstlane(p[i]); }
+// What a workgroup keeps of the batch in LDS: units before each sequence, row
+// boundaries (within [0, n_rows]) and PagedSeq::base.
+struct Seqs {
+    int *before, *row0, *base;
+    int n;
+    __device__ Seqs(int* p, int n_seq) : before(p), row0(p + n_seq + 1), base(p + 2 * n_seq + 2), n(n_seq) {}
+    static __device__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+    __device__ PagedSeq operator[](int b) const {
+        const int r0 = row0[b], r1 = row0[b + 1], k = base[b];
+        return {uniform(r0), max(uniform(r1) - uniform(r0), 0), uniform(k)};
+    }
+    // The first sequence whose units end behind u: 64 looked at together.
+    __device__ int find(int u) const {
+        const int lane = threadIdx.x & 63;
+        int lo = 0, step = 1;
+        if (n > 64) {
+            step = (n + 63) / 64;
+            const int i = (lane + 1) * step;
+            lo = step * __builtin_popcountll(__ballot(i < n && before[min(i, n)] <= u));
+        } else {
+            step = 64;
+        }
+        lo += __builtin_popcountll(__ballot(lane < step && lo + lane + 1 < n && before[min(lo + lane + 1, n)] <= u));
+        return uniform(lo);
+    }
 };
 
 template <typename T>
@@ -242,21 +264,20 @@ struct Kernel {
     };
 
     // Positions (from the segment's first one on) that packed token row t of a segment sees.
-    static __device__ int limit_of(const PagedAttendArgs& a, const Work& s, int t, const int* row0) {
+    static __device__ int limit_of(const Work& s, int t, const Seqs& sq) {
         int base = s.base, r0 = s.row0;
         if (s.seq < 0) {
-            int lo = 0, hi = a.b.n_seq;  // row0[lo] <= t < row0[hi] (LDS copy)
+            int lo = 0, hi = sq.n;  // row0[lo] <= t < row0[hi]
+            if (sq.row0[0] > t || sq.row0[hi] <= t) return 0;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (row0[mid] <= t)
+                if (sq.row0[mid] <= t)
                     lo = mid;
                 else
                     hi = mid;
             }
-            if (row0[0] > t || row0[a.b.n_seq] <= t) return 0;
-            const PagedSeq q = paged_seq(row0[lo], row0[lo + 1], gptr(a.b.kv_len)[lo], a.b.n_rows, a.b.capacity);
-            base = q.base;
-            r0 = q.r0;
+            base = sq.base[lo];
+            r0 = sq.row0[lo];
         }
         return min(max(base + t - r0 + 1, 0), s.kv_end) - s.kv;
     }
@@ -278,7 +299,7 @@ struct Kernel {
     // O^T = V^T P^T.  That order is the same for V's operand: transposing
     // reads of four keys each.
     static __device__ __forceinline__ void rows128(const PagedAttendArgs& a, const Work& s, const Loader& ld,
-                                                   TER_LDS char* ring, const int* row0, int* shared, int& tick,
+                                                   TER_LDS char* ring, const Seqs& sq, int* shared, int& tick,
                                                    int w, int lane) {
         int* const lows = shared;                 // [kWaves]
         int* const flag = shared + kWaves;        // [NST] the tick at which a tile of a stage held odd values
@@ -286,29 +307,28 @@ struct Kernel {
         const int r = 32 * w + col, tok = r / a.group, t = s.tok0 + tok;
         const int h = s.kvh * a.group + (r - tok * a.group);
         const bool live = r < s.rows;
-        const int lim = live ? limit_of(a, s, t, row0) : 0;
+        const int lim = live ? limit_of(s, t, sq) : 0;
         v8 q[HD / 16];
         {
             const char* p = a.q + (live ? (long long)t * a.q_stride + (long long)h * L::ROW : 0) + half * 16;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) q[c] = *gptr(reinterpret_cast<const v8*>(p + c * 32));
         }
-        // the fewest positions that a row sees, the most that one of this wave does
-        int lo = live ? lim : 0x7FFFFFFF, hi = lim;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            lo = min(lo, __shfl_xor(lo, m));
-            hi = max(hi, __shfl_xor(hi, m));
-        }
+        // What every row sees, and what none of this wave's sees more than.
+        // (On the prefix: all of it, or as if some row saw nothing.)
+        int lo, hi;
         if (s.seq >= 0) {
-            lo = paged_limit({0, 0, s.base}, s.tok0 - s.row0, s.kv_end) - s.kv;
+            lo = min(max(s.base + s.tok0 - s.row0 + 1, 0), s.kv_end) - s.kv;
+            hi = 32 * w < s.rows ? min(max(s.base + s.tok0 + (min(32 * w + 32, s.rows) - 1) / a.group - s.row0 + 1, 0),
+                                       s.kv_end) - s.kv
+                                 : 0;
         } else {
-            if (lane == 0) lows[w] = lo;
+            if (lane == 0) lows[w] = 0;
+            if (live && lim < s.kv_end) lows[w] = 1;
             __syncthreads();
-            lo = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+            lo = __builtin_amdgcn_readfirstlane(lows[0] | lows[1] | lows[2] | lows[3]) ? 0 : s.kv_end;
+            hi = 32 * w < s.rows ? s.kv_end : 0;
         }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
 
         f32x16 o[HD / 32];
 #pragma unroll
@@ -558,11 +578,11 @@ struct Kernel {
     // before their sums meet in LDS at the end.
     template <bool kSolo>
     static __device__ __forceinline__ void rows16(const PagedAttendArgs& a, const Work& s, const Loader& ld,
-                                                  TER_LDS char* ring, const int* row0, int w, int lane) {
+                                                  TER_LDS char* ring, const Seqs& sq, int w, int lane) {
         const int quad = lane >> 4, col = lane & 15;
         const int tok = col / a.group, t = s.tok0 + tok, h = s.kvh * a.group + (col - tok * a.group);
         const bool live = col < s.rows;
-        const int lim = live ? limit_of(a, s, t, row0) : 0;
+        const int lim = live ? limit_of(s, t, sq) : 0;
         const int first = s.j0 * kPagedKeys + (kSolo ? 0 : 16 * w), stride = kSolo ? 16 : kPagedKeys;
         const int n = kSolo ? max(1, (min(s.j1 * kPagedKeys, s.kv_end - s.kv) - first + 15) / 16) : s.j1 - s.j0;
         int pg = ld.page(a, s, first), put = 0, todo = 0;
@@ -581,10 +601,11 @@ struct Kernel {
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) q[c] = *gptr(reinterpret_cast<const v8*>(p + c * 64));
         }
-        int lo = live ? lim : 0x7FFFFFFF;
-#pragma unroll
-        for (int m = 1; m < 16; m <<= 1) lo = min(lo, __shfl_xor(lo, m));
-        lo = __builtin_amdgcn_readfirstlane(lo);
+        int lo = 0;  // what every row sees (on the prefix: all of it or nothing)
+        if (s.seq >= 0)
+            lo = min(max(s.base + s.tok0 - s.row0 + 1, 0), s.kv_end) - s.kv;
+        else if (__ballot(live && lim < s.kv_end) == 0)
+            lo = s.kv_end;
         f32x4 o[HD / 16];
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -745,26 +766,36 @@ struct Kernel {
     }
 };
 
-// Units before each sequence (paged_plan.h), [n_seq + 1] in LDS; `row0` a copy
-// of the row boundaries beside it.
-__device__ __forceinline__ int count_units(const PagedAttendArgs& a, const PagedLine& l, int* before, int* row0, int* tmp) {
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false);
+}
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then the last
+// lanes of the rows before.
+__device__ __forceinline__ int wave_prefix(int v) {
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15
+    return dpp_add<0x143, 0xC>(v);  // row_bcast:31
+}
+
+// Fills sq; returns the units of the whole line.
+__device__ __forceinline__ int count_units(const PagedAttendArgs& a, const PagedLine& l, const Seqs& sq, int* tmp) {
     const int n = a.b.n_seq, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int each = (n + kThreads - 1) / kThreads;
+    const int each = (n + kThreads - 1) / kThreads, i0 = tid * each, i1 = min(n, i0 + each);
     int sum = 0;
-    for (int i = tid * each; i < min(n, (tid + 1) * each); ++i) {
+    for (int i = i0; i < i1; ++i) {
         const int r0 = gptr(a.b.row0)[i], r1 = gptr(a.b.row0)[i + 1];
-        row0[i] = r0;
-        if (i == n - 1) row0[n] = r1;
-        const int u = paged_units(paged_seq(r0, r1, gptr(a.b.kv_len)[i], a.b.n_rows, a.b.capacity), l.q, l.kv0) * a.nkv;
-        before[i] = sum;
-        sum += u;
+        const PagedSeq s = paged_seq(r0, r1, gptr(a.b.kv_len)[i], a.b.n_rows, a.b.capacity);
+        sq.row0[i] = s.r0;
+        sq.base[i] = s.base;
+        if (i == n - 1) sq.row0[n] = min(max(r1, 0), a.b.n_rows);
+        sq.before[i] = sum;
+        sum += paged_units(s, l.q, l.kv0) * a.nkv;
     }
-    int inc = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(inc, d);
-        if (lane >= d) inc += v;
-    }
+    const int inc = wave_prefix(sum);
     if (lane == 63) tmp[w] = inc;
     __syncthreads();
     int add = l.prefix_units + inc - sum, total = l.prefix_units;
@@ -773,8 +804,8 @@ __device__ __forceinline__ int count_units(const PagedAttendArgs& a, const Paged
         if (k < w) add += tmp[k];
         total += tmp[k];
     }
-    for (int i = tid * each; i < min(n, (tid + 1) * each); ++i) before[i] += add;
-    if (tid == 0) before[n] = total;
+    for (int i = i0; i < i1; ++i) sq.before[i] += add;
+    if (tid == 0) sq.before[n] = total;
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(total);
 }
@@ -783,16 +814,15 @@ template <typename T, int HD>
 __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a) {
     typedef Kernel<T, HD> K;
     extern __shared__ __align__(1024) unsigned char lds[];
-    int* before = reinterpret_cast<int*>(lds + K::RING);
-    int* row0 = before + a.b.n_seq + 1;
-    int* tmp = row0 + a.b.n_seq + 1;
+    int* tmp = reinterpret_cast<int*>(lds + K::RING);  // [kWaves + 3]
+    const Seqs sq(tmp + kWaves + 3, a.b.n_seq);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TER_LDS char* ring = (TER_LDS char*)lds;
 
     PagedLine l = paged_line(a.tokens_log2, a.shared, a.b.n_rows, a.nkv);
-    const int total = count_units(a, l, before, row0, tmp);
+    const int total = count_units(a, l, sq, tmp);
     if (a.shared && blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = before[i];
+        for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = sq.before[i];
     paged_cut(l, total, a.max_wg, a.min_per, a.uncut);
     // neighbouring ranges on one XCD (blocks go round the 8 XCDs): they read the same keys
     // (blocks beyond the last range have the numbers behind it: each number once)
@@ -803,9 +833,12 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         return;
     }
 
-    const ConstInts rows{a.b.row0}, lens{a.b.kv_len};
+    PagedSeq q{};  // the sequence of the segment found last
     auto segment = [&](int u) {
-        return paged_segment(l, u, rows, lens, a.b.n_seq, a.b.n_rows, a.b.capacity, a.nkv, LdsInts{before});
+        if (u < l.prefix_units) return paged_segment(l, u, a.nkv, 0, q, 0, 0);
+        const int b = sq.find(u), b0 = sq.before[b], b1 = sq.before[b + 1];
+        q = sq[b];
+        return paged_segment(l, u, a.nkv, b, q, Seqs::uniform(b0), Seqs::uniform(b1));
     };
     auto cut = [&](int i) {
         const int u = paged_cut_at(l, i);
@@ -815,13 +848,12 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
     if (threadIdx.x < K::NST) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
-    const int u0 = cut(g), u1 = cut(g + 1);
+    const int u1 = cut(g + 1), u0 = cut(g);
     if (u0 >= u1) {
         if (threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
         return;
     }
     PagedSegment sg = segment(u0);
-    PagedSeq q{};
     int turn = -1;  // of a run of short segments: the wave whose turn it is
     for (int u = u0;;) {
         const int end = min(u1, sg.start + sg.n);
@@ -839,7 +871,6 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
             s.row0 = s.base = 0;
             s.table = a.b.pages;
         } else {
-            q = paged_seq(rows[sg.seq], rows[sg.seq + 1], lens[sg.seq], a.b.n_rows, a.b.capacity);
             const int i = sg.tile << l.q;
             s.tok0 = q.r0 + i;
             s.n_tok = min(q.n - i, 1 << l.q);
@@ -863,14 +894,14 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
             // short ones beside others: the waves take turns, each by itself
             if (turn < 0) __syncthreads();
             turn = (turn + 1) & (kWaves - 1);
-            if (turn == w) K::template rows16<true>(a, s, ld, ring, row0, w, lane);
+            if (turn == w) K::template rows16<true>(a, s, ld, ring, sq, w, lane);
         } else {
             turn = -1;
             __syncthreads();  // the ring is free
             if (s.rows > 16)
-                K::rows128(a, s, ld, ring, row0, tmp, tick, w, lane);
+                K::rows128(a, s, ld, ring, sq, tmp, tick, w, lane);
             else
-                K::template rows16<false>(a, s, ld, ring, row0, w, lane);
+                K::template rows16<false>(a, s, ld, ring, sq, w, lane);
         }
         u = end;
         if (u >= u1) break;
@@ -1018,9 +1049,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
 template <typename T, int HD>
 hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
-    const int lds = Kernel<T, HD>::RING + (2 * (a.b.n_seq + 1) + kWaves + 3) * 4;
+    const int lds = Kernel<T, HD>::RING + (3 * a.b.n_seq + 2 + kWaves + 3) * 4;
     const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
-    hipError_t e = limit.allow(Kernel<T, HD>::RING + (2 * (TER_HIP_PAGED_SEQ_MAX + 1) + kWaves + 3) * 4, {fn});
+    hipError_t e = limit.allow(Kernel<T, HD>::RING + (3 * TER_HIP_PAGED_SEQ_MAX + 2 + kWaves + 3) * 4, {fn});
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.max_wg), dim3(kThreads), lds, st, a);
     e = hipGetLastError();

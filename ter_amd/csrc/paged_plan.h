@@ -112,6 +112,7 @@ struct PagedLine {
     int prefix_units;          // of all KV heads
     int total;
     int n_wg, near;            // ranges; cuts closer than `near` to an edge move there
+    int step, rest;            // total = step * n_wg + rest
 };
 TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
     PagedLine l{};
@@ -128,12 +129,19 @@ TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
 TER_HD void paged_cut(PagedLine& l, int total, int max_wg, int min_per, int uncut) {
     l.total = total;
     l.n_wg = paged_min(max_wg, (total + min_per - 1) / min_per);
-    l.near = paged_max(paged_max(1, l.n_wg ? total / l.n_wg / 8 : 0), (uncut + 1) / 2);
+    l.step = l.n_wg ? (int)((unsigned)total / (unsigned)l.n_wg) : 0;
+    l.rest = total - l.step * l.n_wg;
+    l.near = paged_max(paged_max(1, l.step / 8), (uncut + 1) / 2);
 }
-TER_HD int paged_cut_at(const PagedLine& l, int g) { return (int)((long long)l.total * g / l.n_wg); }
-// The first cut at unit u or behind it.
+// floor(total * g / n_wg)
+TER_HD int paged_cut_at(const PagedLine& l, int g) {
+    return l.step * g + (int)((unsigned)(l.rest * g) / (unsigned)l.n_wg);
+}
+// The first cut at unit u or behind it: ceil(u * n_wg / total).  (In binary64
+// exactly: the quotient is below 2^11, and at least 2^-31 off an integer if it
+// is none.)
 TER_HD int paged_cut_from(const PagedLine& l, int u) {
-    return u <= 0 ? 0 : (int)(((long long)u * l.n_wg + l.total - 1) / l.total);
+    return u <= 0 ? 0 : (int)__builtin_ceil((double)u * l.n_wg / l.total);
 }
 
 struct PagedSegment {
@@ -142,33 +150,23 @@ struct PagedSegment {
     int kvh, tile;  // KV head, row tile
 };
 
-// The segment of unit u (0 <= u < total).  before: units before each sequence
-// (prefix units included), [n_seq + 1].
-template <class Ints, class Before>
-TER_HD PagedSegment paged_segment(const PagedLine& l, int u, Ints row0, Ints kv_len, int n_seq, int n_rows, int cap,
-                                  int nkv, Before before) {
+// The segment of unit u (0 <= u < total): b is the first sequence with units
+// behind u (of no matter for the prefix), s its rows, b0 and b1 the units
+// before it and behind it.
+TER_HD PagedSegment paged_segment(const PagedLine& l, int u, int nkv, int b, const PagedSeq& s, int b0, int b1) {
     PagedSegment g;
     if (u < l.prefix_units) {
-        const int i = u / l.prefix_length;
+        const unsigned i = (unsigned)u / (unsigned)l.prefix_length;
         g.seq = -1;
-        g.kvh = i / l.prefix_rows;
-        g.tile = i - g.kvh * l.prefix_rows;
-        g.start = i * l.prefix_length;
+        g.kvh = (int)(i / (unsigned)l.prefix_rows);
+        g.tile = (int)i - g.kvh * l.prefix_rows;
+        g.start = (int)i * l.prefix_length;
         g.n = l.prefix_length;
         return g;
     }
-    int lo = 0, hi = n_seq - 1;  // the last sequence that begins at u or before (empty ones before it end there too)
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (before[mid] <= u)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    const PagedSeq s = paged_seq(row0[lo], row0[lo + 1], kv_len[lo], n_rows, cap);
-    const int b0 = before[lo], each = (before[lo + 1] - b0) / nkv, at = u - b0;
-    g.seq = lo;
-    g.kvh = at / each;
+    const int each = (int)((unsigned)(b1 - b0) / (unsigned)nkv), at = u - b0;
+    g.seq = b;
+    g.kvh = (int)((unsigned)at / (unsigned)each);
     const int r = at - g.kvh * each;
     g.tile = paged_row_tile_of(s, r, l.q, l.kv0);
     g.start = b0 + g.kvh * each + paged_length_before(s, g.tile, l.q, l.kv0);

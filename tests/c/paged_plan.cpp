@@ -70,12 +70,20 @@ int main() {
         CHECK(total == before.back());
         if (!total) continue;
         paged_cut(l, total, in(1, 600), in(1, 4), in(0, 3) ? 1 : in(2, 20));
+        for (int w = 0; w <= l.n_wg; ++w) CHECK(paged_cut_at(l, w) == (long long)total * w / l.n_wg);
+        for (int i = 0; i < 20; ++i) {
+            const int u = in(0, total);
+            CHECK(paged_cut_from(l, u) == ((long long)u * l.n_wg + total - 1) / total);
+        }
         // the device's way: each range by itself
         std::vector<int> done(total, 0);
         std::map<std::pair<int, int>, int> slots;  // (segment start, range) -> slot
         std::set<int> used;
         auto find = [&](int u) {
-            return paged_segment(l, u, row0.data(), len.data(), n_seq, n_rows, cap, nkv, before.data());
+            int b = 0;
+            while (u >= l.prefix_units && before[b + 1] <= u) ++b;
+            return paged_segment(l, u, nkv, b, paged_seq(row0[b], row0[b + 1], len[b], n_rows, cap), before[b],
+                                 before[b + 1]);
         };
         auto cut = [&](int g) {
             const int u = paged_cut_at(l, g);
