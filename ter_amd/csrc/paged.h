@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "paged_plan.h"
 #include "ter_hip_paged.h"
 
 namespace terhip {
@@ -48,7 +49,7 @@ struct PagedAttendArgs {
     int nh, nkv, group, tokens_log2;
     int shared;                      // a multiple of 16
     unsigned page_magic;             // ceil(2^32 / (page_size / 16)); 0 for pages of 16
-    int max_wg, min_per, uncut;      // paged_cut()
+    PagedCuts cuts_by;
     // the workspace (paged_attend_layout)
     int* cuts;                       // [max_wg][8] where a range begins inside a segment: rows of the row tile
                                      //   (0: it does not), first token row, KV head, first and last range of it
@@ -63,7 +64,8 @@ struct PagedAttendArgs {
 // How a call is cut, and where its parts lie in the workspace (offsets in
 // bytes; the rows of `whole` are there with a shared prefix only).
 struct PagedAttendLayout {
-    int tokens_log2, max_wg, min_per, uncut, slot_rows;
+    int tokens_log2, slot_rows;
+    PagedCuts cuts_by;
     size_t cuts, before, slots, slot_stats, whole, whole_stats, bytes;
 };
 PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared);

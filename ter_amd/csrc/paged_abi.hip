@@ -198,9 +198,7 @@ int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
     a.shared = shared;
     const unsigned d = (unsigned)a.c.page_size / 16;  // x / d = x * magic >> 32 for x < 2^17, d <= 4096
     a.page_magic = d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d);
-    a.max_wg = p.max_wg;
-    a.min_per = p.min_per;
-    a.uncut = p.uncut;
+    a.cuts_by = p.cuts_by;
     a.slot_rows = p.slot_rows;
     char* w = static_cast<char*>(ws);
     a.cuts = reinterpret_cast<int*>(w + p.cuts);

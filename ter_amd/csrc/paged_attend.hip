@@ -218,48 +218,74 @@ struct Kernel {
 
     // ---- loads: wave w takes rows 16 w .. 16 w + 15 of K and V
     struct Loader {
-        unsigned ko[L::NI], vo[L::NI];  // byte offsets of this lane's piece in the 16 rows
+        unsigned row, kp, vp;  // byte offset of this lane's first row, its pieces of K and V there
         unsigned lds;
-        int w;
         __device__ void init(const PagedAttendArgs& a, unsigned lds_off, int wave, int lane) {
-            w = wave;
             lds = lds_off + wave * 16 * L::ROW;
             const int r0 = lane / L::PIECES, p = lane % L::PIECES;
-#pragma unroll
-            for (int i = 0; i < L::NI; ++i) {
-                const int r = i * L::RPI + r0;
-                ko[i] = r * a.c.pos_stride + (p ^ L::swizzle_k(r)) * 16;
-                vo[i] = r * a.c.pos_stride + (p ^ L::swizzle_v(r)) * 16;
+            row = r0 * a.c.pos_stride;
+            kp = (p ^ L::swizzle_k(r0)) * 16;
+            vp = (p ^ L::swizzle_v(r0)) * 16;
+        }
+        // (instruction i: rows i * RPI further on, whose K swizzle differs in
+        // one bit or two, whose V swizzle is the same)
+        __device__ __forceinline__ unsigned k_at(const PagedAttendArgs& a, int i) const {
+            return (kp ^ (L::swizzle_k(i * L::RPI) * 16)) + (row + i * L::RPI * a.c.pos_stride);
+        }
+        __device__ __forceinline__ unsigned v_at(const PagedAttendArgs& a, int i) const {
+            return vp + (row + i * L::RPI * a.c.pos_stride);
+        }
+        // Where the next 64 groups of 16 positions are, one a lane: offset
+        // into K and V, bytes from there on that may be read (0: none).  From
+        // these a step takes its own with three lane reads; found one by one,
+        // by scalar loads and products, they took longer than its first
+        // matrix products, and the loads were waited for with every LDS read.
+        struct Groups {
+            unsigned lo, hi, bytes;
+        };
+        // `stride` positions apart, from position `at` of the segment on.
+        static __device__ __forceinline__ void locate(Groups& g, const PagedAttendArgs& a, const Work& s, int at,
+                                                      int stride, int lane) {
+            const int pos = s.kv + at + lane * stride;
+            g = {0u, 0u, 0u};
+            if (pos < s.kv_end) {
+                const unsigned x = (unsigned)pos >> 4, i = a.page_magic ? __umulhi(x, a.page_magic) : x;
+                const int page = gptr(s.table)[i];
+                if (page >= 0 && page < a.c.n_pages) {
+                    const unsigned long long o = (unsigned long long)page * (unsigned long long)a.c.page_stride +
+                                                 (unsigned long long)(pos - (int)i * a.c.page_size) * (unsigned)a.c.pos_stride +
+                                                 (unsigned long long)s.kvh * (unsigned)a.c.head_stride;
+                    g.lo = (unsigned)o;
+                    g.hi = (unsigned)(o >> 32);
+                    g.bytes = (unsigned)(min(s.kv_end - pos, 16) - 1) * a.c.pos_stride + L::ROW;
+                }
             }
+            asm volatile("" : "+v"(g.lo), "+v"(g.hi), "+v"(g.bytes));  // (waited for here)
         }
-        // The page of 16 positions from `at` on (counted from the segment's
-        // first one; -1: none), and the load of them into this wave's rows.
-        __device__ int page(const PagedAttendArgs& a, const Work& s, int at) const {
-            const int pos = s.kv + at;
-            if (pos >= s.kv_end) return -1;
-            const unsigned x = (unsigned)pos >> 4;
-            const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
-            return ConstInts{s.table}[i];
+        // A load of 2 * NI instructions, K first, to be issued one by one.
+        struct Pending {
+            u32x4 kr, vr;
+            unsigned to;
+        };
+        __device__ __forceinline__ Pending prepare(const PagedAttendArgs& a, const Groups& g, int i, int stage) const {
+            const unsigned long long o = (unsigned)__builtin_amdgcn_readlane(g.lo, i) |
+                                         (unsigned long long)(unsigned)__builtin_amdgcn_readlane(g.hi, i) << 32;
+            const unsigned bytes = (unsigned)__builtin_amdgcn_readlane(g.bytes, i);
+            const unsigned long long kb = (unsigned long long)a.c.k + o, vb = (unsigned long long)a.c.v + o;
+            return {{(unsigned)kb, (unsigned)(kb >> 32) & 0xFFFFu, bytes, 0x00020000u},
+                    {(unsigned)vb, (unsigned)(vb >> 32) & 0xFFFFu, bytes, 0x00020000u},
+                    lds + stage * L::BYTES};
         }
-        __device__ void issue(const PagedAttendArgs& a, const Work& s, int at, int page, int stage) const {
-            const int pos = s.kv + at;
-            const unsigned x = (unsigned)pos >> 4;
-            const unsigned i = a.page_magic ? (unsigned)(((unsigned long long)x * a.page_magic) >> 32) : x;
-            const int slot = pos - (int)i * a.c.page_size;
-            int n = min(s.kv_end - pos, 16);
-            if (page < 0 || page >= a.c.n_pages) n = 0;
-            const unsigned bytes = n > 0 ? (unsigned)(n - 1) * a.c.pos_stride + L::ROW : 0u;
-            const long long o = n > 0 ? page * a.c.page_stride + (long long)slot * a.c.pos_stride +
-                                            (long long)s.kvh * a.c.head_stride
-                                      : 0;
-            const unsigned long long kb = (unsigned long long)(a.c.k + o), vb = (unsigned long long)(a.c.v + o);
-            const u32x4 kr = {(unsigned)kb, (unsigned)(kb >> 32) & 0xFFFFu, bytes, 0x00020000u};
-            const u32x4 vr = {(unsigned)vb, (unsigned)(vb >> 32) & 0xFFFFu, bytes, 0x00020000u};
-            const unsigned d = lds + stage * L::BYTES;
+        __device__ __forceinline__ void piece(const PagedAttendArgs& a, const Pending& p, int i) const {
+            if (i < L::NI)
+                load_to_lds(p.kr, k_at(a, i), p.to + i * 1024);
+            else
+                load_to_lds(p.vr, v_at(a, i - L::NI), p.to + L::V + (i - L::NI) * 1024);
+        }
+        __device__ __forceinline__ void issue(const PagedAttendArgs& a, const Groups& g, int at, int stage) const {
+            const Pending p = prepare(a, g, at, stage);
 #pragma unroll
-            for (int i = 0; i < L::NI; ++i) load_to_lds(kr, ko[i], d + i * 1024);
-#pragma unroll
-            for (int i = 0; i < L::NI; ++i) load_to_lds(vr, vo[i], d + L::V + i * 1024);
+            for (int i = 0; i < 2 * L::NI; ++i) piece(a, p, i);
         }
     };
 
@@ -339,27 +365,38 @@ struct Kernel {
 
         // LDS offsets: K pieces of row col (+ 32 by offset); V rows of the
         // lane's transposing read
-        int ka[HD / 16], va[HD / 32];
-#pragma unroll
-        for (int c = 0; c < HD / 16; ++c) ka[c] = col * L::ROW + (((2 * c + half) ^ L::swizzle_k(col)) * 16);
+        // (pieces further on by exclusive or: rows and stages are multiples of
+        // 128 bytes)
+        const int ka = col * L::ROW + ((half ^ L::swizzle_k(col)) * 16);
         const int vr = 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-            va[d] = L::V + vr * L::ROW +
-                    (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
-
+        const int va = L::V + vr * L::ROW + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) +
+                       8 * (lane & 1);
         const auto mine = [&](int j) { return j * kPagedKeys + 16 * w; };
         // NST - 1 tiles ahead of the one in work
-        int pg = ld.page(a, s, mine(s.j0)), put = 0, todo = s.j0;
+        typename Loader::Groups groups;
+        int put = 0, todo = s.j0;
+        auto group = [&]() {
+            const int i = (todo - s.j0) & 63;
+            if (i == 0) Loader::locate(groups, a, s, mine(todo), kPagedKeys, lane);
+            ++todo;
+            return i;
+        };
         auto fetch = [&]() {
             if (todo < s.j1) {
-                ld.issue(a, s, mine(todo), pg, put);
-                if (++todo < s.j1) pg = ld.page(a, s, mine(todo));
+                ld.issue(a, groups, group(), put);
                 put = after(put);
             }
         };
 #pragma unroll
         for (int i = 0; i < NST - 1; ++i) fetch();
+        // The same in pieces, spread over a step: a wave that issues all of
+        // them at once waits a quarter of the step for the address unit.
+        // (Behind the last tile they load what nobody reads, into a stage that is free.)
+        typename Loader::Pending next;
+        auto prepare = [&]() {
+            next = ld.prepare(a, groups, group(), put);
+            put = after(put);
+        };
         int stage = 0, j = s.j0;
         auto landed = [&]() {  // this wave's rows of tile j are in LDS
             if (NST > 2 && j + 1 < s.j1)
@@ -422,14 +459,14 @@ struct Kernel {
         // the scheduling groups below.)
         auto step = [&](auto masked) {
             constexpr bool kMasked = decltype(masked)::value;
-            const TER_LDS char* tile = ring + stage * L::BYTES;
+            const int kt = (int)(size_t)ring + stage * L::BYTES + ka, vt = (int)(size_t)ring + stage * L::BYTES + va;
             f32x16 x[2];
             v8 k[HD / 16], p[2][2], y[2][HD / 32];
             float al = 1.f;
-            auto read_k = [&](int b, int c) { k[c] = *(const TER_LDS v8*)(tile + ka[c] + b * 32 * L::ROW); };
+            auto read_k = [&](int b, int c) { k[c] = *((const TER_LDS v8*)(size_t)(unsigned)(kt ^ (32 * c)) + b * 2 * L::ROW); };
             auto scores = [&](int b, int c) { x[b] = E::mma32(k[c], q[c], x[b]); };
             auto read_v = [&](int c, int d) {
-                const TER_LDS char* v = tile + va[d] + c * 16 * L::ROW;
+                const TER_LDS char* v = (const TER_LDS char*)(size_t)(unsigned)(vt ^ (64 * d)) + c * 16 * L::ROW;
                 const v4 y0 = E::read_tr(v), y1 = E::read_tr(v + 8 * L::ROW);
                 y[c & 1][d] = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
             };
@@ -477,27 +514,29 @@ struct Kernel {
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) read_k(0, c);
             __builtin_amdgcn_sched_barrier(0);
-            fetch();
+            prepare();
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[0][i] = x[1][i] = 0.f;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
                 scores(0, c);
                 read_k(1, c);
+                if (c % 4 == 2) ld.piece(a, next, c / 4);  // NI / 2
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (decide(0)) rescale();
             __builtin_amdgcn_sched_barrier(0);
+            // (in this order: two weights for each of eight places in the code)
 #pragma unroll
-            for (int c = 0; c < HD / 16; ++c) scores(1, c);
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d) read_v(0, d);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) weight(0, i);
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // a matrix product
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                // an LDS read
-                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (HD / 16), 0);  // vector work
+            for (int i = 0; i < 8; ++i) {
+                if (i % (128 / HD) == 0) {
+                    const int c = i / (128 / HD);
+                    scores(1, c);
+                    if (c % 2 == 0) ld.piece(a, next, L::NI / 2 + c / 2);  // NI
+                    if (c >= HD / 32) read_v(0, c - HD / 32);
+                }
+                weight(0, 2 * i);
+                __builtin_amdgcn_sched_barrier(0);
             }
             // (weights are formed here, not where they are used)
             asm volatile("" : "+v"(p[0][0]), "+v"(p[0][1]), "+v"(l));
@@ -506,22 +545,19 @@ struct Kernel {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) read_v(1, d);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 0; d < HD / 32; ++d) {
-                    value(c, d);
-                    read_v(2 + c, d);
-                }
             const float sum = l;
             l = 0.f;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) weight(1, i);
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (HD / 16), 0);
+            for (int i = 0; i < 8; ++i) {
+                if (i % (128 / HD) == 0) {
+                    const int c = i / 4, d = i / (128 / HD) % (HD / 32);
+                    value(c, d);
+                    read_v(2 + c, d);
+                    if (i % (16 / L::NI) == 2) ld.piece(a, next, L::NI * 3 / 2 + i / (16 / L::NI));  // NI / 2
+                }
+                weight(1, 2 * i);
+                __builtin_amdgcn_sched_barrier(0);
             }
             asm volatile("" : "+v"(p[1][0]), "+v"(p[1][1]), "+v"(l));
             __builtin_amdgcn_sched_barrier(0);
@@ -547,6 +583,7 @@ struct Kernel {
             else
                 fetch();  // no row of this wave sees it
         }
+        wait_loads<0>();
         l += lane_xor32(l);
         if (!live) return;
         if (s.dst == 0) {
@@ -585,11 +622,13 @@ struct Kernel {
         const int lim = live ? limit_of(s, t, sq) : 0;
         const int first = s.j0 * kPagedKeys + (kSolo ? 0 : 16 * w), stride = kSolo ? 16 : kPagedKeys;
         const int n = kSolo ? max(1, (min(s.j1 * kPagedKeys, s.kv_end - s.kv) - first + 15) / 16) : s.j1 - s.j0;
-        int pg = ld.page(a, s, first), put = 0, todo = 0;
+        typename Loader::Groups groups;
+        int put = 0, todo = 0;
         auto fetch = [&]() {
             if (todo < n) {
-                ld.issue(a, s, first + todo * stride, pg, put);
-                if (++todo < n) pg = ld.page(a, s, first + todo * stride);
+                if ((todo & 63) == 0) Loader::locate(groups, a, s, first + todo * stride, stride, lane);
+                ld.issue(a, groups, todo & 63, put);
+                ++todo;
                 put = after(put);
             }
         };
@@ -823,11 +862,11 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
     const int total = count_units(a, l, sq, tmp);
     if (a.shared && blockIdx.x == 0)
         for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = sq.before[i];
-    paged_cut(l, total, a.max_wg, a.min_per, a.uncut);
+    paged_cut(l, total, a.cuts_by);
     // neighbouring ranges on one XCD (blocks go round the 8 XCDs): they read the same keys
     // (blocks beyond the last range have the numbers behind it: each number once)
     const int chunk = (l.n_wg + 7) / 8, x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8);
-    const int g = y < chunk ? x * chunk + y : 8 * chunk + x * (a.max_wg / 8 - chunk) + y - chunk;
+    const int g = y < chunk ? x * chunk + y : 8 * chunk + x * (a.cuts_by.max_wg / 8 - chunk) + y - chunk;
     if (g >= l.n_wg) {
         if (threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
         return;
@@ -840,23 +879,22 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         q = sq[b];
         return paged_segment(l, u, a.nkv, b, q, Seqs::uniform(b0), Seqs::uniform(b1));
     };
-    auto cut = [&](int i) {
-        const int u = paged_cut_at(l, i);
-        return u >= total ? total : paged_snap(l, segment(u), u);
-    };
-    int tick = 0;
-    if (threadIdx.x < K::NST) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
-    const int u1 = cut(g + 1), u0 = cut(g);
-    if (u0 >= u1) {
-        if (threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
-        return;
-    }
+    int tick = 0;
+    if (threadIdx.x < K::NST) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
+    const int raw1 = paged_cut_at(l, g + 1);
+    int u0 = paged_cut_at(l, g);
     PagedSegment sg = segment(u0);
+    u0 = paged_snap(l, sg, u0);
+    if (u0 == sg.start + sg.n && u0 < total) sg = segment(u0);
     int turn = -1;  // of a run of short segments: the wave whose turn it is
     for (int u = u0;;) {
-        const int end = min(u1, sg.start + sg.n);
+        const int end = raw1 >= sg.start + sg.n ? sg.start + sg.n : paged_snap(l, sg, raw1);
+        if (end <= u) {
+            if (u == u0 && threadIdx.x == 0) gptr(a.cuts)[8 * g] = 0;
+            break;
+        }
         Work s;
         s.seq = sg.seq;
         s.kvh = sg.kvh;
@@ -885,12 +923,7 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         const int slot = 2 * g + (u == sg.start ? 1 : 0);
         s.slot = a.slots + (long long)slot * a.slot_rows * HD;
         s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
-        if (u == u0 && threadIdx.x == 0) {  // what the joining kernel has to know of this cut
-            const PagedParts p = paged_parts(l, sg.start, sg.n);
-            *gptr(reinterpret_cast<i32x4*>(a.cuts + 8 * g)) = i32x4{u == sg.start ? 0 : s.rows, s.tok0, s.kvh, p.first};
-            gptr(a.cuts)[8 * g + 4] = p.last;
-        }
-        if (s.rows <= 16 && s.j1 - s.j0 <= kSolo && (u > u0 || end < u1)) {
+        if (s.rows <= 16 && s.j1 - s.j0 <= kSolo && (u > u0 || raw1 > end)) {
             // short ones beside others: the waves take turns, each by itself
             if (turn < 0) __syncthreads();
             turn = (turn + 1) & (kWaves - 1);
@@ -903,8 +936,13 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
             else
                 K::template rows16<false>(a, s, ld, ring, sq, w, lane);
         }
+        if (u == u0 && threadIdx.x == 0) {  // what the joining kernel has to know of this cut
+            const PagedParts p = paged_parts(l, sg.start, sg.n);
+            *gptr(reinterpret_cast<i32x4*>(a.cuts + 8 * g)) = i32x4{u == sg.start ? 0 : s.rows, s.tok0, s.kvh, p.first};
+            gptr(a.cuts)[8 * g + 4] = p.last;
+        }
         u = end;
-        if (u >= u1) break;
+        if (u < sg.start + sg.n || u >= total) break;
         if (!paged_advance(l, sg, q, a.nkv)) sg = segment(u);
     }
 }
@@ -1014,7 +1052,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
     const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
     const PagedSeq s = paged_seq(rows[b], rows[b + 1], lens[b], a.b.n_rows, a.b.capacity);
     PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
-    paged_cut(l, before[a.b.n_seq], a.max_wg, a.min_per, a.uncut);
+    paged_cut(l, before[a.b.n_seq], a.cuts_by);
     const int tile = (t - s.r0) >> q, b0 = before[b], each = (before[b + 1] - b0) / a.nkv;
     const PagedParts own = paged_parts(l, b0 + kvh * each + paged_length_before(s, tile, q, l.kv0),
                                        paged_length(s, tile, q, l.kv0));
@@ -1053,14 +1091,14 @@ hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
     hipError_t e = limit.allow(Kernel<T, HD>::RING + (3 * TER_HIP_PAGED_SEQ_MAX + 2 + kWaves + 3) * 4, {fn});
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.max_wg), dim3(kThreads), lds, st, a);
+    hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.cuts_by.max_wg), dim3(kThreads), lds, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (!a.shared && a.uncut * kPagedKeys > a.b.capacity + a.b.n_rows) return hipSuccess;  // nothing is cut
+    if (!a.shared && a.cuts_by.uncut * kPagedKeys > a.b.capacity + a.b.n_rows) return hipSuccess;  // nothing is cut
     if (a.shared)
         hipLaunchKernelGGL((paged_join_shared_kernel<T, HD>), dim3(a.b.n_rows, a.nkv), dim3(kThreads), 0, st, a);
     else
-        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(a.max_wg, 4), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(a.cuts_by.max_wg, 4), dim3(kThreads), 0, st, a);
     return hipGetLastError();
 }
 
@@ -1072,17 +1110,25 @@ PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_
     p.tokens_log2 = paged_tokens_log2(group);
     int dev = 0;
     int cus = hipGetDevice(&dev) == hipSuccess ? device_cu_count(dev) : 256;
-    p.max_wg = ((hd == 128 ? Kernel<_Float16, 128>::PER_CU : Kernel<_Float16, 64>::PER_CU) * cus + 7) / 8 * 8;
-    p.min_per = 2;
-    p.uncut = capacity + n_rows <= 512 ? 9 : 1;
+    const int64_t tiles = ((int64_t)n_rows >> p.tokens_log2) + n_seq;
+    // no more ranges than there can be work for
+    const int64_t units = nkv * (tiles * (kPagedLead + 1 + min((int64_t)capacity + n_rows, (int64_t)1 << 30) / kPagedKeys) +
+                                 (shared ? tiles * (kPagedLead + 1 + shared / kPagedKeys) : 0));
+    PagedCuts& c = p.cuts_by;
+    c.resident = (hd == 128 ? Kernel<_Float16, 128>::PER_CU : Kernel<_Float16, 64>::PER_CU) * cus;
+    c.min_per = 2;
+    c.target = 96;
+    c.uncut = capacity + n_rows <= 512 ? 9 : 1;
+    c.max_wg = (int)min((int64_t)4 * c.resident, (units + c.min_per - 1) / c.min_per);
+    c.max_wg = (c.max_wg + 7) / 8 * 8;
     p.slot_rows = min(kPagedRows, (int)min((long long)n_rows * group, (long long)(1 << p.tokens_log2) * group));
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
         return at;
     };
-    const size_t slots = 2 * (size_t)p.max_wg * p.slot_rows, whole = shared ? 2 * (size_t)n_rows * nh : 0;
-    p.cuts = take((size_t)p.max_wg * 32);
+    const size_t slots = 2 * (size_t)c.max_wg * p.slot_rows, whole = shared ? 2 * (size_t)n_rows * nh : 0;
+    p.cuts = take((size_t)c.max_wg * 32);
     p.before = take(shared ? (size_t)(n_seq + 1) * 4 : 0);
     p.slot_stats = take(slots * 2 * 4);
     p.whole_stats = take(whole * 2 * 4);

@@ -65,26 +65,27 @@ TER_HD int paged_key_tiles(const PagedSeq& s, int rt, int q, int kv0) {
     const int a = s.base - kv0 + paged_min(s.n, (rt + 1) << q);
     return a <= kPagedKeys ? 1 : (a + kPagedKeys - 1) / kPagedKeys;
 }
-// Key tiles of row tiles 0 .. n - 1, all of them full.
-TER_HD long long paged_key_tiles_before(const PagedSeq& s, int n, int q, int kv0) {
+// Key tiles of row tiles 0 .. n - 1, all of them full.  (Sums modulo 2^32, of
+// which the result is less.)
+TER_HD int paged_key_tiles_before(const PagedSeq& s, int n, int q, int kv0) {
     const int c = s.base - kv0, room = kPagedKeys - c;
     const int ones = paged_min(n, room >= (1 << q) ? room >> q : 0);  // tiles of at most 64 positions
     if (ones == n) return n;
-    const long long m = n - ones;
+    const unsigned m = (unsigned)(n - ones);
     if (q >= 6)  // ceil((c + 2^q i) / 64), i = ones + 1 .. n
-        return ones + m * ((c + 63) >> 6) + ((m * (ones + 1 + n) / 2) << (q - 6));
+        return (int)((unsigned)ones + m * (unsigned)((c + 63) >> 6) + ((m * (unsigned)(ones + 1 + n) / 2) << (q - 6)));
     // ceil(x / R) for x = e + ones + 1 .. e + n, R row tiles to a key tile
     const int lr = 6 - q, e = (c + (1 << q) - 1) >> q;
-    const long long x1 = e + n, x0 = e + ones, a1 = x1 >> lr, a0 = x0 >> lr, r = (1 << lr) - 1;
-    return ones + (((a1 * (a1 + 1) / 2) << lr) + (x1 & r) * (a1 + 1)) -
-           (((a0 * (a0 + 1) / 2) << lr) + (x0 & r) * (a0 + 1));
+    const unsigned x1 = (unsigned)(e + n), x0 = (unsigned)(e + ones), a1 = x1 >> lr, a0 = x0 >> lr, r = (1u << lr) - 1;
+    return (int)((unsigned)ones + (((a1 * (a1 + 1) / 2) << lr) + (x1 & r) * (a1 + 1)) -
+                 (((a0 * (a0 + 1) / 2) << lr) + (x0 & r) * (a0 + 1)));
 }
 // Units of a segment, of the row tiles before it, of a sequence for one KV head.
 TER_HD int paged_length(const PagedSeq& s, int rt, int q, int kv0) {
     return kPagedLead + paged_key_tiles(s, rt, q, kv0);
 }
 TER_HD int paged_length_before(const PagedSeq& s, int n, int q, int kv0) {
-    return n * kPagedLead + (int)paged_key_tiles_before(s, n, q, kv0);
+    return n * kPagedLead + paged_key_tiles_before(s, n, q, kv0);
 }
 TER_HD int paged_units(const PagedSeq& s, int q, int kv0) {
     const int t = paged_row_tiles(s, q);
@@ -123,15 +124,26 @@ TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
     l.prefix_units = l.prefix_length * l.prefix_rows * nkv;
     return l;
 }
-// total: prefix units and those of the sequences.  max_wg: workgroups of the
-// launch.  min_per: fewer units than that are not worth a workgroup.  uncut:
+// How the line is cut.  resident: workgroups that run at the same time; more
+// ranges than that, of `target` units or more, if there is work for them: the
+// hardware starts them as others end, which evens out what equal ranges do not
+// (of two workgroups of a CU the older one is served first and ends a quarter
+// earlier).  min_per: fewer units than that are not worth a workgroup.  uncut:
 // segments of fewer key tiles are never cut.
-TER_HD void paged_cut(PagedLine& l, int total, int max_wg, int min_per, int uncut) {
+struct PagedCuts {
+    int max_wg, resident, target, min_per, uncut;
+};
+TER_HD void paged_cut(PagedLine& l, int total, const PagedCuts& c) {
     l.total = total;
-    l.n_wg = paged_min(max_wg, (total + min_per - 1) / min_per);
+    l.n_wg = (int)(((unsigned)total + (unsigned)c.min_per - 1) / (unsigned)c.min_per);
+    int part = 8;
+    if (l.n_wg > c.resident) {
+        l.n_wg = paged_max(c.resident, paged_min(c.max_wg, (int)((unsigned)total / (unsigned)c.target)));
+        if (l.n_wg > c.resident) part = 2;
+    }
     l.step = l.n_wg ? (int)((unsigned)total / (unsigned)l.n_wg) : 0;
     l.rest = total - l.step * l.n_wg;
-    l.near = paged_max(paged_max(1, l.step / 8), (uncut + 1) / 2);
+    l.near = paged_max(paged_max(1, l.step / part), (c.uncut + 1) / 2);
 }
 // floor(total * g / n_wg)
 TER_HD int paged_cut_at(const PagedLine& l, int g) {

@@ -69,7 +69,9 @@ int main() {
         for (auto& g : segs) g.start = total, total += g.n;
         CHECK(total == before.back());
         if (!total) continue;
-        paged_cut(l, total, in(1, 600), in(1, 4), in(0, 3) ? 1 : in(2, 20));
+        const int resident = in(1, 600);
+        paged_cut(l, total, {resident * in(1, 4), resident, in(1, 40), in(1, 4), in(0, 3) ? 1 : in(2, 20)});
+        CHECK(l.n_wg >= 1);
         for (int w = 0; w <= l.n_wg; ++w) CHECK(paged_cut_at(l, w) == (long long)total * w / l.n_wg);
         for (int i = 0; i < 20; ++i) {
             const int u = in(0, total);
@@ -107,11 +109,19 @@ int main() {
             }
         }
         for (int w = 0; w < l.n_wg; ++w) {
-            const int u0 = cut(w), u1 = cut(w + 1);
-            CHECK(u0 <= u1);
-            for (int u = u0; u < u1;) {
-                const PagedSegment g = find(u);
-                const int e = paged_min(u1, g.start + g.n);
+            // as the kernel does: from its cut on, segment by segment
+            const int raw0 = paged_cut_at(l, w), raw1 = paged_cut_at(l, w + 1);
+            if (raw0 >= total) continue;
+            PagedSegment g = find(raw0);
+            int u = paged_snap(l, g, raw0);
+            if (u == g.start + g.n) {
+                if (u >= total) continue;
+                g = find(u);
+            }
+            CHECK(u == cut(w));
+            while (u < total) {
+                const int e = raw1 >= g.start + g.n ? g.start + g.n : paged_snap(l, g, raw1);
+                if (e <= u) break;
                 for (int i = u; i < e; ++i) ++done[i];
                 CHECK(u == g.start || u > g.start + kPagedLead);
                 CHECK(e > g.start + kPagedLead);
@@ -121,7 +131,10 @@ int main() {
                     slots[{g.start, w}] = slot;
                 }
                 u = e;
+                if (u < g.start + g.n || u >= total) break;
+                g = find(u);
             }
+            CHECK(u == cut(w + 1));
         }
         for (int d : done) CHECK(d == 1);
         size_t seen = 0;
