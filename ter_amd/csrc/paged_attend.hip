@@ -17,7 +17,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kSolo = 8;  // key tiles up to which a segment of few rows may be one wave's
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -103,11 +102,19 @@ struct Elem<__bf16> {
 // 16 bytes a lane from memory straight to LDS at lds_off + 16 * lane.  Inline
 // asm without outputs: the compiler's own wait insertion would make every LDS
 // read wait for the loads of the next tile; the waits are explicit instead.
+// kOnce: read by nobody else, so not kept in the caches.
+template <bool kOnce>
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned lds_off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(lds_off), "v"(voff), "s"(rsrc)
-                 : "memory");
+    if constexpr (kOnce)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                     :
+                     : "s"(lds_off), "v"(voff), "s"(rsrc)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(lds_off), "v"(voff), "s"(rsrc)
+                     : "memory");
 }
 // Waits until at most N loads are in flight, and for this wave's LDS reads.
 template <int N>
@@ -206,13 +213,11 @@ struct Kernel {
     typedef typename E::v4 v4;
     typedef typename E::v2 v2;
     typedef Tile<HD> L;
-    // Stages of the ring, and workgroups of a CU (by LDS and registers): 64 KB
-    // each and two of them at head_dim 128; 48 KB and three at 64, where a
-    // stage is half as large and more of them have to be in flight.
-    static constexpr int NST = HD == 128 ? 2 : 3;
+    // Two stages of the ring, and the workgroups of a CU that registers (and,
+    // at head_dim 128, LDS) leave room for.  (More stages at head_dim 64 made
+    // no difference: 3 instead of 2, batches of single tokens within 1%.)
     static constexpr int PER_CU = HD == 128 ? 2 : 3;
-    static constexpr int RING = NST * L::BYTES;
-    static __device__ __forceinline__ int after(int stage) { return stage + 1 == NST ? 0 : stage + 1; }
+    static constexpr int RING = 2 * L::BYTES;
     // An offset stays while the largest weight is at most 2^kSlack above its start
     static constexpr float kSlack = 7.f;
 
@@ -276,16 +281,18 @@ struct Kernel {
                     {(unsigned)vb, (unsigned)(vb >> 32) & 0xFFFFu, bytes, 0x00020000u},
                     lds + stage * L::BYTES};
         }
+        template <bool kOnce>
         __device__ __forceinline__ void piece(const PagedAttendArgs& a, const Pending& p, int i) const {
             if (i < L::NI)
-                load_to_lds(p.kr, k_at(a, i), p.to + i * 1024);
+                load_to_lds<kOnce>(p.kr, k_at(a, i), p.to + i * 1024);
             else
-                load_to_lds(p.vr, v_at(a, i - L::NI), p.to + L::V + (i - L::NI) * 1024);
+                load_to_lds<kOnce>(p.vr, v_at(a, i - L::NI), p.to + L::V + (i - L::NI) * 1024);
         }
+        template <bool kOnce>
         __device__ __forceinline__ void issue(const PagedAttendArgs& a, const Groups& g, int at, int stage) const {
             const Pending p = prepare(a, g, at, stage);
 #pragma unroll
-            for (int i = 0; i < 2 * L::NI; ++i) piece(a, p, i);
+            for (int i = 0; i < 2 * L::NI; ++i) piece<kOnce>(a, p, i);
         }
     };
 
@@ -328,7 +335,7 @@ struct Kernel {
                                                    TER_LDS char* ring, const Seqs& sq, int* shared, int& tick,
                                                    int w, int lane) {
         int* const lows = shared;                 // [kWaves]
-        int* const flag = shared + kWaves;        // [NST] the tick at which a tile of a stage held odd values
+        int* const flag = shared + kWaves;        // [2] the tick at which a tile of a stage held odd values
         const int half = lane >> 5, col = lane & 31;
         const int r = 32 * w + col, tok = r / a.group, t = s.tok0 + tok;
         const int h = s.kvh * a.group + (r - tok * a.group);
@@ -372,7 +379,7 @@ struct Kernel {
         const int va = L::V + vr * L::ROW + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) +
                        8 * (lane & 1);
         const auto mine = [&](int j) { return j * kPagedKeys + 16 * w; };
-        // NST - 1 tiles ahead of the one in work
+        // one tile ahead of the one in work
         typename Loader::Groups groups;
         int put = 0, todo = s.j0;
         auto group = [&]() {
@@ -383,29 +390,22 @@ struct Kernel {
         };
         auto fetch = [&]() {
             if (todo < s.j1) {
-                ld.issue(a, groups, group(), put);
-                put = after(put);
+                ld.template issue<false>(a, groups, group(), put);
+                put ^= 1;
             }
         };
-#pragma unroll
-        for (int i = 0; i < NST - 1; ++i) fetch();
+        fetch();
         // The same in pieces, spread over a step: a wave that issues all of
         // them at once waits a quarter of the step for the address unit.
         // (Behind the last tile they load what nobody reads, into a stage that is free.)
         typename Loader::Pending next;
         auto prepare = [&]() {
             next = ld.prepare(a, groups, group(), put);
-            put = after(put);
+            put ^= 1;
         };
         int stage = 0, j = s.j0;
-        auto landed = [&]() {  // this wave's rows of tile j are in LDS
-            if (NST > 2 && j + 1 < s.j1)
-                wait_loads<2 * L::NI>();
-            else
-                wait_loads<0>();
-        };
-        auto arrive = [&]() {
-            landed();
+        auto arrive = [&]() {  // tile j is in LDS
+            wait_loads<0>();
             barrier_only();
         };
         // The same for a tile that some row does not see whole.  Values there
@@ -413,7 +413,7 @@ struct Kernel {
         // are added to the sums of the rows that see them and set to zero in
         // LDS.  Each wave looks at the rows that it loaded.
         auto arrive_masked = [&]() {
-            landed();
+            wait_loads<0>();
             TER_LDS char* const vt = ring + stage * L::BYTES + L::V;
             TER_LDS u32x4* const own = (TER_LDS u32x4*)(vt + w * 16 * L::ROW + lane * 16);
             unsigned odd = 0;
@@ -521,7 +521,7 @@ struct Kernel {
             for (int c = 0; c < HD / 16; ++c) {
                 scores(0, c);
                 read_k(1, c);
-                if (c % 4 == 2) ld.piece(a, next, c / 4);  // NI / 2
+                if (c % 4 == 2) ld.template piece<false>(a, next, c / 4);  // NI / 2
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (decide(0)) rescale();
@@ -532,7 +532,7 @@ struct Kernel {
                 if (i % (128 / HD) == 0) {
                     const int c = i / (128 / HD);
                     scores(1, c);
-                    if (c % 2 == 0) ld.piece(a, next, L::NI / 2 + c / 2);  // NI
+                    if (c % 2 == 0) ld.template piece<false>(a, next, L::NI / 2 + c / 2);  // NI
                     if (c >= HD / 32) read_v(0, c - HD / 32);
                 }
                 weight(0, 2 * i);
@@ -554,7 +554,7 @@ struct Kernel {
                     const int c = i / 4, d = i / (128 / HD) % (HD / 32);
                     value(c, d);
                     read_v(2 + c, d);
-                    if (i % (16 / L::NI) == 2) ld.piece(a, next, L::NI * 3 / 2 + i / (16 / L::NI));  // NI / 2
+                    if (i % (16 / L::NI) == 2) ld.template piece<false>(a, next, L::NI * 3 / 2 + i / (16 / L::NI));  // NI / 2
                 }
                 weight(1, 2 * i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -572,11 +572,11 @@ struct Kernel {
         };
         // tiles that every row sees whole, then the others
         const int full = min(s.j1, max(s.j0, lo / kPagedKeys));
-        for (; j < full; ++j, stage = after(stage)) {
+        for (; j < full; ++j, stage ^= 1) {
             arrive();
             step(std::false_type{});
         }
-        for (; j < s.j1; ++j, stage = after(stage)) {
+        for (; j < s.j1; ++j, stage ^= 1) {
             arrive_masked();
             if (j * kPagedKeys < hi)
                 step(std::true_type{});
@@ -627,13 +627,13 @@ struct Kernel {
         auto fetch = [&]() {
             if (todo < n) {
                 if ((todo & 63) == 0) Loader::locate(groups, a, s, first + todo * stride, stride, lane);
-                ld.issue(a, groups, todo & 63, put);
+                ld.template issue<true>(a, groups, todo & 63, put);
                 ++todo;
-                put = after(put);
+                put ^= 1;
             }
         };
-#pragma unroll
-        for (int i = 0; i < NST; ++i) fetch();
+        fetch();
+        fetch();
         v8 q[HD / 32];
         {
             const char* p = a.q + (live ? (long long)t * a.q_stride + (long long)h * L::ROW : 0) + quad * 16;
@@ -660,11 +660,9 @@ struct Kernel {
         // loop: inside it that wait would be one for all loads in flight.
         wait_loads<0>();
         int stage = 0;
-        for (int i = 0; i < n; ++i, stage = after(stage)) {
+        for (int i = 0; i < n; ++i, stage ^= 1) {
             // the next keys' loads may still be in flight
-            if (NST > 2 && i + 2 < n)
-                wait_loads<4 * L::NI>();
-            else if (i + 1 < n)
+            if (i + 1 < n)
                 wait_loads<2 * L::NI>();
             else
                 wait_loads<0>();
@@ -832,7 +830,7 @@ __device__ __forceinline__ int count_units(const PagedAttendArgs& a, const Paged
         sq.base[i] = s.base;
         if (i == n - 1) sq.row0[n] = min(max(r1, 0), a.b.n_rows);
         sq.before[i] = sum;
-        sum += paged_units(s, l.q, l.kv0) * a.nkv;
+        sum += paged_units(s, l.group, l.q, l.kv0) * a.nkv;
     }
     const int inc = wave_prefix(sum);
     if (lane == 63) tmp[w] = inc;
@@ -853,12 +851,12 @@ template <typename T, int HD>
 __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a) {
     typedef Kernel<T, HD> K;
     extern __shared__ __align__(1024) unsigned char lds[];
-    int* tmp = reinterpret_cast<int*>(lds + K::RING);  // [kWaves + 3]
-    const Seqs sq(tmp + kWaves + 3, a.b.n_seq);
+    int* tmp = reinterpret_cast<int*>(lds + K::RING);  // [kWaves + 2]
+    const Seqs sq(tmp + kWaves + 2, a.b.n_seq);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TER_LDS char* ring = (TER_LDS char*)lds;
 
-    PagedLine l = paged_line(a.tokens_log2, a.shared, a.b.n_rows, a.nkv);
+    PagedLine l = paged_line(a.group, a.tokens_log2, a.shared, a.b.n_rows, a.nkv);
     const int total = count_units(a, l, sq, tmp);
     if (a.shared && blockIdx.x == 0)
         for (int i = threadIdx.x; i <= a.b.n_seq; i += kThreads) gptr(a.before)[i] = sq.before[i];
@@ -882,7 +880,7 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
     typename K::Loader ld;
     ld.init(a, (unsigned)(size_t)ring, w, lane);
     int tick = 0;
-    if (threadIdx.x < K::NST) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
+    if (threadIdx.x < 2) tmp[kWaves + threadIdx.x] = 0;  // (a barrier comes before each segment)
     const int raw1 = paged_cut_at(l, g + 1);
     int u0 = paged_cut_at(l, g);
     PagedSegment sg = segment(u0);
@@ -899,7 +897,7 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         s.seq = sg.seq;
         s.kvh = sg.kvh;
         s.j0 = max(u - sg.start - kPagedLead, 0);
-        s.j1 = end - sg.start - kPagedLead;
+        s.j1 = sg.lead ? end - sg.start - kPagedLead : paged_key_tiles(q, 0, l.q, l.kv0);
         const bool whole = u == sg.start && end == sg.start + sg.n;
         if (sg.seq < 0) {
             s.tok0 = sg.tile << l.q;
@@ -923,7 +921,7 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         const int slot = 2 * g + (u == sg.start ? 1 : 0);
         s.slot = a.slots + (long long)slot * a.slot_rows * HD;
         s.slot_stats = a.slot_stats + (long long)slot * a.slot_rows * 2;
-        if (s.rows <= 16 && s.j1 - s.j0 <= kSolo && (u > u0 || raw1 > end)) {
+        if (sg.lead == 0 && (u > u0 || raw1 > end)) {
             // short ones beside others: the waves take turns, each by itself
             if (turn < 0) __syncthreads();
             turn = (turn + 1) & (kWaves - 1);
@@ -931,13 +929,13 @@ __global__ __launch_bounds__(kThreads, (Kernel<T, HD>::PER_CU)) void paged_atten
         } else {
             turn = -1;
             __syncthreads();  // the ring is free
-            if (s.rows > 16)
+            if (s.rows > kPagedFew)
                 K::rows128(a, s, ld, ring, sq, tmp, tick, w, lane);
             else
                 K::template rows16<false>(a, s, ld, ring, sq, w, lane);
         }
         if (u == u0 && threadIdx.x == 0) {  // what the joining kernel has to know of this cut
-            const PagedParts p = paged_parts(l, sg.start, sg.n);
+            const PagedParts p = paged_parts(l, sg.start, sg.n, sg.lead);
             *gptr(reinterpret_cast<i32x4*>(a.cuts + 8 * g)) = i32x4{u == sg.start ? 0 : s.rows, s.tok0, s.kvh, p.first};
             gptr(a.cuts)[8 * g + 4] = p.last;
         }
@@ -1051,12 +1049,13 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
     if (b < 0) return;
     const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
     const PagedSeq s = paged_seq(rows[b], rows[b + 1], lens[b], a.b.n_rows, a.b.capacity);
-    PagedLine l = paged_line(q, a.shared, a.b.n_rows, a.nkv);
+    PagedLine l = paged_line(a.group, q, a.shared, a.b.n_rows, a.nkv);
     paged_cut(l, before[a.b.n_seq], a.cuts_by);
     const int tile = (t - s.r0) >> q, b0 = before[b], each = (before[b + 1] - b0) / a.nkv;
     const PagedParts own = paged_parts(l, b0 + kvh * each + paged_length_before(s, tile, q, l.kv0),
-                                       paged_length(s, tile, q, l.kv0));
-    const PagedParts pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_length, l.prefix_length);
+                                       paged_length(s, tile, a.group, q, l.kv0),
+                                       paged_solid(s, a.group, q, l.kv0) ? 0 : kPagedLead);
+    const PagedParts pre = paged_parts(l, (kvh * l.prefix_rows + (t >> q)) * l.prefix_length, l.prefix_length, kPagedLead);
     const int n_own = own.last - own.first + 1, n_pre = pre.last - pre.first + 1;
     const int own_row = ((t - s.r0) & ((1 << q) - 1)) * a.group, pre_row = (t & ((1 << q) - 1)) * a.group;
     int S = J::GROUPS;
@@ -1087,9 +1086,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
 template <typename T, int HD>
 hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
-    const int lds = Kernel<T, HD>::RING + (3 * a.b.n_seq + 2 + kWaves + 3) * 4;
+    const int lds = Kernel<T, HD>::RING + (3 * a.b.n_seq + 2 + kWaves + 2) * 4;
     const void* fn = reinterpret_cast<const void*>(&paged_attend_kernel<T, HD>);
-    hipError_t e = limit.allow(Kernel<T, HD>::RING + (3 * TER_HIP_PAGED_SEQ_MAX + 2 + kWaves + 3) * 4, {fn});
+    hipError_t e = limit.allow(Kernel<T, HD>::RING + (3 * TER_HIP_PAGED_SEQ_MAX + 2 + kWaves + 2) * 4, {fn});
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_attend_kernel<T, HD>), dim3(a.cuts_by.max_wg), dim3(kThreads), lds, st, a);
     e = hipGetLastError();

@@ -7,10 +7,11 @@
 // all its key tiles, a unit one key tile of one segment.  All units of a launch
 // form one line,
 //   [ shared prefix: KV head, row tile over all rows ][ sequence, KV head, row tile ],
-// where every segment begins with kPagedLead units of no work: what its start
-// and end cost beside its key tiles (queries and first tiles from memory,
-// results to it) is about as much.  The line
-// is cut into equal ranges, one for each workgroup, whatever the lengths
+// where a segment has kPagedLead units more than key tiles, at its beginning:
+// what its start and end cost beside them (queries and first tiles from memory,
+// results to it) is about as much.  A segment of at most 16 rows and 8 key
+// tiles is never cut, and counts less: one wave does it alone, while others do
+// theirs.  The line is cut into equal ranges, one for each workgroup, whatever the lengths
 // are: a long sequence is spread over many workgroups, many short ones share
 // one.  A cut close to a segment's edge is moved there.  A segment that is cut
 // leaves one partial result in each range that holds a part of it; they
@@ -32,6 +33,8 @@ namespace terhip {
 constexpr int kPagedKeys = 64;   // positions of a key tile
 constexpr int kPagedRows = 128;  // rows of a row tile
 constexpr int kPagedLead = 3;
+constexpr int kPagedFew = 16;    // rows and key tiles of a segment that is never cut
+constexpr int kPagedShort = 8;
 
 TER_HD int paged_min(int a, int b) { return a < b ? a : b; }
 TER_HD int paged_max(int a, int b) { return a > b ? a : b; }
@@ -80,16 +83,21 @@ TER_HD int paged_key_tiles_before(const PagedSeq& s, int n, int q, int kv0) {
     return (int)((unsigned)ones + (((a1 * (a1 + 1) / 2) << lr) + (x1 & r) * (a1 + 1)) -
                  (((a0 * (a0 + 1) / 2) << lr) + (x0 & r) * (a0 + 1)));
 }
+// Whether the only segment of a sequence and KV head is one that is never cut.
+TER_HD bool paged_solid(const PagedSeq& s, int group, int q, int kv0) {
+    return s.n * group <= kPagedFew && s.n <= 1 << q && paged_key_tiles(s, 0, q, kv0) <= kPagedShort;
+}
 // Units of a segment, of the row tiles before it, of a sequence for one KV head.
-TER_HD int paged_length(const PagedSeq& s, int rt, int q, int kv0) {
-    return kPagedLead + paged_key_tiles(s, rt, q, kv0);
+TER_HD int paged_length(const PagedSeq& s, int rt, int group, int q, int kv0) {
+    const int n = paged_key_tiles(s, rt, q, kv0);
+    return paged_solid(s, group, q, kv0) ? 1 + (n + 1) / 2 : kPagedLead + n;
 }
 TER_HD int paged_length_before(const PagedSeq& s, int n, int q, int kv0) {
     return n * kPagedLead + paged_key_tiles_before(s, n, q, kv0);
 }
-TER_HD int paged_units(const PagedSeq& s, int q, int kv0) {
+TER_HD int paged_units(const PagedSeq& s, int group, int q, int kv0) {
     const int t = paged_row_tiles(s, q);
-    return t ? paged_length_before(s, t - 1, q, kv0) + paged_length(s, t - 1, q, kv0) : 0;
+    return t ? paged_length_before(s, t - 1, q, kv0) + paged_length(s, t - 1, group, q, kv0) : 0;
 }
 // The row tile that holds unit r of a sequence and KV head.
 TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
@@ -107,7 +115,7 @@ TER_HD int paged_row_tile_of(const PagedSeq& s, int r, int q, int kv0) {
 // One launch's line of units.  The ranges: workgroup g of n_wg takes the units
 // from cut g to cut g + 1, cut g being at or near total * g / n_wg.
 struct PagedLine {
-    int q, kv0;                // row tile, first position behind the prefix
+    int group, q, kv0;         // query heads of a KV head, row tile, first position behind the prefix
     int prefix_length;         // units of a row tile on the prefix
     int prefix_rows;           // row tiles over all rows
     int prefix_units;          // of all KV heads
@@ -115,8 +123,9 @@ struct PagedLine {
     int n_wg, near;            // ranges; cuts closer than `near` to an edge move there
     int step, rest;            // total = step * n_wg + rest
 };
-TER_HD PagedLine paged_line(int q, int shared, int n_rows, int nkv) {
+TER_HD PagedLine paged_line(int group, int q, int shared, int n_rows, int nkv) {
     PagedLine l{};
+    l.group = group;
     l.q = q;
     l.kv0 = shared;
     l.prefix_length = shared ? kPagedLead + (shared + kPagedKeys - 1) / kPagedKeys : 0;
@@ -160,6 +169,7 @@ struct PagedSegment {
     int start, n;   // first unit, units
     int seq;        // -1: the prefix
     int kvh, tile;  // KV head, row tile
+    int lead;       // units before its first key tile (0: never cut)
 };
 
 // The segment of unit u (0 <= u < total): b is the first sequence with units
@@ -174,6 +184,7 @@ TER_HD PagedSegment paged_segment(const PagedLine& l, int u, int nkv, int b, con
         g.tile = (int)i - g.kvh * l.prefix_rows;
         g.start = (int)i * l.prefix_length;
         g.n = l.prefix_length;
+        g.lead = kPagedLead;
         return g;
     }
     const int each = (int)((unsigned)(b1 - b0) / (unsigned)nkv), at = u - b0;
@@ -182,7 +193,8 @@ TER_HD PagedSegment paged_segment(const PagedLine& l, int u, int nkv, int b, con
     const int r = at - g.kvh * each;
     g.tile = paged_row_tile_of(s, r, l.q, l.kv0);
     g.start = b0 + g.kvh * each + paged_length_before(s, g.tile, l.q, l.kv0);
-    g.n = paged_length(s, g.tile, l.q, l.kv0);
+    g.n = paged_length(s, g.tile, l.group, l.q, l.kv0);
+    g.lead = paged_solid(s, l.group, l.q, l.kv0) ? 0 : kPagedLead;
     return g;
 }
 // To the segment behind g where that is of the same sequence s (or of the
@@ -196,14 +208,15 @@ TER_HD bool paged_advance(const PagedLine& l, PagedSegment& g, const PagedSeq& s
     else
         return false;
     g.start += g.n;
-    if (g.seq >= 0) g.n = paged_length(s, g.tile, l.q, l.kv0);
+    if (g.seq >= 0) g.n = paged_length(s, g.tile, l.group, l.q, l.kv0);
     return true;
 }
 
 // Where a cut at unit u of segment g goes.
 TER_HD int paged_snap(const PagedLine& l, const PagedSegment& g, int u) {
     const int off = u - g.start;
-    return off < kPagedLead + l.near ? g.start : g.n - off < l.near ? g.start + g.n : u;
+    if (g.lead == 0) return 2 * off < g.n ? g.start : g.start + g.n;
+    return off < g.lead + l.near ? g.start : g.n - off < l.near ? g.start + g.n : u;
 }
 
 // The ranges that hold parts of a segment: first .. last, one if it is not cut.
@@ -212,8 +225,12 @@ TER_HD int paged_snap(const PagedLine& l, const PagedSegment& g, int u) {
 struct PagedParts {
     int first, last;
 };
-TER_HD PagedParts paged_parts(const PagedLine& l, int start, int n) {
+TER_HD PagedParts paged_parts(const PagedLine& l, int start, int n, int lead) {
     PagedParts p;
+    if (lead == 0) {
+        p.first = p.last = 0;
+        return p;
+    }
     // cuts from start + lead + near to start + n - near stay inside
     const int c0 = paged_cut_from(l, start + kPagedLead + l.near), c1 = paged_cut_from(l, start + n - l.near + 1) - 1;
     p.first = c0 - 1;

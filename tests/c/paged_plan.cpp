@@ -38,13 +38,13 @@ int main() {
         }
         const int n_rows = paged_max(0, in(0, 9) ? row0.back() : row0.back() - in(0, 5)) + (in(0, 5) ? 0 : 3);
         const int shared = in(0, 2) ? 0 : 16 * in(0, cap / 16);
-        PagedLine l = paged_line(q, shared, n_rows, nkv);
+        PagedLine l = paged_line(group, q, shared, n_rows, nkv);
         // plain counting
         std::vector<int> before(1, l.prefix_units);
         std::vector<PagedSegment> segs;
         for (int h = 0; h < nkv && shared; ++h)
             for (int t = 0; t < (n_rows + (1 << q) - 1) >> q; ++t)
-                segs.push_back({0, kPagedLead + (shared + 63) / 64, -1, h, t});
+                segs.push_back({0, kPagedLead + (shared + 63) / 64, -1, h, t, kPagedLead});
         for (int b = 0; b < n_seq; ++b) {
             const PagedSeq s = paged_seq(row0[b], row0[b + 1], len[b], n_rows, cap);
             CHECK(s.r0 >= 0 && s.n >= 0 && s.r0 + s.n <= n_rows);
@@ -57,12 +57,14 @@ int main() {
                 CHECK(n >= 1 && n * 64 >= see);
                 if (s.base + last + 1 <= cap) CHECK(n == paged_max(1, (see + 63) / 64));
                 CHECK(paged_length_before(s, tiles, q, shared) == units);
-                CHECK(paged_length(s, tiles, q, shared) == n + kPagedLead);
-                units += n + kPagedLead;
+                const bool solid = s.n * group <= 16 && tiles == 0 && i + (1 << q) >= s.n && n <= 8;
+                CHECK(paged_length(s, tiles, group, q, shared) == (solid ? 1 + (n + 1) / 2 : n + kPagedLead));
+                CHECK(solid == paged_solid(s, group, q, shared));
+                units += solid ? 1 + (n + 1) / 2 : n + kPagedLead;
             }
-            CHECK(tiles == paged_row_tiles(s, q) && units == paged_units(s, q, shared));
+            CHECK(tiles == paged_row_tiles(s, q) && units == paged_units(s, group, q, shared));
             for (int h = 0; h < nkv; ++h)
-                for (int t = 0; t < tiles; ++t) segs.push_back({0, paged_length(s, t, q, shared), b, h, t});
+                for (int t = 0; t < tiles; ++t) segs.push_back({0, paged_length(s, t, group, q, shared), b, h, t, paged_solid(s, group, q, shared) ? 0 : kPagedLead});
             before.push_back(before.back() + units * nkv);
         }
         int total = 0;
@@ -97,13 +99,13 @@ int main() {
             if (in(0, 3) && u != segs[k].start) continue;
             const PagedSegment g = find(u);
             CHECK(g.start == segs[k].start && g.n == segs[k].n && g.seq == segs[k].seq && g.kvh == segs[k].kvh &&
-                  g.tile == segs[k].tile);
+                  g.tile == segs[k].tile && g.lead == segs[k].lead);
             PagedSegment next = g;
             const PagedSeq s = g.seq < 0 ? PagedSeq{} : paged_seq(row0[g.seq], row0[g.seq + 1], len[g.seq], n_rows, cap);
             if (paged_advance(l, next, s, nkv)) {
                 const PagedSegment& m = segs[k + 1];
                 CHECK(next.start == m.start && next.n == m.n && next.seq == m.seq && next.kvh == m.kvh &&
-                      next.tile == m.tile);
+                      next.tile == m.tile && next.lead == m.lead);
             } else {
                 CHECK(k + 1 == segs.size() || segs[k + 1].seq != g.seq);
             }
@@ -124,7 +126,7 @@ int main() {
                 if (e <= u) break;
                 for (int i = u; i < e; ++i) ++done[i];
                 CHECK(u == g.start || u > g.start + kPagedLead);
-                CHECK(e > g.start + kPagedLead);
+                CHECK(e > g.start + g.lead && (g.lead || (u == g.start && e == u + g.n)));
                 if (u > g.start || e < g.start + g.n) {
                     const int slot = u == g.start ? 2 * w + 1 : 2 * w;
                     CHECK(used.insert(slot).second);
@@ -139,7 +141,7 @@ int main() {
         for (int d : done) CHECK(d == 1);
         size_t seen = 0;
         for (auto& g : segs) {
-            const PagedParts p = paged_parts(l, g.start, g.n);
+            const PagedParts p = paged_parts(l, g.start, g.n, g.lead);
             if (p.first == p.last) {
                 CHECK(!slots.count({g.start, p.first}));
                 continue;
