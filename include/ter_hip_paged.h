@@ -26,7 +26,8 @@
  *     attend reads zeros as its keys and values;
  *   - rows at positions below 0 (kv_len[b] less than the rows given): append
  *     leaves them, attend writes zeros.
- * row0 must not decrease.  Two rows of one call must not have the same page
+ * row0 must not decrease (where it does, results of the rows concerned are
+ * undefined; accesses stay in bounds).  Two rows of one call must not have the same page
  * and slot (append); pages may be shared between sequences for reading.
  */
 #ifndef TER_HIP_PAGED_H

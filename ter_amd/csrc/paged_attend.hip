@@ -804,12 +804,13 @@ struct Kernel {
 };
 
 template <int kCtrl, int kRows>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false);
+__device__ __forceinline__ unsigned dpp_add(unsigned v) {
+    return __builtin_elementwise_add_sat(
+        v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, false));
 }
-// Inclusive prefix sum over the wave: within rows of 16 lanes, then the last
-// lanes of the rows before.
-__device__ __forceinline__ int wave_prefix(int v) {
+// Inclusive prefix sum over the wave, saturating: within rows of 16 lanes, then
+// the last lanes of the rows before.
+__device__ __forceinline__ unsigned wave_prefix(unsigned v) {
     v = dpp_add<0x111, 0xF>(v);  // row_shr:1
     v = dpp_add<0x112, 0xF>(v);
     v = dpp_add<0x114, 0xF>(v);
@@ -818,33 +819,35 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return dpp_add<0x143, 0xC>(v);  // row_bcast:31
 }
 
-// Fills sq; returns the units of the whole line.
+// Fills sq; returns the units of the whole line.  They fit 31 bits if row0 does
+// not decrease; a batch whose sequences overlap may have more: then none is done.
 __device__ __forceinline__ int count_units(const PagedAttendArgs& a, const PagedLine& l, const Seqs& sq, int* tmp) {
     const int n = a.b.n_seq, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int each = (n + kThreads - 1) / kThreads, i0 = tid * each, i1 = min(n, i0 + each);
-    int sum = 0;
+    unsigned sum = 0;
     for (int i = i0; i < i1; ++i) {
         const int r0 = gptr(a.b.row0)[i], r1 = gptr(a.b.row0)[i + 1];
         const PagedSeq s = paged_seq(r0, r1, gptr(a.b.kv_len)[i], a.b.n_rows, a.b.capacity);
         sq.row0[i] = s.r0;
         sq.base[i] = s.base;
         if (i == n - 1) sq.row0[n] = min(max(r1, 0), a.b.n_rows);
-        sq.before[i] = sum;
-        sum += paged_units(s, l.group, l.q, l.kv0) * a.nkv;
+        sq.before[i] = (int)sum;
+        sum = __builtin_elementwise_add_sat(sum, (unsigned)(paged_units(s, l.group, l.q, l.kv0) * a.nkv));
     }
-    const int inc = wave_prefix(sum);
-    if (lane == 63) tmp[w] = inc;
+    const unsigned inc = wave_prefix(sum);
+    if (lane == 63) tmp[w] = (int)inc;
     __syncthreads();
-    int add = l.prefix_units + inc - sum, total = l.prefix_units;
+    unsigned add = l.prefix_units + inc - sum, total = l.prefix_units;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-        if (k < w) add += tmp[k];
-        total += tmp[k];
+        if (k < w) add += (unsigned)tmp[k];
+        total = __builtin_elementwise_add_sat(total, (unsigned)tmp[k]);
     }
-    for (int i = i0; i < i1; ++i) sq.before[i] += add;
-    if (tid == 0) sq.before[n] = total;
+    if (total > 0x7FFFFFFFu) total = 0;
+    for (int i = i0; i < i1; ++i) sq.before[i] += (int)add;
+    if (tid == 0) sq.before[n] = (int)total;
     __syncthreads();
-    return __builtin_amdgcn_readfirstlane(total);
+    return __builtin_amdgcn_readfirstlane((int)total);
 }
 
 template <typename T, int HD>
@@ -1050,7 +1053,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
     const ConstInts rows{a.b.row0}, lens{a.b.kv_len}, before{a.before};
     const PagedSeq s = paged_seq(rows[b], rows[b + 1], lens[b], a.b.n_rows, a.b.capacity);
     PagedLine l = paged_line(a.group, q, a.shared, a.b.n_rows, a.nkv);
-    paged_cut(l, before[a.b.n_seq], a.cuts_by);
+    const int total = before[a.b.n_seq];
+    if (t - s.r0 >= s.n || total == 0) return;  // (row0 decreases somewhere)
+    paged_cut(l, total, a.cuts_by);
     const int tile = (t - s.r0) >> q, b0 = before[b], each = (before[b + 1] - b0) / a.nkv;
     const PagedParts own = paged_parts(l, b0 + kvh * each + paged_length_before(s, tile, q, l.kv0),
                                        paged_length(s, tile, a.group, q, l.kv0),

@@ -159,6 +159,33 @@ def test_refusals(fake):
     """)
 
 
+def test_refusals_of_size(fake):
+    """More work than units are counted in; a scale that is no number once
+    multiplied by log2(e); a workspace for another call."""
+    fake("""
+    x = context(128, 1, 64)
+    c = cache(page_stride=4096 * 64, pos_stride=64, head_stride=64, page_size=4096)
+    b = batch(n_seq=1024, max_pages=256, pages_stride=256)
+    kw = dict(qs=128 * 64, os=128 * 64)
+    assert attend(x, b, c, n=L.PAGED_ROWS_MAX, **kw) == L.ERR_SHAPE and b"too many" in lib.ter_hip_last_error()
+    assert not any(l.startswith("launch") for l in log())
+    assert attend(x, b, c, n=1024, **kw) == 0
+    for scale in (1e39, 2e38, -0.5):
+        assert attend(h, batch(), cache(), scale=scale) == L.ERR_SHAPE
+    assert attend(h, batch(), cache(), scale=1e38) == 0
+    log()
+    small = lib.ter_hip_paged_attend_ws(h, C.byref(batch()), C.byref(cache()), 7, 0)
+    large = lib.ter_hip_paged_attend_ws(h, C.byref(batch()), C.byref(cache()), 7, 16)
+    assert 0 < small < large
+    assert attend(h, batch(), cache(), shared=16, nb=small) == L.ERR_SHAPE
+    assert attend(h, batch(), cache(), shared=15, nb=small) == 0
+    for bad in (dict(n=-1), dict(n=0), dict(n=1 << 20), dict(shared=-1)):
+        a = dict(n=7, shared=0)
+        a.update(bad)
+        assert lib.ter_hip_paged_attend_ws(h, C.byref(batch()), C.byref(cache()), a["n"], a["shared"]) == 0
+    """)
+
+
 def test_launches_and_errors(fake):
     """Nothing to do launches nothing; a failed launch is reported; another
     device than the context's is refused."""

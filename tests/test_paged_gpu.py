@@ -120,6 +120,68 @@ def test_masked_infinities_and_nan(cuda):
         compare(out[57:99][:, :, keep], want[57:99][:, :, keep], tol[57:99][:, :, keep], "other elements")
 
 
+@pytest.mark.parametrize("shared", [0, 16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_masked_nan_of_few_rows(cuda, hd, shared):
+    """The same where a sequence has few rows, short ones among long: keys and
+    values of every sequence's last position are NaN, which its last row only
+    sees."""
+    import ter_amd as T
+    seqs = [(3, 20), (2, 33), (4, 700), (5, 290), (2, 18), (1, 40), (16, 64)]
+    b = Batch(seqs, hd=hd, nh=2, nkv=2, common=16, seed=4)
+    want, tol = b.attend()
+    for s, n in enumerate(b.lens):
+        b.k[b.table[s, (n - 1) // 16], (n - 1) % 16] = math.nan
+        b.v[b.table[s, (n - 1) // 16], (n - 1) % 16] = math.nan
+    cache, batch = b.on_device(T)
+    out = context(b).attend(b.q.cuda(), cache, batch, shared=shared).cpu()
+    for s in range(len(seqs)):
+        at, end = int(b.first[s]), int(b.first[s + 1]) - 1
+        compare(out[at:end], want[at:end], tol[at:end], f"sequence {s}")
+        assert torch.isnan(out[end]).all()
+
+
+@pytest.mark.parametrize("nh,nkv,seqs", [(128, 1, [(1, 5000), (3, 900)]), (17, 1, [(1, 6000), (9, 1500)]),
+                                         (6, 2, [(2, 9000), (1, 10), (1, 30)])])
+def test_long_sequences_of_few_rows(cuda, nh, nkv, seqs):
+    """Cut among many workgroups, groups of every size."""
+    check_attend(Batch(seqs, nh=nh, nkv=nkv, page=64, dtype=BF16, seed=nh))
+
+
+@pytest.mark.parametrize("shared", [0, 32])
+def test_row0_that_decreases(cuda, shared):
+    """Not allowed, and without a meaning for the rows it confuses; the others
+    are right and nothing else is written."""
+    import ter_amd as T
+    b = Batch([(4, 40), (4, 50), (4, 60), (4, 70)], common=32, spare_rows=6)
+    cache, batch = b.on_device(T)
+    wild = T.PagedBatch(torch.tensor([0, 4, 12, 7, 16], dtype=torch.int32, device="cuda"), batch.kv_len, batch.pages)
+    out = torch.full((b.t, b.nh, b.hd), 7.0, dtype=b.dtype, device="cuda")
+    ctx = context(b)
+    ctx.attend(b.q.cuda(), cache, wild, shared=shared, out=out)
+    want, tol = b.attend()
+    compare(out[:4], want[:4], tol[:4])
+    assert (out[16:] == 7.0).all()
+    k = torch.zeros(b.t, b.nkv, b.hd, dtype=b.dtype, device="cuda")
+    ctx.append(None, k, k, cache, wild)
+    torch.cuda.synchronize()
+
+
+def test_overlapping_sequences_beyond_counting(cuda):
+    """The same with more work than a call can have: none is done."""
+    import ter_amd as T
+    n = 1024
+    kd = torch.zeros(1, 4096, 1, 64, dtype=F16, device="cuda")
+    row0 = torch.tensor([0, n] * 512 + [0], dtype=torch.int32, device="cuda")
+    batch = T.PagedBatch(row0, torch.full((1024,), 1 << 20, dtype=torch.int32, device="cuda"),
+                         torch.zeros(1024, 256, dtype=torch.int32, device="cuda"))
+    out = torch.full((n, 128, 64), 7.0, dtype=F16, device="cuda")
+    for shared in (0, 4096):
+        T.PagedAttention(128, 1, 64, 16, THETA).attend(torch.zeros_like(out), T.PagedCache(kd, kd), batch, shared=shared,
+                                                       out=out)
+        assert (out == 7.0).all()
+
+
 def test_peaked_and_flat_scores(cuda):
     """Scores so far apart that all but one weight vanishes, growing along the
     sequence (the running maximum moves at every step), and all equal."""
