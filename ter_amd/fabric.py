@@ -667,11 +667,9 @@ class PagedAttention:
             if q_out is None:
                 q_out = self._empty(n, stream)
             os = self._rows(q_out, self.n_heads, n, "q_out")
-        with _Device(self._dev):
-            rc = L.lib().ter_hip_paged_append(self._h, batch._ref, cache._ref, n, *(
-                (None, 0) if q is None else (q.data_ptr(), qs)), k.data_ptr(), ks, v.data_ptr(), vs, *(
-                (None, 0) if q is None else (q_out.data_ptr(), os)), _stream(stream))
-        L.check(rc, "ter_hip_paged_append")
+        self._launch("ter_hip_paged_append", stream, self._h, batch._ref, cache._ref, n, *(
+            (None, 0) if q is None else (q.data_ptr(), qs)), k.data_ptr(), ks, v.data_ptr(), vs, *(
+            (None, 0) if q is None else (q_out.data_ptr(), os)))
         return q_out
 
     def attend(self, q, cache: PagedCache, batch: PagedBatch, shared: int = 0, scale: Optional[float] = None, out=None,
@@ -688,24 +686,37 @@ class PagedAttention:
         if out is None:
             out = self._empty(n, stream)
         os = self._rows(out, self.n_heads, n, "out")
-        lib = L.lib()
-        need = lib.ter_hip_paged_attend_ws(self._h, batch._ref, cache._ref, n, shared)
+        need = L.lib().ter_hip_paged_attend_ws(self._h, batch._ref, cache._ref, n, shared)
         # a workspace of its own for every call, from the allocator of the
         # stream (or graph) that runs it
         ws = self._empty(need, stream, True) if need else None
-        with _Device(self._dev):
-            rc = lib.ter_hip_paged_attend(self._h, batch._ref, cache._ref, n, q.data_ptr(), qs, out.data_ptr(), os,
-                                          shared, scale or 0.0, _ptr(ws), need, _stream(stream))
-        L.check(rc, "ter_hip_paged_attend")
+        self._launch("ter_hip_paged_attend", stream, self._h, batch._ref, cache._ref, n, q.data_ptr(), qs,
+                     out.data_ptr(), os, shared, scale or 0.0, _ptr(ws), need)
         return out
 
     def _empty(self, n: int, stream, raw: bool = False):
         torch = _torch()
-        shape, dtype = (n, torch.uint8) if raw else ((n, self.n_heads, self.head_dim), self.dtype)
-        if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self._dev)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self._dev)):
-            return torch.empty(shape, dtype=dtype, device=self._dev)
+        if stream is not None:
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self._dev)):
+                return self._empty(n, None, raw)
+        # (sizes one by one: as a tuple they take 0.4 us more)
+        if raw:
+            return torch.empty(n, dtype=torch.uint8, device=self._dev)
+        return torch.empty(n, self.n_heads, self.head_dim, dtype=self.dtype, device=self._dev)
+
+    def _launch(self, name: str, stream, *args):
+        """Calls the function on the context's device and its current stream,
+        or the given one."""
+        torch, fn = _torch(), getattr(L.lib(), name)
+        was = torch._C._cuda_getDevice()
+        if was != self._dev:
+            torch.cuda.set_device(self._dev)
+        try:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev) if stream is None else stream)
+        finally:
+            if was != self._dev:
+                torch.cuda.set_device(was)
+        L.check(rc, name)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -717,26 +728,6 @@ class PagedAttention:
             self.close()
         except Exception:
             pass
-
-
-class _Device:
-    """Makes a device current where it is not (launches go to the current one)."""
-
-    __slots__ = ("dev", "was")
-
-    def __init__(self, dev: int):
-        self.dev = dev
-
-    def __enter__(self):
-        torch = _torch()
-        was = torch._C._cuda_getDevice()
-        self.was = was if was != self.dev else None
-        if self.was is not None:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *_):
-        if self.was is not None:
-            _torch().cuda.set_device(self.was)
 
 
 def _held(it: dict) -> list:
