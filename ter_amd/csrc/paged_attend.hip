@@ -983,8 +983,9 @@ struct Join {
                 f32x2 st[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
+                    if (i0 + u * S >= n) break;
                     const float *ps, *pt;
-                    place(min(i0 + u * S, n - 1), ps, pt);
+                    place(i0 + u * S, ps, pt);
                     v[u] = *gptr(reinterpret_cast<const f32x4*>(ps + e));
                     st[u] = *gptr(reinterpret_cast<const f32x2*>(pt));
                 }
