@@ -1121,6 +1121,14 @@ PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_
                                  (shared ? tiles * (kPagedLead + 1 + shared / kPagedKeys) : 0));
     PagedCuts& c = p.cuts_by;
     c.resident = (hd == 128 ? Kernel<_Float16, 128>::PER_CU : Kernel<_Float16, 64>::PER_CU) * cus;
+    // Rows that keep the matrix cores busy, one at a time: prompts of a batch
+    // 124 us with equal ranges, 118 so, prompts among single tokens 79 and 75.
+    // Single tokens alone share the memory evenly: 87 us with equal ranges, 90
+    // so.  (With a prefix the joining kernel, in which each row looks for its
+    // ranges, loses more than this gains: 37 and 39 us.)
+    c.rounds = c.resident / cus;
+    c.round = cus / 8;
+    c.skew = cus % 8 == 0 && !shared && (int64_t)n_rows * group > kPagedFew * n_seq ? (hd == 128 ? 3 : 2) : 0;
     c.min_per = 2;
     c.target = 96;
     c.uncut = capacity + n_rows <= 512 ? 9 : 1;

@@ -121,7 +121,7 @@ struct PagedLine {
     int prefix_units;          // of all KV heads
     int total;
     int n_wg, near;            // ranges; cuts closer than `near` to an edge move there
-    int step, rest;            // total = step * n_wg + rest
+    int skew, rounds, round;   // 0: equal ranges; else PagedCuts::skew, workgroups of a CU, CUs of an XCD
 };
 TER_HD PagedLine paged_line(int group, int q, int shared, int n_rows, int nkv) {
     PagedLine l{};
@@ -141,6 +141,7 @@ TER_HD PagedLine paged_line(int group, int q, int shared, int n_rows, int nkv) {
 // segments of fewer key tiles are never cut.
 struct PagedCuts {
     int max_wg, resident, target, min_per, uncut;
+    int skew, rounds, round;
 };
 TER_HD void paged_cut(PagedLine& l, int total, const PagedCuts& c) {
     l.total = total;
@@ -150,19 +151,39 @@ TER_HD void paged_cut(PagedLine& l, int total, const PagedCuts& c) {
         l.n_wg = paged_max(c.resident, paged_min(c.max_wg, (int)((unsigned)total / (unsigned)c.target)));
         if (l.n_wg > c.resident) part = 2;
     }
-    l.step = l.n_wg ? (int)((unsigned)total / (unsigned)l.n_wg) : 0;
-    l.rest = total - l.step * l.n_wg;
-    l.near = paged_max(paged_max(1, l.step / part), (c.uncut + 1) / 2);
+    const int step = l.n_wg ? (int)((unsigned)total / (unsigned)l.n_wg) : 0;
+    l.near = paged_max(paged_max(1, step / part), (c.uncut + 1) / 2);
+    l.skew = l.n_wg == c.resident && step >= 4 ? c.skew : 0;  // (so that no range is empty)
+    l.rounds = c.rounds;
+    l.round = c.round;
 }
-// floor(total * g / n_wg)
+// Sixteenths of a mean range before range g.
+TER_HD int paged_share_before(const PagedLine& l, int g) {
+    if (!l.skew) return 16 * g;
+    const int chunk = l.rounds * l.round, x = (int)((unsigned)g / (unsigned)chunk), y = g - x * chunk;
+    const int r = (int)((unsigned)y / (unsigned)l.round), i = y - r * l.round;
+    return 16 * g + l.skew * (r * (l.rounds - r) * l.round + (l.rounds - 1 - 2 * r) * i);
+}
+// floor(total * share before g / all shares).  (In binary64 exactly: the
+// quotient is below 2^31, and at least 2^-16 off an integer if it is none.)
 TER_HD int paged_cut_at(const PagedLine& l, int g) {
-    return l.step * g + (int)((unsigned)(l.rest * g) / (unsigned)l.n_wg);
+    return (int)((double)l.total * paged_share_before(l, g) / (16 * l.n_wg));
 }
-// The first cut at unit u or behind it: ceil(u * n_wg / total).  (In binary64
-// exactly: the quotient is below 2^11, and at least 2^-31 off an integer if it
-// is none.)
+// The first cut at unit u or behind it: with at least ceil(u * all shares /
+// total) before it.  (Exactly: below 2^16, at least 2^-31 off an integer.)
 TER_HD int paged_cut_from(const PagedLine& l, int u) {
-    return u <= 0 ? 0 : (int)__builtin_ceil((double)u * l.n_wg / l.total);
+    if (u <= 0) return 0;
+    const int a = (int)__builtin_ceil((double)u * (16 * l.n_wg) / l.total);
+    if (!l.skew) return (a + 15) / 16;
+    const int chunk = l.rounds * l.round, x = (int)((unsigned)a / (unsigned)(16 * chunk));
+    int at = a - 16 * chunk * x, g = x * chunk;
+    for (int r = 0; r < l.rounds; ++r) {
+        const int w = 16 + l.skew * (l.rounds - 1 - 2 * r);
+        if (at <= w * l.round) return g + (at + w - 1) / w;
+        at -= w * l.round;
+        g += l.round;
+    }
+    return g;
 }
 
 struct PagedSegment {

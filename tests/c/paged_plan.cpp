@@ -71,13 +71,24 @@ int main() {
         for (auto& g : segs) g.start = total, total += g.n;
         CHECK(total == before.back());
         if (!total) continue;
-        const int resident = in(1, 600);
-        paged_cut(l, total, {resident * in(1, 4), resident, in(1, 40), in(1, 4), in(0, 3) ? 1 : in(2, 20)});
+        // (with a skew: workgroups of CUs in rounds, 8 times as many)
+        const int skew = in(0, 1) ? in(1, 3) : 0, rounds = in(1, 4), round = in(1, 20);
+        const int resident = skew ? 8 * rounds * round : in(1, 600);
+        paged_cut(l, total, {resident * in(1, 4), resident, in(1, 40), in(1, 4), in(0, 3) ? 1 : in(2, 20), skew, rounds,
+                             round});
         CHECK(l.n_wg >= 1);
-        for (int w = 0; w <= l.n_wg; ++w) CHECK(paged_cut_at(l, w) == (long long)total * w / l.n_wg);
+        std::vector<long long> share(1, 0);
+        for (int w = 0; w < l.n_wg; ++w) {
+            const int r = w / round % rounds;
+            share.push_back(share.back() + 16 + (skew && l.n_wg == resident && total >= 4 * resident ? skew * (rounds - 1 - 2 * r) : 0));
+        }
+        CHECK(share.back() == 16 * l.n_wg);
+        for (int w = 0; w <= l.n_wg; ++w) CHECK(paged_cut_at(l, w) == total * share[w] / share.back());
         for (int i = 0; i < 20; ++i) {
             const int u = in(0, total);
-            CHECK(paged_cut_from(l, u) == ((long long)u * l.n_wg + total - 1) / total);
+            int w = 0;
+            while (total * share[w] < u * share.back()) ++w;
+            CHECK(paged_cut_from(l, u) == w);
         }
         // the device's way: each range by itself
         std::vector<int> done(total, 0);
