@@ -8,6 +8,23 @@
 // binary32 with an o near minus the largest x so far; where that grows by
 // enough, sums are multiplied by 2^(new o - old o).  Partial results (sums and
 // their o) of different ranges of positions are joined the same way.
+//
+// Weights are rounded to the element type for the second product (half a step
+// of it each, as the inputs are); scores, sums and statistics stay binary32.
+//
+// What bounds it, on an MI355X whose large copies run at 4.85 TB/s and whose
+// large matrix products at 1,150 (fp16) to 1,210 (bf16) TFLOP/s:
+//   single tokens: memory.  96 sequences of up to 4,095 positions (32 heads on
+//     8 of 64, 421 MB of keys and values) 84 us, 5.0 TB/s; one sequence of
+//     65,521 positions (20 on 5 of 128, 168 MB) 33 us, 5.1 TB/s, and 7 to join.
+//   prompts: a SIMD's matrix and vector work, which overlap in part only (two
+//     waves that alternate them take the matrix time and 0.4 of the vector
+//     time).  One prompt of 16,384 tokens (20 on 5 of 128, bf16) 1.49 ms, 924
+//     TFLOP/s, the matrix cores busy 44% of the cycles at the 1.7 GHz that this
+//     load runs at.  A workgroup of 256 rows, twice the rows a wave and half
+//     the LDS reads a product, took 1.70 ms: one wave a SIMD hides less.
+//   small calls: latency.  A workgroup needs 3 to 5 us to find its range and
+//     have its first tiles, two launches 9 us of the host.
 #include "common.h"
 #include "paged.h"
 #include "paged_plan.h"
