@@ -237,6 +237,10 @@ struct Kernel {
     static constexpr int RING = 2 * L::BYTES;
     // An offset stays while the largest weight is at most 2^kSlack above its start
     static constexpr float kSlack = 7.f;
+    // The offset while all scores are -infinity (masked or not): their weights
+    // are zero with any finite one, and with this one a partial result without
+    // another score counts for nothing beside one that has some.
+    static constexpr float kNoScore = 3e38f;
 
     // ---- loads: wave w takes rows 16 w .. 16 w + 15 of K and V
     struct Loader {
@@ -385,7 +389,7 @@ struct Kernel {
         for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-        float l = 0.f, top = -__builtin_inff(), off = 0.f;
+        float l = 0.f, top = -__builtin_inff(), off = kNoScore;
 
         // LDS offsets: K pieces of row col (+ 32 by offset); V rows of the
         // lane's transposing read
@@ -504,7 +508,7 @@ struct Kernel {
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[b][i]);
                 mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
                 if (__ballot(mx > top + kSlack)) {
-                    const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
+                    const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? kNoScore : E::kOffset - nt;
                     al = top == -__builtin_inff() ? 1.f : shrink(no - off);
                     top = nt;
                     off = no;
@@ -665,7 +669,7 @@ struct Kernel {
         f32x4 o[HD / 16];
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float l = 0.f, top = -__builtin_inff(), off = 0.f;
+        float l = 0.f, top = -__builtin_inff(), off = kNoScore;
         const int kr = 16 * w + col, vr = 16 * w + 4 * quad + (col >> 2);
         int ka[HD / 32], va[HD / 16];
 #pragma unroll
@@ -737,7 +741,7 @@ struct Kernel {
             mx = fmaxf(mx, lane_xor16(mx));
             mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
             if (__ballot(mx > top + kSlack)) {
-                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? 0.f : E::kOffset - nt;
+                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? kNoScore : E::kOffset - nt;
                 const float al = top == -__builtin_inff() ? 1.f : shrink(no - off);
                 top = nt;
                 off = no;

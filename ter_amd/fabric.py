@@ -655,7 +655,8 @@ class PagedAttention:
     def append(self, q, k, v, cache: PagedCache, batch: PagedBatch, q_out=None, stream=None):
         """Writes k and v [T][n_kv_heads][head_dim] to their pages, keys
         rotated, and returns the rotated q (in q_out; q itself is fine).  q
-        None: keys and values only."""
+        None: keys and values only.  Rows of no sequence are not touched, those
+        of a new q_out hold anything."""
         self._check(cache, batch)
         n = k.shape[0]
         ks, vs = self._rows(k, self.n_kv_heads, n, "k"), self._rows(v, self.n_kv_heads, n, "v")
@@ -676,13 +677,14 @@ class PagedAttention:
                stream=None):
         """softmax(scale q K^T) V of every row of q (rotated) over the positions
         up to its own; scale defaults to 1 / sqrt(head_dim).  shared: that many
-        first positions are the same pages in every sequence, and are computed
-        once for all of them."""
+        first positions are the same pages in every sequence (those of sequence
+        0 are read), and are computed once for all of them.  Rows of no
+        sequence are not touched, those of a new out hold anything."""
         self._check(cache, batch)
         n = q.shape[0]
         qs = self._rows(q, self.n_heads, n, "q")
-        if scale is not None and not scale > 0:
-            raise ValueError("scale must be > 0")
+        if scale is not None and not C.c_float(scale).value > 0:
+            raise ValueError("scale must be > 0 (in binary32)")
         if out is None:
             out = self._empty(n, stream)
         os = self._rows(out, self.n_heads, n, "out")

@@ -182,6 +182,35 @@ def test_overlapping_sequences_beyond_counting(cuda):
         assert (out == 7.0).all()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_of_minus_infinity(cuda, hd, rows):
+    """Keys that no weight can fall on, whole tiles and ranges of them, beside
+    scores far below zero: the others' softmax, NaN where there are no others."""
+    import ter_amd as T
+    n = 3000
+    b = Batch([(rows, n), (rows, 130)], hd=hd, nh=4, nkv=1, page=64, dtype=BF16, seed=6)
+    b.q = b.q.abs() + 0.5
+    b.k = torch.where(torch.isnan(b.k), b.k, -(b.k.abs() * 8 + 4))  # scores: about -10 sqrt(hd)
+    # 2,000 positions of the first sequence, all of the second
+    for s, (lo, hi) in enumerate(((0, 2000), (0, 130))):
+        for p in range(lo, hi):
+            b.k[b.table[s, p // 64], p % 64, :, 0] = -math.inf
+    cache, batch = b.on_device(T)
+    out = context(b).attend(b.q.cuda(), cache, batch).double().cpu()
+    assert torch.isnan(out[rows:]).all()
+    k, v = b.positions(0, b.k)[2000:, 0], b.positions(0, b.v)[2000:, 0]
+    for i in range(rows):
+        m = n - rows + i + 1 - 2000
+        for h in range(4):
+            q = b.q[i, h].double()
+            w = torch.softmax((k[:m] @ q) / math.sqrt(hd), 0)
+            mean = w @ v[:m].abs()
+            ds = float((k[:m].abs() @ q.abs()).max()) / math.sqrt(hd) * (hd + 8) * 2.0 ** -24 + 16 * 2.0 ** -24
+            rel = 2 * ds + 2.0 ** -8 + (n + 64) * 2.0 ** -24
+            assert ((out[i, h] - w @ v[:m]).abs() <= mean * rel + ((w @ v[:m]).abs() + mean * rel) * 2.0 ** -8).all(), (i, h)
+
+
 def test_peaked_and_flat_scores(cuda):
     """Scores so far apart that all but one weight vanishes, growing along the
     sequence (the running maximum moves at every step), and all equal."""
@@ -566,8 +595,9 @@ def test_python_refusals(cuda):
             ctx.attend(bad, cache, batch)
     with pytest.raises(ValueError):
         ctx.attend(q, cache, batch, out=torch.empty_like(q)[:2])
-    with pytest.raises(ValueError):
-        ctx.attend(q, cache, batch, scale=0.0)
+    for scale in (0.0, 1e-50, math.nan):
+        with pytest.raises(ValueError):
+            ctx.attend(q, cache, batch, scale=scale)
     with pytest.raises(ValueError):
         ctx.append(q, k, k[:2], cache, batch)
     with pytest.raises(ValueError):
