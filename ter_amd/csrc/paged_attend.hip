@@ -1152,7 +1152,10 @@ PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_
     c.skew = cus % 8 == 0 && !shared && (int64_t)n_rows * group > kPagedFew * n_seq ? (hd == 128 ? 3 : 2) : 0;
     c.min_per = 2;
     c.target = 96;
-    c.uncut = capacity + n_rows <= 512 ? 9 : 1;
+    // Short tables: with nothing cut there is nothing to join, one launch less
+    // (with a prefix there always is: four tokens behind 448 positions 15.8 us
+    // uncut, 13.6 cut).
+    c.uncut = !shared && capacity + n_rows <= 512 ? 9 : 1;
     c.max_wg = (int)min((int64_t)4 * c.resident, (units + c.min_per - 1) / c.min_per);
     c.max_wg = (c.max_wg + 7) / 8 * 8;
     p.slot_rows = min(kPagedRows, (int)min((long long)n_rows * group, (long long)(1 << p.tokens_log2) * group));
