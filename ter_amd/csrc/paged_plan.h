@@ -151,6 +151,7 @@ TER_HD void paged_cut(PagedLine& l, int total, const PagedCuts& c) {
         l.n_wg = paged_max(c.resident, paged_min(c.max_wg, (int)((unsigned)total / (unsigned)c.target)));
         if (l.n_wg > c.resident) part = 2;
     }
+    l.n_wg = paged_min(l.n_wg, c.max_wg);  // (more work than the host knows of: sequences that overlap)
     const int step = l.n_wg ? (int)((unsigned)total / (unsigned)l.n_wg) : 0;
     l.near = paged_max(paged_max(1, step / part), (c.uncut + 1) / 2);
     l.skew = l.n_wg == c.resident && step >= 4 ? c.skew : 0;  // (so that no range is empty)

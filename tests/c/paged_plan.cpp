@@ -74,9 +74,10 @@ int main() {
         // (with a skew: workgroups of CUs in rounds, 8 times as many)
         const int skew = in(0, 1) ? in(1, 3) : 0, rounds = in(1, 4), round = in(1, 20);
         const int resident = skew ? 8 * rounds * round : in(1, 600);
-        paged_cut(l, total, {resident * in(1, 4), resident, in(1, 40), in(1, 4), in(0, 3) ? 1 : in(2, 20), skew, rounds,
-                             round});
-        CHECK(l.n_wg >= 1);
+        // (fewer than the resident ones where the host knows of less work, whatever the tables hold)
+        const int max_wg = in(0, 3) ? resident * in(1, 4) : in(1, resident);
+        paged_cut(l, total, {max_wg, resident, in(1, 40), in(1, 4), in(0, 3) ? 1 : in(2, 20), skew, rounds, round});
+        CHECK(l.n_wg >= 1 && l.n_wg <= max_wg);
         std::vector<long long> share(1, 0);
         for (int w = 0; w < l.n_wg; ++w) {
             const int r = w / round % rounds;

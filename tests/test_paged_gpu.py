@@ -167,6 +167,29 @@ def test_row0_that_decreases(cuda, shared):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("shared", [0, 16])
+def test_overlapping_sequences_keep_to_the_workspace(cuda, shared):
+    """More row tiles than rows could have: no more ranges than the workspace
+    has places for."""
+    import ter_amd as T
+    from ter_amd import _lib as L
+    n = 20
+    kd = torch.zeros(4, 16, 1, 64, dtype=F16, device="cuda")
+    batch = T.PagedBatch(torch.tensor([0, n] * 10 + [0], dtype=torch.int32, device="cuda"),
+                         torch.full((n,), 60, dtype=torch.int32, device="cuda"),
+                         torch.arange(4, dtype=torch.int32, device="cuda").repeat(n, 1))
+    ctx = T.PagedAttention(128, 1, 64, 64, THETA)
+    cache = T.PagedCache(kd, kd)
+    q = torch.zeros(n, 128, 64, dtype=F16, device="cuda")
+    out = torch.empty_like(q)
+    need = L.lib().ter_hip_paged_attend_ws(ctx._h, batch._ref, cache._ref, n, shared)
+    ws = torch.full((need + (1 << 24),), 165, dtype=torch.uint8, device="cuda")
+    rc = L.lib().ter_hip_paged_attend(ctx._h, batch._ref, cache._ref, n, q.data_ptr(), 128 * 64, out.data_ptr(), 128 * 64,
+                                      shared, 0.0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert (ws[need:] == 165).all()
+
+
 def test_overlapping_sequences_beyond_counting(cuda):
     """The same with more work than a call can have: none is done."""
     import ter_amd as T
