@@ -119,19 +119,22 @@ struct Elem<__bf16> {
 // 16 bytes a lane from memory straight to LDS at lds_off + 16 * lane.  Inline
 // asm without outputs: the compiler's own wait insertion would make every LDS
 // read wait for the loads of the next tile; the waits are explicit instead.
+// (Also the one that hardware does not enforce: a buffer load reads its
+// descriptor five wait states or more after a lane read wrote a part of it.
+// Behind fewer it may be bounded by the size of another load.)
 // kOnce: read by nobody else, so not kept in the caches.
 template <bool kOnce>
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned lds_off) {
     if constexpr (kOnce)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                      :
                      : "s"(lds_off), "v"(voff), "s"(rsrc)
-                     : "memory");
+                     : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(lds_off), "v"(voff), "s"(rsrc)
-                     : "memory");
+                     : "memory", "m0");
 }
 // Waits until at most N loads are in flight, and for this wave's LDS reads.
 template <int N>
