@@ -380,8 +380,8 @@ struct Kernel {
                                        s.kv_end) - s.kv
                                  : 0;
         } else {
-            if (lane == 0) lows[w] = 0;
-            if (live && lim < s.kv_end) lows[w] = 1;
+            const bool some = __ballot(live && lim < s.kv_end) != 0;
+            if (lane == 0) lows[w] = some;  // (one lane: stores of several lanes to one place have no order)
             __syncthreads();
             lo = __builtin_amdgcn_readfirstlane(lows[0] | lows[1] | lows[2] | lows[3]) ? 0 : s.kv_end;
             hi = 32 * w < s.rows ? s.kv_end : 0;
