@@ -200,15 +200,24 @@ __device__ __forceinline__ float shrink(float x) { return fmaxf(__builtin_amdgcn
 // An MFMA's result may be read by another kind of instruction only some wait
 // states later (up to 20), which hardware does not enforce and the compiler
 // fills.  It has left out the wait where the reader is the first instruction
-// behind a branch (an element of the scores read as it was before), so every
-// such result passes through here first.
+// behind a branch (an element of the scores read as it was before), so scores
+// pass through here before their maximum, and sums before they are multiplied
+// or stored.  (tests/test_paged_waits.py checks the built code.)
 template <class V>
 __device__ __forceinline__ void settle(V& x) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x));
 }
-template <class V>
-__device__ __forceinline__ void settle(V& x, V& y) {
-    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x), "+v"(y));
+// (one wait for all of them)
+template <class V, int N>
+__device__ __forceinline__ void settle_all(V (&x)[N]) {
+    static_assert(N == 2 || N == 4 || N == 8, "sums of a row");
+    if constexpr (N == 2)
+        asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));
+    else if constexpr (N == 4)
+        asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+    else
+        asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+                     : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
 }
 
 // A segment's work as one workgroup sees it (all uniform).
@@ -452,8 +461,7 @@ struct Kernel {
             wait_lds();
             barrier_only();
             if (__builtin_amdgcn_readfirstlane(flag[stage]) != tick) return;
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d) settle(o[d]);
+            settle_all(o);
 #pragma clang loop unroll(disable)
             for (int k = 0; k < kPagedKeys; ++k) {
                 const bool sees = j * kPagedKeys + k < lim;
@@ -521,6 +529,7 @@ struct Kernel {
             };
             auto rescale = [&]() {
                 l *= al;
+                settle_all(o);
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -608,6 +617,7 @@ struct Kernel {
                 fetch();  // no row of this wave sees it
         }
         wait_loads<0>();
+        settle_all(o);
         l += lane_xor32(l);
         if (!live) return;
         if (s.dst == 0) {
@@ -702,8 +712,7 @@ struct Kernel {
                     for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
                 }
                 if (__ballot(odd != 0)) {
-#pragma unroll
-                    for (int d = 0; d < HD / 16; ++d) settle(o[d]);
+                    settle_all(o);
 #pragma clang loop unroll(disable)
                     for (int k = 0; k < 16; ++k) {
                         const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW + (quad & 1) * 8;
@@ -749,6 +758,7 @@ struct Kernel {
                 top = nt;
                 off = no;
                 l *= al;
+                settle_all(o);
 #pragma unroll
                 for (int d = 0; d < HD / 16; ++d) o[d] *= al;
             }
@@ -764,6 +774,7 @@ struct Kernel {
             wait_lds();  // these keys' reads are done: their place is free
             fetch();
         }
+        settle_all(o);
         l += lane_xor16(l);
         l += lane_xor32(l);
         if (kSolo) {
