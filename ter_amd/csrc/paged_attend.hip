@@ -220,6 +220,13 @@ __device__ __forceinline__ void settle_all(V (&x)[N]) {
                      : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
 }
 
+// What is computed from x behind here is not moved in front of it.  Rows of
+// either kind start so: with the places of their lanes in LDS computed once for
+// all segments, the kernels kept both kinds' in registers, and at head_dim 64,
+// with 168 of them, some went to scratch memory (96 single tokens 91 us instead
+// of 85).
+__device__ __forceinline__ void hide(int& x) { asm volatile("" : "+v"(x)); }
+
 // A segment's work as one workgroup sees it (all uniform).
 struct Work {
     int kv, kv_end;      // first position of the segment's key tile 0; positions from kv_end on are zeros
@@ -367,6 +374,7 @@ struct Kernel {
     static __device__ __forceinline__ void rows128(const PagedAttendArgs& a, const Work& s, const Loader& ld,
                                                    TER_LDS char* ring, const Seqs& sq, int* shared, int& tick,
                                                    int w, int lane) {
+        hide(lane);
         int* const lows = shared;                 // [kWaves]
         int* const flag = shared + kWaves;        // [2] the tick at which a tile of a stage held odd values
         const int half = lane >> 5, col = lane & 31;
@@ -650,6 +658,7 @@ struct Kernel {
     template <bool kSolo>
     static __device__ __forceinline__ void rows16(const PagedAttendArgs& a, const Work& s, const Loader& ld,
                                                   TER_LDS char* ring, const Seqs& sq, int w, int lane) {
+        hide(lane);
         const int quad = lane >> 4, col = lane & 15;
         const int tok = col / a.group, t = s.tok0 + tok, h = s.kvh * a.group + (col - tok * a.group);
         const bool live = col < s.rows;

@@ -145,6 +145,13 @@ def test_the_check_itself():
     assert faults(mma, mma, "s_nop 7", "s_nop 3", "global_store_dword v50, v3, s[0:1]", end) == 0
 
 
+def test_registers_suffice(tmp_path):
+    """No scratch memory in the attention kernels: it is one more wait for all
+    loads in flight, and memory for every wave."""
+    for name, k in kernels(tmp_path, "paged_attend_kernel").items():
+        assert not any(op.startswith("scratch_") for _, op, _ in k.code), name
+
+
 def test_wait_states(tmp_path):
     found = kernels(tmp_path, "paged_attend_kernel")
     assert len(found) == 4
