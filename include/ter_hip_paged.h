@@ -99,7 +99,8 @@ int ter_hip_paged_append(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
 /* Causal attention of the rows over the pages (their own positions included:
  * append first): out[r][h] = sum_{s <= p(r)} softmax_s(scale * q[r][h] . K[s])
  * V[s].  q holds rotated queries, laid out as for append; out likewise.  scale
- * > 0, or 0 for 1 / sqrt(head_dim).
+ * > 0, or 0 for 1 / sqrt(head_dim).  Scores q . K may have any size that
+ * binary32 holds, and their products with scale any at all.
  *
  * shared: the first `shared` positions of every sequence are the same pages
  * (row 0 of the table is read for them); rounded down to a multiple of 16.

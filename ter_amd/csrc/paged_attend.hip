@@ -220,6 +220,38 @@ __device__ __forceinline__ void settle_all(V (&x)[N]) {
                      : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
 }
 
+__device__ __forceinline__ bool minus_zero(float x) { return __builtin_bit_cast(unsigned, x) == 0x80000000u; }
+
+// Four elements of a row's partial results, added up.  Beside its sums one has
+// their offset and the sum of their weights, or (a far level, see there) the
+// score that was subtracted and minus that sum.  An infinite offset: it has no
+// weights, and -0 as their sum if the row sees no position of the range at all
+// (such sums add up to -0 among themselves only).
+template <typename T>
+struct PartSum {
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float l = -0.f, ref = 0.f, off = __builtin_inff();
+    __device__ __forceinline__ void add(f32x4 v, f32x2 st, float scale2) {
+        const float inf = __builtin_inff();
+        // (a sum that is NaN has any sign; the result is NaN with either)
+        const bool far = __builtin_signbit(st[1]) && st[0] != inf;
+        const float r = far ? st[0] : 0.f, o = far ? Elem<T>::kOffset : st[0], lv = far ? -st[1] : st[1];
+        // 2^d takes sums to the new level; the larger level's stay
+        float d = __builtin_fmaf(ref - r, scale2, -off) + o;
+        d = off == inf ? -inf : d;
+        const float f = __builtin_amdgcn_exp2f(fminf(-fabsf(d), 0.f)), f0 = d < 0.f ? f : 1.f, f1 = d < 0.f ? 1.f : f;
+        l = l * f0 + lv * f1;
+        y = y * f0 + v * f1;
+        ref = d < 0.f ? r : ref;
+        off = d < 0.f ? o : off;
+    }
+    __device__ __forceinline__ f32x2 stats() const { return ref != 0.f ? f32x2{ref, -l} : f32x2{off, l}; }
+    __device__ __forceinline__ typename Elem<T>::v4 result() const {
+        const float inv = minus_zero(l) ? 0.f : 1.f / l;
+        return {(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
+    }
+};
+
 // What is computed from x behind here is not moved in front of it.  Rows of
 // either kind start so: with the places of their lanes in LDS computed once for
 // all segments, the kernels kept both kinds' in registers, and at head_dim 64,
@@ -256,10 +288,42 @@ struct Kernel {
     static constexpr int RING = 2 * L::BYTES;
     // An offset stays while the largest weight is at most 2^kSlack above its start
     static constexpr float kSlack = 7.f;
-    // The offset while all scores are -infinity (masked or not): their weights
-    // are zero with any finite one, and with this one a partial result without
-    // another score counts for nothing beside one that has some.
-    static constexpr float kNoScore = 3e38f;
+
+    // What a row's scores x (before their scaling) are turned into weights
+    // with: 2^(x scale2 + off), off near -max x scale2.  That product is
+    // rounded, by 2^-4 below 2^20, but by whole units from 2^24 on, and the
+    // largest weight would be that far from where it belongs, up to infinite
+    // or zero.  From 2^20 on ("far") the weights are 2^((x - ref) scale2 +
+    // kOffset) with the largest score itself as ref: x - ref is exact near it.
+    // A far row looks at its level for every score: what rows need that are
+    // not is then one comparison.
+    struct Level {
+        float lim = -__builtin_inff();  // nothing to do while no score is above this
+        float off = -0.f;               // far: ref; -0 while all scores are -infinity (masked or not: their
+                                        //   weights are zero with any offset, and no other level has this one)
+        __device__ bool far() const { return lim == -__builtin_inff() && !minus_zero(off); }
+        // For scores above lim, mx the largest: to the level that it asks for.
+        // Returns what sums so far are to be multiplied by.  (Constants pass
+        // through asm: held in registers for this path, which is rarely taken,
+        // they cost more elsewhere.)
+        __device__ float move(float mx, float scale2) {
+            float k = E::kOffset, slack = kSlack;
+            asm volatile("" : "+v"(k), "+v"(slack), "+v"(scale2));
+            const bool was = far(), none = minus_zero(off);
+            if (!(mx > (was ? off : lim))) return 1.f;
+            const float t = mx * scale2, ref = was ? off : 0.f, from = was ? k : off;
+            const bool f = fabsf(t) >= 1048576.f && mx < __builtin_inff();
+            const float to = f ? k : k - t;
+            lim = f ? -__builtin_inff() : __builtin_fmaf(slack, __builtin_amdgcn_rcpf(scale2), mx);
+            off = f ? mx : to;
+            return none ? 1.f : shrink(__builtin_fmaf(ref - (f ? mx : 0.f), scale2, -from) + to);
+        }
+        // A partial result's two numbers, with l for the sum of its weights.
+        __device__ f32x2 stats(bool sees, float l) const {
+            const bool none = minus_zero(off);
+            return f32x2{none ? __builtin_inff() : off, none ? (sees ? l : -0.f) : far() ? -l : l};
+        }
+    };
 
     // ---- loads: wave w takes rows 16 w .. 16 w + 15 of K and V
     struct Loader {
@@ -409,7 +473,8 @@ struct Kernel {
         for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-        float l = 0.f, top = -__builtin_inff(), off = kNoScore;
+        float l = 0.f;
+        Level level;
 
         // LDS offsets: K pieces of row col (+ 32 by offset); V rows of the
         // lane's transposing read
@@ -502,7 +567,7 @@ struct Kernel {
             const int kt = (int)(size_t)ring + stage * L::BYTES + ka, vt = (int)(size_t)ring + stage * L::BYTES + va;
             f32x16 x[2];
             v8 k[HD / 16], p[2][2], y[2][HD / 32];
-            float al = 1.f;
+            float al = 1.f, wo;
             auto read_k = [&](int b, int c) { k[c] = *((const TER_LDS v8*)(size_t)(unsigned)(kt ^ (32 * c)) + b * 2 * L::ROW); };
             auto scores = [&](int b, int c) { x[b] = E::mma32(k[c], q[c], x[b]); };
             auto read_v = [&](int c, int d) {
@@ -525,15 +590,20 @@ struct Kernel {
                 float mx = x[b][0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[b][i]);
-                mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
-                if (__ballot(mx > top + kSlack)) {
-                    const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? kNoScore : E::kOffset - nt;
-                    al = top == -__builtin_inff() ? 1.f : shrink(no - off);
-                    top = nt;
-                    off = no;
-                    return true;
+                mx = fmaxf(mx, lane_xor32(mx));
+                const bool look = __ballot(mx > level.lim) != 0;
+                wo = level.off;
+                if (look) {
+                    al = level.move(mx, a.scale2);
+                    wo = level.off;
+                    if (__ballot(level.far())) {
+                        const float ref = level.far() ? level.off : 0.f;
+                        wo = level.far() ? E::kOffset : level.off;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[b][i] -= ref;
+                    }
                 }
-                return false;
+                return look;
             };
             auto rescale = [&]() {
                 l *= al;
@@ -544,8 +614,8 @@ struct Kernel {
                     for (int i = 0; i < 16; ++i) o[d][i] *= al;
             };
             auto weight = [&](int b, int i) {  // elements i, i + 1
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, off));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, off));
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, wo));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, wo));
                 l += e0;
                 l += e1;
                 p[b][i >> 3][i & 7] = (T)e0;
@@ -649,7 +719,7 @@ struct Kernel {
                 *gptr(reinterpret_cast<f32x4*>(p + 32 * d + 2 * i)) =
                     f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
         if (half == 0)
-            *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, t, h))) = f32x2{lim > s.j0 * kPagedKeys ? off : __builtin_inff(), l};
+            *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, t, h))) = level.stats(lim > s.j0 * kPagedKeys, l);
     }
 
     // ---- up to 16 rows, 16 keys at a time.  kSolo: by one wave.  Else wave w
@@ -691,7 +761,8 @@ struct Kernel {
         f32x4 o[HD / 16];
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float l = 0.f, top = -__builtin_inff(), off = kNoScore;
+        float l = 0.f;
+        Level level;
         const int kr = 16 * w + col, vr = 16 * w + 4 * quad + (col >> 2);
         int ka[HD / 32], va[HD / 16];
 #pragma unroll
@@ -760,21 +831,26 @@ struct Kernel {
             }
             float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             mx = fmaxf(mx, lane_xor16(mx));
-            mx = fmaxf(mx, lane_xor32(mx)) * a.scale2;
-            if (__ballot(mx > top + kSlack)) {
-                const float nt = fmaxf(top, mx), no = nt == -__builtin_inff() ? kNoScore : E::kOffset - nt;
-                const float al = top == -__builtin_inff() ? 1.f : shrink(no - off);
-                top = nt;
-                off = no;
+            mx = fmaxf(mx, lane_xor32(mx));
+            float wo = level.off;
+            if (__ballot(mx > level.lim)) {
+                const float al = level.move(mx, a.scale2);
                 l *= al;
                 settle_all(o);
 #pragma unroll
                 for (int d = 0; d < HD / 16; ++d) o[d] *= al;
+                wo = level.off;
+                if (__ballot(level.far())) {
+                    const float ref = level.far() ? level.off : 0.f;
+                    wo = level.far() ? E::kOffset : level.off;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] -= ref;
+                }
             }
             v4 p;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.scale2, off));
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.scale2, wo));
                 l += e;
                 p[i] = (T)e;
             }
@@ -801,7 +877,7 @@ struct Kernel {
 #pragma unroll
                 for (int d = 0; d < HD / 16; ++d) *gptr(reinterpret_cast<f32x4*>(p + 16 * d)) = o[d];
                 if (quad == 0)
-                    *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, col, t, h))) = f32x2{lim > first ? off : __builtin_inff(), l};
+                    *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, col, t, h))) = level.stats(lim > first, l);
             }
             return;
         }
@@ -813,35 +889,21 @@ struct Kernel {
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d)
                 *(TER_LDS f32x4*)(sums + (w * 16 + col) * HD + 16 * d + 4 * quad) = o[d];
-            if (quad == 0) {
-                stats[(w * 16 + col) * 2] = lim > first ? off : __builtin_inff();
-                stats[(w * 16 + col) * 2 + 1] = l;
-            }
+            if (quad == 0) *(TER_LDS f32x2*)(stats + (w * 16 + col) * 2) = level.stats(lim > first, l);
         }
         __syncthreads();
         for (int i = w * 64 + lane; i < s.rows * (HD / 4); i += kThreads) {
             const int r = i / (HD / 4), e = (i - r * (HD / 4)) * 4;
-            float f[kWaves], least = __builtin_inff(), tl = 0.f;
+            PartSum<T> sum;
 #pragma unroll
-            for (int k = 0; k < kWaves; ++k) least = fminf(least, stats[(k * 16 + r) * 2]);
-            f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < kWaves; ++k) {
-                const float ok = stats[(k * 16 + r) * 2];
-                f[k] = ok == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(least - ok);
-                if (f[k] != 0.f || stats[(k * 16 + r) * 2 + 1] != stats[(k * 16 + r) * 2 + 1]) {  // (NaN stays)
-                    tl += f[k] * stats[(k * 16 + r) * 2 + 1];
-                    y += f[k] * *(TER_LDS f32x4*)(sums + (k * 16 + r) * HD + e);
-                }
-            }
+            for (int k = 0; k < kWaves; ++k)
+                sum.add(*(TER_LDS f32x4*)(sums + (k * 16 + r) * HD + e), *(TER_LDS f32x2*)(stats + (k * 16 + r) * 2), a.scale2);
             const int rt = s.tok0 + r / a.group, rh = s.kvh * a.group + r % a.group;
             if (s.dst == 0) {
-                const float inv = least == __builtin_inff() ? 0.f : 1.f / tl;
-                const v4 z = {(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
-                *gptr(reinterpret_cast<v4*>(a.out + (long long)rt * a.out_stride + (long long)rh * L::ROW + e * 2)) = z;
+                *gptr(reinterpret_cast<v4*>(a.out + (long long)rt * a.out_stride + (long long)rh * L::ROW + e * 2)) = sum.result();
             } else {
-                *gptr(reinterpret_cast<f32x4*>(sums_of(a, s, r, rt, rh) + e)) = y;
-                if (e == 0) *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, rt, rh))) = f32x2{least, tl};
+                *gptr(reinterpret_cast<f32x4*>(sums_of(a, s, r, rt, rh) + e)) = sum.y;
+                if (e == 0) *gptr(reinterpret_cast<f32x2*>(stats_of(a, s, r, rt, rh))) = sum.stats();
             }
         }
     }
@@ -999,27 +1061,15 @@ struct Join {
     static constexpr int TPR = HD / 4, GROUPS = kThreads / TPR;
     typedef typename Elem<T>::v4 v4;
     struct Lds {
-        float sums[GROUPS][HD], stats[GROUPS][2];
-    };
-    struct Sum {
-        f32x4 y = {0.f, 0.f, 0.f, 0.f};
-        float l = 0.f, off = __builtin_inff();
-        __device__ void add(f32x4 v, float lv, float o) {
-            if (o == __builtin_inff()) return;  // nothing seen there
-            const float no = fminf(off, o);
-            const float f0 = off == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(no - off);
-            const float f1 = __builtin_amdgcn_exp2f(no - o);
-            l = l * f0 + lv * f1;
-            y = y * f0 + v * f1;
-            off = no;
-        }
+        float sums[GROUPS][HD];
+        f32x2 stats[GROUPS];
     };
     // Partial result i of n of a row: place(i, sums, stats).  All threads call
     // it; those of a row's first group return with the whole, `live` rows write it.
     template <class Place>
-    static __device__ void row(Lds& lds, int S, int n, bool live, Place place, char* out) {
+    static __device__ void row(Lds& lds, int S, int n, bool live, float scale2, Place place, char* out) {
         const int grp = threadIdx.x / TPR, e = (threadIdx.x % TPR) * 4, sub = grp & (S - 1);
-        Sum t;
+        PartSum<T> t;
         if (live) {
             constexpr int U = 4;  // partial results in flight
             for (int i0 = sub; i0 < n; i0 += U * S) {
@@ -1035,27 +1085,19 @@ struct Join {
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (i0 + u * S < n) t.add(v[u], st[u][1], st[u][0]);
+                    if (i0 + u * S < n) t.add(v[u], st[u], scale2);
             }
         }
         if (S > 1) {
             __syncthreads();
             *reinterpret_cast<f32x4*>(&lds.sums[grp][e]) = t.y;
-            if (e == 0) {
-                lds.stats[grp][0] = t.off;
-                lds.stats[grp][1] = t.l;
-            }
+            if (e == 0) lds.stats[grp] = t.stats();
             __syncthreads();
             if (sub == 0)
                 for (int k = 1; k < S; ++k)
-                    t.add(*reinterpret_cast<const f32x4*>(&lds.sums[grp + k][e]), lds.stats[grp + k][1],
-                          lds.stats[grp + k][0]);
+                    t.add(*reinterpret_cast<const f32x4*>(&lds.sums[grp + k][e]), lds.stats[grp + k], scale2);
         }
-        if (live && sub == 0) {
-            const float inv = t.off == __builtin_inff() ? 0.f : 1.f / t.l;
-            const v4 z = {(T)(t.y[0] * inv), (T)(t.y[1] * inv), (T)(t.y[2] * inv), (T)(t.y[3] * inv)};
-            *gptr(reinterpret_cast<v4*>(out + e * 2)) = z;
-        }
+        if (live && sub == 0) *gptr(reinterpret_cast<v4*>(out + e * 2)) = t.result();
     }
 };
 
@@ -1076,7 +1118,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttendArgs a)
     for (int r0 = worker * per; r0 < rows; r0 += workers * per) {
         const int r = r0 + grp / S, tok = r / a.group, t = tok0 + tok, h = kvh * a.group + r - tok * a.group;
         J::row(
-            lds, S, n, r < rows,
+            lds, S, n, r < rows, a.scale2,
             [&](int i, const float*& sums, const float*& stats) {
                 const long long at = (long long)(2 * (first + i) + (i == 0 ? 1 : 0)) * a.slot_rows + r;
                 sums = a.slots + at * HD;
@@ -1114,7 +1156,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_shared_kernel(PagedAttend
     for (int i0 = 0; i0 < a.group; i0 += per) {
         const int i = i0 + grp / S, h = kvh * a.group + i;
         J::row(
-            lds, S, n_own + n_pre, i < a.group,
+            lds, S, n_own + n_pre, i < a.group, a.scale2,
             [&](int k, const float*& sums, const float*& stats) {
                 const bool is_pre = k >= n_own;
                 const PagedParts& p = is_pre ? pre : own;
