@@ -68,7 +68,9 @@ struct PagedAttendLayout {
     PagedCuts cuts_by;
     size_t cuts, before, slots, slot_stats, whole, whole_stats, bytes;
 };
-PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared);
+// (bytes 0: the device cannot be asked for its CUs)
+PagedAttendLayout paged_attend_layout(int device, int nh, int nkv, int hd, int n_seq, int n_rows, int capacity,
+                                      int shared);
 
 hipError_t launch_paged_rope_table(float* tab, int hd, int max_pos, double theta, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendArgs& a, int hd, bool neox, bool bf16, hipStream_t st);

@@ -159,7 +159,8 @@ size_t ter_hip_paged_attend_ws(const ter_hip_paged_t* ctx, const ter_hip_paged_b
     PagedBatch b;
     PagedCache c;
     if (check_batch(ctx, batch, cache, n_rows, &b, &c) || n_rows == 0 || b.n_seq == 0 || shared < 0) return 0;
-    return paged_attend_layout(ctx->nh, ctx->nkv, ctx->hd, b.n_seq, n_rows, b.capacity, shared / 16 * 16).bytes;
+    return paged_attend_layout(ctx->device, ctx->nh, ctx->nkv, ctx->hd, b.n_seq, n_rows, b.capacity, shared / 16 * 16)
+        .bytes;
 }
 
 int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t* batch,
@@ -177,7 +178,8 @@ int ter_hip_paged_attend(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
     if ((rc = check_rows("out", out, out_stride, (int64_t)ctx->nh * ctx->hd))) return rc;
     shared = shared / 16 * 16;
     const PagedAttendLayout p =
-        paged_attend_layout(ctx->nh, ctx->nkv, ctx->hd, batch->n_seq, n_rows, a.b.capacity, shared);
+        paged_attend_layout(ctx->device, ctx->nh, ctx->nkv, ctx->hd, batch->n_seq, n_rows, a.b.capacity, shared);
+    if (p.bytes == 0) return fail(TER_HIP_ERR_HIP, "cannot query CU count");
     // units are counted in 31 bits (a sequence's rows may lie behind its whole table)
     const int64_t tiles = ((int64_t)n_rows >> p.tokens_log2) + batch->n_seq;
     if (tiles * ctx->nkv * (((int64_t)a.b.capacity + n_rows) / 64 + 10 + shared / 64) > 0x7FFFFFFFll)

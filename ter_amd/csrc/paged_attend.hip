@@ -1195,12 +1195,13 @@ hipError_t launch(const PagedAttendArgs& a, hipStream_t st) {
 
 }  // namespace
 
-PagedAttendLayout paged_attend_layout(int nh, int nkv, int hd, int n_seq, int n_rows, int capacity, int shared) {
+PagedAttendLayout paged_attend_layout(int device, int nh, int nkv, int hd, int n_seq, int n_rows, int capacity,
+                                      int shared) {
     PagedAttendLayout p{};
+    const int cus = device_cu_count(device);
+    if (cus <= 0) return p;
     const int group = nh / nkv;
     p.tokens_log2 = paged_tokens_log2(group);
-    int dev = 0;
-    int cus = hipGetDevice(&dev) == hipSuccess ? device_cu_count(dev) : 256;
     const int64_t tiles = ((int64_t)n_rows >> p.tokens_log2) + n_seq;
     // no more ranges than there can be work for
     const int64_t units = nkv * (tiles * (kPagedLead + 1 + min((int64_t)capacity + n_rows, (int64_t)1 << 30) / kPagedKeys) +
