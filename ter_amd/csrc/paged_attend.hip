@@ -220,6 +220,18 @@ __device__ __forceinline__ void settle_all(V (&x)[N]) {
                      : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
 }
 
+// Whether all sums are finite.
+template <class V, int N>
+__device__ __forceinline__ bool all_finite(const V (&x)[N]) {
+    float m = 0.f;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / 4); i += 2)
+            m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(x[d][i]), fabsf(x[d][i + 1])), m);
+    return m < __builtin_inff();
+}
+
 __device__ __forceinline__ bool minus_zero(float x) { return __builtin_bit_cast(unsigned, x) == 0x80000000u; }
 
 // Four elements of a row's partial results, added up.  Beside its sums one has
@@ -236,10 +248,11 @@ struct PartSum {
         // (a sum that is NaN has any sign; the result is NaN with either)
         const bool far = __builtin_signbit(st[1]) && st[0] != inf;
         const float r = far ? st[0] : 0.f, o = far ? Elem<T>::kOffset : st[0], lv = far ? -st[1] : st[1];
-        // 2^d takes sums to the new level; the larger level's stay
+        // 2^d takes sums to the new level; the larger level's stay.  (Never
+        // less than 2^-126, as in shrink, of which no finite sum is left.)
         float d = __builtin_fmaf(ref - r, scale2, -off) + o;
         d = off == inf ? -inf : d;
-        const float f = __builtin_amdgcn_exp2f(fminf(-fabsf(d), 0.f)), f0 = d < 0.f ? f : 1.f, f1 = d < 0.f ? 1.f : f;
+        const float f = __builtin_amdgcn_exp2f(fmaxf(-fabsf(d), -126.f)), f0 = d < 0.f ? f : 1.f, f1 = d < 0.f ? 1.f : f;
         l = l * f0 + lv * f1;
         y = y * f0 + v * f1;
         ref = d < 0.f ? r : ref;
@@ -469,11 +482,7 @@ struct Kernel {
         }
 
         f32x16 o[HD / 32];
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-        float l = 0.f;
+        float l;
         Level level;
 
         // LDS offsets: K pieces of row col (+ 32 by offset); V rows of the
@@ -500,7 +509,6 @@ struct Kernel {
                 put ^= 1;
             }
         };
-        fetch();
         // The same in pieces, spread over a step: a wave that issues all of
         // them at once waits a quarter of the step for the address unit.
         // (Behind the last tile they load what nobody reads, into a stage that is free.)
@@ -682,20 +690,36 @@ struct Kernel {
                 for (int d = 0; d < HD / 32; ++d) value(c, d);
         };
         // tiles that every row sees whole, then the others
-        const int full = min(s.j1, max(s.j0, lo / kPagedKeys));
-        for (; j < full; ++j, stage ^= 1) {
-            arrive();
-            step(std::false_type{});
+        for (int full = min(s.j1, max(s.j0, lo / kPagedKeys));; full = s.j0) {
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+            l = 0.f;
+            level = Level{};
+            fetch();
+            for (; j < full; ++j, stage ^= 1) {
+                arrive();
+                step(std::false_type{});
+            }
+            for (; j < s.j1; ++j, stage ^= 1) {
+                arrive_masked();
+                if (j * kPagedKeys < hi)
+                    step(std::true_type{});
+                else
+                    fetch();  // no row of this wave sees it
+            }
+            wait_loads<0>();
+            settle_all(o);
+            if (full == s.j0) break;
+            // Infinite or NaN: once more, with every tile's values looked at
+            const bool odd = __ballot(live && !all_finite(o)) != 0;
+            if (lane == 0) lows[w] = odd;
+            __syncthreads();
+            if (!__builtin_amdgcn_readfirstlane(lows[0] | lows[1] | lows[2] | lows[3])) break;
+            put = stage = 0;
+            j = todo = s.j0;
         }
-        for (; j < s.j1; ++j, stage ^= 1) {
-            arrive_masked();
-            if (j * kPagedKeys < hi)
-                step(std::true_type{});
-            else
-                fetch();  // no row of this wave sees it
-        }
-        wait_loads<0>();
-        settle_all(o);
         l += lane_xor32(l);
         if (!live) return;
         if (s.dst == 0) {
@@ -759,9 +783,7 @@ struct Kernel {
         else if (__ballot(live && lim < s.kv_end) == 0)
             lo = s.kv_end;
         f32x4 o[HD / 16];
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
+        float l;
         Level level;
         const int kr = 16 * w + col, vr = 16 * w + 4 * quad + (col >> 2);
         int ka[HD / 32], va[HD / 16];
@@ -770,96 +792,108 @@ struct Kernel {
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d)
             va[d] = L::V + vr * L::ROW + (((2 * d + ((lane & 3) >> 1)) ^ L::swizzle_v(vr)) * 16) + 8 * (lane & 1);
-        // The queries, which the compiler waits for, have to be here before the
-        // loop: inside it that wait would be one for all loads in flight.
-        wait_loads<0>();
-        int stage = 0;
-        for (int i = 0; i < n; ++i, stage ^= 1) {
-            // the next keys' loads may still be in flight
-            if (i + 1 < n)
-                wait_loads<2 * L::NI>();
-            else
-                wait_loads<0>();
-            const int at = first + i * stride;
-            TER_LDS char* tile = ring + stage * L::BYTES;
-            if (at + 16 > lo) {  // (as in rows128, by each wave for its own keys)
-                TER_LDS u32x4* const mine = (TER_LDS u32x4*)(tile + L::V + w * 16 * L::ROW + lane * 16);
-                unsigned odd = 0;
+        for (bool again = false;; again = true) {
 #pragma unroll
-                for (int i = 0; i < L::NI; ++i) {
-                    const u32x4 y = mine[64 * i];
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
-                }
-                if (__ballot(odd != 0)) {
-                    settle_all(o);
-#pragma clang loop unroll(disable)
-                    for (int k = 0; k < 16; ++k) {
-                        const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW + (quad & 1) * 8;
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d)
-                            add_odd<T>(o[d], 0,
-                                       *(const TER_LDS u32x2*)(v + ((2 * d + (quad >> 1)) ^ L::swizzle_v(16 * w + k)) * 16),
-                                       at + k < lim);
-                    }
+            for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+            l = 0.f;
+            level = Level{};
+            // The queries, which the compiler waits for, have to be here before the
+            // loop: inside it that wait would be one for all loads in flight.
+            wait_loads<0>();
+            int stage = 0;
+            for (int i = 0; i < n; ++i, stage ^= 1) {
+                // the next keys' loads may still be in flight
+                if (i + 1 < n)
+                    wait_loads<2 * L::NI>();
+                else
+                    wait_loads<0>();
+                const int at = first + i * stride;
+                TER_LDS char* tile = ring + stage * L::BYTES;
+                if (at + 16 > lo) {  // (as in rows128, by each wave for its own keys)
+                    TER_LDS u32x4* const mine = (TER_LDS u32x4*)(tile + L::V + w * 16 * L::ROW + lane * 16);
+                    unsigned odd = 0;
 #pragma unroll
                     for (int i = 0; i < L::NI; ++i) {
-                        u32x4 y = mine[64 * i];
+                        const u32x4 y = mine[64 * i];
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) y[m] = without_odd<T>(y[m]);
-                        mine[64 * i] = y;
+                        for (int m = 0; m < 4; ++m) odd |= odd_halves<T>(y[m]);
                     }
-                    wait_lds();
+                    if (__ballot(odd != 0)) {
+                        settle_all(o);
+#pragma clang loop unroll(disable)
+                        for (int k = 0; k < 16; ++k) {
+                            const TER_LDS char* v = tile + L::V + (16 * w + k) * L::ROW + (quad & 1) * 8;
+#pragma unroll
+                            for (int d = 0; d < HD / 16; ++d)
+                                add_odd<T>(o[d], 0,
+                                           *(const TER_LDS u32x2*)(v + ((2 * d + (quad >> 1)) ^ L::swizzle_v(16 * w + k)) * 16),
+                                           at + k < lim);
+                        }
+#pragma unroll
+                        for (int i = 0; i < L::NI; ++i) {
+                            u32x4 y = mine[64 * i];
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) y[m] = without_odd<T>(y[m]);
+                            mine[64 * i] = y;
+                        }
+                        wait_lds();
+                    }
                 }
-            }
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            v8 k[HD / 32];
-            v4 y[HD / 16];
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                v8 k[HD / 32];
+                v4 y[HD / 16];
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) k[c] = *(const TER_LDS v8*)(tile + ka[c]);
+                for (int c = 0; c < HD / 32; ++c) k[c] = *(const TER_LDS v8*)(tile + ka[c]);
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) y[d] = E::read_tr(tile + va[d]);
-            __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product
+                for (int d = 0; d < HD / 16; ++d) y[d] = E::read_tr(tile + va[d]);
+                __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) x = E::mma16(k[c], q[c], x);
-            settle(x);
-            if (at + 16 > lo) {
-                const int see = lim - at - 4 * quad;
+                for (int c = 0; c < HD / 32; ++c) x = E::mma16(k[c], q[c], x);
+                settle(x);
+                if (at + 16 > lo) {
+                    const int see = lim - at - 4 * quad;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k >= see) x[k] = -__builtin_inff();
-            }
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, lane_xor16(mx));
-            mx = fmaxf(mx, lane_xor32(mx));
-            float wo = level.off;
-            if (__ballot(mx > level.lim)) {
-                const float al = level.move(mx, a.scale2);
-                l *= al;
-                settle_all(o);
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d) o[d] *= al;
-                wo = level.off;
-                if (__ballot(level.far())) {
-                    const float ref = level.far() ? level.off : 0.f;
-                    wo = level.far() ? E::kOffset : level.off;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] -= ref;
+                    for (int k = 0; k < 4; ++k)
+                        if (k >= see) x[k] = -__builtin_inff();
                 }
-            }
-            v4 p;
+                float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                mx = fmaxf(mx, lane_xor16(mx));
+                mx = fmaxf(mx, lane_xor32(mx));
+                float wo = level.off;
+                if (__ballot(mx > level.lim)) {
+                    const float al = level.move(mx, a.scale2);
+                    l *= al;
+                    settle_all(o);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.scale2, wo));
-                l += e;
-                p[i] = (T)e;
-            }
+                    for (int d = 0; d < HD / 16; ++d) o[d] *= al;
+                    wo = level.off;
+                    if (__ballot(level.far())) {
+                        const float ref = level.far() ? level.off : 0.f;
+                        wo = level.far() ? E::kOffset : level.off;
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(y[d], p, o[d]);
-            wait_lds();  // these keys' reads are done: their place is free
+                        for (int k = 0; k < 4; ++k) x[k] -= ref;
+                    }
+                }
+                v4 p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.scale2, wo));
+                    l += e;
+                    p[i] = (T)e;
+                }
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) o[d] = E::mma16k16(y[d], p, o[d]);
+                wait_lds();  // these keys' reads are done: their place is free
+                fetch();
+            }
+            settle_all(o);
+            // Infinite or NaN: once more, with every key's values looked at
+            if (again || !__ballot(live && !all_finite(o))) break;
+            lo = -0x7FFFFFFF;
+            put = todo = 0;
+            fetch();
             fetch();
         }
-        settle_all(o);
         l += lane_xor16(l);
         l += lane_xor32(l);
         if (kSolo) {
