@@ -102,6 +102,13 @@ int ter_hip_paged_append(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
  * > 0, or 0 for 1 / sqrt(head_dim).  Scores q . K may have any size that
  * binary32 holds, and their products with scale any at all.
  *
+ * Rounding: scores, the softmax and all sums are binary32, the result is
+ * rounded once.  On its way into the product with V a weight is rounded to two
+ * elements of the cache's type (22 bits of fp16, 16 of bf16) where a KV head's
+ * query heads times the sequence's rows in a tile are 16 or fewer, as those of
+ * single tokens are, and to one element (11 or 8 bits) where they are more: of
+ * prompts, and of all sequences' rows together on a shared prefix.
+ *
  * shared: the first `shared` positions of every sequence are the same pages
  * (row 0 of the table is read for them); rounded down to a multiple of 16.
  * Results are those of shared = 0 up to rounding: those positions are

@@ -678,8 +678,11 @@ class PagedAttention:
         """softmax(scale q K^T) V of every row of q (rotated) over the positions
         up to its own; scale defaults to 1 / sqrt(head_dim).  shared: that many
         first positions are the same pages in every sequence (those of sequence
-        0 are read), and are computed once for all of them.  Rows of no
-        sequence are not touched, those of a new out hold anything."""
+        0 are read), and are computed once for all of them.  Scores and sums
+        are binary32; weights are rounded to the cache's type before they meet
+        V, those of single tokens (16 or fewer rows of a KV head) to two
+        elements of it.  Rows of no sequence are not touched, those of a new
+        out hold anything."""
         self._check(cache, batch)
         n = q.shape[0]
         qs = self._rows(q, self.n_heads, n, "q")

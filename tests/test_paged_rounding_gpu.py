@@ -1,13 +1,50 @@
-"""What the paged attention rounds on the way, and what of it must not show."""
+"""What the paged attention rounds: of few rows (at most 16 of a KV head and
+sequence, as single tokens are) nothing between the inputs and the result but in
+binary32 and to twice the element type's bits."""
 import math
 
 import pytest
 import torch
 
-from paged_ref import Batch, compare
+from paged_ref import Batch, compare, half_step, smallest
 from test_paged_gpu import BF16, F16, context
 
 pytestmark = pytest.mark.gpu
+
+
+def expected(b):
+    """(result, bound) of the rows: paged_ref.Batch.attend's, but weights are
+    held in two elements (half a step of half a step)."""
+    u, f32, scale = half_step(b.dtype), 2.0 ** -24, 1 / math.sqrt(b.hd)
+    want = torch.full((b.t, b.nh, b.hd), math.nan, dtype=torch.float64)
+    tol = want.clone()
+    for s, (n, r) in enumerate(zip(b.lens, b.rows)):
+        k, v = b.positions(s, b.k), b.positions(s, b.v)
+        hidden = torch.arange(n) > torch.arange(n - r, n)[:, None]
+        at = slice(int(b.first[s]), int(b.first[s + 1]))
+        for h in range(b.nh):
+            g, q = h * b.nkv // b.nh, b.q[at, h].double()
+            w = torch.softmax((q @ k[:, g].T * scale).masked_fill_(hidden, -math.inf), -1)
+            y, mean = w @ v[:, g], w @ v[:, g].abs()
+            ds = (q.abs() @ k[:, g].abs().T * scale).amax(-1, keepdim=True) * (b.hd + 8) * f32 + 16 * f32
+            rel = 2 * ds + u * u + (n + 64) * f32
+            few = n * 2.0 ** -33 * float(v.abs().max()) if b.dtype == F16 else 0.0
+            want[at, h] = y
+            tol[at, h] = mean * rel + few + (y.abs() + mean * rel) * u + smallest(b.dtype)
+    return want, tol
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("shape", [dict(nh=4, nkv=2, hd=64), dict(nh=5, nkv=1, hd=128)], ids=["hd64", "hd128"])
+@pytest.mark.parametrize("seqs", [
+    [(1, n) for n in (1, 2, 3, 5, 17, 40, 130)], [(3, 3), (2, 20), (3, 300), (1, 700)], [(1, 6000), (3, 2500), (2, 9)],
+], ids=["single", "few", "cut"])
+def test_few_rows_keep_their_weights(cuda, seqs, shape, dtype):
+    import ter_amd as T
+    b = Batch(seqs, dtype=dtype, seed=8, page=32, **shape)
+    cache, batch = b.on_device(T)
+    want, tol = expected(b)
+    compare(context(b).attend(b.q.cuda(), cache, batch), want, tol)
 
 
 @pytest.mark.parametrize("shape", [dict(nh=4, nkv=2, hd=64), dict(nh=4, nkv=1, hd=128)], ids=["hd64", "hd128"])
