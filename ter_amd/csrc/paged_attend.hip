@@ -1266,7 +1266,11 @@ PagedAttendLayout paged_attend_layout(int device, int nh, int nkv, int hd, int n
     // (with a prefix there always is: four tokens behind 448 positions 15.8 us
     // uncut, 13.6 cut).
     c.uncut = !shared && capacity + n_rows <= 512 ? 9 : 1;
-    c.max_wg = (int)min((int64_t)4 * c.resident, (units + c.min_per - 1) / c.min_per);
+    // (as paged_cut has it for the most units there can be: each range needs
+    // two places in the workspace, 96 single tokens 52 MB so instead of 208
+    // with four times the resident ones)
+    c.max_wg = (int)min(max((int64_t)c.resident, min((int64_t)4 * c.resident, units / c.target)),
+                        (units + c.min_per - 1) / c.min_per);
     c.max_wg = (c.max_wg + 7) / 8 * 8;
     p.slot_rows = min(kPagedRows, (int)min((long long)n_rows * group, (long long)(1 << p.tokens_log2) * group));
     auto take = [&](size_t n) {

@@ -68,3 +68,29 @@ def test_device_that_cannot_be_asked(unlike):
     unlike.unlike_break(0)
     assert attend(h, batch(), cache()) == 0 and any(l.startswith("launch") for l in log())
     """)
+
+
+def test_workspace_holds_the_ranges_that_there_can_be(unlike):
+    """Two places for each: not for four times the workgroups that run at a
+    time where the tables have no work for them."""
+    unlike("""
+    def need(n_seq, rows, cap, nh=32, nkv=8, hd=64):
+        x = context(nh, nkv, hd)
+        c = cache(page_stride=64 * nkv * hd, pos_stride=nkv * hd, head_stride=hd, page_size=64)
+        b = batch(n_seq=n_seq, max_pages=cap // 64, pages_stride=cap // 64)
+        n = lib.ter_hip_paged_attend_ws(x, C.byref(b), C.byref(c), rows, 0)
+        assert attend(x, b, c, n=rows, qs=nh * hd, os=nh * hd, nb=n) == 0
+        lib.ter_hip_paged_destroy(x)
+        grid = [int(l.split()[2]) for l in log() if "paged_attend" in l and l.startswith("launch")]
+        return n, grid[0]
+    # 256 CUs, three workgroups of each: 96 single tokens of up to 4096
+    # positions are 96 * 8 * (64 + 3) units at most, fewer than 96 a range
+    n, grid = need(96, 96, 4096)
+    assert grid == 768 and n < 2 * 768 * 128 * (64 + 2) * 4 + (1 << 20)
+    # one prompt of 16384: more ranges than workgroups
+    n, grid = need(1, 16384, 16384, 20, 5, 128)
+    assert grid == 4 * 512
+    # little work
+    n, grid = need(1, 1, 64)
+    assert grid < 64
+    """)
