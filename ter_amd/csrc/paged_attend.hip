@@ -111,7 +111,9 @@ struct Elem<__bf16> {
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     typedef short s4 __attribute__((ext_vector_type(4)));
-    static constexpr float kOffset = 0.f;
+    // Values may be near binary32's largest: with weights of at most 2^-25 no
+    // sum of 2^20 of them leaves it, and weights have 2^-94 to go.
+    static constexpr float kOffset = -32.f;
     static __device__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) {

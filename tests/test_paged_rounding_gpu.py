@@ -92,3 +92,20 @@ def test_infinite_values_of_vanishing_weight(cuda, power, rows, shared, shape, d
     keep = [d for d in range(b.hd) if d != 7]
     want, tol = b.attend()
     compare(out[..., keep], want[..., keep], tol[..., keep])
+
+
+@pytest.mark.parametrize("shape", [dict(nh=4, nkv=2, hd=64), dict(nh=4, nkv=1, hd=128)], ids=["hd64", "hd128"])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("shared", [0, 64])
+def test_values_near_the_largest(cuda, shared, shape, dtype):
+    """No sum on the way leaves binary32."""
+    import ter_amd as T
+    seqs = [(60, 160), (1, 70), (3, 2500), (100, 900), (1, 6000)]
+    b = Batch(seqs, dtype=dtype, seed=12, page=16, common=shared, **shape)
+    top = torch.finfo(dtype).max
+    b.v = torch.where(torch.isnan(b.v), b.v, (b.v.float().clamp(-1, 1) * top).to(dtype))
+    cache, batch = b.on_device(T)
+    out = context(b).attend(b.q.cuda(), cache, batch, shared=shared)
+    assert torch.isfinite(out).all()
+    want, tol = b.attend()
+    compare(out, want, tol)
