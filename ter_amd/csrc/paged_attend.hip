@@ -17,7 +17,8 @@
 // to one, half a step as the inputs are (0.00026-0.00029 and 0.0023).  Two there
 // make 5,600 rows of prompts 148 us instead of 118, one prompt of 16,384 2.0 ms
 // instead of 1.5, single tokens behind a shared prefix 40.5 us instead of 36;
-// of few rows they cost nothing that shows.
+// of few rows they cost nothing that shows.  Rounded weights are what their sum
+// adds up, too: a result lies between the values whatever the rounding.
 //
 // What bounds it, on an MI355X whose large copies run at 4.85 TB/s and whose
 // large matrix products at 1,150 (fp16) to 1,210 (bf16) TFLOP/s:
@@ -99,6 +100,7 @@ struct Elem<_Float16> {
     static __device__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+    static __device__ float add(v2 e, float l) { return __builtin_amdgcn_fdot2(e, v2{1, 1}, l, false); }
     static __device__ v4 read_tr(const TER_LDS char* p) {
         typedef __fp16 h4 __attribute__((ext_vector_type(4)));
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((TER_LDS h4*)p));
@@ -119,6 +121,7 @@ struct Elem<__bf16> {
     static __device__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
     }
+    static __device__ float add(v2 e, float l) { return __builtin_amdgcn_fdot2_f32_bf16(e, v2{1, 1}, l, false); }
     static __device__ v4 read_tr(const TER_LDS char* p) {
         return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((TER_LDS v4*)p);
     }
@@ -633,10 +636,10 @@ struct Kernel {
             auto weight = [&](int b, int i) {  // elements i, i + 1
                 const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], a.scale2, wo));
                 const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], a.scale2, wo));
-                l += e0;
-                l += e1;
-                p[b][i >> 3][i & 7] = (T)e0;
-                p[b][i >> 3][(i & 7) + 1] = (T)e1;
+                const v2 e = {(T)e0, (T)e1};
+                p[b][i >> 3][i & 7] = e[0];
+                p[b][i >> 3][(i & 7) + 1] = e[1];
+                l = E::add(e, l);
             };
 
 #pragma unroll

@@ -97,6 +97,24 @@ def test_infinite_values_of_vanishing_weight(cuda, power, rows, shared, shape, d
 @pytest.mark.parametrize("shape", [dict(nh=4, nkv=2, hd=64), dict(nh=4, nkv=1, hd=128)], ids=["hd64", "hd128"])
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("shared", [0, 64])
+@pytest.mark.parametrize("value", ["1.5", "max", "-max"])
+def test_equal_values(cuda, value, shared, shape, dtype):
+    """Where all values are one number so is every result, up to the type's
+    largest: sums of n terms in binary32 are off by less than half a step."""
+    import ter_amd as T
+    seqs = [(60, 160), (1, 70), (3, 2500), (100, 900), (1, 3900), (70, 70)]
+    b = Batch(seqs, dtype=dtype, seed=11, page=16, common=shared, spread=1.5, **shape)
+    x = 1.5 if value == "1.5" else torch.finfo(dtype).max * (-1 if value[0] == "-" else 1)
+    b.v = torch.where(torch.isnan(b.v), b.v, torch.full_like(b.v, x))
+    assert max(b.lens) * 2.0 ** -23 < half_step(dtype)
+    cache, batch = b.on_device(T)
+    out = context(b).attend(b.q.cuda(), cache, batch, shared=shared)
+    assert (out == x).all(), out[out != x][:4]
+
+
+@pytest.mark.parametrize("shape", [dict(nh=4, nkv=2, hd=64), dict(nh=4, nkv=1, hd=128)], ids=["hd64", "hd128"])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("shared", [0, 64])
 def test_values_near_the_largest(cuda, shared, shape, dtype):
     """No sum on the way leaves binary32."""
     import ter_amd as T
