@@ -23,14 +23,15 @@
 // What bounds it, on an MI355X whose large copies run at 4.85 TB/s and whose
 // large matrix products at 1,150 (fp16) to 1,210 (bf16) TFLOP/s:
 //   single tokens: memory.  96 sequences of up to 4,095 positions (32 heads on
-//     8 of 64, 421 MB of keys and values) 84 us, 5.0 TB/s; one sequence of
-//     65,521 positions (20 on 5 of 128, 168 MB) 33 us, 5.1 TB/s, and 7 to join.
+//     8 of 64, 421 MB of keys and values) 86 us, 4.9 TB/s; one sequence of
+//     65,521 positions (20 on 5 of 128, 168 MB) 31 us, 5.4 TB/s, and 8 to join.
 //   prompts: a SIMD's matrix and vector work, which overlap in part only (two
 //     waves that alternate them take the matrix time and 0.4 of the vector
-//     time).  One prompt of 16,384 tokens (20 on 5 of 128, bf16) 1.49 ms, 924
-//     TFLOP/s, the matrix cores busy 44% of the cycles at the 1.7 GHz that this
-//     load runs at.  A workgroup of 256 rows, twice the rows a wave and half
-//     the LDS reads a product, took 1.70 ms: one wave a SIMD hides less.
+//     time).  One prompt of 16,384 tokens (20 on 5 of 128, bf16) 1.47 to 1.55
+//     ms, 890 to 935 TFLOP/s; in a run of 1.64 ms with counters (838 TFLOP/s)
+//     the matrix cores were busy 42% of the cycles, at 1.9 GHz.  A workgroup of
+//     256 rows, twice the rows a wave and half the LDS reads a product, took
+//     1.70 ms: one wave a SIMD hides less.
 //   small calls: latency.  A workgroup needs 3 to 5 us to find its range and
 //     have its first tiles, two launches 9 us of the host.
 #include "common.h"
