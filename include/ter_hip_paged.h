@@ -107,7 +107,9 @@ int ter_hip_paged_append(const ter_hip_paged_t* ctx, const ter_hip_paged_batch_t
  * elements of the cache's type (22 bits of fp16, 16 of bf16) where a KV head's
  * query heads times the sequence's rows in a tile are 16 or fewer, as those of
  * single tokens are, and to one element (11 or 8 bits) where they are more: of
- * prompts, and of all sequences' rows together on a shared prefix.
+ * prompts, and of all sequences' rows together on a shared prefix.  In fp16
+ * weights below 2^-33 of a row's largest are zero.  Where a row sees infinite
+ * values or NaN its result has them, whatever their weights.
  *
  * shared: the first `shared` positions of every sequence are the same pages
  * (row 0 of the table is read for them); rounded down to a multiple of 16.

@@ -127,3 +127,36 @@ def test_values_near_the_largest(cuda, shared, shape, dtype):
     assert torch.isfinite(out).all()
     want, tol = b.attend()
     compare(out, want, tol)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_many_small_weights(cuda, dtype, hd, rows):
+    """2^17 weights of 2^-23 of the largest, subnormal in fp16, are a 64th of
+    the sum: in it and in the product with the values alike."""
+    import ter_amd as T
+    n, page = 1 << 17, 64
+    k = torch.zeros(2, page, 1, hd, dtype=dtype, device="cuda")
+    k[0, 0] = 1.0  # page 0 is the first one only: one score of hd, zeros behind it
+    v = torch.ones_like(k)
+    q = torch.ones(rows, 4, hd, dtype=dtype, device="cuda")
+    table = torch.ones(1, n // page, dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    cache = T.PagedCache(k, v)
+    batch = T.PagedBatch(torch.tensor([0, rows], dtype=torch.int32, device="cuda"),
+                         torch.tensor([n], dtype=torch.int32, device="cuda"), table)
+    ctx = T.PagedAttention(4, 1, hd, 16, 1e4, dtype=dtype)
+    scale = 23 * math.log(2) / hd
+    # (sums of equal numbers in binary32, pieces of at most 2^12 of a lane, joined: 2^-11 would be seen)
+    assert (ctx.attend(q, cache, batch, scale=scale) == 1.0).all()
+    v[0, 0] = 0.0
+    m = torch.arange(n - rows, n, dtype=torch.float64) + 1
+    small = (m - 1) * 2.0 ** -23
+    want = (small / (1 + small))[:, None, None].expand(rows, 4, hd)
+    # an exponent of 23 from a rounded scale (2^-24 of it) and exp2, half a
+    # step of 2^-15 in subnormals of 2^-24, or of the element type, and of the
+    # result; sums of 2^17 terms in lanes and pieces of at most 2^12
+    u = half_step(dtype)
+    rel = 23 * 2.0 ** -23 + max(2.0 ** -10, u) + 2.0 ** -11 + u
+    compare(ctx.attend(q, cache, batch, scale=scale), want, want * rel)
