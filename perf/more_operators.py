@@ -15,9 +15,9 @@ one-row lm_head and argmax.
   sample   w_i = exp((l_i - max l) / T).  In the order of falling logits (of
            equal ones the lower index first): the first top_k; of those, the
            ones whose predecessors have less than top_p of the top_k's mass; of
-           those, the ones with w_i >= min_p.  The token is the lowest index at
-           which the sum of the kept w_i so far, in the order of indices,
-           exceeds u times their whole sum.  T = 0 takes the largest logit.
+           those, the ones with w_i >= min_p.  The token is the first, in the
+           same order, at which the sum of the kept w_i so far exceeds u times
+           their whole sum.  T = 0 takes the largest logit.
 
 `own` says which side run() computes: the plain form in elementary torch
 operations, or the calls of the framework.  The sizes are those of
@@ -200,11 +200,11 @@ def _sample(s):
     ranked = w.gather(1, order) * (torch.arange(v, device="cuda") < k)
     before = ranked.cumsum(1) - ranked
     keep = (before < p * ranked.sum(1, keepdim=True)) & (ranked >= q) & (torch.arange(v, device="cuda") < k)
-    kept = torch.zeros_like(w).scatter_(1, order, ranked * keep)
-    upto = kept.cumsum(1)
+    upto = (ranked * keep).cumsum(1)
     total = upto[:, -1:]
-    token = (upto <= s["u"].double()[:, None] * total).sum(1, keepdim=True)
-    return dict(token=token[:, 0].to(torch.int32), prob=(kept.gather(1, token) / total)[:, 0].float())
+    at = (upto <= s["u"].double()[:, None] * total).sum(1, keepdim=True)
+    token, prob = order.gather(1, at), ranked.gather(1, at) / total
+    return dict(token=token[:, 0].to(torch.int32), prob=prob[:, 0].float())
 
 
 def exact(case, seed):
@@ -240,7 +240,7 @@ def exact(case, seed):
         first = order[:int(ks[r])] if 0 < ks[r] < v else order
         mass = np.cumsum(w[first])
         n = 1 + int(np.searchsorted(mass, np.longdouble(ps[r]) * mass[-1]))
-        kept = np.sort(first[:n][w[first[:n]] >= qs[r]])
+        kept = first[:n][w[first[:n]] >= qs[r]]
         sums = np.cumsum(w[kept])
         i = int(np.searchsorted(sums, np.longdouble(u[r]) * sums[-1], side="right"))
         token[r], prob[r] = kept[i], w[kept[i]] / sums[-1]
