@@ -261,6 +261,51 @@ PAGED_SIGNATURES = [
                                        _P, C.c_size_t, _P]),
 ]
 
+T_F16, T_BF16, T_F32, T_I8, T_I32 = 0, 1, 2, 3, 4
+INT8_K_MAX = 131071
+INT8_N_MAX = 1 << 23
+INT8_M_MAX = 1 << 23
+INT8_Y_MAX = 1 << 36
+SAMPLE_V_MAX = 1 << 19
+SAMPLE_ROWS_MAX = 1 << 20
+
+
+class W8(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scale", C.c_void_p), ("bytes", C.c_size_t), ("K", C.c_int32),
+                ("N", C.c_int32)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scale", C.c_void_p), ("stride", C.c_int64), ("type", C.c_int32),
+                ("n", C.c_int32)]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [("temperature_dev", C.c_void_p), ("top_k_dev", C.c_void_p), ("top_p_dev", C.c_void_p),
+                ("min_p_dev", C.c_void_p), ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+
+_W8, _R = C.POINTER(W8), C.POINTER(Rows)
+
+# (name, result, argument types) of every symbol of include/ter_hip_int8.h
+INT8_SIGNATURES = [
+    ("ter_hip_w8_bytes", C.c_size_t, [C.c_int32, C.c_int32]),
+    ("ter_hip_w8_init", C.c_int, [_W8, _P, C.c_size_t, C.c_int32, C.c_int32]),
+    ("ter_hip_w8_pack", C.c_int, [_W8, _P, C.c_int64, _P, _P]),
+    ("ter_hip_w8_quantize", C.c_int, [_W8, _P, C.c_int32, C.c_int64, _P]),
+    ("ter_hip_w8_unpack", C.c_int, [_W8, _P, _P, _P]),
+    ("ter_hip_w8_mm_ws", C.c_size_t, [_W8, _R]),
+    ("ter_hip_w8_mm", C.c_int, [_W8, _R, _P, C.c_int64, C.c_int32, _P, C.c_size_t, _P]),
+]
+
+# (name, result, argument types) of every symbol of include/ter_hip_sample.h
+SAMPLE_SIGNATURES = [
+    ("ter_hip_sample_ws", C.c_size_t, [C.c_int32, C.c_int32]),
+    ("ter_hip_sample", C.c_int, [_P, C.c_int32, C.c_int64, C.c_int32, C.c_int32, _P, C.POINTER(SampleParams), _P, _P,
+                                 _P, C.c_size_t, _P]),
+]
+
 _lib = None
 
 
@@ -291,7 +336,7 @@ def lib():
         except ImportError:
             pass
         L = C.CDLL(LIB_PATH)
-        for name, res, args in SIGNATURES + PAGED_SIGNATURES:
+        for name, res, args in SIGNATURES + PAGED_SIGNATURES + INT8_SIGNATURES + SAMPLE_SIGNATURES:
             f = getattr(L, name)
             f.restype = res
             f.argtypes = args

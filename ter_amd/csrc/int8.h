@@ -1,0 +1,53 @@
+// int8.h -- shared definitions of the 8-bit products (include/ter_hip_int8.h).
+//
+// Weight layout.  Channels are cut into strips of 16 and K into units of 128
+// (zero-padded).  A tile is one strip x 64 values of K in the order in which
+// v_mfma_i32_16x16x64_i8 takes an operand: lane l's 16 bytes, row l % 16 of
+// the strip, k = 16 * (l / 16) .. + 15, at byte 16 * l of 1024.  Tile (strip
+// s, k-tile t) is at (s * 2 Ku + t) * 1024, Ku = ceil(K / 128): one wave reads
+// an operand with one 16-byte load a lane over 1 KiB without gaps, from memory
+// straight to registers or, past LDS, without bank conflicts.
+//
+// Two strips hold 32 channels, dealt to them by fours: row 4 g + r of strip
+// 2 p + t is channel 32 p + 8 g + 4 t + r.  The weights are the product's A
+// operand, so a lane's sums are rows 4 g .. 4 g + 3 (g = l / 16) of token
+// l % 16: of the two strips together, 8 consecutive channels of one token,
+// which are one 16-byte store in 16 bits, 64 contiguous bytes a token and wave.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ter_hip_int8.h"
+
+namespace terhip {
+
+constexpr int kI8Unit = 128;  // K is padded to this
+__host__ __device__ inline int i8_units(int K) { return (K + kI8Unit - 1) / kI8Unit; }
+__host__ __device__ inline int i8_pairs(int N) { return (N + 31) / 32; }  // of strips
+inline size_t i8_tile_bytes(int K, int N) { return (size_t)i8_pairs(N) * i8_units(K) * 4096; }
+
+struct Int8MmArgs {
+    const uint8_t* w;     // tiles
+    const float* ws;      // [32 pairs] (zero behind N)
+    const int8_t* x;      // [M] rows, 16-byte aligned, a multiple of 16 values each
+    const float* xs;      // [M], or null (y_type I32)
+    char* y;
+    long long ldx, ldy;   // bytes, elements
+    int M, N, Kx, Ku;     // Kx: values of a row of x (a multiple of 16; those from K on meet zero weights)
+    int y_type;
+};
+
+hipError_t launch_w8_pack(const int8_t* q, long long stride, const float* scale, uint8_t* tiles, float* out_scale,
+                          int K, int N, hipStream_t st);
+hipError_t launch_w8_quantize(const void* src, int type, long long stride, uint8_t* tiles, float* out_scale, int K,
+                              int N, hipStream_t st);
+hipError_t launch_w8_unpack(const uint8_t* tiles, const float* scale, int8_t* q, float* out_scale, int K, int N,
+                            hipStream_t st);
+// Rows to int8 rows ldq bytes apart (a multiple of 16) with zeros behind K;
+// scales [M] for types other than TER_HIP_T_I8.
+hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                        hipStream_t st);
+hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st);
+
+}  // namespace terhip

@@ -1,0 +1,240 @@
+// int8_pack.hip -- weights in 8 bits to and from the tiles of int8.h, and the
+// rows of a product in 8 bits: quantized by their largest magnitude, or
+// integers laid out at 16-byte alignment.
+//
+// Quantizing reads a row twice (its largest magnitude, then its values) by one
+// workgroup: the second time from the cache.
+#include "common.h"
+#include "int8.h"
+
+namespace terhip {
+namespace {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<TER_HIP_T_F16> {
+    typedef uint16_t T;
+    static __device__ float get(T v) { return half_bits_to_float(v); }
+};
+template <>
+struct Elem<TER_HIP_T_BF16> {
+    typedef uint16_t T;
+    static __device__ float get(T v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
+};
+template <>
+struct Elem<TER_HIP_T_F32> {
+    typedef float T;
+    static __device__ float get(T v) { return v; }
+};
+
+// The largest magnitude of a workgroup's values as bits (an infinity or NaN is
+// larger than any number), to every thread.
+__device__ unsigned block_max(unsigned v, unsigned* red) {
+    for (int s = 32; s; s >>= 1) {
+        const unsigned o = (unsigned)__shfl_xor((int)v, s);
+        v = o > v ? o : v;
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) v = red[i] > v ? red[i] : v;
+    __syncthreads();
+    return v;
+}
+
+struct Quant {
+    float s, inv;
+};
+
+// The steps of quant_rows_kernel (pack.hip), binary32, each rounded.
+__device__ __forceinline__ Quant quant_of(unsigned amax_bits) {
+#pragma clang fp contract(off)
+    Quant q;
+    q.s = 127.0f / (__builtin_bit_cast(float, amax_bits) + 1e-9f);
+    q.inv = 1.0f / q.s;
+    if (amax_bits >= 0x7F800000u) {  // an infinity or NaN in the row
+        q.s = 0.f;
+        q.inv = __builtin_nanf("");
+    }
+    return q;
+}
+
+__device__ __forceinline__ int quantize(float v, float s) {
+#pragma clang fp contract(off)
+    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_rintf(v * s), -128.f), 127.f);  // (of NaN -128)
+}
+
+// Largest magnitude of row `row` of K elements.
+template <int TYPE>
+__device__ unsigned row_amax(const typename Elem<TYPE>::T* row, int K, unsigned* red) {
+    unsigned m = 0;
+    for (int k = threadIdx.x; k < K; k += blockDim.x) {
+        const unsigned b = __builtin_bit_cast(unsigned, Elem<TYPE>::get(gptr(row)[k])) & 0x7FFFFFFFu;
+        m = b > m ? b : m;
+    }
+    return block_max(m, red);
+}
+
+// One workgroup a row: int8 rows, 16 values a thread.
+template <int TYPE>
+__global__ __launch_bounds__(256) void rows8_quant_kernel(const void* __restrict__ x, long long stride, int K,
+                                                          int8_t* __restrict__ q, long long ldq,
+                                                          float* __restrict__ scale) {
+    typedef typename Elem<TYPE>::T T;
+    __shared__ unsigned red[4];
+    const T* row = static_cast<const T*>(x) + (long long)blockIdx.x * stride;
+    const Quant z = quant_of(row_amax<TYPE>(row, K, red));
+    if (threadIdx.x == 0) gptr(scale)[blockIdx.x] = z.inv;
+    int8_t* out = q + (long long)blockIdx.x * ldq;
+    for (int k = threadIdx.x * 4; k < ldq; k += 1024) {
+        unsigned v = 0;
+        for (int i = 0; i < 4; ++i)
+            if (k + i < K) v |= ((unsigned)quantize(Elem<TYPE>::get(gptr(row)[k + i]), z.s) & 255u) << (8 * i);
+        *reinterpret_cast<TER_GLOBAL unsigned*>(gptr(out) + k) = v;
+    }
+}
+
+// Integer rows at any alignment to aligned ones, 16 bytes a thread.
+__global__ __launch_bounds__(256) void rows8_copy_kernel(const int8_t* __restrict__ x, long long stride, int K,
+                                                         int8_t* __restrict__ q, long long ldq, int chunks,
+                                                         long long total) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256ll * gridDim.x) {
+        const long long m = i / chunks;
+        const int k0 = (int)(i - m * chunks) * 16;
+        const int8_t* row = x + m * stride;
+        u32x4 v;
+        for (int j = 0; j < 4; ++j) {
+            unsigned d = 0;
+            for (int b = 0; b < 4; ++b) {
+                const int k = k0 + 4 * j + b;
+                if (k < K) d |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+            }
+            v[j] = d;
+        }
+        *reinterpret_cast<TER_GLOBAL u32x4*>(gptr(q) + m * ldq + k0) = v;
+    }
+}
+
+// Chunk c (16 values of K) of channel n within the tiles.
+__device__ __forceinline__ long long chunk_at(int n, int c, int Ku) {
+    const int strip = 2 * (n >> 5) + ((n >> 2) & 1), row = 4 * ((n >> 3) & 3) + (n & 3);
+    return ((long long)strip * (2 * Ku) + (c >> 2)) * 1024 + ((c & 3) * 16 + row) * 16;
+}
+
+// One workgroup a channel (those that pad the last strip are zero).
+template <int TYPE>
+__global__ __launch_bounds__(256) void w8_quantize_kernel(const void* __restrict__ src, long long stride, int K, int N,
+                                                          int Ku, uint8_t* __restrict__ tiles,
+                                                          float* __restrict__ scale) {
+    typedef typename Elem<TYPE>::T T;
+    __shared__ unsigned red[4];
+    const int n = blockIdx.x;
+    const T* row = static_cast<const T*>(src) + (long long)(n < N ? n : 0) * stride;
+    Quant z{};
+    if (n < N) z = quant_of(row_amax<TYPE>(row, K, red));  // (by workgroups)
+    if (threadIdx.x == 0) gptr(scale)[n] = z.inv;
+    for (int c = threadIdx.x; c < 8 * Ku; c += 256) {
+        u32x4 v;
+        for (int j = 0; j < 4; ++j) {
+            unsigned d = 0;
+            for (int b = 0; b < 4; ++b) {
+                const int k = c * 16 + 4 * j + b;
+                if (n < N && k < K) d |= ((unsigned)quantize(Elem<TYPE>::get(gptr(row)[k]), z.s) & 255u) << (8 * b);
+            }
+            v[j] = d;
+        }
+        *reinterpret_cast<TER_GLOBAL u32x4*>(gptr(tiles) + chunk_at(n, c, Ku)) = v;
+    }
+}
+
+// One thread a chunk.
+__global__ __launch_bounds__(256) void w8_pack_kernel(const int8_t* __restrict__ q, long long stride,
+                                                      const float* __restrict__ src_scale, int K, int N, int Ku,
+                                                      uint8_t* __restrict__ tiles, float* __restrict__ scale,
+                                                      long long total) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256ll * gridDim.x) {
+        const int n = (int)(i / (8 * Ku)), c = (int)(i % (8 * Ku));
+        if (c == 0) gptr(scale)[n] = n < N ? gptr(src_scale)[n] : 0.f;
+        const int8_t* row = q + (long long)n * stride;
+        u32x4 v;
+        for (int j = 0; j < 4; ++j) {
+            unsigned d = 0;
+            for (int b = 0; b < 4; ++b) {
+                const int k = c * 16 + 4 * j + b;
+                if (n < N && k < K) d |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+            }
+            v[j] = d;
+        }
+        *reinterpret_cast<TER_GLOBAL u32x4*>(gptr(tiles) + chunk_at(n, c, Ku)) = v;
+    }
+}
+
+__global__ __launch_bounds__(256) void w8_unpack_kernel(const uint8_t* __restrict__ tiles,
+                                                        const float* __restrict__ scale, int K, int N, int Ku,
+                                                        int8_t* __restrict__ q, float* __restrict__ out_scale,
+                                                        long long total) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256ll * gridDim.x) {
+        const int n = (int)(i / K), k = (int)(i % K);
+        if (q) gptr(q)[i] = (int8_t)gptr(tiles)[chunk_at(n, k >> 4, Ku) + (k & 15)];
+        if (out_scale && k == 0) gptr(out_scale)[n] = gptr(scale)[n];
+    }
+}
+
+inline unsigned grid_of(long long n) { return (unsigned)(n < (1ll << 30) ? (n + 255) / 256 : 1 << 22); }
+
+}  // namespace
+
+hipError_t launch_w8_pack(const int8_t* q, long long stride, const float* scale, uint8_t* tiles, float* out_scale,
+                          int K, int N, hipStream_t st) {
+    const int Ku = i8_units(K);
+    const long long n = (long long)i8_pairs(N) * 32 * 8 * Ku;
+    hipLaunchKernelGGL(w8_pack_kernel, dim3(grid_of(n)), dim3(256), 0, st, q, stride, scale, K, N, Ku, tiles, out_scale,
+                       n);
+    return hipGetLastError();
+}
+
+hipError_t launch_w8_quantize(const void* src, int type, long long stride, uint8_t* tiles, float* out_scale, int K,
+                              int N, hipStream_t st) {
+    const dim3 grid(i8_pairs(N) * 32);
+    const int Ku = i8_units(K);
+    if (type == TER_HIP_T_F16)
+        hipLaunchKernelGGL(w8_quantize_kernel<TER_HIP_T_F16>, grid, dim3(256), 0, st, src, stride, K, N, Ku, tiles,
+                           out_scale);
+    else if (type == TER_HIP_T_BF16)
+        hipLaunchKernelGGL(w8_quantize_kernel<TER_HIP_T_BF16>, grid, dim3(256), 0, st, src, stride, K, N, Ku, tiles,
+                           out_scale);
+    else
+        hipLaunchKernelGGL(w8_quantize_kernel<TER_HIP_T_F32>, grid, dim3(256), 0, st, src, stride, K, N, Ku, tiles,
+                           out_scale);
+    return hipGetLastError();
+}
+
+hipError_t launch_w8_unpack(const uint8_t* tiles, const float* scale, int8_t* q, float* out_scale, int K, int N,
+                            hipStream_t st) {
+    const long long n = (long long)N * K;
+    hipLaunchKernelGGL(w8_unpack_kernel, dim3(grid_of(n)), dim3(256), 0, st, tiles, scale, K, N, i8_units(K), q,
+                       out_scale, n);
+    return hipGetLastError();
+}
+
+hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                        hipStream_t st) {
+    if (type == TER_HIP_T_I8) {
+        const int chunks = (int)(ldq / 16);
+        const long long n = (long long)M * chunks;
+        hipLaunchKernelGGL(rows8_copy_kernel, dim3(grid_of(n)), dim3(256), 0, st, static_cast<const int8_t*>(x), stride,
+                           K, q, ldq, chunks, n);
+    } else if (type == TER_HIP_T_F16) {
+        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_F16>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+    } else if (type == TER_HIP_T_BF16) {
+        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_BF16>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+    } else {
+        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_F32>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace terhip

@@ -735,6 +735,207 @@ class PagedAttention:
             pass
 
 
+def _row_types():
+    torch = _torch()
+    return {torch.float16: L.T_F16, torch.bfloat16: L.T_BF16, torch.float32: L.T_F32, torch.int8: L.T_I8,
+            torch.int32: L.T_I32}
+
+
+_types = None
+
+
+def _type_of(dtype, among, name: str) -> int:
+    """The TER_HIP_T_* of a torch type, one of `among`."""
+    global _types
+    if _types is None:
+        _types = _row_types()
+    t = _types.get(dtype, -1)
+    if t not in among:
+        raise TypeError(f"{name} cannot be {dtype}")
+    return t
+
+
+def _matrix(t, name: str, device: Optional[int] = None, width: Optional[int] = None) -> int:
+    """Checks a CUDA matrix with contiguous rows; returns their stride."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or (device is not None and t.get_device() != device):
+        raise TypeError(f"{name} must be a CUDA tensor" + ("" if device is None else f" on cuda:{device}"))
+    s = t.shape
+    if len(s) != 2 or (width is not None and s[1] != width):
+        raise ValueError(f"{name} must be [rows][{'columns' if width is None else width}], got {list(s)}")
+    st = t.stride()
+    if s[1] > 1 and st[1] != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    # (the stride of a dimension of size 1 says nothing)
+    return st[0] if s[0] > 1 else max(s[1], 1)
+
+
+def _vector(t, name: str, dtype, n: int, device: int):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda or t.get_device() != device:
+        raise TypeError(f"{name} must be a {dtype} tensor on cuda:{device}")
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be [{n}], contiguous")
+    return t
+
+
+def _launch_on(device: int, name: str, stream, *args):
+    """Calls the function on `device` and its current stream, or the given one."""
+    torch, fn = _torch(), getattr(L.lib(), name)
+    was = torch._C._cuda_getDevice()
+    if was != device:
+        torch.cuda.set_device(device)
+    try:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream)
+    finally:
+        if was != device:
+            torch.cuda.set_device(was)
+    if rc:
+        L.check(rc, name)
+
+
+def _empty_on(device: int, stream, shape, dtype):
+    """A tensor of the allocator of the stream (or graph) that will use it."""
+    torch = _torch()
+    if stream is not None:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+class PackedInt8:
+    """A weight in 8-bit integers, N channels of K values with a scale for each
+    channel, resident on the device in the layout that mm_int8 streams
+    (ter_hip_w8_*).  Beside PackedTrits, for what is not ternary: a head, an
+    embedding, a projection."""
+
+    def __init__(self, K: int, N: int, device=None):
+        torch = _torch()
+        self.K, self.N = int(K), int(N)
+        nbytes = L.lib().ter_hip_w8_bytes(self.K, self.N) if 0 < self.K < 1 << 31 and 0 < self.N < 1 << 31 else 0
+        if nbytes == 0:
+            raise ValueError(f"bad shape K={K} N={N}")
+        self.buf = torch.empty(nbytes, dtype=torch.uint8, device="cuda" if device is None else device)
+        self.w8 = L.W8()
+        L.check(L.lib().ter_hip_w8_init(C.byref(self.w8), self.buf.data_ptr(), nbytes, self.K, self.N),
+                "ter_hip_w8_init")
+        self._ref = C.byref(self.w8)
+        self._dev = self.buf.get_device()
+
+    @classmethod
+    def from_int8(cls, q, scale, stream=None) -> "PackedInt8":
+        """From integers q int8 [N][K] and their scales fp32 [N]."""
+        torch = _torch()
+        st = _matrix(q, "q")
+        _type_of(q.dtype, (L.T_I8,), "q")
+        _vector(scale, "scale", torch.float32, q.shape[0], q.get_device())
+        w = cls(q.shape[1], q.shape[0], device=q.device)
+        _launch_on(w._dev, "ter_hip_w8_pack", stream, w._ref, q.data_ptr(), st, scale.data_ptr())
+        return w
+
+    @classmethod
+    def quantize(cls, w, stream=None) -> "PackedInt8":
+        """From fp16, bf16 or fp32 w [N][K], each channel by its largest
+        magnitude (the steps of quant_int8)."""
+        st = _matrix(w, "w")
+        ty = _type_of(w.dtype, (L.T_F16, L.T_BF16, L.T_F32), "w")
+        p = cls(w.shape[1], w.shape[0], device=w.device)
+        _launch_on(p._dev, "ter_hip_w8_quantize", stream, p._ref, w.data_ptr(), ty, st)
+        return p
+
+    def to_int8(self, stream=None):
+        """(q int8 [N][K], scale fp32 [N])."""
+        torch = _torch()
+        q = _empty_on(self._dev, stream, (self.N, self.K), torch.int8)
+        scale = _empty_on(self._dev, stream, (self.N,), torch.float32)
+        _launch_on(self._dev, "ter_hip_w8_unpack", stream, self._ref, q.data_ptr(), scale.data_ptr())
+        return q, scale
+
+
+def mm_int8(W: PackedInt8, x, x_scale=None, dtype=None, out=None, stream=None):
+    """y[m][n] = (sum_k x[m][k] W[n][k]) * (x_scale[m] * W.scale[n]), the sum
+    exact in int32.  x: int8 [M][K] with x_scale fp32 [M], or fp16, bf16 or
+    fp32 [M][K], whose rows are quantized within the call (quant_int8 steps;
+    a row with an infinity or NaN gives NaN); rows may be parts of wider ones.
+    y [M][N] is `out` or a new tensor of type `dtype`: fp16, bf16, fp32, or,
+    of int8 rows, int32 for the bare sums; by default x's type, or fp32 of int8
+    rows.  Returns y."""
+    torch = _torch()
+    dev = W._dev
+    xs = _matrix(x, "x", dev, W.K)
+    xt = _type_of(x.dtype, (L.T_F16, L.T_BF16, L.T_F32, L.T_I8), "x")
+    M = x.shape[0]
+    if out is not None:
+        if dtype is not None and dtype != out.dtype:
+            raise TypeError(f"out is {out.dtype}, not {dtype}")
+        dtype = out.dtype
+    elif dtype is None:
+        dtype = torch.float32 if xt == L.T_I8 else x.dtype
+    yt = _type_of(dtype, (L.T_F16, L.T_BF16, L.T_F32) + ((L.T_I32,) if xt == L.T_I8 else ()), "the result")
+    if xt != L.T_I8:
+        if x_scale is not None:
+            raise ValueError("x_scale goes with int8 rows")
+    elif yt != L.T_I32:
+        _vector(x_scale, "x_scale", torch.float32, M, dev)
+    if out is None:
+        out = _empty_on(dev, stream, (M, W.N), dtype)
+        ys = W.N
+    else:
+        ys = _matrix(out, "out", dev, W.N)
+        if out.shape[0] != M:
+            raise ValueError(f"out must be [{M}][{W.N}]")
+    rows = L.Rows(x.data_ptr(), _ptr(x_scale), xs, xt, M)
+    need = L.lib().ter_hip_w8_mm_ws(W._ref, C.byref(rows))
+    # a workspace of its own for every call, from the allocator of the stream
+    # (or graph) that runs it
+    ws = _empty_on(dev, stream, (need,), torch.uint8) if need else None
+    _launch_on(dev, "ter_hip_w8_mm", stream, W._ref, C.byref(rows), out.data_ptr(), ys, yt, _ptr(ws), need)
+    return out
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, prob_out=None, stream=None):
+    """A token for each row of logits [M][V] (fp16, bf16 or fp32, rows possibly
+    parts of wider ones), drawn with the random numbers u fp32 [M] in [0, 1).
+    In the order of falling logits (of equal ones the lower index first) the
+    first top_k are kept, of those the ones whose predecessors have less than
+    top_p of the top_k's probability, of those the ones with at least min_p of
+    the largest probability; the token is the first at which the kept
+    probabilities sum to more than u of their whole.  temperature 0 takes the
+    largest logit, top_k 0, top_p 1 and min_p 0 keep all.  Each setting is a
+    number or a CUDA tensor [M] (fp32; top_k int32), read when the launch runs.
+    Logits of -infinity or NaN are never drawn; a row of nothing else gives -1.
+    Returns the tokens, int32 [M] (`out`); prob_out fp32 [M] receives the
+    probability with which each was drawn."""
+    torch = _torch()
+    st = _matrix(logits, "logits")
+    ty = _type_of(logits.dtype, (L.T_F16, L.T_BF16, L.T_F32), "logits")
+    dev = logits.get_device()
+    M, V = logits.shape
+    _vector(u, "u", torch.float32, M, dev)
+    p = L.SampleParams()
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            setattr(p, name + "_dev", _vector(v, name, dtype, M, dev).data_ptr())
+        elif name == "top_k":
+            if v != int(v) or not 0 <= v:
+                raise ValueError("top_k must be a whole number >= 0")
+            p.top_k = min(int(v), (1 << 31) - 1)
+        else:
+            setattr(p, name, v)
+    if out is None:
+        out = _empty_on(dev, stream, (M,), torch.int32)
+    else:
+        _vector(out, "out", torch.int32, M, dev)
+    if prob_out is not None:
+        _vector(prob_out, "prob_out", torch.float32, M, dev)
+    need = L.lib().ter_hip_sample_ws(M, V)
+    ws = _empty_on(dev, stream, (need,), torch.uint8) if need else None
+    _launch_on(dev, "ter_hip_sample", stream, logits.data_ptr(), ty, st, M, V, u.data_ptr(), C.byref(p),
+               out.data_ptr(), _ptr(prob_out), _ptr(ws), need)
+    return out
+
+
 def _held(it: dict) -> list:
     """What a plan built from item `it` must keep alive: the device table
     holds raw pointers into the weight buffer (as it was when the plan was
