@@ -8,6 +8,28 @@
 
 namespace terhip {
 
+constexpr int kBins = 2048;   // of a row's histogram (sample.hip)
+constexpr int kList = 8192;   // elements listed at most: else the general path
+constexpr int kSlices = 64;   // workgroups of a row at most
+
+// Workspace of a row that several workgroups work on.
+struct SampleRow {
+    unsigned long long mass[kBins];
+    unsigned long long list[kList];
+    unsigned count[kBins];
+    float slice_max[kSlices];
+    unsigned n;  // elements listed (more than kList: not all are)
+    unsigned pad[3];
+};
+
+// Workgroups of a row: 1 where rows alone fill the GPU (a call needs no
+// workspace then).
+inline int sample_slices(int rows, int V) {
+    const int want = (V + 4095) / 4096, fit = 512 / (rows > 0 ? rows : 1);
+    const int n = want < fit ? want : fit;
+    return n < kSlices ? n : kSlices;
+}
+
 struct SampleArgs {
     const char* logits;
     long long stride;  // bytes
@@ -16,6 +38,8 @@ struct SampleArgs {
     ter_hip_sample_params_t p;
     int32_t* token;
     float* prob;  // or null
+    SampleRow* ws;
+    int slices;
 };
 
 hipError_t launch_sample(const SampleArgs& a, int type, hipStream_t st);

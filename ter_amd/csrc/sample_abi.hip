@@ -21,8 +21,8 @@ bool shape_ok(int rows, int V) {
 extern "C" {
 
 size_t ter_hip_sample_ws(int32_t rows, int32_t V) {
-    if (!shape_ok(rows, V)) return 0;
-    return 0;
+    if (!shape_ok(rows, V) || sample_slices(rows, V) <= 1) return 0;
+    return (size_t)rows * sizeof(SampleRow);
 }
 
 int ter_hip_sample(const void* logits, int32_t type, int64_t stride, int32_t rows, int32_t V, const float* u,
@@ -59,6 +59,8 @@ int ter_hip_sample(const void* logits, int32_t type, int64_t stride, int32_t row
     a.p = p;
     a.token = token;
     a.prob = prob;
+    a.ws = static_cast<SampleRow*>(ws);
+    a.slices = sample_slices(rows, V);
     const hipError_t e = launch_sample(a, type, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "sampling launch");
     return TER_HIP_OK;
