@@ -17,10 +17,14 @@ struct SampleRow {
     unsigned long long mass[kBins];
     unsigned long long list[kList];
     unsigned count[kBins];
-    float slice_max[kSlices];
+    unsigned long long run_mass[3], total, least_mass;
+    unsigned run_count[3];
+    int lo[3], hi[3];
     unsigned n;  // elements listed (more than kList: not all are)
-    unsigned pad[3];
+    float slice_high[kSlices], slice_low[kSlices];
+    unsigned pad[4];
 };
+static_assert(sizeof(SampleRow) % 16 == 0, "");
 
 // Workgroups of a row: 1 where rows alone fill the GPU (a call needs no
 // workspace then).

@@ -52,12 +52,14 @@ constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest lo
 // (ln 2 / 512)^4 / 24 = 2^-42.7), 2^(n >> 8) by the exponent.  t is rounded
 // twice, relative 2^-52 of at most 2^13.5: 2^-47 of the result.
 struct Weights {
-    const double* table;  // 2^(j / 256), in LDS
+    const double* table;  // 2^(44 + j / 256), in LDS
     double m, c;
 
     __device__ __forceinline__ double scaled(float x) const {
-        double t = ((double)x - m) * c;
-        t = __builtin_fmax(t, -12032.0);  // 2^-47; also of -infinity, and of NaN (-infinity times 0)
+        // (from -12032, 2^-47, on all the same; also of -infinity, and of NaN, -infinity times 0)
+        return of(__builtin_fmax(((double)x - m) * c, -12032.0));
+    }
+    __device__ __forceinline__ double of(double t) const {
         const double tn = t + 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer, in the low bits
         const int n = (int)__builtin_bit_cast(u64, tn);
         const double r = t - (tn - 6755399441055744.0);
@@ -65,12 +67,15 @@ struct Weights {
         double p = __builtin_fma(r, a * a * a / 6, a * a / 2);
         p = __builtin_fma(r, p, a);
         p = __builtin_fma(r, p, 1.0);
-        return __builtin_ldexp(table[n & 255] * p, 44 + (n >> 8));
+        return __builtin_ldexp(table[n & 255] * p, n >> 8);
     }
-    __device__ __forceinline__ u64 operator()(float x) const {
-        // (below 2^52 the low bits of a number added to 2^52 are its nearest integer)
-        return __builtin_bit_cast(u64, scaled(x) + 4503599627370496.0) - 0x4330000000000000ull;
+    // (below 2^52 the low bits of a number added to 2^52 are its nearest integer)
+    static __device__ __forceinline__ u64 whole(double v) {
+        return __builtin_bit_cast(u64, v + 4503599627370496.0) - 0x4330000000000000ull;
     }
+    __device__ __forceinline__ u64 operator()(float x) const { return whole(scaled(x)); }
+    // the same for logits less than 32 T below the largest; anything for others
+    __device__ __forceinline__ u64 quick(float x) const { return whole(of(((double)x - m) * c)); }
 };
 
 __device__ __forceinline__ Weights weights_of(const double* table, float m, double T) {
@@ -303,30 +308,34 @@ __device__ void sample_row(const SampleArgs& a, int row, const double* table, Sh
     }
 }
 
-
-// ---- the usual path: two levels ----
+// ---- the usual path: bins of bins ----
 //
-// The row is cut into bins of falling weight: bin b of logit x is
-// floor((m - x) / T * (kBins - 1) / 31.5), clipped to kBins - 1, in binary32.
-// Its steps are monotonic, so bins stand in the order of the logits and one
-// holds all elements between two values; from 31.5 on weights are 0, so the
-// last bin has none (and is not counted up).  A histogram of numbers or of
-// weights over the bins finds the bin of each cut and of the draw; the elements
-// of those bins, few, are then listed, sorted, and the places found exactly.
-// A cut moves what later ones start from, so before the list is there a later
-// place is known to a bin or two only: all of them are listed.
+// The row is cut into bins of falling logits: bin floor(y), y = (m - x) /
+// range * (kBins - 2), in binary32, where range is the smallest of 31.5 T and
+// the row's own.  Its steps are monotonic, so bins stand in the order of the
+// logits and one holds all elements between two values.  The last bin, kBins -
+// 1, takes what has no weight (31.5 T and more below m) and is not counted.  A
+// histogram of numbers or of weights over the bins finds the bin of each cut
+// and of the draw.  A cut moves what later ones start from, so a later place
+// is known to a bin or two only: all of them are listed.  The same again over
+// the listed elements, a bin cut into up to 256, leaves a few elements, which
+// one wave compares with each other, or many equal ones.
 constexpr int kCountK = 1024; // up to this top_k everything kept is listed, and weights are computed for the list alone
+constexpr int kFew = 64;      // elements compared by one wave
+constexpr int kValues = 8;    // different values among more elements than that
 
 struct Bins {
     float mh, cb;  // m / 2; bins for half a logit
-    __device__ __forceinline__ int operator()(float x) const {
-        // (halves do not overflow; NaN and -infinity: the last; +infinity: the first)
-        return (int)(unsigned)__builtin_fminf(__builtin_fmaf(x, -0.5f, mh) * cb, (float)(kBins - 1));
+    __device__ __forceinline__ float operator()(float x) const {
+        return __builtin_fmaf(x, -0.5f, mh) * cb;  // (halves do not overflow; NaN of NaN, +infinity of -infinity)
     }
 };
+constexpr float kLast = (float)(kBins - 1);
 
-__device__ __forceinline__ Bins bins_of(float m, double T) {
-    return Bins{0.5f * m, (float)__builtin_fmin(2.0 * (kBins - 1) / 31.5 / T, 3e38)};
+// m, low: the largest logit and the smallest that is a number.
+__device__ __forceinline__ Bins bins_of(float m, float low, double T) {
+    const double range = __builtin_fmin(31.5 * T, ((double)m - (double)low) * 1.001);
+    return Bins{0.5f * m, (float)__builtin_fmin(2.0 * (kBins - 2) / range, 3e38)};
 }
 
 // What a row's histogram counts.
@@ -335,7 +344,12 @@ __device__ __forceinline__ int mode_of(const Settings& s, int V) {
     return s.k <= kCountK && s.k < V ? kCount : s.k < V ? kBoth : kMass;
 }
 
-struct Lds {
+struct LdsSmall {
+    u64 wave_mass[kWaves];
+    unsigned wave_count[kWaves];
+};
+
+struct Lds : LdsSmall {
     double table[256];
     union {
         struct {
@@ -345,36 +359,38 @@ struct Lds {
         };
         Shared general;
     };
-    u64 wave_mass[kWaves];
-    unsigned wave_count[kWaves];
-    u64 place[8];
-    int cross[8];
+    // places of a level: bin, sums at its start and end
+    int at[8];
+    u64 from[8], to[8];
+    u64 least_mass;       // sum of the weights that min-p keeps
     int n;
 };
 
-// f(x) or f(x, i) of elements [i0, i1) of a row by `nt` threads, 16 bytes a
+// f(x, i) of elements [i0, i1) of a row by the workgroup's threads, 16 bytes a
 // load, four loads in flight.
 template <int TYPE, typename F>
-__device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0, int i1, int t, int nt, F f) {
+__device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0, int i1, F f) {
     typedef typename Logit<TYPE>::T T;
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
     constexpr int VE = 16 / (int)sizeof(T), U = 4;
+    const int t = threadIdx.x;
     const TER_GLOBAL T* p = gptr(row) + i0;
     const int n = i1 - i0;
     int head = (int)((0 - reinterpret_cast<uintptr_t>(row + i0)) & 15) / (int)sizeof(T);
     head = head < n ? head : n;
     const int nv = (n - head) / VE, tail = head + nv * VE;
-    if (t < head) f(Logit<TYPE>::raw(p[t]), i0 + t);
-    if (t < n - tail) f(Logit<TYPE>::raw(p[tail + t]), i0 + tail + t);
+    // (the elements outside of whole vectors: at most 2 VE - 2, one a thread)
+    const int odd = t < head ? t : t - head < n - tail ? tail + t - head : -1;
+    if (odd >= 0) f(Logit<TYPE>::raw(p[odd]), i0 + odd);
     const TER_GLOBAL u32x4* v = reinterpret_cast<const TER_GLOBAL u32x4*>(p + head);
-    for (int a = t; a < nv; a += U * nt) {
+    for (int a = t; a < nv; a += U * kThreads) {
         u32x4 r[U];
 #pragma unroll
-        for (int q = 0; q < U; ++q) r[q] = v[a + q * nt < nv ? a + q * nt : nv - 1];
+        for (int q = 0; q < U; ++q) r[q] = v[a + q * kThreads < nv ? a + q * kThreads : nv - 1];
 #pragma unroll
         for (int q = 0; q < U; ++q) {
-            if (a + q * nt >= nv) break;
-            const int i = i0 + head + (a + q * nt) * VE;
+            if (a + q * kThreads >= nv) break;
+            const int i = i0 + head + (a + q * kThreads) * VE;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned w = r[q][e];
@@ -389,24 +405,36 @@ __device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0,
     }
 }
 
-// The largest logit of [i0, i1), to every thread of the workgroup.
+// The largest logit of a row or slice, and the smallest that is a number.
+struct Extent {
+    float high, low;
+    __device__ void join(float h, float l) {
+        high = __builtin_fmaxf(high, h);
+        low = __builtin_fminf(low, l);
+    }
+};
+
 template <int TYPE>
-__device__ float largest_of(const typename Logit<TYPE>::T* row, int i0, int i1, Lds& sh) {
-    float m = -__builtin_inff();
-    each<TYPE>(row, i0, i1, threadIdx.x, kThreads, [&](float x, int) { m = __builtin_fmaxf(m, x); });
-    for (int s = 1; s < 64; s <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, s));
-    if ((threadIdx.x & 63) == 0) sh.wave_count[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, m);
+__device__ Extent extent_of(const typename Logit<TYPE>::T* row, int i0, int i1, LdsSmall& sh) {
+    Extent x{-__builtin_inff(), __builtin_inff()};
+    each<TYPE>(row, i0, i1, [&](float v, int) { x.join(v, v == -__builtin_inff() ? x.low : v); });
+    for (int s = 1; s < 64; s <<= 1) x.join(__shfl_xor(x.high, s), __shfl_xor(x.low, s));
+    if ((threadIdx.x & 63) == 0) {
+        sh.wave_count[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, x.high);
+        sh.wave_mass[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, x.low);
+    }
     __syncthreads();
-    for (int i = 0; i < kWaves; ++i) m = __builtin_fmaxf(m, __builtin_bit_cast(float, sh.wave_count[i]));
+    for (int i = 0; i < kWaves; ++i)
+        x.join(__builtin_bit_cast(float, sh.wave_count[i]), __builtin_bit_cast(float, (unsigned)sh.wave_mass[i]));
     __syncthreads();
-    return cleaned(m);
+    return x;
 }
 
 // Index of the first element equal to m (V: none).
 template <int TYPE>
 __device__ int first_of(const typename Logit<TYPE>::T* row, int V, float m, Lds& sh) {
     int at = V;
-    each<TYPE>(row, 0, V, threadIdx.x, kThreads, [&](float x, int i) { at = cleaned(x) == m && i < at ? i : at; });
+    each<TYPE>(row, 0, V, [&](float x, int i) { at = cleaned(x) == m && i < at ? i : at; });
     for (int s = 1; s < 64; s <<= 1) {
         const int o = __shfl_xor(at, s);
         at = o < at ? o : at;
@@ -423,35 +451,45 @@ __device__ __forceinline__ void clear_bins(Lds& sh) {
         sh.mass[i] = 0;
         sh.count[i] = 0;
     }
+    if (threadIdx.x == 0) sh.least_mass = 0;
+    __syncthreads();
 }
 
-// Elements [i0, i1) into the histogram in LDS.
+// Elements [i0, i1) into the histogram in LDS.  (What is computed of elements
+// of the last bin is not used: their weights may be anything.)
 template <int TYPE>
-__device__ void fill_bins(const typename Logit<TYPE>::T* row, int i0, int i1, int mode, const Bins& bin,
+__device__ void fill_bins(const typename Logit<TYPE>::T* row, int i0, int i1, int mode, u64 least, const Bins& y,
                           const Weights& w, Lds& sh) {
     if (mode == kCount) {
-        each<TYPE>(row, i0, i1, threadIdx.x, kThreads, [&](float x, int) {
-            const int b = bin(x);
+        each<TYPE>(row, i0, i1, [&](float x, int) {
+            const int b = (int)__builtin_fminf(y(x), kLast);
             if (b < kBins - 1) atomicAdd(&sh.count[b], 1u);
         });
-    } else if (mode == kMass) {
-        each<TYPE>(row, i0, i1, threadIdx.x, kThreads, [&](float x, int) {
-            const int b = bin(x);
-            if (b < kBins - 1) atomicAdd(&sh.mass[b], w(x));
+    } else if (mode == kMass && !least) {
+        each<TYPE>(row, i0, i1, [&](float x, int) {
+            const u64 e = w.quick(x);
+            const int b = (int)__builtin_fminf(y(x), kLast);
+            if (b < kBins - 1) atomicAdd(&sh.mass[b], e);
         });
     } else {
-        each<TYPE>(row, i0, i1, threadIdx.x, kThreads, [&](float x, int) {
-            const int b = bin(x);
+        u64 kept = 0;
+        each<TYPE>(row, i0, i1, [&](float x, int) {
+            const u64 e = w.quick(x);
+            const int b = (int)__builtin_fminf(y(x), kLast);
             if (b < kBins - 1) {
-                atomicAdd(&sh.count[b], 1u);
-                atomicAdd(&sh.mass[b], w(x));
+                if (mode != kMass) atomicAdd(&sh.count[b], 1u);
+                atomicAdd(&sh.mass[b], e);
+                kept += e >= least ? e : 0;
             }
         });
+        kept = wave_sum(kept);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.least_mass, kept);
     }
+    __syncthreads();
 }
 
-// Exclusive running sums over a workgroup's threads of m and n; the whole in *tm.
-__device__ void block_scan(u64& m, unsigned& n, u64* tm, Lds& sh) {
+// Exclusive running sums over a workgroup's threads; the whole in *all.
+__device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, Lds& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 im = m;
     unsigned in = n;
@@ -468,241 +506,436 @@ __device__ void block_scan(u64& m, unsigned& n, u64* tm, Lds& sh) {
         sh.wave_count[wave] = in;
     }
     __syncthreads();
-    u64 bm = 0, all = 0;
+    u64 bm = 0, sum = 0;
     unsigned bn = 0;
     for (int i = 0; i < kWaves; ++i) {
         const u64 e = sh.wave_mass[i];
         bm += i < wave ? e : 0;
         bn += i < wave ? sh.wave_count[i] : 0;
-        all += e;
+        sum += e;
     }
     m = bm + im - m;
     n = bn + in - n;
-    *tm = all;
+    *all = sum;
     __syncthreads();
 }
-
-// The bins to list, from the histogram in LDS, which becomes its running sums.
-struct Ranges {
-    int lo[4], hi[4];  // (lo > hi: none)
-    int bk;            // bin of the last element of the top_k (kBins - 1: weightless, or no top_k)
-    u64 total;         // sum of all weights (not of mode kCount)
-    u64 least_before;  // sum of the weights before bin lo[2]
-    __device__ __forceinline__ bool has(int b) const {
-        bool r = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r = r || (b >= lo[i] && b <= hi[i]);
-        return r;
-    }
-};
 
 __device__ __forceinline__ u64 p_target(float p, u64 sum) {
     const double want = __builtin_ceil((double)p * (double)sum);
     return want > 1.0 ? (u64)want - 1 : 0;
 }
 
-__device__ Ranges ranges_of(const Settings& s, int V, int mode, Lds& sh) {
+constexpr int kNone = 1 << 20;
+
+// The bins of a level that hold the places, up to three runs of them in their
+// order, and the sums in front of each run.
+struct Runs {
+    int lo[3], hi[3];  // kNone: no run
+    u64 mass[3];
+    unsigned count[3];
+    u64 total;         // sum of all weights (not before the list in mode kCount)
+    u64 least_mass;
+};
+
+__device__ __forceinline__ void swap_runs(Runs& r, int i, int j) {
+    if (r.lo[j] >= r.lo[i]) return;
+    const int l = r.lo[i], h = r.hi[i];
+    r.lo[i] = r.lo[j];
+    r.hi[i] = r.hi[j];
+    r.lo[j] = l;
+    r.hi[j] = h;
+}
+
+// One level: the histogram in LDS becomes its running sums, each run's bins
+// [start[i], start[i + 1]) from the sums that `before` has in front of it
+// (null: one run from 0), and the places are found in it.  Listing of all up
+// to the last element of the top_k where there are no weights (weighted =
+// false).
+__device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted, const Runs* before, const int* start, Lds& sh) {
     constexpr int PER = kBins / kThreads;  // bins of a thread
     const int b0 = threadIdx.x * PER;
-    u64 m[PER], ms = 0;
-    unsigned n[PER], ns = 0;
+    u64 m[PER], e[PER], ms = 0;
+    unsigned n[PER], c[PER], ns = 0;
     for (int i = 0; i < PER; ++i) {
         m[i] = ms;
         n[i] = ns;
-        ms += sh.mass[b0 + i];
-        ns += sh.count[b0 + i];
+        ms += e[i] = sh.mass[b0 + i];
+        ns += c[i] = sh.count[b0 + i];
     }
-    const u64 thread_mass = ms;
-    const unsigned thread_count = ns;
-    Ranges r;
+    Runs r;
     block_scan(ms, ns, &r.total, sh);
     for (int i = 0; i < PER; ++i) {
         sh.mass[b0 + i] = m[i] += ms;
         sh.count[b0 + i] = n[i] += ns;
     }
-    const u64 mass_end = ms + thread_mass;
-    const unsigned count_end = ns + thread_count;
-    // the bin in which a running sum exceeds a target
+    if (threadIdx.x < 8) sh.at[threadIdx.x] = kNone;
+    __syncthreads();
+    if (before) {
+        u64 dm[3];
+        unsigned dn[3];
+        for (int i = 0; i < 3; ++i) {
+            const int f = start[i] < kBins ? start[i] : 0;
+            dm[i] = before->mass[i] - sh.mass[f];
+            dn[i] = before->count[i] - sh.count[f];
+        }
+        __syncthreads();
+        for (int i = 0; i < PER; ++i) {
+            const int b = b0 + i, k = b >= start[2] ? 2 : b >= start[1] ? 1 : 0;
+            sh.mass[b] = m[i] += k == 2 ? dm[2] : k == 1 ? dm[1] : dm[0];
+            sh.count[b] = n[i] += k == 2 ? dn[2] : k == 1 ? dn[1] : dn[0];
+        }
+        if (before->total) r.total = before->total;
+    }
+    r.least_mass = before && before->total ? before->least_mass : sh.least_mass;
+    // the bin in which the running sum exceeds a target
     auto cross = [&](u64 target, int slot) {
         for (int i = 0; i < PER; ++i)
-            if (m[i] <= target && target < (i + 1 < PER ? m[i + 1] : mass_end)) sh.cross[slot] = b0 + i;
+            if (m[i] <= target && target - m[i] < e[i]) {
+                sh.at[slot] = b0 + i;
+                sh.from[slot] = m[i];
+                sh.to[slot] = m[i] + e[i];
+            }
     };
-    if (threadIdx.x == 0)
-        for (int i = 0; i < 8; ++i) sh.cross[i] = kBins - 1;
-    __syncthreads();
-    if (s.k < V)
+    if (s.k < V) {
         for (int i = 0; i < PER; ++i)
-            if (n[i] <= (unsigned)(s.k - 1) && (unsigned)(s.k - 1) < (i + 1 < PER ? n[i + 1] : count_end))
-                sh.cross[0] = b0 + i;
-    __syncthreads();
-    r.bk = sh.cross[0];
-    for (int i = 0; i < 4; ++i) {
-        r.lo[i] = 1;
-        r.hi[i] = 0;
+            if (n[i] <= (unsigned)(s.k - 1) && (unsigned)(s.k - 1) - n[i] < c[i]) {
+                sh.at[0] = b0 + i;
+                sh.from[0] = m[i];
+                sh.to[0] = m[i] + e[i];
+            }
+        __syncthreads();
     }
-    r.least_before = 0;
-    if (mode == kCount) {
+    const int bk = sh.at[0];  // (kNone: no top_k, or its last element has no weight)
+    for (int i = 0; i < 3; ++i) r.lo[i] = r.hi[i] = kNone;
+    if (!weighted) {
         r.lo[0] = 0;
-        r.hi[0] = r.bk < kBins - 1 ? r.bk : kBins - 2;
+        r.hi[0] = bk != kNone ? bk : kBins - 2;
+        r.total = 0;
+    } else {
+        u64 lo = r.total, hi = r.total;  // the sum of what is kept, so far
+        if (bk != kNone) {
+            r.lo[0] = r.hi[0] = bk;
+            lo = sh.from[0];
+            hi = sh.to[0];
+        }
+        if (s.p < 1.f) {
+            cross(p_target(s.p, lo), 1);
+            cross(p_target(s.p, hi), 2);
+            __syncthreads();
+            r.lo[1] = sh.at[1];
+            r.hi[1] = sh.at[2];
+            const u64 a = sh.from[1], b = sh.to[2];
+            lo = a < lo ? a : lo;
+            hi = b < hi ? b : hi;
+        }
+        if (s.least) {
+            lo = r.least_mass < lo ? r.least_mass : lo;
+            hi = r.least_mass < hi ? r.least_mass : hi;
+        }
+        cross((u64)(s.u * (double)lo), 3);
+        cross((u64)(s.u * (double)hi), 4);
         __syncthreads();
-        return r;
+        r.lo[2] = sh.at[3];
+        r.hi[2] = sh.at[4];
+        // in their order, those that touch as one
+        swap_runs(r, 0, 1);
+        swap_runs(r, 1, 2);
+        swap_runs(r, 0, 1);
+        if (r.lo[2] != kNone && r.lo[2] <= r.hi[1] + 1) {
+            r.hi[1] = r.hi[2] > r.hi[1] ? r.hi[2] : r.hi[1];
+            r.lo[2] = r.hi[2] = kNone;
+        }
+        if (r.lo[1] != kNone && r.lo[1] <= r.hi[0] + 1) {
+            r.hi[0] = r.hi[1] > r.hi[0] ? r.hi[1] : r.hi[0];
+            r.lo[1] = r.lo[2];
+            r.hi[1] = r.hi[2];
+            r.lo[2] = r.hi[2] = kNone;
+            if (r.lo[1] != kNone && r.lo[1] <= r.hi[0] + 1) {
+                r.hi[0] = r.hi[1] > r.hi[0] ? r.hi[1] : r.hi[0];
+                r.lo[1] = r.hi[1] = kNone;
+            }
+        }
     }
-    u64 lo = r.total, hi = r.total;  // the sum of what is kept, so far
-    if (r.bk < kBins - 1) {
-        lo = sh.mass[r.bk];
-        hi = sh.mass[r.bk + 1];
-        r.lo[0] = r.hi[0] = r.bk;
+    for (int i = 0; i < 3; ++i) {
+        const int f = r.lo[i] < kBins ? r.lo[i] : 0;
+        r.mass[i] = sh.mass[f];
+        r.count[i] = sh.count[f];
     }
-    if (s.p < 1.f) {
-        cross(p_target(s.p, lo), 1);
-        cross(p_target(s.p, hi), 2);
-        __syncthreads();
-        const int bl = sh.cross[1], bh = sh.cross[2];  // (both below the last: their targets are below the total)
-        r.lo[1] = bl;
-        r.hi[1] = bh;
-        const u64 a = sh.mass[bl], b = sh.mass[bh + 1];
-        lo = a < lo ? a : lo;
-        hi = b < hi ? b : hi;
-    }
-    if (s.least) {
-        // where weights fall below `least` (2^-44 or more: bin 1983 at most): the bin of that logit, give or take
-        // the rounding of its place
-        const int c = (int)(-log((double)s.least / kOne) * ((kBins - 1) / 31.5));
-        r.lo[2] = c > 0 ? c - 1 : 0;
-        r.hi[2] = c + 1;
-        const u64 a = r.least_before = sh.mass[r.lo[2]], b = sh.mass[r.hi[2] + 1];
-        lo = a < lo ? a : lo;
-        hi = b < hi ? b : hi;
-    }
-    cross((u64)(s.u * (double)lo), 3);
-    cross((u64)(s.u * (double)hi), 4);
-    __syncthreads();
-    r.lo[3] = sh.cross[3];
-    r.hi[3] = sh.cross[4];
     __syncthreads();
     return r;
 }
 
-// The list's n elements (key and index, inverted key first), padded to a power
-// of two, into their order.
-__device__ void sort_list(u64* list, int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-                const int a = (i & -j) * 2 + (i & (j - 1)), b = a + j;
-                const u64 x = list[a], y = list[b];
-                if ((x > y) == ((a & k) == 0)) {
-                    list[a] = y;
-                    list[b] = x;
-                }
-            }
-            __syncthreads();
+__device__ __forceinline__ u64 entry_of(float x, int i) { return (u64)~key_of(cleaned(x)) << 32 | (unsigned)i; }
+__device__ __forceinline__ float entry_value(u64 l) { return value_of(~(unsigned)(l >> 32)); }
+
+// Lists the elements of runs r among [i0, i1): sh.n of them, those past kList
+// left out.
+template <int TYPE, int NR>
+__device__ __forceinline__ void list_runs(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r,
+                                          Lds& sh) {
+    float lo[NR], hi[NR];
+    for (int i = 0; i < NR; ++i) {
+        lo[i] = (float)r.lo[i];
+        hi[i] = (float)(r.hi[i] + 1);
+    }
+    each<TYPE>(x, i0, i1, [&](float v, int i) {
+        const float b = y(v);
+        bool in = false;
+#pragma unroll
+        for (int k = 0; k < NR; ++k) in |= (b >= lo[k]) & (b < hi[k]);
+        if (in) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < kList) sh.list[at] = entry_of(v, i);
         }
+    });
 }
 
-__device__ __forceinline__ u64 entry_of(float x, int i) { return (u64)~key_of(cleaned(x)) << 32 | (unsigned)i; }
-
-// The token from the listed elements of ranges r, whose running sums are in
-// LDS; false where a place is not among them.
-__device__ bool finish_row(const SampleArgs& a, int row, const Settings& s, int mode, const Bins& bin, const Weights& w,
-                           const Ranges& r, int n, Lds& sh) {
-    constexpr int PER = kList / kThreads;
-    sort_list(sh.list, n);
-    const int per = (n + kThreads - 1) / kThreads, i0 = threadIdx.x * per;
-    const int n0 = n - i0 < per ? n - i0 : per;  // elements of this thread (below 0: none)
-    auto value = [&](int i) { return value_of(~(unsigned)(sh.list[i0 + i] >> 32)); };
-    u64 e[PER], before = 0;
-    unsigned none = 0;
-    for (int i = 0; i < PER; ++i) {
-        e[i] = i < n0 ? w(value(i)) : 0;
-        before += e[i];
-    }
-    u64 all;
-    block_scan(before, none, &all, sh);
-    // running sums over the whole row: of the bin's start, and of its elements so far
-    if (mode != kCount) {
-        u64 p = before;
-        for (int i = 0; i < PER; ++i) {
-            if (i >= n0) break;
-            const int b = bin(value(i));
-            if (i0 + i == 0 || bin(value(i - 1)) != b) {
-                sh.mass[b] -= p;
-                sh.count[b] -= (unsigned)(i0 + i);
-            }
-            p += e[i];
-        }
-    }
-    if (threadIdx.x < 8) sh.place[threadIdx.x] = 0;
+template <int TYPE>
+__device__ void fill_list(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r, Lds& sh) {
+    if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    u64 at[PER];
-    unsigned rank[PER];
-    for (int i = 0; i < PER; ++i) {
-        at[i] = before;
-        rank[i] = (unsigned)(i0 + i);
-        if (mode != kCount && i < n0) {
-            const int b = bin(value(i));
-            at[i] += sh.mass[b];
-            rank[i] += sh.count[b];
-        }
-        before += e[i];
-    }
-    // places are written as their running sum, which is above 0
-    u64 sum = mode == kCount ? all : r.total;
-    if (r.bk < kBins - 1) {
-        for (int i = 0; i < PER; ++i)
-            if (i < n0 && rank[i] == (unsigned)(s.k - 1)) sh.place[0] = at[i] + e[i];
-        __syncthreads();
-        sum = sh.place[0];
+    if (r.lo[1] == kNone)
+        list_runs<TYPE, 1>(x, i0, i1, y, r, sh);
+    else if (r.lo[2] == kNone)
+        list_runs<TYPE, 2>(x, i0, i1, y, r, sh);
+    else
+        list_runs<TYPE, 3>(x, i0, i1, y, r, sh);
+    __syncthreads();
+}
+
+// One element of a group that is small or of few values: its sums in front.
+struct Spot {
+    u64 before, mass;       // sum of the weights in front of it; its own (of all equal ones)
+    unsigned rank, number;  // elements in front of it; equal ones
+};
+
+// The places among the spots that a wave's lanes hold (`here`: this lane has
+// one), each kept sum exact: the sum of all kept, and where u lies.
+__device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, u64 weight, bool here, const Runs& r, u64* target) {
+    auto pick = [&](bool mine, u64 v) -> u64 {
+        const u64 b = __ballot(mine);
+        if (!b) return 0;
+        return (u64)__shfl((long long)v, __builtin_ctzll(b));
+    };
+    u64 sum = r.total;
+    if (s.k < V) {
+        const unsigned k = (unsigned)(s.k - 1);
+        const u64 got = pick(here && z.rank <= k && k - z.rank < z.number, z.before + (k - z.rank + 1) * weight);
+        sum = got ? got : sum;  // (none: the top_k's last element has no weight)
     }
     u64 kept = sum;
     if (s.p < 1.f) {
-        const u64 target = p_target(s.p, sum);
-        for (int i = 0; i < PER; ++i)
-            if (i < n0 && at[i] <= target && target < at[i] + e[i]) sh.place[1] = at[i] + e[i];
-        __syncthreads();
-        kept = sh.place[1] < kept ? sh.place[1] : kept;
+        const u64 t = p_target(s.p, sum);
+        const bool mine = here && z.before <= t && t - z.before < z.mass;
+        const u64 got = pick(mine, z.before + (mine ? (t - z.before) / weight + 1 : 0) * weight);
+        if (!got) return 0;
+        kept = got < kept ? got : kept;
     }
-    if (s.least) {
-        u64 most = threadIdx.x == 0 ? r.least_before : 0;
-        for (int i = 0; i < PER; ++i)
-            if (i < n0 && e[i] >= s.least) most = at[i] + e[i] > most ? at[i] + e[i] : most;
-        if (most) atomicMax(&sh.place[2], most);
-        __syncthreads();
-        kept = sh.place[2] < kept ? sh.place[2] : kept;
-    }
-    const u64 target = (u64)(s.u * (double)kept);
-    for (int i = 0; i < PER; ++i)
-        if (i < n0 && at[i] <= target && target < at[i] + e[i]) {
-            const u64 l = sh.list[i0 + i];
-            gptr(a.token)[row] = (int32_t)(unsigned)l;
-            if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(value(i)) / (double)kept);
-            sh.place[3] = 1;
+    if (s.least && r.least_mass < kept) kept = r.least_mass;
+    *target = (u64)(s.u * (double)kept);
+    return kept;
+}
+
+// The k <= kFew elements at the front of the list, one a lane of the first wave.
+template <typename B>
+__device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
+                           int k, Lds& sh) {
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        const bool here = lane < k;
+        const u64 l = here ? sh.list[lane] : ~0ull;
+        const float x = entry_value(l);
+        const u64 e = here ? w(x) : 0;
+        const int b = here ? bin(x) : -1;
+        Spot z{here ? sh.mass[b] : 0, e, here ? sh.count[b] : 0, 1};
+        for (int i = 0; i < k; ++i) {
+            const u64 ol = (u64)__shfl((long long)l, i), oe = (u64)__shfl((long long)e, i);
+            const bool ahead = __shfl(b, i) == b && ol < l;
+            z.before += ahead ? oe : 0;
+            z.rank += ahead;
         }
+        u64 target = 0;
+        const u64 sum = kept_of(s, a.V, z, e, here, q, &target);
+        const bool mine = sum && here && z.before <= target && target - z.before < e;
+        if (mine) {
+            gptr(a.token)[row] = (int32_t)(unsigned)l;
+            if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
+        }
+        const bool found = __ballot(mine) != 0;
+        if (lane == 0) sh.at[7] = found;
+    }
     __syncthreads();
-    return kept != 0 && sh.place[3] != 0;
+    return sh.at[7] != 0;
 }
 
-__device__ __forceinline__ void fill_table(double* table) {
-    if (threadIdx.x < 256) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 256));
+// More elements than that, of up to kValues values: the values one after
+// another, then the token among equal ones by its index.
+template <typename B>
+__device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
+                            int k, Lds& sh) {
+    const int lane = threadIdx.x & 63;
+    unsigned* const values = sh.wave_count;  // inverted keys, rising: falling logits
+    unsigned* const numbers = values + kValues;
+    static_assert(2 * kValues <= kWaves, "");
+    if (threadIdx.x < kWaves) sh.wave_count[threadIdx.x] = threadIdx.x < kValues ? ~0u : 0u;
     __syncthreads();
-}
-
-// Rows that need no sums: of nothing to draw, and at temperature 0.
-template <int TYPE>
-__device__ __forceinline__ bool settled(const SampleArgs& a, int row, const typename Logit<TYPE>::T* x, float m, double T,
-                                        Lds& sh) {
-    const bool none = m == -__builtin_inff();
-    if (!none && T > 0.0) return false;
-    const int i = none ? -1 : first_of<TYPE>(x, a.V, m, sh);
-    if (threadIdx.x == 0) {
-        gptr(a.token)[row] = i;
-        if (a.prob) gptr(a.prob)[row] = none ? 0.f : 1.f;
+    unsigned last = 0;  // (0 inverted is a NaN's key)
+    int nv = 0;
+    for (;; ++nv) {
+        unsigned v = ~0u;
+        for (int i = threadIdx.x; i < k; i += kThreads) {
+            const unsigned e = (unsigned)(sh.list[i] >> 32);
+            v = e > last && e < v ? e : v;
+        }
+        for (int d = 1; d < 64; d <<= 1) {
+            const unsigned o = (unsigned)__shfl_xor((int)v, d);
+            v = o < v ? o : v;
+        }
+        if (nv == kValues) {  // one too many?
+            const bool more = __syncthreads_or(v != ~0u);
+            if (more) return false;
+            break;
+        }
+        if (lane == 0) atomicMin(&values[nv], v);
+        __syncthreads();
+        last = values[nv];
+        if (last == ~0u) break;
+        unsigned c = 0;
+        for (int i = threadIdx.x; i - (int)threadIdx.x < k; i += kThreads)
+            c += __builtin_popcountll(__ballot(i < k && (unsigned)(sh.list[i] >> 32) == last));
+        if (lane == 0 && c) atomicAdd(&numbers[nv], c);
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const bool here = lane < nv;
+        const float x = value_of(~(here ? values[lane] : 0x7FFFFFFFu));
+        const unsigned c = here ? numbers[lane] : 0;
+        const u64 e = here ? w(x) : 0;
+        const int b = here ? bin(x) : -1;
+        Spot z{here ? sh.mass[b] : 0, e * c, here ? sh.count[b] : 0, c};
+        for (int i = 0; i < nv; ++i) {
+            const u64 oe = (u64)__shfl((long long)z.mass, i);
+            const unsigned oc = (unsigned)__shfl((int)c, i);
+            const bool ahead = __shfl(b, i) == b && i < lane;
+            z.before += ahead ? oe : 0;
+            z.rank += ahead ? oc : 0;
+        }
+        u64 target = 0;
+        const u64 sum = kept_of(s, a.V, z, e, here, q, &target);
+        const bool mine = sum && here && z.before <= target && target - z.before < z.mass;
+        if (mine) {
+            sh.at[5] = (int)((target - z.before) / e);
+            sh.at[6] = (int)values[lane];
+            if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
+        }
+        const bool found = __ballot(mine) != 0;
+        if (lane == 0) sh.at[7] = found;
+    }
+    __syncthreads();
+    if (!sh.at[7]) return false;
+    const unsigned rank = (unsigned)sh.at[5], key = (unsigned)sh.at[6];
+    // of the equal ones the one with `rank` lower indices: by the index's upper bits, then among those that share them
+    static_assert(TER_HIP_SAMPLE_V_MAX <= kBins << 8, "");
+    clear_bins(sh);
+    for (int i = threadIdx.x; i < k; i += kThreads)
+        if ((unsigned)(sh.list[i] >> 32) == key) atomicAdd(&sh.count[(unsigned)sh.list[i] >> 8], 1u);
+    __syncthreads();
+    constexpr int PER = kBins / kThreads;
+    const int b0 = threadIdx.x * PER;
+    u64 none = 0, all;
+    unsigned n = 0;
+    for (int i = 0; i < PER; ++i) n += sh.count[b0 + i];
+    block_scan(none, n, &all, sh);
+    for (int i = 0; i < PER; ++i) {
+        const unsigned c = sh.count[b0 + i];
+        if (n <= rank && rank - n < c) {
+            sh.at[0] = b0 + i;
+            sh.at[1] = (int)(rank - n);
+        }
+        n += c;
+    }
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const int bucket = sh.at[0];
+    for (int i = threadIdx.x; i < k; i += kThreads)
+        if ((unsigned)(sh.list[i] >> 32) == key && (int)((unsigned)sh.list[i] >> 8) == bucket)
+            sh.mass[atomicAdd(&sh.n, 1)] = (unsigned)sh.list[i];  // (256 at most)
+    __syncthreads();
+    if ((int)threadIdx.x < sh.n) {
+        const u64 me = sh.mass[threadIdx.x];
+        int lower = 0;
+        for (int i = 0; i < sh.n; ++i) lower += sh.mass[i] < me;
+        if (lower == sh.at[1]) gptr(a.token)[row] = (int32_t)me;
     }
     return true;
+}
+
+// The token from the n elements in the list, which are all of runs r; false
+// where its place is not found (too many elements close together).
+__device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w, const Runs& r,
+                           int n, Lds& sh) {
+    // the runs' bins, each cut into 2^shift
+    int bins = 0, first[3], start[3], shift = 8;
+    for (int i = 0; i < 3; ++i) {
+        first[i] = bins;
+        bins += r.lo[i] != kNone ? r.hi[i] - r.lo[i] + 1 : 0;
+    }
+    while ((bins << shift) > kBins) --shift;
+    int off[3];
+    for (int i = 0; i < 3; ++i) {
+        start[i] = r.lo[i] != kNone ? first[i] << shift : kNone;
+        off[i] = (first[i] - r.lo[i]) * (1 << shift);
+    }
+    auto bin = [&](float x) {
+        const int f = (int)(y(x) * 256.f), b = f >> 8;  // (exact; below 0 by a rounding: the first)
+        const int i = (f >> (8 - shift)) + (b >= r.lo[2] ? off[2] : b >= r.lo[1] ? off[1] : off[0]);
+        return i < 0 ? 0 : i < kBins ? i : kBins - 1;
+    };
+    clear_bins(sh);
+    u64 kept = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const float x = entry_value(sh.list[i]);
+        const u64 e = w(x);
+        const int b = bin(x);
+        atomicAdd(&sh.mass[b], e);
+        atomicAdd(&sh.count[b], 1u);
+        kept += e >= s.least ? e : 0;
+    }
+    if (r.total == 0 && s.least) {
+        kept = wave_sum(kept);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.least_mass, kept);
+    }
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const Runs q = level_of(s, a.V, true, &r, start, sh);
+    // the elements of its runs, to the front of the list
+    const int per = (n + kThreads - 1) / kThreads;
+    u64 keep[kList / kThreads];
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) {
+        if (i >= per) break;
+        const int at = i * kThreads + (int)threadIdx.x;
+        keep[i] = at < n ? sh.list[at] : 0;
+        const int b = at < n ? bin(entry_value(keep[i])) : -1;
+        const bool in = (b >= q.lo[0] && b <= q.hi[0]) || (b >= q.lo[1] && b <= q.hi[1]) || (b >= q.lo[2] && b <= q.hi[2]);
+        m = m * 2 + in;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) {
+        if (i >= per) break;
+        if (m >> (per - 1 - i) & 1) sh.list[atomicAdd(&sh.n, 1)] = keep[i];
+    }
+    __syncthreads();
+    const int k = sh.n;
+    return k <= kFew ? finish_few(a, row, s, bin, w, q, k, sh) : finish_many(a, row, s, bin, w, q, k, sh);
+}
+
+// 2^44 times 2^(j / 256).
+__device__ __forceinline__ void fill_table(double* table) {
+    if (threadIdx.x < 256) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 256) + 44.0);
+    __syncthreads();
 }
 
 template <int TYPE>
@@ -710,17 +943,21 @@ __device__ __forceinline__ const typename Logit<TYPE>::T* row_of(const SampleArg
     return reinterpret_cast<const typename Logit<TYPE>::T*>(a.logits + (long long)row * a.stride);
 }
 
-// Lists the elements of r among [i0, i1): sh.n of them, those past kList left out.
+// Rows that need no sums: of nothing to draw, and at temperature 0.
+__device__ __forceinline__ bool no_sums(const Extent& x, const Settings& s) {
+    return x.high == -__builtin_inff() || s.T == 0.0;
+}
+// Rows with an infinite logit go the general path.
+__device__ __forceinline__ bool infinite(const Extent& x) { return x.high == __builtin_inff(); }
+
 template <int TYPE>
-__device__ void fill_list(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& bin, const Ranges& r, Lds& sh) {
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
-    each<TYPE>(x, i0, i1, threadIdx.x, kThreads, [&](float v, int i) {
-        if (!r.has(bin(v))) return;
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kList) sh.list[at] = entry_of(v, i);
-    });
-    __syncthreads();
+__device__ void settle(const SampleArgs& a, int row, const Extent& x, Lds& sh) {
+    const bool none = x.high == -__builtin_inff();
+    const int i = none ? -1 : first_of<TYPE>(row_of<TYPE>(a, row), a.V, cleaned(x.high), sh);
+    if (threadIdx.x == 0) {
+        gptr(a.token)[row] = i;
+        if (a.prob) gptr(a.prob)[row] = none ? 0.f : 1.f;
+    }
 }
 
 // One workgroup a row, start to end.
@@ -729,107 +966,119 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
     __shared__ Lds sh;
     const int row = blockIdx.x;
     const auto* x = row_of<TYPE>(a, row);
-    fill_table(sh.table);
-    const float m = largest_of<TYPE>(x, 0, a.V, sh);
     const Settings s = settings_of(a, row);
-    if (settled<TYPE>(a, row, x, m, s.T, sh)) return;
-    const Bins bin = bins_of(m, s.T);
-    const Weights w = weights_of(sh.table, m, s.T);
-    const int mode = mode_of(s, a.V);
-    clear_bins(sh);
-    __syncthreads();
-    fill_bins<TYPE>(x, 0, a.V, mode, bin, w, sh);
-    __syncthreads();
-    const Ranges r = ranges_of(s, a.V, mode, sh);
-    fill_list<TYPE>(x, 0, a.V, bin, r, sh);
-    const int n = sh.n;
-    if (n <= kList && finish_row(a, row, s, mode, bin, w, r, n, sh)) return;
-    __syncthreads();
+    fill_table(sh.table);
+    const Extent ext = extent_of<TYPE>(x, 0, a.V, sh);
+    if (no_sums(ext, s)) {
+        settle<TYPE>(a, row, ext, sh);
+        return;
+    }
+    if (!infinite(ext)) {
+        const Bins y = bins_of(ext.high, ext.low, s.T);
+        const Weights w = weights_of(sh.table, cleaned(ext.high), s.T);
+        const int mode = mode_of(s, a.V);
+        clear_bins(sh);
+        fill_bins<TYPE>(x, 0, a.V, mode, s.least, y, w, sh);
+        const Runs r = level_of(s, a.V, mode != kCount, nullptr, nullptr, sh);
+        fill_list<TYPE>(x, 0, a.V, y, r, sh);
+        const int n = sh.n;
+        if (n <= kList && finish_row(a, row, s, y, w, r, n, sh)) return;
+        __syncthreads();
+    }
     sample_row<TYPE>(a, row, sh.table, sh.general);
 }
 
 // ---- few rows: slices of a row by many workgroups, four launches ----
 
-__device__ __forceinline__ void slice_of(const SampleArgs& a, int& row, int& i0, int& i1) {
+__device__ __forceinline__ void slice_of(const SampleArgs& a, int& row, int& g, int& i0, int& i1) {
     row = blockIdx.x / a.slices;
-    const int g = blockIdx.x - row * a.slices;
+    g = blockIdx.x - row * a.slices;
     const int per = ((a.V + a.slices - 1) / a.slices + 7) / 8 * 8;
     i0 = g * per < a.V ? g * per : a.V;
     i1 = i0 + per < a.V ? i0 + per : a.V;
 }
 
-__device__ __forceinline__ SampleRow* ws_of(const SampleArgs& a, int row) { return a.ws + row; }
-
-__device__ __forceinline__ float row_max(const SampleArgs& a, const SampleRow* z) {
-    float m = -__builtin_inff();
-    for (int i = 0; i < a.slices; ++i) m = __builtin_fmaxf(m, gptr(z->slice_max)[i]);
-    return m;
+__device__ __forceinline__ Extent row_extent(const SampleArgs& a, const SampleRow* z) {
+    Extent x{-__builtin_inff(), __builtin_inff()};
+    const int i = threadIdx.x & 63;
+    if (i < a.slices) x = Extent{gptr(z->slice_high)[i], gptr(z->slice_low)[i]};
+    for (int s = 1; s < 64; s <<= 1) x.join(__shfl_xor(x.high, s), __shfl_xor(x.low, s));
+    return x;
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
-    __shared__ Lds sh;
-    int row, i0, i1;
-    slice_of(a, row, i0, i1);
-    const int g = blockIdx.x - row * a.slices;
-    SampleRow* z = ws_of(a, row);
+    __shared__ LdsSmall sh;
+    int row, g, i0, i1;
+    slice_of(a, row, g, i0, i1);
+    SampleRow* z = a.ws + row;
     // the row's sums, cleared for the next launch
     for (int i = g * kThreads + threadIdx.x; i < kBins; i += a.slices * kThreads) {
         gptr(z->mass)[i] = 0;
         gptr(z->count)[i] = 0;
     }
-    const float m = largest_of<TYPE>(row_of<TYPE>(a, row), i0, i1, sh);
+    const Extent x = extent_of<TYPE>(row_of<TYPE>(a, row), i0, i1, sh);
     if (threadIdx.x == 0) {
-        gptr(z->slice_max)[g] = m;
-        if (g == 0) *gptr(&z->n) = 0;
+        gptr(z->slice_high)[g] = x.high;
+        gptr(z->slice_low)[g] = x.low;
+        if (g == 0) {
+            *gptr(&z->n) = 0;
+            *gptr(&z->least_mass) = 0;
+        }
     }
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
     __shared__ Lds sh;
-    int row, i0, i1;
-    slice_of(a, row, i0, i1);
-    SampleRow* z = ws_of(a, row);
-    const float m = row_max(a, z);
+    int row, g, i0, i1;
+    slice_of(a, row, g, i0, i1);
+    SampleRow* z = a.ws + row;
+    const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
-    if (m == -__builtin_inff() || s.T == 0.0) return;
+    if (no_sums(x, s) || infinite(x)) return;
     const int mode = mode_of(s, a.V);
     if (mode != kCount) fill_table(sh.table);
     clear_bins(sh);
-    __syncthreads();
-    fill_bins<TYPE>(row_of<TYPE>(a, row), i0, i1, mode, bins_of(m, s.T), weights_of(sh.table, m, s.T), sh);
-    __syncthreads();
+    fill_bins<TYPE>(row_of<TYPE>(a, row), i0, i1, mode, s.least, bins_of(x.high, x.low, s.T),
+                    weights_of(sh.table, x.high, s.T), sh);
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
         if (mode != kCount && sh.mass[i]) atomicAdd(&z->mass[i], sh.mass[i]);
         if (mode != kMass && sh.count[i]) atomicAdd(&z->count[i], sh.count[i]);
     }
-}
-
-__device__ __forceinline__ void load_bins(const SampleRow* z, Lds& sh) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        sh.mass[i] = gptr(z->mass)[i];
-        sh.count[i] = gptr(z->count)[i];
-    }
-    __syncthreads();
+    if (threadIdx.x == 0 && sh.least_mass) atomicAdd(&z->least_mass, sh.least_mass);
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void sample_list_kernel(SampleArgs a) {
     __shared__ Lds sh;
-    int row, i0, i1;
-    slice_of(a, row, i0, i1);
-    SampleRow* z = ws_of(a, row);
-    const float m = row_max(a, z);
+    int row, g, i0, i1;
+    slice_of(a, row, g, i0, i1);
+    SampleRow* z = a.ws + row;
+    const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
-    if (m == -__builtin_inff() || s.T == 0.0) return;
-    load_bins(z, sh);
-    const Ranges r = ranges_of(s, a.V, mode_of(s, a.V), sh);
-    fill_list<TYPE>(row_of<TYPE>(a, row), i0, i1, bins_of(m, s.T), r, sh);
-    const int n = sh.n;
-    if (threadIdx.x == 0) sh.cross[0] = n ? (int)atomicAdd(&z->n, (unsigned)n) : 0;  // (V at most in all)
+    if (no_sums(x, s) || infinite(x)) return;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        sh.mass[i] = gptr(z->mass)[i];
+        sh.count[i] = gptr(z->count)[i];
+    }
+    if (threadIdx.x == 0) sh.least_mass = *gptr(&z->least_mass);
     __syncthreads();
-    const int at = sh.cross[0];
+    const Runs r = level_of(s, a.V, mode_of(s, a.V) != kCount, nullptr, nullptr, sh);
+    if (g == 0 && threadIdx.x == 0) {
+        for (int i = 0; i < 3; ++i) {
+            z->lo[i] = r.lo[i];
+            z->hi[i] = r.hi[i];
+            z->run_mass[i] = r.mass[i];
+            z->run_count[i] = r.count[i];
+        }
+        z->total = r.total;
+    }
+    fill_list<TYPE>(row_of<TYPE>(a, row), i0, i1, bins_of(x.high, x.low, s.T), r, sh);
+    const int n = sh.n;
+    if (threadIdx.x == 0) sh.at[0] = n ? (int)atomicAdd(&z->n, (unsigned)n) : 0;  // (V at most in all)
+    __syncthreads();
+    const int at = sh.at[0];
     for (int i = threadIdx.x; i < n && i < kList && at + i < kList; i += kThreads) gptr(z->list)[at + i] = sh.list[i];
 }
 
@@ -837,21 +1086,30 @@ template <int TYPE>
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     __shared__ Lds sh;
     const int row = blockIdx.x;
-    const SampleRow* z = ws_of(a, row);
-    const float m = row_max(a, z);
+    const SampleRow* z = a.ws + row;
+    const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
-    if (settled<TYPE>(a, row, row_of<TYPE>(a, row), m, s.T, sh)) return;
-    const int mode = mode_of(s, a.V);
-    fill_table(sh.table);
-    load_bins(z, sh);
-    const Ranges r = ranges_of(s, a.V, mode, sh);
     const int n = (int)*gptr(&z->n);
-    if (n <= kList) {
+    Runs r;
+    for (int i = 0; i < 3; ++i) {
+        r.lo[i] = gptr(z->lo)[i];
+        r.hi[i] = gptr(z->hi)[i];
+        r.mass[i] = gptr(z->run_mass)[i];
+        r.count[i] = gptr(z->run_count)[i];
+    }
+    r.total = *gptr(&z->total);
+    r.least_mass = *gptr(&z->least_mass);
+    if (no_sums(x, s)) {
+        settle<TYPE>(a, row, x, sh);
+        return;
+    }
+    fill_table(sh.table);
+    if (!infinite(x) && n <= kList) {
         for (int i = threadIdx.x; i < n; i += kThreads) sh.list[i] = gptr(z->list)[i];
         __syncthreads();
-        if (finish_row(a, row, s, mode, bins_of(m, s.T), weights_of(sh.table, m, s.T), r, n, sh)) return;
+        if (finish_row(a, row, s, bins_of(x.high, x.low, s.T), weights_of(sh.table, x.high, s.T), r, n, sh)) return;
+        __syncthreads();
     }
-    __syncthreads();
     sample_row<TYPE>(a, row, sh.table, sh.general);
 }
 
