@@ -15,8 +15,6 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-
 template <int TYPE>
 struct Logit {
     typedef uint16_t T;
@@ -106,7 +104,9 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
     return s;
 }
 
+template <int NT>
 struct Shared {
+    static constexpr int kWaves = NT / 64;
     u64 mass[256];
     unsigned count[256];
     u64 red[kWaves];
@@ -122,14 +122,16 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
 }
 
 // A row by its elements, one workgroup.
-template <int TYPE>
+template <int TYPE, int kThreads>
 struct Row {
+    static constexpr int kWaves = kThreads / 64;
     typedef typename Logit<TYPE>::T T;
+    typedef Shared<kThreads> Sh;
     const TER_GLOBAL T* x;
     int V;
     __device__ float operator[](int i) const { return cleaned(Logit<TYPE>::raw(x[i])); }
 
-    __device__ unsigned largest(Shared& sh) const {
+    __device__ unsigned largest(Sh& sh) const {
         unsigned k = 0;
         for (int i = threadIdx.x; i < V; i += kThreads) {
             const unsigned e = key_of((*this)[i]);
@@ -147,7 +149,7 @@ struct Row {
     }
 
     // Sum of the weights that are `least` or more.
-    __device__ u64 mass(Shared& sh, const Weights& w, u64 least) const {
+    __device__ u64 mass(Sh& sh, const Weights& w, u64 least) const {
         u64 s = 0;
         for (int i = threadIdx.x; i < V; i += kThreads) {
             const u64 e = w((*this)[i]);
@@ -163,7 +165,7 @@ struct Row {
     }
 
     // Index of element `rank` (from 0, by index) of those with key `key`.
-    __device__ int tie(Shared& sh, unsigned key, unsigned rank) const {
+    __device__ int tie(Sh& sh, unsigned key, unsigned rank) const {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const int per = ((V + kWaves - 1) / kWaves + 63) / 64 * 64, from = wave * per;
         const int to = from + per < V ? from + per : V;
@@ -201,7 +203,7 @@ struct Row {
     // or the number where by_count) exceeds target, which the whole exceeds:
     // byte by byte of the key, each by a histogram of the elements that agree
     // so far.
-    __device__ Place find(Shared& sh, const Weights& w, bool by_count, u64 target) const {
+    __device__ Place find(Sh& sh, const Weights& w, bool by_count, u64 target) const {
         Place at = {0, 0, 0};
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (int i = threadIdx.x; i < 256; i += kThreads) {
@@ -266,9 +268,9 @@ struct Row {
 
 // One row by one workgroup: a search through the row's values for each cut and
 // for the draw.  Right for every row; the general path.
-template <int TYPE>
-__device__ void sample_row(const SampleArgs& a, int row, const double* table, Shared& sh) {
-    Row<TYPE> x{gptr(reinterpret_cast<const typename Logit<TYPE>::T*>(a.logits + (long long)row * a.stride)), a.V};
+template <int TYPE, int NT>
+__device__ void sample_row(const SampleArgs& a, int row, const double* table, Shared<NT>& sh) {
+    Row<TYPE, NT> x{gptr(reinterpret_cast<const typename Logit<TYPE>::T*>(a.logits + (long long)row * a.stride)), a.V};
     const unsigned top = x.largest(sh);
     const Settings s = settings_of(a, row);
     if (top == key_of(-__builtin_inff()) || s.T == 0.0) {
@@ -323,6 +325,7 @@ __device__ void sample_row(const SampleArgs& a, int row, const double* table, Sh
 constexpr int kCountK = 1024; // up to this top_k everything kept is listed, and weights are computed for the list alone
 constexpr int kFew = 64;      // elements compared by one wave
 constexpr int kValues = 8;    // different values among more elements than that
+constexpr int kSecond = 3072; // elements of the second list
 
 struct Bins {
     float mh, cb;  // m / 2; bins for half a logit
@@ -344,21 +347,20 @@ __device__ __forceinline__ int mode_of(const Settings& s, int V) {
     return s.k <= kCountK && s.k < V ? kCount : s.k < V ? kBoth : kMass;
 }
 
-struct LdsSmall {
+// A workgroup's LDS: for the extent of its logits, for a histogram, for the list
+// too, and to the end.
+template <int NT>
+struct LdsScan {
+    static constexpr int kThreads = NT, kWaves = NT / 64;
     u64 wave_mass[kWaves];
     unsigned wave_count[kWaves];
 };
 
-struct Lds : LdsSmall {
+template <int NT>
+struct LdsBins : LdsScan<NT> {
     double table[256];
-    union {
-        struct {
-            u64 mass[kBins];
-            unsigned count[kBins];
-            u64 list[kList];
-        };
-        Shared general;
-    };
+    u64 mass[kBins];
+    unsigned count[kBins];
     // places of a level: bin, sums at its start and end
     int at[8];
     u64 from[8], to[8];
@@ -366,9 +368,24 @@ struct Lds : LdsSmall {
     int n;
 };
 
+template <int NT, int LIST>
+struct LdsList : LdsBins<NT> {
+    static constexpr int kCapacity = LIST;
+    u64 list[LIST];
+};
+
+template <int NT>
+struct Lds : LdsList<NT, kList> {
+    union {
+        u64 second[kSecond];
+        Shared<NT> general;
+    };
+    unsigned values[kValues], numbers[kValues];
+};
+
 // f(x, i) of elements [i0, i1) of a row by the workgroup's threads, 16 bytes a
 // load, four loads in flight.
-template <int TYPE, typename F>
+template <int TYPE, int kThreads, typename F>
 __device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0, int i1, F f) {
     typedef typename Logit<TYPE>::T T;
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -414,40 +431,42 @@ struct Extent {
     }
 };
 
-template <int TYPE>
-__device__ Extent extent_of(const typename Logit<TYPE>::T* row, int i0, int i1, LdsSmall& sh) {
+template <int TYPE, int NT>
+__device__ Extent extent_of(const typename Logit<TYPE>::T* row, int i0, int i1, LdsScan<NT>& sh) {
     Extent x{-__builtin_inff(), __builtin_inff()};
-    each<TYPE>(row, i0, i1, [&](float v, int) { x.join(v, v == -__builtin_inff() ? x.low : v); });
+    each<TYPE, NT>(row, i0, i1, [&](float v, int) { x.join(v, v == -__builtin_inff() ? x.low : v); });
     for (int s = 1; s < 64; s <<= 1) x.join(__shfl_xor(x.high, s), __shfl_xor(x.low, s));
     if ((threadIdx.x & 63) == 0) {
         sh.wave_count[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, x.high);
         sh.wave_mass[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, x.low);
     }
     __syncthreads();
-    for (int i = 0; i < kWaves; ++i)
+    for (int i = 0; i < NT / 64; ++i)
         x.join(__builtin_bit_cast(float, sh.wave_count[i]), __builtin_bit_cast(float, (unsigned)sh.wave_mass[i]));
     __syncthreads();
     return x;
 }
 
 // Index of the first element equal to m (V: none).
-template <int TYPE>
-__device__ int first_of(const typename Logit<TYPE>::T* row, int V, float m, Lds& sh) {
+template <int TYPE, int NT>
+__device__ int first_of(const typename Logit<TYPE>::T* row, int V, float m, LdsScan<NT>& sh) {
     int at = V;
-    each<TYPE>(row, 0, V, [&](float x, int i) { at = cleaned(x) == m && i < at ? i : at; });
+    each<TYPE, NT>(row, 0, V, [&](float x, int i) { at = cleaned(x) == m && i < at ? i : at; });
     for (int s = 1; s < 64; s <<= 1) {
         const int o = __shfl_xor(at, s);
         at = o < at ? o : at;
     }
     if ((threadIdx.x & 63) == 0) sh.wave_count[threadIdx.x >> 6] = (unsigned)at;
     __syncthreads();
-    for (int i = 0; i < kWaves; ++i) at = (int)sh.wave_count[i] < at ? (int)sh.wave_count[i] : at;
+    for (int i = 0; i < NT / 64; ++i) at = (int)sh.wave_count[i] < at ? (int)sh.wave_count[i] : at;
     __syncthreads();
     return at;
 }
 
-__device__ __forceinline__ void clear_bins(Lds& sh) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+template <int NT>
+__device__ __forceinline__ void clear_bins(LdsBins<NT>& sh) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kBins; i += NT) {
         sh.mass[i] = 0;
         sh.count[i] = 0;
     }
@@ -457,23 +476,23 @@ __device__ __forceinline__ void clear_bins(Lds& sh) {
 
 // Elements [i0, i1) into the histogram in LDS.  (What is computed of elements
 // of the last bin is not used: their weights may be anything.)
-template <int TYPE>
+template <int TYPE, int NT>
 __device__ void fill_bins(const typename Logit<TYPE>::T* row, int i0, int i1, int mode, u64 least, const Bins& y,
-                          const Weights& w, Lds& sh) {
+                          const Weights& w, LdsBins<NT>& sh) {
     if (mode == kCount) {
-        each<TYPE>(row, i0, i1, [&](float x, int) {
+        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
             const int b = (int)__builtin_fminf(y(x), kLast);
             if (b < kBins - 1) atomicAdd(&sh.count[b], 1u);
         });
     } else if (mode == kMass && !least) {
-        each<TYPE>(row, i0, i1, [&](float x, int) {
+        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
             const u64 e = w.quick(x);
             const int b = (int)__builtin_fminf(y(x), kLast);
             if (b < kBins - 1) atomicAdd(&sh.mass[b], e);
         });
     } else {
         u64 kept = 0;
-        each<TYPE>(row, i0, i1, [&](float x, int) {
+        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
             const u64 e = w.quick(x);
             const int b = (int)__builtin_fminf(y(x), kLast);
             if (b < kBins - 1) {
@@ -489,7 +508,8 @@ __device__ void fill_bins(const typename Logit<TYPE>::T* row, int i0, int i1, in
 }
 
 // Exclusive running sums over a workgroup's threads; the whole in *all.
-__device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, Lds& sh) {
+template <int NT>
+__device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, LdsScan<NT>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 im = m;
     unsigned in = n;
@@ -508,7 +528,8 @@ __device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, Lds& s
     __syncthreads();
     u64 bm = 0, sum = 0;
     unsigned bn = 0;
-    for (int i = 0; i < kWaves; ++i) {
+#pragma unroll 1
+    for (int i = 0; i < NT / 64; ++i) {
         const u64 e = sh.wave_mass[i];
         bm += i < wave ? e : 0;
         bn += i < wave ? sh.wave_count[i] : 0;
@@ -551,11 +572,14 @@ __device__ __forceinline__ void swap_runs(Runs& r, int i, int j) {
 // (null: one run from 0), and the places are found in it.  Listing of all up
 // to the last element of the top_k where there are no weights (weighted =
 // false).
-__device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted, const Runs* before, const int* start, Lds& sh) {
-    constexpr int PER = kBins / kThreads;  // bins of a thread
+template <int NT>
+__device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted, const Runs* before, const int* start,
+                                         LdsBins<NT>& sh) {
+    constexpr int PER = kBins / NT;  // bins of a thread
     const int b0 = threadIdx.x * PER;
     u64 m[PER], e[PER], ms = 0;
     unsigned n[PER], c[PER], ns = 0;
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
         m[i] = ms;
         n[i] = ns;
@@ -564,6 +588,7 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
     }
     Runs r;
     block_scan(ms, ns, &r.total, sh);
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
         sh.mass[b0 + i] = m[i] += ms;
         sh.count[b0 + i] = n[i] += ns;
@@ -573,12 +598,14 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
     if (before) {
         u64 dm[3];
         unsigned dn[3];
+#pragma unroll
         for (int i = 0; i < 3; ++i) {
             const int f = start[i] < kBins ? start[i] : 0;
             dm[i] = before->mass[i] - sh.mass[f];
             dn[i] = before->count[i] - sh.count[f];
         }
         __syncthreads();
+#pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int b = b0 + i, k = b >= start[2] ? 2 : b >= start[1] ? 1 : 0;
             sh.mass[b] = m[i] += k == 2 ? dm[2] : k == 1 ? dm[1] : dm[0];
@@ -589,6 +616,7 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
     r.least_mass = before && before->total ? before->least_mass : sh.least_mass;
     // the bin in which the running sum exceeds a target
     auto cross = [&](u64 target, int slot) {
+#pragma unroll
         for (int i = 0; i < PER; ++i)
             if (m[i] <= target && target - m[i] < e[i]) {
                 sh.at[slot] = b0 + i;
@@ -597,6 +625,7 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
             }
     };
     if (s.k < V) {
+#pragma unroll
         for (int i = 0; i < PER; ++i)
             if (n[i] <= (unsigned)(s.k - 1) && (unsigned)(s.k - 1) - n[i] < c[i]) {
                 sh.at[0] = b0 + i;
@@ -606,6 +635,7 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
         __syncthreads();
     }
     const int bk = sh.at[0];  // (kNone: no top_k, or its last element has no weight)
+#pragma unroll
     for (int i = 0; i < 3; ++i) r.lo[i] = r.hi[i] = kNone;
     if (!weighted) {
         r.lo[0] = 0;
@@ -656,6 +686,7 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
             }
         }
     }
+#pragma unroll
     for (int i = 0; i < 3; ++i) {
         const int f = r.lo[i] < kBins ? r.lo[i] : 0;
         r.mass[i] = sh.mass[f];
@@ -668,30 +699,32 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
 __device__ __forceinline__ u64 entry_of(float x, int i) { return (u64)~key_of(cleaned(x)) << 32 | (unsigned)i; }
 __device__ __forceinline__ float entry_value(u64 l) { return value_of(~(unsigned)(l >> 32)); }
 
-// Lists the elements of runs r among [i0, i1): sh.n of them, those past kList
+// Lists the elements of runs r among [i0, i1): sh.n of them, those past LIST
 // left out.
-template <int TYPE, int NR>
+template <int TYPE, int NR, int NT, int LIST>
 __device__ __forceinline__ void list_runs(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r,
-                                          Lds& sh) {
+                                          LdsList<NT, LIST>& sh) {
     float lo[NR], hi[NR];
+#pragma unroll
     for (int i = 0; i < NR; ++i) {
         lo[i] = (float)r.lo[i];
         hi[i] = (float)(r.hi[i] + 1);
     }
-    each<TYPE>(x, i0, i1, [&](float v, int i) {
+    each<TYPE, NT>(x, i0, i1, [&](float v, int i) {
         const float b = y(v);
         bool in = false;
 #pragma unroll
         for (int k = 0; k < NR; ++k) in |= (b >= lo[k]) & (b < hi[k]);
         if (in) {
             const int at = atomicAdd(&sh.n, 1);
-            if (at < kList) sh.list[at] = entry_of(v, i);
+            if (at < LIST) sh.list[at] = entry_of(v, i);
         }
     });
 }
 
-template <int TYPE>
-__device__ void fill_list(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r, Lds& sh) {
+template <int TYPE, int NT, int LIST>
+__device__ void fill_list(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r,
+                          LdsList<NT, LIST>& sh) {
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     if (r.lo[1] == kNone)
@@ -701,6 +734,14 @@ __device__ void fill_list(const typename Logit<TYPE>::T* x, int i0, int i1, cons
     else
         list_runs<TYPE, 3>(x, i0, i1, y, r, sh);
     __syncthreads();
+}
+
+// a / b, where it is below 2^20 (in binary64, off by one at most, and put right).
+__device__ __forceinline__ unsigned ratio(u64 a, u64 b) {
+    unsigned q = (unsigned)((double)a / (double)b);
+    q -= q * b > a;
+    q += (q + 1) * b <= a;
+    return q;
 }
 
 // One element of a group that is small or of few values: its sums in front.
@@ -727,7 +768,7 @@ __device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, 
     if (s.p < 1.f) {
         const u64 t = p_target(s.p, sum);
         const bool mine = here && z.before <= t && t - z.before < z.mass;
-        const u64 got = pick(mine, z.before + (mine ? (t - z.before) / weight + 1 : 0) * weight);
+        const u64 got = pick(mine, z.before + (mine ? ratio(t - z.before, weight) + 1 : 0) * weight);
         if (!got) return 0;
         kept = got < kept ? got : kept;
     }
@@ -737,13 +778,13 @@ __device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, 
 }
 
 // The k <= kFew elements at the front of the list, one a lane of the first wave.
-template <typename B>
+template <int NT, typename B>
 __device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
-                           int k, Lds& sh) {
+                           int k, Lds<NT>& sh) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         const bool here = lane < k;
-        const u64 l = here ? sh.list[lane] : ~0ull;
+        const u64 l = here ? sh.second[lane] : ~0ull;
         const float x = entry_value(l);
         const u64 e = here ? w(x) : 0;
         const int b = here ? bin(x) : -1;
@@ -770,21 +811,21 @@ __device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const S
 
 // More elements than that, of up to kValues values: the values one after
 // another, then the token among equal ones by its index.
-template <typename B>
+template <int NT, typename B>
 __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
-                            int k, Lds& sh) {
+                            int k, Lds<NT>& sh) {
     const int lane = threadIdx.x & 63;
-    unsigned* const values = sh.wave_count;  // inverted keys, rising: falling logits
-    unsigned* const numbers = values + kValues;
-    static_assert(2 * kValues <= kWaves, "");
-    if (threadIdx.x < kWaves) sh.wave_count[threadIdx.x] = threadIdx.x < kValues ? ~0u : 0u;
+    if (threadIdx.x < kValues) {
+        sh.values[threadIdx.x] = ~0u;  // inverted keys, rising: falling logits
+        sh.numbers[threadIdx.x] = 0;
+    }
     __syncthreads();
     unsigned last = 0;  // (0 inverted is a NaN's key)
     int nv = 0;
     for (;; ++nv) {
         unsigned v = ~0u;
-        for (int i = threadIdx.x; i < k; i += kThreads) {
-            const unsigned e = (unsigned)(sh.list[i] >> 32);
+        for (int i = threadIdx.x; i < k; i += NT) {
+            const unsigned e = (unsigned)(sh.second[i] >> 32);
             v = e > last && e < v ? e : v;
         }
         for (int d = 1; d < 64; d <<= 1) {
@@ -796,20 +837,20 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
             if (more) return false;
             break;
         }
-        if (lane == 0) atomicMin(&values[nv], v);
+        if (lane == 0) atomicMin(&sh.values[nv], v);
         __syncthreads();
-        last = values[nv];
+        last = sh.values[nv];
         if (last == ~0u) break;
         unsigned c = 0;
-        for (int i = threadIdx.x; i - (int)threadIdx.x < k; i += kThreads)
-            c += __builtin_popcountll(__ballot(i < k && (unsigned)(sh.list[i] >> 32) == last));
-        if (lane == 0 && c) atomicAdd(&numbers[nv], c);
+        for (int i = threadIdx.x; i - (int)threadIdx.x < k; i += NT)
+            c += __builtin_popcountll(__ballot(i < k && (unsigned)(sh.second[i] >> 32) == last));
+        if (lane == 0 && c) atomicAdd(&sh.numbers[nv], c);
     }
     __syncthreads();
     if (threadIdx.x < 64) {
         const bool here = lane < nv;
-        const float x = value_of(~(here ? values[lane] : 0x7FFFFFFFu));
-        const unsigned c = here ? numbers[lane] : 0;
+        const float x = value_of(~(here ? sh.values[lane] : 0x7FFFFFFFu));
+        const unsigned c = here ? sh.numbers[lane] : 0;
         const u64 e = here ? w(x) : 0;
         const int b = here ? bin(x) : -1;
         Spot z{here ? sh.mass[b] : 0, e * c, here ? sh.count[b] : 0, c};
@@ -824,8 +865,8 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
         const u64 sum = kept_of(s, a.V, z, e, here, q, &target);
         const bool mine = sum && here && z.before <= target && target - z.before < z.mass;
         if (mine) {
-            sh.at[5] = (int)((target - z.before) / e);
-            sh.at[6] = (int)values[lane];
+            sh.at[5] = (int)ratio(target - z.before, e);
+            sh.at[6] = (int)sh.values[lane];
             if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
         }
         const bool found = __ballot(mine) != 0;
@@ -837,15 +878,17 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
     // of the equal ones the one with `rank` lower indices: by the index's upper bits, then among those that share them
     static_assert(TER_HIP_SAMPLE_V_MAX <= kBins << 8, "");
     clear_bins(sh);
-    for (int i = threadIdx.x; i < k; i += kThreads)
-        if ((unsigned)(sh.list[i] >> 32) == key) atomicAdd(&sh.count[(unsigned)sh.list[i] >> 8], 1u);
+    for (int i = threadIdx.x; i < k; i += NT)
+        if ((unsigned)(sh.second[i] >> 32) == key) atomicAdd(&sh.count[(unsigned)sh.second[i] >> 8], 1u);
     __syncthreads();
-    constexpr int PER = kBins / kThreads;
+    constexpr int PER = kBins / NT;
     const int b0 = threadIdx.x * PER;
     u64 none = 0, all;
     unsigned n = 0;
+#pragma unroll
     for (int i = 0; i < PER; ++i) n += sh.count[b0 + i];
     block_scan(none, n, &all, sh);
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
         const unsigned c = sh.count[b0 + i];
         if (n <= rank && rank - n < c) {
@@ -857,9 +900,9 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     const int bucket = sh.at[0];
-    for (int i = threadIdx.x; i < k; i += kThreads)
-        if ((unsigned)(sh.list[i] >> 32) == key && (int)((unsigned)sh.list[i] >> 8) == bucket)
-            sh.mass[atomicAdd(&sh.n, 1)] = (unsigned)sh.list[i];  // (256 at most)
+    for (int i = threadIdx.x; i < k; i += NT)
+        if ((unsigned)(sh.second[i] >> 32) == key && (int)((unsigned)sh.second[i] >> 8) == bucket)
+            sh.mass[atomicAdd(&sh.n, 1)] = (unsigned)sh.second[i];  // (256 at most)
     __syncthreads();
     if ((int)threadIdx.x < sh.n) {
         const u64 me = sh.mass[threadIdx.x];
@@ -872,16 +915,19 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
 
 // The token from the n elements in the list, which are all of runs r; false
 // where its place is not found (too many elements close together).
-__device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w, const Runs& r,
-                           int n, Lds& sh) {
+template <int NT>
+__device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w,
+                                           const Runs& r, int n, Lds<NT>& sh) {
     // the runs' bins, each cut into 2^shift
     int bins = 0, first[3], start[3], shift = 8;
+#pragma unroll
     for (int i = 0; i < 3; ++i) {
         first[i] = bins;
         bins += r.lo[i] != kNone ? r.hi[i] - r.lo[i] + 1 : 0;
     }
     while ((bins << shift) > kBins) --shift;
     int off[3];
+#pragma unroll
     for (int i = 0; i < 3; ++i) {
         start[i] = r.lo[i] != kNone ? first[i] << shift : kNone;
         off[i] = (first[i] - r.lo[i]) * (1 << shift);
@@ -893,7 +939,8 @@ __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const S
     };
     clear_bins(sh);
     u64 kept = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += NT) {
         const float x = entry_value(sh.list[i]);
         const u64 e = w(x);
         const int b = bin(x);
@@ -908,28 +955,20 @@ __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const S
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     const Runs q = level_of(s, a.V, true, &r, start, sh);
-    // the elements of its runs, to the front of the list
-    const int per = (n + kThreads - 1) / kThreads;
-    u64 keep[kList / kThreads];
-    int m = 0;
-#pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) {
-        if (i >= per) break;
-        const int at = i * kThreads + (int)threadIdx.x;
-        keep[i] = at < n ? sh.list[at] : 0;
-        const int b = at < n ? bin(entry_value(keep[i])) : -1;
-        const bool in = (b >= q.lo[0] && b <= q.hi[0]) || (b >= q.lo[1] && b <= q.hi[1]) || (b >= q.lo[2] && b <= q.hi[2]);
-        m = m * 2 + in;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) {
-        if (i >= per) break;
-        if (m >> (per - 1 - i) & 1) sh.list[atomicAdd(&sh.n, 1)] = keep[i];
+    // the elements of its runs
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const u64 e = sh.list[i];
+        const int b = bin(entry_value(e));
+        if ((b >= q.lo[0] && b <= q.hi[0]) || (b >= q.lo[1] && b <= q.hi[1]) || (b >= q.lo[2] && b <= q.hi[2])) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < kSecond) sh.second[at] = e;
+        }
     }
     __syncthreads();
     const int k = sh.n;
-    return k <= kFew ? finish_few(a, row, s, bin, w, q, k, sh) : finish_many(a, row, s, bin, w, q, k, sh);
+    if (k <= kFew) return finish_few(a, row, s, bin, w, q, k, sh);
+    return k <= kSecond && finish_many(a, row, s, bin, w, q, k, sh);
 }
 
 // 2^44 times 2^(j / 256).
@@ -950,8 +989,8 @@ __device__ __forceinline__ bool no_sums(const Extent& x, const Settings& s) {
 // Rows with an infinite logit go the general path.
 __device__ __forceinline__ bool infinite(const Extent& x) { return x.high == __builtin_inff(); }
 
-template <int TYPE>
-__device__ void settle(const SampleArgs& a, int row, const Extent& x, Lds& sh) {
+template <int TYPE, int NT>
+__device__ void settle(const SampleArgs& a, int row, const Extent& x, LdsScan<NT>& sh) {
     const bool none = x.high == -__builtin_inff();
     const int i = none ? -1 : first_of<TYPE>(row_of<TYPE>(a, row), a.V, cleaned(x.high), sh);
     if (threadIdx.x == 0) {
@@ -960,10 +999,13 @@ __device__ void settle(const SampleArgs& a, int row, const Extent& x, Lds& sh) {
     }
 }
 
+constexpr int kRowThreads = 1024, kSliceThreads = 512;
+constexpr int kSliceList = 4096;
+
 // One workgroup a row, start to end.
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
-    __shared__ Lds sh;
+__global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) {
+    __shared__ Lds<kRowThreads> sh;
     const int row = blockIdx.x;
     const auto* x = row_of<TYPE>(a, row);
     const Settings s = settings_of(a, row);
@@ -1007,13 +1049,14 @@ __device__ __forceinline__ Extent row_extent(const SampleArgs& a, const SampleRo
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
-    __shared__ LdsSmall sh;
+__global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ LdsScan<NT> sh;
     int row, g, i0, i1;
     slice_of(a, row, g, i0, i1);
     SampleRow* z = a.ws + row;
     // the row's sums, cleared for the next launch
-    for (int i = g * kThreads + threadIdx.x; i < kBins; i += a.slices * kThreads) {
+    for (int i = g * NT + threadIdx.x; i < kBins; i += a.slices * NT) {
         gptr(z->mass)[i] = 0;
         gptr(z->count)[i] = 0;
     }
@@ -1029,8 +1072,9 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
-    __shared__ Lds sh;
+__global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ LdsBins<NT> sh;
     int row, g, i0, i1;
     slice_of(a, row, g, i0, i1);
     SampleRow* z = a.ws + row;
@@ -1042,7 +1086,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
     clear_bins(sh);
     fill_bins<TYPE>(row_of<TYPE>(a, row), i0, i1, mode, s.least, bins_of(x.high, x.low, s.T),
                     weights_of(sh.table, x.high, s.T), sh);
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    for (int i = threadIdx.x; i < kBins; i += NT) {
         if (mode != kCount && sh.mass[i]) atomicAdd(&z->mass[i], sh.mass[i]);
         if (mode != kMass && sh.count[i]) atomicAdd(&z->count[i], sh.count[i]);
     }
@@ -1050,15 +1094,16 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_list_kernel(SampleArgs a) {
-    __shared__ Lds sh;
+__global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ LdsList<NT, kSliceList> sh;
     int row, g, i0, i1;
     slice_of(a, row, g, i0, i1);
     SampleRow* z = a.ws + row;
     const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
     if (no_sums(x, s) || infinite(x)) return;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    for (int i = threadIdx.x; i < kBins; i += NT) {
         sh.mass[i] = gptr(z->mass)[i];
         sh.count[i] = gptr(z->count)[i];
     }
@@ -1066,6 +1111,7 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(SampleArgs a) {
     __syncthreads();
     const Runs r = level_of(s, a.V, mode_of(s, a.V) != kCount, nullptr, nullptr, sh);
     if (g == 0 && threadIdx.x == 0) {
+#pragma unroll
         for (int i = 0; i < 3; ++i) {
             z->lo[i] = r.lo[i];
             z->hi[i] = r.hi[i];
@@ -1076,21 +1122,24 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(SampleArgs a) {
     }
     fill_list<TYPE>(row_of<TYPE>(a, row), i0, i1, bins_of(x.high, x.low, s.T), r, sh);
     const int n = sh.n;
-    if (threadIdx.x == 0) sh.at[0] = n ? (int)atomicAdd(&z->n, (unsigned)n) : 0;  // (V at most in all)
+    // (more than the slice's list holds: none of the row's list is used)
+    if (threadIdx.x == 0) sh.at[0] = n ? (int)atomicAdd(&z->n, (unsigned)(n <= kSliceList ? n : kList + 1)) : 0;
     __syncthreads();
     const int at = sh.at[0];
-    for (int i = threadIdx.x; i < n && i < kList && at + i < kList; i += kThreads) gptr(z->list)[at + i] = sh.list[i];
+    for (int i = threadIdx.x; i < n && i < kSliceList && at + i < kList; i += NT) gptr(z->list)[at + i] = sh.list[i];
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
-    __shared__ Lds sh;
+__global__ __launch_bounds__(kSliceThreads) void sample_finish_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ Lds<NT> sh;
     const int row = blockIdx.x;
     const SampleRow* z = a.ws + row;
     const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
     const int n = (int)*gptr(&z->n);
     Runs r;
+#pragma unroll
     for (int i = 0; i < 3; ++i) {
         r.lo[i] = gptr(z->lo)[i];
         r.hi[i] = gptr(z->hi)[i];
@@ -1105,7 +1154,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
     fill_table(sh.table);
     if (!infinite(x) && n <= kList) {
-        for (int i = threadIdx.x; i < n; i += kThreads) sh.list[i] = gptr(z->list)[i];
+        for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = gptr(z->list)[i];
         __syncthreads();
         if (finish_row(a, row, s, bins_of(x.high, x.low, s.T), weights_of(sh.table, x.high, s.T), r, n, sh)) return;
         __syncthreads();
@@ -1115,9 +1164,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
 
 template <int TYPE>
 hipError_t launch(const SampleArgs& a, hipStream_t st) {
-    const dim3 rows(a.rows), block(kThreads);
+    const dim3 rows(a.rows), block(kSliceThreads);
     if (a.slices <= 1) {
-        hipLaunchKernelGGL(sample_rows_kernel<TYPE>, rows, block, 0, st, a);
+        hipLaunchKernelGGL(sample_rows_kernel<TYPE>, rows, dim3(kRowThreads), 0, st, a);
         return hipGetLastError();
     }
     const dim3 grid(a.rows * a.slices);
