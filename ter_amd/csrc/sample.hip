@@ -65,7 +65,9 @@ struct Weights {
         double p = __builtin_fma(r, a * a * a / 6, a * a / 2);
         p = __builtin_fma(r, p, a);
         p = __builtin_fma(r, p, 1.0);
-        return __builtin_ldexp(table[n & 255] * p, n >> 8);
+        // (the table's number times 2^(n >> 8): into its exponent)
+        const u64 e = __builtin_bit_cast(u64, table[n & 255]) + ((u64)(unsigned)((n & ~255) << 12) << 32);
+        return __builtin_bit_cast(double, e) * p;
     }
     // (below 2^52 the low bits of a number added to 2^52 are its nearest integer)
     static __device__ __forceinline__ u64 whole(double v) {
@@ -269,7 +271,7 @@ struct Row {
 // One row by one workgroup: a search through the row's values for each cut and
 // for the draw.  Right for every row; the general path.
 template <int TYPE, int NT>
-__device__ void sample_row(const SampleArgs& a, int row, const double* table, Shared<NT>& sh) {
+__device__ __forceinline__ void sample_row(const SampleArgs& a, int row, const double* table, Shared<NT>& sh) {
     Row<TYPE, NT> x{gptr(reinterpret_cast<const typename Logit<TYPE>::T*>(a.logits + (long long)row * a.stride)), a.V};
     const unsigned top = x.largest(sh);
     const Settings s = settings_of(a, row);
@@ -334,6 +336,7 @@ struct Bins {
     }
 };
 constexpr float kLast = (float)(kBins - 1);
+constexpr int kSpare = 64;
 
 // m, low: the largest logit and the smallest that is a number.
 __device__ __forceinline__ Bins bins_of(float m, float low, double T) {
@@ -359,8 +362,8 @@ struct LdsScan {
 template <int NT>
 struct LdsBins : LdsScan<NT> {
     double table[256];
-    u64 mass[kBins];
-    unsigned count[kBins];
+    u64 mass[kBins + kSpare];
+    unsigned count[kBins + kSpare];
     // places of a level: bin, sums at its start and end
     int at[8];
     u64 from[8], to[8];
@@ -383,8 +386,8 @@ struct Lds : LdsList<NT, kList> {
     unsigned values[kValues], numbers[kValues];
 };
 
-// f(x, i) of elements [i0, i1) of a row by the workgroup's threads, 16 bytes a
-// load, four loads in flight.
+// f(x, i), x an array of consecutive elements from i on, of all elements [i0,
+// i1) of a row by the workgroup's threads, 16 bytes a load, four loads in flight.
 template <int TYPE, int kThreads, typename F>
 __device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0, int i1, F f) {
     typedef typename Logit<TYPE>::T T;
@@ -398,7 +401,10 @@ __device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0,
     const int nv = (n - head) / VE, tail = head + nv * VE;
     // (the elements outside of whole vectors: at most 2 VE - 2, one a thread)
     const int odd = t < head ? t : t - head < n - tail ? tail + t - head : -1;
-    if (odd >= 0) f(Logit<TYPE>::raw(p[odd]), i0 + odd);
+    if (odd >= 0) {
+        const float x[1] = {Logit<TYPE>::raw(p[odd])};
+        f(x, i0 + odd);
+    }
     const TER_GLOBAL u32x4* v = reinterpret_cast<const TER_GLOBAL u32x4*>(p + head);
     for (int a = t; a < nv; a += U * kThreads) {
         u32x4 r[U];
@@ -407,20 +413,24 @@ __device__ __forceinline__ void each(const typename Logit<TYPE>::T* row, int i0,
 #pragma unroll
         for (int q = 0; q < U; ++q) {
             if (a + q * kThreads >= nv) break;
-            const int i = i0 + head + (a + q * kThreads) * VE;
+            float x[VE];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned w = r[q][e];
                 if constexpr (TYPE == TER_HIP_T_F32) {
-                    f(__builtin_bit_cast(float, w), i + e);
+                    x[e] = __builtin_bit_cast(float, w);
                 } else {
-                    f(Logit<TYPE>::raw((uint16_t)w), i + 2 * e);
-                    f(Logit<TYPE>::raw((uint16_t)(w >> 16)), i + 2 * e + 1);
+                    x[2 * e] = Logit<TYPE>::raw((uint16_t)w);
+                    x[2 * e + 1] = Logit<TYPE>::raw((uint16_t)(w >> 16));
                 }
             }
+            f(x, i0 + head + (a + q * kThreads) * VE);
         }
     }
 }
+
+template <typename A>
+constexpr int length_of(const A& x) { return (int)(sizeof(x) / sizeof(x[0])); }
 
 // The largest logit of a row or slice, and the smallest that is a number.
 struct Extent {
@@ -434,7 +444,10 @@ struct Extent {
 template <int TYPE, int NT>
 __device__ Extent extent_of(const typename Logit<TYPE>::T* row, int i0, int i1, LdsScan<NT>& sh) {
     Extent x{-__builtin_inff(), __builtin_inff()};
-    each<TYPE, NT>(row, i0, i1, [&](float v, int) { x.join(v, v == -__builtin_inff() ? x.low : v); });
+    each<TYPE, NT>(row, i0, i1, [&](const auto& v, int) {
+#pragma unroll
+        for (int e = 0; e < length_of(v); ++e) x.join(v[e], v[e] == -__builtin_inff() ? x.low : v[e]);
+    });
     for (int s = 1; s < 64; s <<= 1) x.join(__shfl_xor(x.high, s), __shfl_xor(x.low, s));
     if ((threadIdx.x & 63) == 0) {
         sh.wave_count[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, x.high);
@@ -451,7 +464,9 @@ __device__ Extent extent_of(const typename Logit<TYPE>::T* row, int i0, int i1, 
 template <int TYPE, int NT>
 __device__ int first_of(const typename Logit<TYPE>::T* row, int V, float m, LdsScan<NT>& sh) {
     int at = V;
-    each<TYPE, NT>(row, 0, V, [&](float x, int i) { at = cleaned(x) == m && i < at ? i : at; });
+    each<TYPE, NT>(row, 0, V, [&](const auto& x, int i) {
+        for (int e = 0; e < length_of(x); ++e) at = cleaned(x[e]) == m && i + e < at ? i + e : at;
+    });
     for (int s = 1; s < 64; s <<= 1) {
         const int o = __shfl_xor(at, s);
         at = o < at ? o : at;
@@ -474,53 +489,77 @@ __device__ __forceinline__ void clear_bins(LdsBins<NT>& sh) {
     __syncthreads();
 }
 
-// Elements [i0, i1) into the histogram in LDS.  (What is computed of elements
-// of the last bin is not used: their weights may be anything.)
+// Elements [i0, i1) into the histogram in LDS.  Those of the last bin go to one
+// of kSpare more by their lane, which nobody reads, so that many do not meet in
+// one place; their weights may be anything.  No branches: the weights of a
+// load's elements are computed side by side.
 template <int TYPE, int NT>
 __device__ void fill_bins(const typename Logit<TYPE>::T* row, int i0, int i1, int mode, u64 least, const Bins& y,
                           const Weights& w, LdsBins<NT>& sh) {
+    const float last = kLast + (float)(threadIdx.x & (kSpare - 1));
     if (mode == kCount) {
-        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
-            const int b = (int)__builtin_fminf(y(x), kLast);
-            if (b < kBins - 1) atomicAdd(&sh.count[b], 1u);
-        });
-    } else if (mode == kMass && !least) {
-        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
-            const u64 e = w.quick(x);
-            const int b = (int)__builtin_fminf(y(x), kLast);
-            if (b < kBins - 1) atomicAdd(&sh.mass[b], e);
+        each<TYPE, NT>(row, i0, i1, [&](const auto& x, int) {
+#pragma unroll
+            for (int e = 0; e < length_of(x); ++e) atomicAdd(&sh.count[(int)__builtin_fminf(y(x[e]), last)], 1u);
         });
     } else {
         u64 kept = 0;
-        each<TYPE, NT>(row, i0, i1, [&](float x, int) {
-            const u64 e = w.quick(x);
-            const int b = (int)__builtin_fminf(y(x), kLast);
-            if (b < kBins - 1) {
-                if (mode != kMass) atomicAdd(&sh.count[b], 1u);
-                atomicAdd(&sh.mass[b], e);
-                kept += e >= least ? e : 0;
+        const bool sums = least != 0, counts = mode != kMass;
+        each<TYPE, NT>(row, i0, i1, [&](const auto& x, int) {
+            constexpr int N = sizeof(x) / sizeof(x[0]);
+            u64 m[N];
+            int b[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                b[e] = (int)__builtin_fminf(y(x[e]), last);
+                m[e] = w.quick(x[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) atomicAdd(&sh.mass[b[e]], m[e]);
+            if (sums) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) kept += b[e] < kBins - 1 && m[e] >= least ? m[e] : 0;
+            }
+            if (counts) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) atomicAdd(&sh.count[b[e]], 1u);
             }
         });
-        kept = wave_sum(kept);
-        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.least_mass, kept);
+        if (sums) {
+            kept = wave_sum(kept);
+            if ((threadIdx.x & 63) == 0) atomicAdd(&sh.least_mass, kept);
+        }
     }
     __syncthreads();
+    if (threadIdx.x == 0) {
+        sh.mass[kBins - 1] = 0;
+        sh.count[kBins - 1] = 0;
+    }
+    __syncthreads();
+}
+
+// m and n plus those of the lane that a DPP control names (0 where there is none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void wave_scan_step(u64& m, unsigned& n) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)m, CTRL, ROWS, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(m >> 32), CTRL, ROWS, 0xF, false);
+    m += (u64)hi << 32 | lo;
+    n += (unsigned)__builtin_amdgcn_update_dpp(0, (int)n, CTRL, ROWS, 0xF, false);
 }
 
 // Exclusive running sums over a workgroup's threads; the whole in *all.
 template <int NT>
 __device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, LdsScan<NT>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // within the wave by DPP: rows of 16 lanes, then the rows' last lanes
     u64 im = m;
     unsigned in = n;
-    for (int s = 1; s < 64; s <<= 1) {
-        const u64 om = (u64)__shfl_up((long long)im, s);
-        const unsigned on = (unsigned)__shfl_up((int)in, s);
-        if (lane >= s) {
-            im += om;
-            in += on;
-        }
-    }
+    wave_scan_step<0x111, 0xF>(im, in);  // row_shr:1
+    wave_scan_step<0x112, 0xF>(im, in);
+    wave_scan_step<0x114, 0xF>(im, in);
+    wave_scan_step<0x118, 0xF>(im, in);
+    wave_scan_step<0x142, 0xA>(im, in);  // row_bcast:15
+    wave_scan_step<0x143, 0xC>(im, in);  // row_bcast:31
     if (lane == 63) {
         sh.wave_mass[wave] = im;
         sh.wave_count[wave] = in;
@@ -528,11 +567,12 @@ __device__ __forceinline__ void block_scan(u64& m, unsigned& n, u64* all, LdsSca
     __syncthreads();
     u64 bm = 0, sum = 0;
     unsigned bn = 0;
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < NT / 64; ++i) {
         const u64 e = sh.wave_mass[i];
+        const unsigned c = sh.wave_count[i];
         bm += i < wave ? e : 0;
-        bn += i < wave ? sh.wave_count[i] : 0;
+        bn += i < wave ? c : 0;
         sum += e;
     }
     m = bm + im - m;
@@ -567,13 +607,13 @@ __device__ __forceinline__ void swap_runs(Runs& r, int i, int j) {
     r.hi[j] = h;
 }
 
-// One level: the histogram in LDS becomes its running sums, each run's bins
-// [start[i], start[i + 1]) from the sums that `before` has in front of it
-// (null: one run from 0), and the places are found in it.  Listing of all up
+// One level: the histogram in LDS becomes its running sums, those of each run
+// of `before` (from bins 0, start1 and start2 on; null: one run of all) from the
+// sums in front of it, and the places are found in it.  Listing of all up
 // to the last element of the top_k where there are no weights (weighted =
 // false).
 template <int NT>
-__device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted, const Runs* before, const int* start,
+__device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted, const Runs* before, int start1, int start2,
                                          LdsBins<NT>& sh) {
     constexpr int PER = kBins / NT;  // bins of a thread
     const int b0 = threadIdx.x * PER;
@@ -596,20 +636,15 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
     if (threadIdx.x < 8) sh.at[threadIdx.x] = kNone;
     __syncthreads();
     if (before) {
-        u64 dm[3];
-        unsigned dn[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const int f = start[i] < kBins ? start[i] : 0;
-            dm[i] = before->mass[i] - sh.mass[f];
-            dn[i] = before->count[i] - sh.count[f];
-        }
+        const int f1 = start1 < kBins ? start1 : 0, f2 = start2 < kBins ? start2 : 0;
+        const u64 m0 = before->mass[0], m1 = before->mass[1] - sh.mass[f1], m2 = before->mass[2] - sh.mass[f2];
+        const unsigned n0 = before->count[0], n1 = before->count[1] - sh.count[f1], n2 = before->count[2] - sh.count[f2];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int b = b0 + i, k = b >= start[2] ? 2 : b >= start[1] ? 1 : 0;
-            sh.mass[b] = m[i] += k == 2 ? dm[2] : k == 1 ? dm[1] : dm[0];
-            sh.count[b] = n[i] += k == 2 ? dn[2] : k == 1 ? dn[1] : dn[0];
+            const int b = b0 + i;
+            sh.mass[b] = m[i] += b >= start2 ? m2 : b >= start1 ? m1 : m0;
+            sh.count[b] = n[i] += b >= start2 ? n2 : b >= start1 ? n1 : n0;
         }
         if (before->total) r.total = before->total;
     }
@@ -710,14 +745,25 @@ __device__ __forceinline__ void list_runs(const typename Logit<TYPE>::T* x, int 
         lo[i] = (float)r.lo[i];
         hi[i] = (float)(r.hi[i] + 1);
     }
-    each<TYPE, NT>(x, i0, i1, [&](float v, int i) {
-        const float b = y(v);
-        bool in = false;
+    each<TYPE, NT>(x, i0, i1, [&](const auto& v, int i) {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+        unsigned in = 0;
 #pragma unroll
-        for (int k = 0; k < NR; ++k) in |= (b >= lo[k]) & (b < hi[k]);
+        for (int e = 0; e < N; ++e) {
+            const float b = y(v[e]);
+            bool one = false;
+#pragma unroll
+            for (int k = 0; k < NR; ++k) one |= (b >= lo[k]) & (b < hi[k]);
+            in |= one ? 1u << e : 0;
+        }
         if (in) {
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < LIST) sh.list[at] = entry_of(v, i);
+            int at = atomicAdd(&sh.n, __builtin_popcount(in));
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (in >> e & 1) {
+                    if (at < LIST) sh.list[at] = entry_of(v[e], i + e);
+                    ++at;
+                }
         }
     });
 }
@@ -918,23 +964,22 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
 template <int NT>
 __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w,
                                            const Runs& r, int n, Lds<NT>& sh) {
-    // the runs' bins, each cut into 2^shift
-    int bins = 0, first[3], start[3], shift = 8;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        first[i] = bins;
-        bins += r.lo[i] != kNone ? r.hi[i] - r.lo[i] + 1 : 0;
-    }
-    while ((bins << shift) > kBins) --shift;
-    int off[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        start[i] = r.lo[i] != kNone ? first[i] << shift : kNone;
-        off[i] = (first[i] - r.lo[i]) * (1 << shift);
-    }
-    auto bin = [&](float x) {
+    // the runs' bins, each cut into 2^shift (no choice between variables: the
+    // compiler makes it an array in LDS, addressed by the dispatch packet, which is in host memory: 10 us)
+    const int len0 = r.hi[0] - r.lo[0] + 1, len1 = r.lo[1] != kNone ? r.hi[1] - r.lo[1] + 1 : 0;
+    const int len2 = r.lo[2] != kNone ? r.hi[2] - r.lo[2] + 1 : 0;
+    int shift = 8;
+    while (((len0 + len1 + len2) << shift) > kBins) --shift;
+    const int start1 = r.lo[1] != kNone ? len0 << shift : kNone;
+    const int start2 = r.lo[2] != kNone ? (len0 + len1) << shift : kNone;
+    const int lo1 = r.lo[1], lo2 = r.lo[2];
+    const int off0 = -r.lo[0] * (1 << shift), off1 = (len0 - lo1) * (1 << shift) - off0;
+    const int off2 = (len0 + len1 - lo2) * (1 << shift) - off1 - off0;
+    auto bin = [=](float x) {
         const int f = (int)(y(x) * 256.f), b = f >> 8;  // (exact; below 0 by a rounding: the first)
-        const int i = (f >> (8 - shift)) + (b >= r.lo[2] ? off[2] : b >= r.lo[1] ? off[1] : off[0]);
+        int i = (f >> (8 - shift)) + off0;
+        i += b >= lo1 ? off1 : 0;
+        i += b >= lo2 ? off2 : 0;
         return i < 0 ? 0 : i < kBins ? i : kBins - 1;
     };
     clear_bins(sh);
@@ -954,7 +999,7 @@ __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const S
     }
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    const Runs q = level_of(s, a.V, true, &r, start, sh);
+    const Runs q = level_of(s, a.V, true, &r, start1, start2, sh);
     // the elements of its runs
 #pragma unroll 1
     for (int i = threadIdx.x; i < n; i += NT) {
@@ -990,7 +1035,7 @@ __device__ __forceinline__ bool no_sums(const Extent& x, const Settings& s) {
 __device__ __forceinline__ bool infinite(const Extent& x) { return x.high == __builtin_inff(); }
 
 template <int TYPE, int NT>
-__device__ void settle(const SampleArgs& a, int row, const Extent& x, LdsScan<NT>& sh) {
+__device__ __forceinline__ void settle(const SampleArgs& a, int row, const Extent& x, LdsScan<NT>& sh) {
     const bool none = x.high == -__builtin_inff();
     const int i = none ? -1 : first_of<TYPE>(row_of<TYPE>(a, row), a.V, cleaned(x.high), sh);
     if (threadIdx.x == 0) {
@@ -1021,7 +1066,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) 
         const int mode = mode_of(s, a.V);
         clear_bins(sh);
         fill_bins<TYPE>(x, 0, a.V, mode, s.least, y, w, sh);
-        const Runs r = level_of(s, a.V, mode != kCount, nullptr, nullptr, sh);
+        const Runs r = level_of(s, a.V, mode != kCount, nullptr, kNone, kNone, sh);
         fill_list<TYPE>(x, 0, a.V, y, r, sh);
         const int n = sh.n;
         if (n <= kList && finish_row(a, row, s, y, w, r, n, sh)) return;
@@ -1109,7 +1154,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
     }
     if (threadIdx.x == 0) sh.least_mass = *gptr(&z->least_mass);
     __syncthreads();
-    const Runs r = level_of(s, a.V, mode_of(s, a.V) != kCount, nullptr, nullptr, sh);
+    const Runs r = level_of(s, a.V, mode_of(s, a.V) != kCount, nullptr, kNone, kNone, sh);
     if (g == 0 && threadIdx.x == 0) {
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
