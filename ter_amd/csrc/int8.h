@@ -49,5 +49,6 @@ hipError_t launch_w8_unpack(const uint8_t* tiles, const float* scale, int8_t* q,
 hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
                         hipStream_t st);
 hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st);
+hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st);  // many rows
 
 }  // namespace terhip

@@ -51,9 +51,11 @@ int check_x(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
     return check_rows("rows", x->data, x->type, x->stride, w->K);
 }
 
-// Whether the kernels read the rows where they are.
+// Whether the kernels read the rows where they are (256 of them within 32-bit
+// offsets).
 bool in_place(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
-    return x->type == TER_HIP_T_I8 && w->K % 16 == 0 && aligned(x->data, 16) && (x->stride % 16 == 0 || x->n == 1);
+    return x->type == TER_HIP_T_I8 && w->K % 16 == 0 && aligned(x->data, 16) &&
+           ((x->stride % 16 == 0 && x->stride <= 1 << 22) || x->n == 1);
 }
 
 size_t row_bytes(const ter_hip_w8_t* w) { return (size_t)i8_units(w->K) * kI8Unit; }

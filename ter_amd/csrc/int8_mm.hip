@@ -2,48 +2,10 @@
 // v_mfma_i32_16x16x64_i8, exact sums in int32.
 #include "common.h"
 #include "int8.h"
+#include "int8_store.h"
 
 namespace terhip {
 namespace {
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-// Scaled results of 8 consecutive channels of one token, `left` of which
-// exist.  ok16: every such group of 8 is 16-byte aligned in y.
-template <int YT>
-__device__ __forceinline__ void store8(char* y, long long at, int left, const int (&sum)[8], float xs,
-                                       const float (&ws)[8], bool wide) {
-#pragma clang fp contract(off)
-    if constexpr (YT == TER_HIP_T_I32 || YT == TER_HIP_T_F32) {
-        unsigned v[8];
-        for (int i = 0; i < 8; ++i)
-            v[i] = YT == TER_HIP_T_I32 ? (unsigned)sum[i] : __builtin_bit_cast(unsigned, (float)sum[i] * (xs * ws[i]));
-        TER_GLOBAL unsigned* p = gptr(reinterpret_cast<unsigned*>(y)) + at;
-        if (wide && left >= 8) {
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p) = u32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p + 4) = u32x4{v[4], v[5], v[6], v[7]};
-        } else {
-            for (int i = 0; i < 8; ++i)
-                if (i < left) p[i] = v[i];
-        }
-    } else {
-        uint16_t v[8];
-        for (int i = 0; i < 8; ++i) {
-            const float f = (float)sum[i] * (xs * ws[i]);
-            v[i] = YT == TER_HIP_T_F16 ? float_to_half_bits(f) : __builtin_bit_cast(uint16_t, (__bf16)f);
-        }
-        TER_GLOBAL uint16_t* p = gptr(reinterpret_cast<uint16_t*>(y)) + at;
-        if (wide && left >= 8) {
-            u32x4 o;
-            for (int i = 0; i < 4; ++i) o[i] = (unsigned)v[2 * i] | (unsigned)v[2 * i + 1] << 16;
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p) = o;
-        } else {
-            for (int i = 0; i < 8; ++i)
-                if (i < left) p[i] = v[i];
-        }
-    }
-}
 
 // A workgroup: 64 rows x 4 strip pairs, one pair a wave, operands straight
 // from memory.
@@ -95,6 +57,7 @@ hipError_t launch(const Int8MmArgs& a, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st) {
+    if (a.M > 64) return launch_int8_gemm(a, st);
     switch (a.y_type) {
         case TER_HIP_T_F16: return launch<TER_HIP_T_F16>(a, st);
         case TER_HIP_T_BF16: return launch<TER_HIP_T_BF16>(a, st);
