@@ -2,8 +2,8 @@
 // rows of a product in 8 bits: quantized by their largest magnitude, or
 // integers laid out at 16-byte alignment.
 //
-// Quantizing reads a row twice (its largest magnitude, then its values) by one
-// workgroup: the second time from the cache.
+// Quantizing is by one workgroup a row.  Weights, and rows of more than 16384
+// values, are read twice (their largest magnitude, then their values).
 #include "common.h"
 #include "int8.h"
 
@@ -11,6 +11,7 @@ namespace terhip {
 namespace {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 template <int TYPE>
 struct Elem;
@@ -78,11 +79,65 @@ __device__ unsigned row_amax(const typename Elem<TYPE>::T* row, int K, unsigned*
     return block_max(m, red);
 }
 
-// One workgroup a row: int8 rows, 16 values a thread.
+// One workgroup of T threads a row, held in registers: 8 NC values a thread,
+// read once.  VEC: rows are 16-byte aligned.
+template <int TYPE, int T, int NC, bool VEC>
+__global__ __launch_bounds__(T) void rows8_quant_kernel(const void* __restrict__ x, long long stride, int K,
+                                                        int8_t* __restrict__ q, long long ldq,
+                                                        float* __restrict__ scale) {
+    typedef typename Elem<TYPE>::T E;
+    __shared__ unsigned red[T / 64];
+    const TER_GLOBAL E* row = gptr(static_cast<const E*>(x) + (long long)blockIdx.x * stride);
+    float v[NC][8];
+    unsigned m = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int k = 8 * (threadIdx.x + T * c);
+        if (VEC && k + 8 <= K) {
+            constexpr int PER = 16 / (int)sizeof(E);
+#pragma unroll
+            for (int h = 0; h < 8 / PER; ++h) {
+                const u32x4 w = *reinterpret_cast<const TER_GLOBAL u32x4*>(row + k + h * PER);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const unsigned d = w[e * (int)sizeof(E) / 4];
+                    if constexpr (sizeof(E) == 4)
+                        v[c][h * PER + e] = Elem<TYPE>::get(__builtin_bit_cast(float, d));
+                    else
+                        v[c][h * PER + e] = Elem<TYPE>::get((uint16_t)(d >> (16 * (e & 1))));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[c][e] = k + e < K ? Elem<TYPE>::get(row[k + e]) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned b = __builtin_bit_cast(unsigned, v[c][e]) & 0x7FFFFFFFu;
+            m = b > m ? b : m;
+        }
+    const Quant z = quant_of(block_max(m, red));
+    if (threadIdx.x == 0) gptr(scale)[blockIdx.x] = z.inv;
+    TER_GLOBAL int8_t* out = gptr(q) + (long long)blockIdx.x * ldq;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int k = 8 * (threadIdx.x + T * c);
+        if (k >= ldq) continue;  // (zeros up to ldq, a multiple of 8)
+        u32x2 d = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e >> 2] |= ((unsigned)quantize(v[c][e], z.s) & 255u) << (8 * (e & 3));
+        *reinterpret_cast<TER_GLOBAL u32x2*>(out + k) = d;
+    }
+}
+
+// The same for rows of any length, read twice.
 template <int TYPE>
-__global__ __launch_bounds__(256) void rows8_quant_kernel(const void* __restrict__ x, long long stride, int K,
-                                                          int8_t* __restrict__ q, long long ldq,
-                                                          float* __restrict__ scale) {
+__global__ __launch_bounds__(256) void rows8_long_kernel(const void* __restrict__ x, long long stride, int K,
+                                                         int8_t* __restrict__ q, long long ldq,
+                                                         float* __restrict__ scale) {
     typedef typename Elem<TYPE>::T T;
     __shared__ unsigned red[4];
     const T* row = static_cast<const T*>(x) + (long long)blockIdx.x * stride;
@@ -185,6 +240,32 @@ __global__ __launch_bounds__(256) void w8_unpack_kernel(const uint8_t* __restric
 
 inline unsigned grid_of(long long n) { return (unsigned)(n < (1ll << 30) ? (n + 255) / 256 : 1 << 22); }
 
+template <int TYPE, int T, int NC>
+void launch_rows_as(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                    hipStream_t st) {
+    constexpr int EL = (int)sizeof(typename Elem<TYPE>::T);
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (stride * EL % 16 == 0 || M == 1);
+    if (vec)
+        hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, true>), dim3(M), dim3(T), 0, st, x, stride, K, q, ldq, scale);
+    else
+        hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, false>), dim3(M), dim3(T), 0, st, x, stride, K, q, ldq, scale);
+}
+
+template <int TYPE>
+void launch_rows_quant(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                       hipStream_t st) {
+    if (ldq <= 2048)
+        launch_rows_as<TYPE, 256, 1>(x, stride, M, K, q, ldq, scale, st);
+    else if (ldq <= 4096)
+        launch_rows_as<TYPE, 512, 1>(x, stride, M, K, q, ldq, scale, st);
+    else if (ldq <= 8192)
+        launch_rows_as<TYPE, 1024, 1>(x, stride, M, K, q, ldq, scale, st);
+    else if (ldq <= 16384)
+        launch_rows_as<TYPE, 1024, 2>(x, stride, M, K, q, ldq, scale, st);
+    else
+        hipLaunchKernelGGL(rows8_long_kernel<TYPE>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+}
+
 }  // namespace
 
 hipError_t launch_w8_pack(const int8_t* q, long long stride, const float* scale, uint8_t* tiles, float* out_scale,
@@ -228,11 +309,11 @@ hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K,
         hipLaunchKernelGGL(rows8_copy_kernel, dim3(grid_of(n)), dim3(256), 0, st, static_cast<const int8_t*>(x), stride,
                            K, q, ldq, chunks, n);
     } else if (type == TER_HIP_T_F16) {
-        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_F16>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+        launch_rows_quant<TER_HIP_T_F16>(x, stride, M, K, q, ldq, scale, st);
     } else if (type == TER_HIP_T_BF16) {
-        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_BF16>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+        launch_rows_quant<TER_HIP_T_BF16>(x, stride, M, K, q, ldq, scale, st);
     } else {
-        hipLaunchKernelGGL(rows8_quant_kernel<TER_HIP_T_F32>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+        launch_rows_quant<TER_HIP_T_F32>(x, stride, M, K, q, ldq, scale, st);
     }
     return hipGetLastError();
 }
