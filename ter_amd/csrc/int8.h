@@ -36,7 +36,20 @@ struct Int8MmArgs {
     long long ldx, ldy;   // bytes, elements
     int M, N, Kx, Ku;     // Kx: values of a row of x (a multiple of 16; those from K on meet zero weights)
     int y_type;
+    int x_type;           // TER_HIP_T_I8, or rows quantized by the product's kernel: x, ldx and Kx are those of its elements
+    int vec;              // such rows are 16-byte aligned
 };
+
+// Rows that the product's kernel quantizes itself: a team of waves holds one
+// in registers, at most kI8Chunks of 8 values a lane where 4 waves work
+// together, fewer where 8 or 16 do.
+constexpr int kI8Chunks = 8;
+__host__ __device__ inline int i8_team(int M, int waves) {
+    return M == 1 ? waves : M == 2 ? waves / 2 : M <= 4 ? waves / 4 : 1;
+}
+inline bool i8_quant_within(int M, int Ku) {
+    return M <= 4 && Ku * 128 <= kI8Chunks * 512 * i8_team(M, 4) && M * Ku <= 128;
+}
 
 hipError_t launch_w8_pack(const int8_t* q, long long stride, const float* scale, uint8_t* tiles, float* out_scale,
                           int K, int N, hipStream_t st);

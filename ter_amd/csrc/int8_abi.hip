@@ -58,10 +58,15 @@ bool in_place(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
            ((x->stride % 16 == 0 && x->stride <= 1 << 22) || x->n == 1);
 }
 
+// Whether the product's kernel quantizes the rows itself.
+bool quant_within(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
+    return x->type != TER_HIP_T_I8 && i8_quant_within(x->n, i8_units(w->K));
+}
+
 size_t row_bytes(const ter_hip_w8_t* w) { return (size_t)i8_units(w->K) * kI8Unit; }
 
 size_t ws_bytes_of(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
-    if (x->n == 0 || in_place(w, x)) return 0;
+    if (x->n == 0 || in_place(w, x) || quant_within(w, x)) return 0;
     return (size_t)x->n * (row_bytes(w) + 4);
 }
 
@@ -158,7 +163,14 @@ int ter_hip_w8_mm(const ter_hip_w8_t* w, const ter_hip_rows_t* x, void* y, int64
     a.N = w->N;
     a.Ku = i8_units(w->K);
     a.y_type = y_type;
-    if (in_place(w, x)) {
+    a.x_type = TER_HIP_T_I8;
+    if (quant_within(w, x)) {
+        a.x = static_cast<const int8_t*>(x->data);
+        a.ldx = x->stride;
+        a.Kx = w->K;
+        a.x_type = x->type;
+        a.vec = aligned(x->data, 16) && (x->n == 1 || x->stride * elem_bytes(x->type) % 16 == 0);
+    } else if (in_place(w, x)) {
         a.x = static_cast<const int8_t*>(x->data);
         a.xs = x->scale;
         a.ldx = x->n == 1 ? w->K : x->stride;

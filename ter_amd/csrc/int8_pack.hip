@@ -6,30 +6,10 @@
 // values, are read twice (their largest magnitude, then their values).
 #include "common.h"
 #include "int8.h"
+#include "int8_quant.h"
 
 namespace terhip {
 namespace {
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
-template <int TYPE>
-struct Elem;
-template <>
-struct Elem<TER_HIP_T_F16> {
-    typedef uint16_t T;
-    static __device__ float get(T v) { return half_bits_to_float(v); }
-};
-template <>
-struct Elem<TER_HIP_T_BF16> {
-    typedef uint16_t T;
-    static __device__ float get(T v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
-};
-template <>
-struct Elem<TER_HIP_T_F32> {
-    typedef float T;
-    static __device__ float get(T v) { return v; }
-};
 
 // The largest magnitude of a workgroup's values as bits (an infinity or NaN is
 // larger than any number), to every thread.
@@ -44,28 +24,6 @@ __device__ unsigned block_max(unsigned v, unsigned* red) {
     for (int i = 1; i < (int)(blockDim.x >> 6); ++i) v = red[i] > v ? red[i] : v;
     __syncthreads();
     return v;
-}
-
-struct Quant {
-    float s, inv;
-};
-
-// The steps of quant_rows_kernel (pack.hip), binary32, each rounded.
-__device__ __forceinline__ Quant quant_of(unsigned amax_bits) {
-#pragma clang fp contract(off)
-    Quant q;
-    q.s = 127.0f / (__builtin_bit_cast(float, amax_bits) + 1e-9f);
-    q.inv = 1.0f / q.s;
-    if (amax_bits >= 0x7F800000u) {  // an infinity or NaN in the row
-        q.s = 0.f;
-        q.inv = __builtin_nanf("");
-    }
-    return q;
-}
-
-__device__ __forceinline__ int quantize(float v, float s) {
-#pragma clang fp contract(off)
-    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_rintf(v * s), -128.f), 127.f);  // (of NaN -128)
 }
 
 // Largest magnitude of row `row` of K elements.
@@ -92,25 +50,7 @@ __global__ __launch_bounds__(T) void rows8_quant_kernel(const void* __restrict__
     unsigned m = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int k = 8 * (threadIdx.x + T * c);
-        if (VEC && k + 8 <= K) {
-            constexpr int PER = 16 / (int)sizeof(E);
-#pragma unroll
-            for (int h = 0; h < 8 / PER; ++h) {
-                const u32x4 w = *reinterpret_cast<const TER_GLOBAL u32x4*>(row + k + h * PER);
-#pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    const unsigned d = w[e * (int)sizeof(E) / 4];
-                    if constexpr (sizeof(E) == 4)
-                        v[c][h * PER + e] = Elem<TYPE>::get(__builtin_bit_cast(float, d));
-                    else
-                        v[c][h * PER + e] = Elem<TYPE>::get((uint16_t)(d >> (16 * (e & 1))));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[c][e] = k + e < K ? Elem<TYPE>::get(row[k + e]) : 0.f;
-        }
+        row8<TYPE>(row, 8 * (threadIdx.x + T * c), K, VEC, v[c]);
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -126,10 +66,7 @@ __global__ __launch_bounds__(T) void rows8_quant_kernel(const void* __restrict__
     for (int c = 0; c < NC; ++c) {
         const int k = 8 * (threadIdx.x + T * c);
         if (k >= ldq) continue;  // (zeros up to ldq, a multiple of 8)
-        u32x2 d = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e >> 2] |= ((unsigned)quantize(v[c][e], z.s) & 255u) << (8 * (e & 3));
-        *reinterpret_cast<TER_GLOBAL u32x2*>(out + k) = d;
+        *reinterpret_cast<TER_GLOBAL u32x2*>(out + k) = quantize8(v[c], z.s);
     }
 }
 

@@ -10,42 +10,44 @@ namespace terhip {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
-// Scaled results of 8 consecutive channels of one token, `left` of which
-// exist.  wide: groups of 8 are 16-byte aligned in y.
-template <int YT>
-__device__ __forceinline__ void store8(char* y, long long at, int left, const int (&sum)[8], float xs,
-                                       const float (&ws)[8], bool wide) {
+// Scaled results of C (4 or 8) consecutive channels of one token, `left` of
+// which exist.  wide: groups of 8 are 16-byte aligned in y.
+template <int YT, int C>
+__device__ __forceinline__ void store_run(char* y, long long at, int left, const int (&sum)[C], float xs,
+                                          const float (&ws)[C], bool wide) {
 #pragma clang fp contract(off)
     if constexpr (YT == TER_HIP_T_I32 || YT == TER_HIP_T_F32) {
-        unsigned v[8];
+        unsigned v[C];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < C; ++i)
             v[i] = YT == TER_HIP_T_I32 ? (unsigned)sum[i] : __builtin_bit_cast(unsigned, (float)sum[i] * (xs * ws[i]));
         TER_GLOBAL unsigned* p = gptr(reinterpret_cast<unsigned*>(y)) + at;
-        if (wide && left >= 8) {
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p) = u32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p + 4) = u32x4{v[4], v[5], v[6], v[7]};
+        if (wide && left >= C) {
+#pragma unroll
+            for (int i = 0; i < C; i += 4)
+                *reinterpret_cast<TER_GLOBAL u32x4*>(p + i) = u32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < C; ++i)
                 if (i < left) p[i] = v[i];
         }
     } else {
-        uint16_t v[8];
+        uint16_t v[C];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < C; ++i) {
             const float f = (float)sum[i] * (xs * ws[i]);
             v[i] = YT == TER_HIP_T_F16 ? float_to_half_bits(f) : __builtin_bit_cast(uint16_t, (__bf16)f);
         }
         TER_GLOBAL uint16_t* p = gptr(reinterpret_cast<uint16_t*>(y)) + at;
-        if (wide && left >= 8) {
-            u32x4 o;
+        if (wide && left >= C) {
+            typedef unsigned int words __attribute__((ext_vector_type(C / 2)));
+            words o;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = (unsigned)v[2 * i] | (unsigned)v[2 * i + 1] << 16;
-            *reinterpret_cast<TER_GLOBAL u32x4*>(p) = o;
+            for (int i = 0; i < C / 2; ++i) o[i] = (unsigned)v[2 * i] | (unsigned)v[2 * i + 1] << 16;
+            *reinterpret_cast<TER_GLOBAL words*>(p) = o;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < C; ++i)
                 if (i < left) p[i] = v[i];
         }
     }
@@ -76,7 +78,7 @@ __device__ __forceinline__ void store_tile(const Int8MmArgs& a, int m0, int n0, 
             if (m >= a.M) continue;
             const i32x4 u = acc[i][2 * p], v = acc[i][2 * p + 1];
             const int sum[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-            store8<YT>(a.y, (long long)m * a.ldy + n, a.N - n, sum, YT == TER_HIP_T_I32 ? 0.f : gptr(a.xs)[m], ws, wide);
+            store_run<YT, 8>(a.y, (long long)m * a.ldy + n, a.N - n, sum, YT == TER_HIP_T_I32 ? 0.f : gptr(a.xs)[m], ws, wide);
         }
     }
 }
