@@ -30,7 +30,7 @@ struct GCfg {
     static constexpr int BM = 16 * MBW * RW, BN = 16 * SW * CW;
     static constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB;
     static constexpr int XL = XB / 1024 / WAVES, WL = WB / 1024 / WAVES;  // loads of a wave and stage
-    static_assert(XB % (1024 * WAVES) == 0 && WB % (1024 * WAVES) == 0 && SW % 2 == 0, "");
+    static_assert(XB % (1024 * WAVES) == 0 && WB % (1024 * WAVES) == 0 && SW % 2 == 0 && SW <= MBW, "");
     static_assert(2 * STAGE <= kLdsMax, "");
 };
 
@@ -53,8 +53,10 @@ __device__ __forceinline__ u32x4 resource(const void* p, unsigned bytes) {
                  (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 
+// Until at most N of this wave's loads are in flight.
+template <int N>
 __device__ __forceinline__ void wait_loads() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void barrier() {
@@ -99,26 +101,61 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         for (int i = 0; i < C::WL; ++i) load_to_lds(wr, wo[i], u * 2048, at + C::XB + (wave * C::WL + i) * 1024);
     };
     const int rw = wave / C::CW, cw = wave % C::CW;
+    const int xat = (rw * C::MBW * 16 + j) * 128, wat = C::XB + cw * C::SW * 2048 + lane * 16;
+    auto read_x = [&](const unsigned char* st, int q) {  // step q of a stage: k-tile q / MBW, row block q % MBW
+        // (rows 16 apart have the same swizzle)
+        return *reinterpret_cast<const i32x4*>(st + xat + q % C::MBW * 2048 + ((q / C::MBW * 4 + g) ^ swizzle(j)) * 16);
+    };
+    auto read_w = [&](const unsigned char* st, int t, int s) {
+        return *reinterpret_cast<const i32x4*>(st + wat + s * 2048 + t * 1024);
+    };
+    // A stage is 2 MBW steps of SW products.  Operands are read kAhead steps
+    // before their products; the stage's reads are over kAhead steps before its
+    // end.  There the wave waits for its loads of the next stage and for the
+    // other waves: then the stage's place is free for the loads of the one after
+    // the next, and the next one's operands are read under the last products.
+    constexpr int STEPS = 2 * C::MBW, kAhead = 3;
     i32x4 acc[C::MBW][C::SW] = {};
+    i32x4 x[kAhead + 1], w[2][C::SW];
     issue(0, 0);
+    if (a.Ku > 1) {
+        issue(1, 1);
+        wait_loads<C::XL + C::WL>();
+    } else {
+        wait_loads<0>();
+    }
+    barrier();
+#pragma unroll
+    for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(lds, 0, s);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) x[q] = read_x(lds, q);
     for (int u = 0; u < a.Ku; ++u) {
-        wait_loads();
-        barrier();
-        if (u + 1 < a.Ku) issue(u + 1, (u + 1) & 1);
         const unsigned char* st = lds + (u & 1) * C::STAGE;
-        const unsigned char* xs = st + (rw * C::MBW * 16 + j) * 128;
-        const unsigned char* ws = st + C::XB + cw * C::SW * 2048 + lane * 16;
+        const unsigned char* next = lds + ((u + 1) & 1) * C::STAGE;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            i32x4 w[C::SW];
+        for (int q = 0; q < STEPS; ++q) {
+            const int t = q / C::MBW, i = q % C::MBW;
+            if (q + kAhead < STEPS)
+                x[(q + kAhead) % (kAhead + 1)] = read_x(st, q + kAhead);
+            else
+                x[(q + kAhead) % (kAhead + 1)] = read_x(next, q + kAhead - STEPS);
+            // weights of the second k-tile: during the first; of the next stage's first: at the end
+            if (t == 0 && i < C::SW) w[1][i] = read_w(st, 1, i);
+            if (q == STEPS - kAhead) {
 #pragma unroll
-            for (int s = 0; s < C::SW; ++s) w[s] = *reinterpret_cast<const i32x4*>(ws + s * 2048 + t * 1024);
+                for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(next, 0, s);
+            }
 #pragma unroll
-            for (int i = 0; i < C::MBW; ++i) {
-                // (rows 16 apart have the same swizzle)
-                const i32x4 x = *reinterpret_cast<const i32x4*>(xs + i * 2048 + ((t * 4 + g) ^ swizzle(j)) * 16);
-#pragma unroll
-                for (int s = 0; s < C::SW; ++s) acc[i][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s], x, acc[i][s], 0, 0, 0);
+            for (int s = 0; s < C::SW; ++s)
+                acc[i][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t][s], x[q % (kAhead + 1)], acc[i][s], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (q == STEPS - kAhead - 1) {
+                // (the step's reads were the stage's last)
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                wait_loads<0>();
+                barrier();
+                if (u + 2 < a.Ku) issue(u + 2, u & 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
