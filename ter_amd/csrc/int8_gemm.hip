@@ -1,10 +1,12 @@
 // int8_gemm.hip -- the 8-bit product of many rows: tiles of rows x channels in
 // LDS, v_mfma_i32_16x16x64_i8.
 //
-// A workgroup of 8 waves (RW x CW) computes BM x BN results.  Per unit of 128
-// values of K both operands come to LDS straight from memory (buffer_load ...
-// lds, 1 KiB an instruction, no registers), two stages, the next unit's loads
-// in flight under the products of the one at hand.
+// A workgroup of 8 waves (RW x CW) computes BM x BN results, tile after tile of
+// its share.  Per unit of 128 values of K both operands come to LDS straight
+// from memory (buffer_load ... lds, 1 KiB an instruction, no registers), NST
+// stages, the next units' loads in flight under the products of the one at
+// hand.  The units of a workgroup's tiles are one sequence: the next tile's
+// first ones are loaded under the last products of a tile and its stores.
 //
 // LDS.  Weights keep their tiles (int8.h): an operand is one ds_read_b128 at 16
 // * lane.  A row of x is 128 bytes, its 16-byte chunk c at position c ^ g(row),
@@ -23,15 +25,16 @@ namespace {
 
 #define TER_LDS __attribute__((address_space(3)))
 
-// MBW row blocks of 16 and SW strips of 16 a wave, RW x CW waves.
-template <int MBW_, int SW_, int RW_, int CW_>
+// MBW row blocks of 16 and SW strips of 16 a wave, RW x CW waves, NST stages.
+template <int MBW_, int SW_, int RW_, int CW_, int NST_>
 struct GCfg {
-    static constexpr int MBW = MBW_, SW = SW_, RW = RW_, CW = CW_, WAVES = RW * CW, THREADS = 64 * WAVES;
+    static constexpr int MBW = MBW_, SW = SW_, RW = RW_, CW = CW_, NST = NST_, WAVES = RW * CW, THREADS = 64 * WAVES;
     static constexpr int BM = 16 * MBW * RW, BN = 16 * SW * CW;
-    static constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB;
-    static constexpr int XL = XB / 1024 / WAVES, WL = WB / 1024 / WAVES;  // loads of a wave and stage
-    static_assert(XB % (1024 * WAVES) == 0 && WB % (1024 * WAVES) == 0 && SW % 2 == 0 && SW <= MBW, "");
-    static_assert(2 * STAGE <= kLdsMax, "");
+    static constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB, LDS = NST * STAGE;
+    // loads of a wave and stage: X runs (the first XR waves one more), W runs
+    static constexpr int XL = XB / 1024 / WAVES, XR = XB / 1024 % WAVES, WL = WB / 1024 / WAVES;
+    static_assert(WB % (1024 * WAVES) == 0 && SW % 2 == 0 && SW <= MBW * 2, "");
+    static_assert(LDS <= kLdsMax && NST >= 2 && (NST - 2) * (XL + 1 + WL) < 64, "");
 };
 
 // 16 bytes a lane from memory to LDS at lds + 16 * lane.  Inline asm without
@@ -67,25 +70,34 @@ __device__ __forceinline__ void barrier() {
 
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ (row >> 3 & 1); }
 
+// Until the loads of the units behind the next one are all that is in flight.
+template <class C, int BEHIND>
+__device__ __forceinline__ void wait_unit(int behind, bool more) {
+    if constexpr (BEHIND == 0) {
+        wait_loads<0>();
+    } else if (behind >= BEHIND) {
+        if (C::XR != 0 && more)
+            wait_loads<BEHIND*(C::XL + 1 + C::WL)>();
+        else
+            wait_loads<BEHIND*(C::XL + C::WL)>();
+    } else {
+        wait_unit<C, BEHIND - 1>(behind, more);
+    }
+}
+
 template <class C, int YT>
 __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int mt, int nt) {
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
-    int tm, tn;
-    tile_of(blockIdx.x, mt, nt, tm, tn);
-    const int m0 = tm * C::BM, s0 = tn * (C::BN / 16);
-    const int rows = a.M - m0 < C::BM ? a.M - m0 : C::BM;
-    const int strips = 2 * i8_pairs(a.N) - s0;
-    const u32x4 xr = resource(a.x + (long long)m0 * a.ldx, (unsigned)((rows - 1) * (int)a.ldx + a.Kx));
-    const u32x4 wr = resource(a.w + (long long)s0 * a.Ku * 2048,
-                              (unsigned)((strips < C::BN / 16 ? strips : C::BN / 16) * a.Ku * 2048));
+    const bool more = wave < C::XR;
     const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((TER_LDS unsigned char*)lds);
     // loads of this wave: X runs of 8 rows, W runs of a tile
-    unsigned xo[C::XL], wo[C::WL];
+    const int run0 = wave * C::XL + (more ? wave : C::XR);
+    unsigned xo[C::XL + 1], wo[C::WL];
 #pragma unroll
-    for (int i = 0; i < C::XL; ++i) {
-        const int row = (wave * C::XL + i) * 8 + (lane >> 3);
+    for (int i = 0; i < C::XL + (C::XR != 0); ++i) {
+        const int row = (run0 + i) * 8 + (lane >> 3);
         xo[i] = (unsigned)(row * (int)a.ldx + ((lane & 7) ^ swizzle(row)) * 16);
     }
 #pragma unroll
@@ -93,12 +105,34 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         const int run = wave * C::WL + i;  // strip run / 2, k-tile run % 2
         wo[i] = (unsigned)((run >> 1) * a.Ku * 2048 + (run & 1) * 1024 + lane * 16);
     }
-    auto issue = [&](int u, int buf) {
-        const unsigned at = base + buf * C::STAGE;
+    // what is loaded: unit iu of tile it
+    int it = blockIdx.x, iu = 0, place = 0;
+    u32x4 xr, wr;
+    auto aim = [&] {
+        int tm, tn;
+        tile_of(it, mt, nt, tm, tn);
+        const int m0 = tm * C::BM, s0 = tn * (C::BN / 16);
+        const int rows = a.M - m0 < C::BM ? a.M - m0 : C::BM;
+        const int strips = 2 * i8_pairs(a.N) - s0;
+        xr = resource(a.x + (long long)m0 * a.ldx, (unsigned)((rows - 1) * (int)a.ldx + a.Kx));
+        wr = resource(a.w + (long long)s0 * a.Ku * 2048,
+                      (unsigned)((strips < C::BN / 16 ? strips : C::BN / 16) * a.Ku * 2048));
+    };
+    const int tiles = mt * nt;
+    auto issue = [&] {  // the next unit, to its place
+        if (it >= tiles) return;
+        const unsigned at = base + place * C::STAGE;
 #pragma unroll
-        for (int i = 0; i < C::XL; ++i) load_to_lds(xr, xo[i], u * 128, at + (wave * C::XL + i) * 1024);
+        for (int i = 0; i < C::XL; ++i) load_to_lds(xr, xo[i], iu * 128, at + (run0 + i) * 1024);
+        if (C::XR != 0 && more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
 #pragma unroll
-        for (int i = 0; i < C::WL; ++i) load_to_lds(wr, wo[i], u * 2048, at + C::XB + (wave * C::WL + i) * 1024);
+        for (int i = 0; i < C::WL; ++i) load_to_lds(wr, wo[i], iu * 2048, at + C::XB + (wave * C::WL + i) * 1024);
+        place = place + 1 == C::NST ? 0 : place + 1;
+        if (++iu == a.Ku) {
+            iu = 0;
+            it += gridDim.x;
+            if (it < tiles) aim();
+        }
     };
     const int rw = wave / C::CW, cw = wave % C::CW;
     const int xat = (rw * C::MBW * 16 + j) * 128, wat = C::XB + cw * C::SW * 2048 + lane * 16;
@@ -111,82 +145,136 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     };
     // A stage is 2 MBW steps of SW products.  Operands are read kAhead steps
     // before their products; the stage's reads are over kAhead steps before its
-    // end.  There the wave waits for its loads of the next stage and for the
-    // other waves: then the stage's place is free for the loads of the one after
-    // the next, and the next one's operands are read under the last products.
-    constexpr int STEPS = 2 * C::MBW, kAhead = 3;
-    i32x4 acc[C::MBW][C::SW] = {};
-    i32x4 x[kAhead + 1], w[2][C::SW];
-    issue(0, 0);
-    if (a.Ku > 1) {
-        issue(1, 1);
-        wait_loads<C::XL + C::WL>();
-    } else {
-        wait_loads<0>();
-    }
+    // end.  There the wave waits for its loads of the next unit and for the
+    // other waves: then the stage's place is free for the loads of a later one,
+    // and the next one's operands are read under the last products.
+    // (kRing operands of x in turn, a divisor of STEPS)
+    constexpr int STEPS = 2 * C::MBW, kRing = C::MBW == 2 ? 2 : C::MBW % 2 ? C::MBW : 4, kAhead = kRing - 1;
+    constexpr int kW = (C::SW + C::MBW - 1) / C::MBW;
+    static_assert(STEPS % kRing == 0 && STEPS - kAhead > C::MBW, "weights of the second k-tile before the stage is free");
+    i32x4 x[kRing], w[2][C::SW];
+    aim();
+#pragma unroll
+    for (int i = 0; i < C::NST; ++i) issue();
+    int left = ((tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * a.Ku;  // units, the one at hand included
+    wait_unit<C, C::NST - 1>(left - 1, more);
     barrier();
+    int cur = 0;
 #pragma unroll
     for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(lds, 0, s);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) x[q] = read_x(lds, q);
-    for (int u = 0; u < a.Ku; ++u) {
-        const unsigned char* st = lds + (u & 1) * C::STAGE;
-        const unsigned char* next = lds + ((u + 1) & 1) * C::STAGE;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        i32x4 acc[C::MBW][C::SW] = {};
+        for (int u = 0; u < a.Ku; ++u) {
+            const unsigned char* st = lds + cur * C::STAGE;
+            cur = cur + 1 == C::NST ? 0 : cur + 1;
+            const unsigned char* next = lds + cur * C::STAGE;
+            --left;
 #pragma unroll
-        for (int q = 0; q < STEPS; ++q) {
-            const int t = q / C::MBW, i = q % C::MBW;
-            if (q + kAhead < STEPS)
-                x[(q + kAhead) % (kAhead + 1)] = read_x(st, q + kAhead);
-            else
-                x[(q + kAhead) % (kAhead + 1)] = read_x(next, q + kAhead - STEPS);
-            // weights of the second k-tile: during the first; of the next stage's first: at the end
-            if (t == 0 && i < C::SW) w[1][i] = read_w(st, 1, i);
-            if (q == STEPS - kAhead) {
+            for (int q = 0; q < STEPS; ++q) {
+                const int t = q / C::MBW, i = q % C::MBW;
+                if (q + kAhead < STEPS)
+                    x[(q + kAhead) % kRing] = read_x(st, q + kAhead);
+                else
+                    x[(q + kAhead) % kRing] = read_x(next, q + kAhead - STEPS);
+                // weights of the second k-tile: during the first; of the next unit's first: at the end
+                if (t == 0) {
 #pragma unroll
-                for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(next, 0, s);
-            }
+                    for (int s = i * kW; s < i * kW + kW && s < C::SW; ++s) w[1][s] = read_w(st, 1, s);
+                }
+                if (q == STEPS - kAhead) {
 #pragma unroll
-            for (int s = 0; s < C::SW; ++s)
-                acc[i][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t][s], x[q % (kAhead + 1)], acc[i][s], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (q == STEPS - kAhead - 1) {
-                // (the step's reads were the stage's last)
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                wait_loads<0>();
-                barrier();
-                if (u + 2 < a.Ku) issue(u + 2, u & 1);
+                    for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(next, 0, s);
+                }
+#pragma unroll
+                for (int s = 0; s < C::SW; ++s)
+                    acc[i][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t][s], x[q % kRing], acc[i][s], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
+                if (q == STEPS - kAhead - 1) {
+                    // (the step's reads were the stage's last)
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    wait_unit<C, C::NST - 2>(left - 1, more);
+                    barrier();
+                    issue();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
+        int tm, tn;
+        tile_of(tile, mt, nt, tm, tn);
+        store_tile<C::MBW, C::SW, YT>(a, tm * C::BM + rw * C::MBW * 16, tn * C::BN + cw * C::SW * 16, acc, lane);
     }
-    store_tile<C::MBW, C::SW, YT>(a, m0 + rw * C::MBW * 16, (s0 + cw * C::SW) * 16, acc, lane);
 }
 
 template <class C, int YT>
-hipError_t launch(const Int8MmArgs& a, hipStream_t st) {
+hipError_t launch(const Int8MmArgs& a, int cus, hipStream_t st) {
     static LdsLimit limit;
-    const hipError_t e = limit.allow(2 * C::STAGE, {reinterpret_cast<const void*>(&int8_gemm_kernel<C, YT>)});
+    const hipError_t e = limit.allow(C::LDS, {reinterpret_cast<const void*>(&int8_gemm_kernel<C, YT>)});
     if (e != hipSuccess) return e;
     const int mt = (a.M + C::BM - 1) / C::BM, nt = (a.N + C::BN - 1) / C::BN;
-    hipLaunchKernelGGL((int8_gemm_kernel<C, YT>), dim3((unsigned)((long long)mt * nt)), dim3(C::THREADS), 2 * C::STAGE, st, a,
-                       mt, nt);
+    const int fit = kLdsMax / C::LDS > 1 ? 2 : 1;
+    const int grid = mt * nt < cus * fit ? mt * nt : cus * fit;
+    hipLaunchKernelGGL((int8_gemm_kernel<C, YT>), dim3(grid), dim3(C::THREADS), C::LDS, st, a, mt, nt);
     return hipGetLastError();
 }
 
 template <class C>
-hipError_t launch_type(const Int8MmArgs& a, hipStream_t st) {
+hipError_t launch_type(const Int8MmArgs& a, int cus, hipStream_t st) {
     switch (a.y_type) {
-        case TER_HIP_T_F16: return launch<C, TER_HIP_T_F16>(a, st);
-        case TER_HIP_T_BF16: return launch<C, TER_HIP_T_BF16>(a, st);
-        case TER_HIP_T_F32: return launch<C, TER_HIP_T_F32>(a, st);
-        default: return launch<C, TER_HIP_T_I32>(a, st);
+        case TER_HIP_T_F16: return launch<C, TER_HIP_T_F16>(a, cus, st);
+        case TER_HIP_T_BF16: return launch<C, TER_HIP_T_BF16>(a, cus, st);
+        case TER_HIP_T_F32: return launch<C, TER_HIP_T_F32>(a, cus, st);
+        default: return launch<C, TER_HIP_T_I32>(a, cus, st);
     }
 }
 
 }  // namespace
 
+// The variants.  A call takes the one whose estimate is the least: rounds of
+// the GPU times (units times `unit` + `tile`), in us, measured on calls that fill
+// it once to many times; `few` is a unit where a CU holds one workgroup of two.
+// 8192 x 8192 x 8192: 1116, 551, 485, 515, 477, 452 and 407 us from the smallest
+// tile to the largest, 128 x 6912 x 2560 (K, N): 20.0, 39, 45, 55, 57, 66, 71.
+namespace {
+struct Variant {
+    int bm, bn, fit;
+    float few, unit, tile;
+};
+constexpr Variant kVariants[] = {
+    {64, 64, 2, 0.33f, 0.55f, 3.f},  {96, 256, 1, 0.78f, 0.78f, 4.f},  {128, 256, 1, 0.95f, 0.95f, 4.5f},
+    {160, 256, 1, 1.15f, 1.15f, 4.5f}, {192, 256, 1, 1.24f, 1.24f, 5.f}, {224, 256, 1, 1.41f, 1.41f, 6.5f},
+    {256, 256, 1, 1.59f, 1.59f, 6.f},
+};
+}  // namespace
+
 hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st) {
-    return launch_type<GCfg<8, 4, 2, 4>>(a, st);
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const int cus = device_cu_count(dev);
+    if (cus <= 0) return hipErrorInvalidDevice;
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < (int)(sizeof(kVariants) / sizeof(kVariants[0])); ++i) {
+        const Variant& v = kVariants[i];
+        const long long tiles = (long long)((a.M + v.bm - 1) / v.bm) * ((a.N + v.bn - 1) / v.bn);
+        const long long rounds = (tiles + (long long)cus * v.fit - 1) / ((long long)cus * v.fit);
+        const float us = (float)rounds * ((float)a.Ku * (tiles <= cus ? v.few : v.unit) + v.tile);
+        if (i == 0 || us < least) {
+            least = us;
+            best = i;
+        }
+    }
+    switch (best) {
+        case 0: return launch_type<GCfg<2, 2, 2, 2, 5>>(a, cus, st);
+        case 1: return launch_type<GCfg<3, 4, 2, 4, 3>>(a, cus, st);
+        case 2: return launch_type<GCfg<4, 4, 4, 2, 3>>(a, cus, st);
+        case 3: return launch_type<GCfg<5, 4, 2, 4, 3>>(a, cus, st);
+        case 4: return launch_type<GCfg<6, 4, 2, 4, 2>>(a, cus, st);
+        case 5: return launch_type<GCfg<7, 4, 2, 4, 2>>(a, cus, st);
+        default: return launch_type<GCfg<8, 4, 2, 4, 2>>(a, cus, st);
+    }
 }
 
 }  // namespace terhip
