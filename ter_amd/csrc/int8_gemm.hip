@@ -25,10 +25,11 @@ namespace {
 
 #define TER_LDS __attribute__((address_space(3)))
 
-// MBW row blocks of 16 and SW strips of 16 a wave, RW x CW waves, NST stages.
-template <int MBW_, int SW_, int RW_, int CW_, int NST_>
+// MBW row blocks of 16 and SW strips of 16 a wave, RW x CW waves, NST stages;
+// a unit's loads are issued over SPREAD steps.
+template <int MBW_, int SW_, int RW_, int CW_, int NST_, int SPREAD_>
 struct GCfg {
-    static constexpr int MBW = MBW_, SW = SW_, RW = RW_, CW = CW_, NST = NST_, WAVES = RW * CW, THREADS = 64 * WAVES;
+    static constexpr int MBW = MBW_, SW = SW_, RW = RW_, CW = CW_, NST = NST_, SPREAD = SPREAD_, WAVES = RW * CW, THREADS = 64 * WAVES;
     static constexpr int BM = 16 * MBW * RW, BN = 16 * SW * CW;
     static constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB, LDS = NST * STAGE;
     // loads of a wave and stage: X runs (the first XR waves one more), W runs
@@ -119,19 +120,23 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
                       (unsigned)((strips < C::BN / 16 ? strips : C::BN / 16) * a.Ku * 2048));
     };
     const int tiles = mt * nt;
-    auto issue = [&] {  // the next unit, to its place
+    constexpr int RUNS = C::XL + (C::XR != 0) + C::WL;
+    auto issue = [&](int i) {  // load i of the next unit, to its place
         if (it >= tiles) return;
         const unsigned at = base + place * C::STAGE;
-#pragma unroll
-        for (int i = 0; i < C::XL; ++i) load_to_lds(xr, xo[i], iu * 128, at + (run0 + i) * 1024);
-        if (C::XR != 0 && more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
-#pragma unroll
-        for (int i = 0; i < C::WL; ++i) load_to_lds(wr, wo[i], iu * 2048, at + C::XB + (wave * C::WL + i) * 1024);
-        place = place + 1 == C::NST ? 0 : place + 1;
-        if (++iu == a.Ku) {
-            iu = 0;
-            it += gridDim.x;
-            if (it < tiles) aim();
+        if (i < C::XL)
+            load_to_lds(xr, xo[i], iu * 128, at + (run0 + i) * 1024);
+        else if (i >= C::XL + C::WL)
+            if (more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
+        if (i >= C::XL && i < C::XL + C::WL)
+            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024);
+        if (i == RUNS - 1) {
+            place = place + 1 == C::NST ? 0 : place + 1;
+            if (++iu == a.Ku) {
+                iu = 0;
+                it += gridDim.x;
+                if (it < tiles) aim();
+            }
         }
     };
     const int rw = wave / C::CW, cw = wave % C::CW;
@@ -155,7 +160,9 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     i32x4 x[kRing], w[2][C::SW];
     aim();
 #pragma unroll
-    for (int i = 0; i < C::NST; ++i) issue();
+    for (int k = 0; k < C::NST; ++k)
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) issue(i);
     int left = ((tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * a.Ku;  // units, the one at hand included
     wait_unit<C, C::NST - 1>(left - 1, more);
     barrier();
@@ -164,6 +171,8 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     for (int s = 0; s < C::SW; ++s) w[0][s] = read_w(lds, 0, s);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) x[q] = read_x(lds, q);
+    constexpr int kSlots = C::SPREAD < STEPS ? C::SPREAD : STEPS - 1;
+    bool loading = false;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         i32x4 acc[C::MBW][C::SW] = {};
         for (int u = 0; u < a.Ku; ++u) {
@@ -196,7 +205,17 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     wait_unit<C, C::NST - 2>(left - 1, more);
                     barrier();
-                    issue();
+                    loading = true;
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    // the loads of a later unit, a few a step: their issue then runs under the products
+                    constexpr int PER = (RUNS + kSlots - 1) / kSlots;
+                    const int slot = (q - (STEPS - kAhead) + STEPS) % STEPS;
+                    if (slot < kSlots && loading) {
+#pragma unroll
+                        for (int i = slot * PER; i < slot * PER + PER && i < RUNS; ++i) issue(i);
+                        if (slot == kSlots - 1) loading = false;
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -234,17 +253,18 @@ hipError_t launch_type(const Int8MmArgs& a, int cus, hipStream_t st) {
 // The variants.  A call takes the one whose estimate is the least: rounds of
 // the GPU times (units times `unit` + `tile`), in us, measured on calls that fill
 // it once to many times; `few` is a unit where a CU holds one workgroup of two.
-// 8192 x 8192 x 8192: 1116, 551, 485, 515, 477, 452 and 407 us from the smallest
-// tile to the largest, 128 x 6912 x 2560 (K, N): 20.0, 39, 45, 55, 57, 66, 71.
+// 8192 x 8192 x 8192: 789, 531, 463, 493, 466, 437 and 407 us from the smallest
+// tile to the largest; 128 rows x 2560 channels, K 6912: 17.8, 36, 42, 51, 55,
+// 58, 67; 1021 x 8192, K 2048: 32.5, 29.7, 22.2, 26, 27.6, 28.8, 31.
 namespace {
 struct Variant {
     int bm, bn, fit;
     float few, unit, tile;
 };
 constexpr Variant kVariants[] = {
-    {64, 64, 2, 0.33f, 0.55f, 3.f},  {96, 256, 1, 0.78f, 0.78f, 4.f},  {128, 256, 1, 0.95f, 0.95f, 4.5f},
-    {160, 256, 1, 1.15f, 1.15f, 4.5f}, {192, 256, 1, 1.24f, 1.24f, 5.f}, {224, 256, 1, 1.41f, 1.41f, 6.5f},
-    {256, 256, 1, 1.59f, 1.59f, 6.f},
+    {64, 64, 2, 0.28f, 0.39f, 3.f},    {96, 256, 1, 0.75f, 0.75f, 4.f},   {128, 256, 1, 0.90f, 0.90f, 4.5f},
+    {160, 256, 1, 1.10f, 1.10f, 5.f},  {192, 256, 1, 1.21f, 1.21f, 6.f},  {224, 256, 1, 1.37f, 1.37f, 7.f},
+    {256, 256, 1, 1.59f, 1.59f, 8.f},
 };
 }  // namespace
 
@@ -267,13 +287,13 @@ hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st) {
         }
     }
     switch (best) {
-        case 0: return launch_type<GCfg<2, 2, 2, 2, 5>>(a, cus, st);
-        case 1: return launch_type<GCfg<3, 4, 2, 4, 3>>(a, cus, st);
-        case 2: return launch_type<GCfg<4, 4, 4, 2, 3>>(a, cus, st);
-        case 3: return launch_type<GCfg<5, 4, 2, 4, 3>>(a, cus, st);
-        case 4: return launch_type<GCfg<6, 4, 2, 4, 2>>(a, cus, st);
-        case 5: return launch_type<GCfg<7, 4, 2, 4, 2>>(a, cus, st);
-        default: return launch_type<GCfg<8, 4, 2, 4, 2>>(a, cus, st);
+        case 0: return launch_type<GCfg<2, 2, 2, 2, 5, 4>>(a, cus, st);
+        case 1: return launch_type<GCfg<3, 4, 2, 4, 3, 8>>(a, cus, st);
+        case 2: return launch_type<GCfg<4, 4, 4, 2, 3, 4>>(a, cus, st);
+        case 3: return launch_type<GCfg<5, 4, 2, 4, 3, 4>>(a, cus, st);
+        case 4: return launch_type<GCfg<6, 4, 2, 4, 2, 4>>(a, cus, st);
+        case 5: return launch_type<GCfg<7, 4, 2, 4, 2, 8>>(a, cus, st);
+        default: return launch_type<GCfg<8, 4, 2, 4, 2, 4>>(a, cus, st);
     }
 }
 

@@ -10,6 +10,40 @@ namespace terhip {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
+template <int C>
+using Words = unsigned int __attribute__((ext_vector_type(C / 2)));
+
+// C (4 or 8) scaled sums in 16 bits.
+template <int YT, int C>
+__device__ __forceinline__ Words<C> words_of(const int (&sum)[C], float xs, const float (&ws)[C]) {
+#pragma clang fp contract(off)
+    Words<C> o;
+#pragma unroll
+    for (int i = 0; i < C; i += 2) {
+        unsigned w = 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float f = (float)sum[i + k] * (xs * ws[i + k]);
+            w |= (unsigned)(YT == TER_HIP_T_F16 ? float_to_half_bits(f) : __builtin_bit_cast(uint16_t, (__bf16)f)) << (16 * k);
+        }
+        o[i / 2] = w;
+    }
+    return o;
+}
+
+// C results of 16 bits from element `at` of y on, `left` of which exist.
+template <int C>
+__device__ __forceinline__ void store_words(char* y, long long at, int left, Words<C> o, bool wide) {
+    TER_GLOBAL uint16_t* p = gptr(reinterpret_cast<uint16_t*>(y)) + at;
+    if (wide && left >= C) {
+        *reinterpret_cast<TER_GLOBAL Words<C>*>(p) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (i < left) p[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
+    }
+}
+
 // Scaled results of C (4 or 8) consecutive channels of one token, `left` of
 // which exist.  wide: groups of 8 are 16-byte aligned in y.
 template <int YT, int C>
@@ -32,24 +66,7 @@ __device__ __forceinline__ void store_run(char* y, long long at, int left, const
                 if (i < left) p[i] = v[i];
         }
     } else {
-        uint16_t v[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const float f = (float)sum[i] * (xs * ws[i]);
-            v[i] = YT == TER_HIP_T_F16 ? float_to_half_bits(f) : __builtin_bit_cast(uint16_t, (__bf16)f);
-        }
-        TER_GLOBAL uint16_t* p = gptr(reinterpret_cast<uint16_t*>(y)) + at;
-        if (wide && left >= C) {
-            typedef unsigned int words __attribute__((ext_vector_type(C / 2)));
-            words o;
-#pragma unroll
-            for (int i = 0; i < C / 2; ++i) o[i] = (unsigned)v[2 * i] | (unsigned)v[2 * i + 1] << 16;
-            *reinterpret_cast<TER_GLOBAL words*>(p) = o;
-        } else {
-#pragma unroll
-            for (int i = 0; i < C; ++i)
-                if (i < left) p[i] = v[i];
-        }
+        store_words<C>(y, at, left, words_of<YT, C>(sum, xs, ws), wide);
     }
 }
 
