@@ -373,12 +373,12 @@ struct LdsBins : LdsScan<NT> {
 
 template <int NT, int LIST>
 struct LdsList : LdsBins<NT> {
-    static constexpr int kCapacity = LIST;
-    u64 list[LIST];
+    unsigned index[LIST];
 };
 
 template <int NT>
 struct Lds : LdsList<NT, kList> {
+    u64 list[kList];
     union {
         u64 second[kSecond];
         Shared<NT> general;
@@ -734,8 +734,8 @@ __device__ __forceinline__ Runs level_of(const Settings& s, int V, bool weighted
 __device__ __forceinline__ u64 entry_of(float x, int i) { return (u64)~key_of(cleaned(x)) << 32 | (unsigned)i; }
 __device__ __forceinline__ float entry_value(u64 l) { return value_of(~(unsigned)(l >> 32)); }
 
-// Lists the elements of runs r among [i0, i1): sh.n of them, those past LIST
-// left out.
+// Lists the elements of runs r among [i0, i1) by their indices: sh.n of them,
+// those past LIST left out.
 template <int TYPE, int NR, int NT, int LIST>
 __device__ __forceinline__ void list_runs(const typename Logit<TYPE>::T* x, int i0, int i1, const Bins& y, const Runs& r,
                                           LdsList<NT, LIST>& sh) {
@@ -758,12 +758,8 @@ __device__ __forceinline__ void list_runs(const typename Logit<TYPE>::T* x, int 
         }
         if (in) {
             int at = atomicAdd(&sh.n, __builtin_popcount(in));
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (in >> e & 1) {
-                    if (at < LIST) sh.list[at] = entry_of(v[e], i + e);
-                    ++at;
-                }
+            for (; in; in &= in - 1, ++at)
+                if (at < LIST) sh.index[at] = (unsigned)(i + __builtin_ctz(in));
         }
     });
 }
@@ -796,13 +792,19 @@ struct Spot {
     unsigned rank, number;  // elements in front of it; equal ones
 };
 
+// The value of lane i, the same for the wave.
+__device__ __forceinline__ u64 lane_of(u64 v, int i) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), i) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, i);
+}
+
 // The places among the spots that a wave's lanes hold (`here`: this lane has
 // one), each kept sum exact: the sum of all kept, and where u lies.
 __device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, u64 weight, bool here, const Runs& r, u64* target) {
     auto pick = [&](bool mine, u64 v) -> u64 {
         const u64 b = __ballot(mine);
         if (!b) return 0;
-        return (u64)__shfl((long long)v, __builtin_ctzll(b));
+        return lane_of(v, __builtin_ctzll(b));
     };
     u64 sum = r.total;
     if (s.k < V) {
@@ -823,33 +825,71 @@ __device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, 
     return kept;
 }
 
-// The k <= kFew elements at the front of the list, one a lane of the first wave.
+// k <= kFew elements, lane i of the first wave with l; b: its bin, whose sums in
+// front are z's.
+__device__ __forceinline__ bool finish_lanes(const SampleArgs& a, int row, const Settings& s, const Weights& w, const Runs& q,
+                                             int k, u64 l, float x, u64 e, int b, Spot z) {
+    const bool here = (int)(threadIdx.x & 63) < k;
+    // (lanes from k on hold the largest entry: behind all.  Eight at a time: one
+    // wave works here, and one by one each waits for the last.)
+    for (int i8 = 0; i8 < k; i8 += 8)
+#pragma unroll
+        for (int i = i8; i < i8 + 8; ++i) {
+            const u64 ol = lane_of(l, i), oe = lane_of(e, i);
+            const bool ahead = __builtin_amdgcn_readlane(b, i) == b && ol < l;
+            z.before += ahead ? oe : 0;
+            z.rank += ahead;
+        }
+    u64 target = 0;
+    const u64 sum = kept_of(s, a.V, z, e, here, q, &target);
+    const bool mine = sum && here && z.before <= target && target - z.before < e;
+    if (mine) {
+        gptr(a.token)[row] = (int32_t)(unsigned)l;
+        if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
+    }
+    return __ballot(mine) != 0;
+}
+
+// The second list, if it has few elements.
 template <int NT, typename B>
 __device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
                            int k, Lds<NT>& sh) {
     if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        const bool here = lane < k;
-        const u64 l = here ? sh.second[lane] : ~0ull;
+        const bool here = (int)threadIdx.x < k;
+        const u64 l = here ? sh.second[threadIdx.x] : ~0ull;
+        const float x = entry_value(l);
+        const int b = here ? bin(x) : -1;
+        const bool found = finish_lanes(a, row, s, w, q, k, l, x, here ? w(x) : 0, b,
+                                        Spot{here ? sh.mass[b] : 0, here ? w(x) : 0, here ? sh.count[b] : 0, 1});
+        if (threadIdx.x == 0) sh.at[7] = found;
+    }
+    __syncthreads();
+    return sh.at[7] != 0;
+}
+
+// The first list, if it has few elements: its runs are the bins.
+template <int NT>
+__device__ __forceinline__ bool finish_short(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w,
+                                             const Runs& r, int n, Lds<NT>& sh) {
+    if (threadIdx.x < 64) {
+        const bool here = (int)threadIdx.x < n;
+        const u64 l = here ? sh.list[threadIdx.x] : ~0ull;
         const float x = entry_value(l);
         const u64 e = here ? w(x) : 0;
-        const int b = here ? bin(x) : -1;
-        Spot z{here ? sh.mass[b] : 0, e, here ? sh.count[b] : 0, 1};
-        for (int i = 0; i < k; ++i) {
-            const u64 ol = (u64)__shfl((long long)l, i), oe = (u64)__shfl((long long)e, i);
-            const bool ahead = __shfl(b, i) == b && ol < l;
-            z.before += ahead ? oe : 0;
-            z.rank += ahead;
+        const int f = (int)y(x);
+        const int b = here ? (f >= r.lo[1]) + (f >= r.lo[2]) : -1;
+        Runs q = r;
+        if (r.total == 0) {
+            q.total = wave_sum(e);
+            q.least_mass = wave_sum(e >= s.least ? e : 0);
         }
-        u64 target = 0;
-        const u64 sum = kept_of(s, a.V, z, e, here, q, &target);
-        const bool mine = sum && here && z.before <= target && target - z.before < e;
-        if (mine) {
-            gptr(a.token)[row] = (int32_t)(unsigned)l;
-            if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
-        }
-        const bool found = __ballot(mine) != 0;
-        if (lane == 0) sh.at[7] = found;
+        Spot z{r.mass[0], e, r.count[0], 1};
+        const u64 m1 = r.mass[1] - z.before, m2 = r.mass[2] - z.before - m1;
+        const unsigned c1 = r.count[1] - z.rank, c2 = r.count[2] - z.rank - c1;
+        z.before += (b >= 1 ? m1 : 0) + (b >= 2 ? m2 : 0);
+        z.rank += (b >= 1 ? c1 : 0) + (b >= 2 ? c2 : 0);
+        const bool found = finish_lanes(a, row, s, w, q, n, l, x, e, b, z);
+        if (threadIdx.x == 0) sh.at[7] = found;
     }
     __syncthreads();
     return sh.at[7] != 0;
@@ -964,6 +1004,7 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
 template <int NT>
 __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const Settings& s, const Bins& y, const Weights& w,
                                            const Runs& r, int n, Lds<NT>& sh) {
+    if (n <= kFew) return finish_short(a, row, s, y, w, r, n, sh);
     // the runs' bins, each cut into 2^shift (no choice between variables: the
     // compiler makes it an array in LDS, addressed by the dispatch packet, which is in host memory: 10 us)
     const int len0 = r.hi[0] - r.lo[0] + 1, len1 = r.lo[1] != kNone ? r.hi[1] - r.lo[1] + 1 : 0;
@@ -1069,7 +1110,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) 
         const Runs r = level_of(s, a.V, mode != kCount, nullptr, kNone, kNone, sh);
         fill_list<TYPE>(x, 0, a.V, y, r, sh);
         const int n = sh.n;
-        if (n <= kList && finish_row(a, row, s, y, w, r, n, sh)) return;
+        if (n <= kList) {
+            for (int i = threadIdx.x; i < n; i += kRowThreads)
+                sh.list[i] = entry_of(Logit<TYPE>::raw(gptr(x)[sh.index[i]]), (int)sh.index[i]);
+            __syncthreads();
+            if (finish_row(a, row, s, y, w, r, n, sh)) return;
+        }
         __syncthreads();
     }
     sample_row<TYPE>(a, row, sh.table, sh.general);
@@ -1148,9 +1194,20 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
     const Extent x = row_extent(a, z);
     const Settings s = settings_of(a, row);
     if (no_sums(x, s) || infinite(x)) return;
-    for (int i = threadIdx.x; i < kBins; i += NT) {
-        sh.mass[i] = gptr(z->mass)[i];
-        sh.count[i] = gptr(z->count)[i];
+    {
+        constexpr int PER = kBins / NT;
+        u64 m[PER];
+        unsigned c[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            m[i] = gptr(z->mass)[threadIdx.x + i * NT];
+            c[i] = gptr(z->count)[threadIdx.x + i * NT];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            sh.mass[threadIdx.x + i * NT] = m[i];
+            sh.count[threadIdx.x + i * NT] = c[i];
+        }
     }
     if (threadIdx.x == 0) sh.least_mass = *gptr(&z->least_mass);
     __syncthreads();
@@ -1171,7 +1228,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
     if (threadIdx.x == 0) sh.at[0] = n ? (int)atomicAdd(&z->n, (unsigned)(n <= kSliceList ? n : kList + 1)) : 0;
     __syncthreads();
     const int at = sh.at[0];
-    for (int i = threadIdx.x; i < n && i < kSliceList && at + i < kList; i += NT) gptr(z->list)[at + i] = sh.list[i];
+    for (int i = threadIdx.x; i < n && i < kSliceList && at + i < kList; i += NT)
+        gptr(z->list)[at + i] = entry_of(Logit<TYPE>::raw(gptr(row_of<TYPE>(a, row))[sh.index[i]]), (int)sh.index[i]);
 }
 
 template <int TYPE>
