@@ -326,8 +326,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int row, const d
 // one wave compares with each other, or many equal ones.
 constexpr int kCountK = 1024; // up to this top_k everything kept is listed, and weights are computed for the list alone
 constexpr int kFew = 64;      // elements compared by one wave
-constexpr int kValues = 8;    // different values among more elements than that
-constexpr int kSecond = 3072; // elements of the second list
+constexpr int kValues = 64;   // different values among more elements than that, by their bins
+constexpr int kOneByOne = 8;  // or one after another
+constexpr int kSecond = 4096; // elements of the second list (a power of two)
 
 struct Bins {
     float mh, cb;  // m / 2; bins for half a logit
@@ -895,55 +896,82 @@ __device__ __forceinline__ bool finish_short(const SampleArgs& a, int row, const
     return sh.at[7] != 0;
 }
 
-// More elements than that, of up to kValues values: the values one after
-// another, then the token among equal ones by its index.
+// The slot of a bin of the runs: those of the first, then of the others.
+__device__ __forceinline__ int slot_of(const Runs& q, int b) {
+    const int n0 = q.hi[0] - q.lo[0] + 1, n1 = q.lo[1] != kNone ? q.hi[1] - q.lo[1] + 1 : 0;
+    int i = b - q.lo[0];
+    i += b >= q.lo[1] ? q.lo[0] + n0 - q.lo[1] : 0;
+    i += b >= q.lo[2] ? q.lo[1] + n1 - q.lo[2] : 0;
+    return i;
+}
+
+// The different values among the k elements of the second list, falling, and
+// their numbers; how many, 0 where they are more than kValues or not found here.
+// Equal logits, as 16 bits have many, stand in a bin by themselves: the bins'
+// values, if the runs have few bins; else the largest value left, one by one.
 template <int NT, typename B>
-__device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
-                            int k, Lds<NT>& sh) {
+__device__ __forceinline__ int values_of(const B& bin, const Runs& q, int k, Lds<NT>& sh) {
     const int lane = threadIdx.x & 63;
-    if (threadIdx.x < kValues) {
-        sh.values[threadIdx.x] = ~0u;  // inverted keys, rising: falling logits
-        sh.numbers[threadIdx.x] = 0;
+    const int last = q.lo[2] != kNone ? q.hi[2] : q.lo[1] != kNone ? q.hi[1] : q.hi[0];
+    const int bins = slot_of(q, last) + 1;
+    if (threadIdx.x < kValues) sh.numbers[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.at[5] = 0;
+    if (bins <= kValues) {
+        for (int i = threadIdx.x; i < k; i += NT)
+            sh.values[slot_of(q, bin(entry_value(sh.second[i])))] = (unsigned)(sh.second[i] >> 32);  // (any one's)
+        __syncthreads();
+        for (int i = threadIdx.x; i < k; i += NT) {
+            const int slot = slot_of(q, bin(entry_value(sh.second[i])));
+            if ((unsigned)(sh.second[i] >> 32) != sh.values[slot]) sh.at[5] = 1;
+            atomicAdd(&sh.numbers[slot], 1u);
+        }
+        __syncthreads();
+        return sh.at[5] ? 0 : bins;
     }
+    if (threadIdx.x < kValues) sh.values[threadIdx.x] = ~0u;
     __syncthreads();
-    unsigned last = 0;  // (0 inverted is a NaN's key)
-    int nv = 0;
-    for (;; ++nv) {
+    unsigned after = 0;  // (inverted keys rise as logits fall; 0 inverted is a NaN's)
+    for (int nv = 0; nv <= kOneByOne; ++nv) {
         unsigned v = ~0u;
         for (int i = threadIdx.x; i < k; i += NT) {
             const unsigned e = (unsigned)(sh.second[i] >> 32);
-            v = e > last && e < v ? e : v;
+            v = e > after && e < v ? e : v;
         }
         for (int d = 1; d < 64; d <<= 1) {
             const unsigned o = (unsigned)__shfl_xor((int)v, d);
             v = o < v ? o : v;
         }
-        if (nv == kValues) {  // one too many?
-            const bool more = __syncthreads_or(v != ~0u);
-            if (more) return false;
-            break;
-        }
-        if (lane == 0) atomicMin(&sh.values[nv], v);
+        if (lane == 0 && v != ~0u) atomicMin(&sh.values[nv], v);
         __syncthreads();
-        last = sh.values[nv];
-        if (last == ~0u) break;
+        after = sh.values[nv];
+        if (after == ~0u) return nv;
         unsigned c = 0;
-        for (int i = threadIdx.x; i - (int)threadIdx.x < k; i += NT)
-            c += __builtin_popcountll(__ballot(i < k && (unsigned)(sh.second[i] >> 32) == last));
+        for (int i = threadIdx.x; i - lane < k; i += NT)
+            c += __builtin_popcountll(__ballot(i < k && (unsigned)(sh.second[i] >> 32) == after));
         if (lane == 0 && c) atomicAdd(&sh.numbers[nv], c);
     }
+    return 0;
+}
+
+// Elements of nv different values: those as spots, then the token among equal
+// ones by its index.
+template <int NT, typename B>
+__device__ __forceinline__ bool finish_values(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w,
+                                              const Runs& q, int k, int nv, Lds<NT>& sh) {
     __syncthreads();
     if (threadIdx.x < 64) {
-        const bool here = lane < nv;
-        const float x = value_of(~(here ? sh.values[lane] : 0x7FFFFFFFu));
-        const unsigned c = here ? sh.numbers[lane] : 0;
+        const int lane = threadIdx.x;
+        const unsigned c = lane < nv ? sh.numbers[lane] : 0;
+        const bool here = c != 0;
+        const unsigned key = here ? sh.values[lane] : 0x7FFFFFFFu;
+        const float x = value_of(~key);
         const u64 e = here ? w(x) : 0;
         const int b = here ? bin(x) : -1;
         Spot z{here ? sh.mass[b] : 0, e * c, here ? sh.count[b] : 0, c};
-        for (int i = 0; i < nv; ++i) {
-            const u64 oe = (u64)__shfl((long long)z.mass, i);
-            const unsigned oc = (unsigned)__shfl((int)c, i);
-            const bool ahead = __shfl(b, i) == b && i < lane;
+        for (int i = 0; i < nv; ++i) {  // (values that share a bin)
+            const u64 oe = lane_of(z.mass, i);
+            const unsigned oc = (unsigned)__builtin_amdgcn_readlane((int)c, i);
+            const bool ahead = __builtin_amdgcn_readlane(b, i) == b && i < lane;
             z.before += ahead ? oe : 0;
             z.rank += ahead ? oc : 0;
         }
@@ -952,7 +980,7 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
         const bool mine = sum && here && z.before <= target && target - z.before < z.mass;
         if (mine) {
             sh.at[5] = (int)ratio(target - z.before, e);
-            sh.at[6] = (int)sh.values[lane];
+            sh.at[6] = (int)key;
             if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(x) / (double)sum);
         }
         const bool found = __ballot(mine) != 0;
@@ -995,6 +1023,96 @@ __device__ __forceinline__ bool finish_many(const SampleArgs& a, int row, const 
         int lower = 0;
         for (int i = 0; i < sh.n; ++i) lower += sh.mass[i] < me;
         if (lower == sh.at[1]) gptr(a.token)[row] = (int32_t)me;
+    }
+    return true;
+}
+
+// Any elements: sorted.
+template <int NT, typename B>
+__device__ __forceinline__ bool finish_sorted(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w,
+                                              const Runs& q, int k, Lds<NT>& sh) {
+    int size = 128;
+    while (size < k) size *= 2;
+    for (int i = k + threadIdx.x; i < size; i += NT) sh.second[i] = ~0ull;
+    __syncthreads();
+    for (int m = 2; m <= size; m *= 2)
+        for (int j = m / 2; j > 0; j /= 2) {
+            for (int i = threadIdx.x; i < size / 2; i += NT) {
+                const int f = (i & -j) * 2 + (i & (j - 1)), g = f + j;
+                const u64 x = sh.second[f], y = sh.second[g];
+                if ((x > y) == ((f & m) == 0)) {
+                    sh.second[f] = y;
+                    sh.second[g] = x;
+                }
+            }
+            __syncthreads();
+        }
+    // Sums in front of each element: those of its bin, and of the bin's elements
+    // before it.  The bin's first takes the list's sum there off the bin's.
+    const int per = (k + NT - 1) / NT, i0 = threadIdx.x * per, i1 = i0 + per < k ? i0 + per : k;
+    u64 sum = 0, all;
+    unsigned none = 0;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) sum += w(entry_value(sh.second[i]));
+    block_scan(sum, none, &all, sh);
+    u64 p = sum;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        const float x = entry_value(sh.second[i]);
+        const int b = bin(x);
+        if (i == 0 || bin(entry_value(sh.second[i - 1])) != b) {
+            sh.mass[b] -= p;
+            sh.count[b] -= (unsigned)i;
+        }
+        p += w(x);
+    }
+    if (threadIdx.x < 8) {
+        sh.at[threadIdx.x] = 0;
+        sh.to[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    // the first element whose running sum is above target: that sum, and the element
+    auto place = [&](u64 target, int slot) {
+        u64 r = sum;
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+            const float x = entry_value(sh.second[i]);
+            const u64 e = w(x), before = sh.mass[bin(x)] + r;
+            if (before <= target && target - before < e) {
+                sh.to[slot] = before + e;
+                sh.at[slot] = i + 1;
+            }
+            r += e;
+        }
+        __syncthreads();
+        return sh.to[slot];
+    };
+    u64 top = q.total;
+    if (s.k < a.V) {
+        u64 r = sum;
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+            const float x = entry_value(sh.second[i]);
+            const int b = bin(x);
+            r += w(x);
+            if (sh.count[b] + (unsigned)i == (unsigned)(s.k - 1)) sh.to[0] = sh.mass[b] + r;
+        }
+        __syncthreads();
+        if (sh.to[0]) top = sh.to[0];
+    }
+    u64 kept = top;
+    if (s.p < 1.f) {
+        const u64 got = place(p_target(s.p, top), 1);
+        if (!got) return false;
+        kept = got < kept ? got : kept;
+    }
+    if (s.least && q.least_mass < kept) kept = q.least_mass;
+    place((u64)(s.u * (double)kept), 2);
+    if (!sh.at[2]) return false;
+    if (threadIdx.x == 0) {
+        const u64 l = sh.second[sh.at[2] - 1];
+        gptr(a.token)[row] = (int32_t)(unsigned)l;
+        if (a.prob) gptr(a.prob)[row] = (float)(w.scaled(entry_value(l)) / (double)kept);
     }
     return true;
 }
@@ -1054,7 +1172,9 @@ __device__ __forceinline__ bool finish_row(const SampleArgs& a, int row, const S
     __syncthreads();
     const int k = sh.n;
     if (k <= kFew) return finish_few(a, row, s, bin, w, q, k, sh);
-    return k <= kSecond && finish_many(a, row, s, bin, w, q, k, sh);
+    if (k > kSecond) return false;
+    const int nv = values_of(bin, q, k, sh);
+    return nv ? finish_values(a, row, s, bin, w, q, k, nv, sh) : finish_sorted(a, row, s, bin, w, q, k, sh);
 }
 
 // 2^44 times 2^(j / 256).
