@@ -253,18 +253,18 @@ hipError_t launch_type(const Int8MmArgs& a, int cus, hipStream_t st) {
 // The variants.  A call takes the one whose estimate is the least: rounds of
 // the GPU times (units times `unit` + `tile`), in us, measured on calls that fill
 // it once to many times; `few` is a unit where a CU holds one workgroup of two.
-// 8192 x 8192 x 8192: 789, 531, 463, 493, 466, 437 and 407 us from the smallest
-// tile to the largest; 128 rows x 2560 channels, K 6912: 17.8, 36, 42, 51, 55,
-// 58, 67; 1021 x 8192, K 2048: 32.5, 29.7, 22.2, 26, 27.6, 28.8, 31.
+// 8192 x 8192 x 8192: 789, 531, 493, 463, 493, 466, 437 and 407 us in the order
+// of the table; 128 rows x 2560 channels, K 6912: 17.8, 36, 46, 42, 51, 55, 58,
+// 67; 1021 x 8192, K 2048: 32.5, 29.7, 23, 22.2, 26, 27.6, 28.8, 31.
 namespace {
 struct Variant {
     int bm, bn, fit;
     float few, unit, tile;
 };
 constexpr Variant kVariants[] = {
-    {64, 64, 2, 0.28f, 0.39f, 3.f},    {96, 256, 1, 0.75f, 0.75f, 4.f},   {128, 256, 1, 0.90f, 0.90f, 4.5f},
-    {160, 256, 1, 1.10f, 1.10f, 5.f},  {192, 256, 1, 1.21f, 1.21f, 6.f},  {224, 256, 1, 1.37f, 1.37f, 7.f},
-    {256, 256, 1, 1.59f, 1.59f, 8.f},
+    {64, 64, 2, 0.28f, 0.39f, 3.f},    {96, 256, 1, 0.75f, 0.75f, 4.f},  {128, 256, 1, 0.93f, 0.93f, 4.5f},
+    {256, 128, 1, 0.90f, 0.90f, 4.5f}, {160, 256, 1, 1.10f, 1.10f, 5.f}, {192, 256, 1, 1.21f, 1.21f, 6.f},
+    {224, 256, 1, 1.37f, 1.37f, 7.f},  {256, 256, 1, 1.59f, 1.59f, 8.f},
 };
 }  // namespace
 
@@ -289,10 +289,11 @@ hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st) {
     switch (best) {
         case 0: return launch_type<GCfg<2, 2, 2, 2, 5, 4>>(a, cus, st);
         case 1: return launch_type<GCfg<3, 4, 2, 4, 3, 8>>(a, cus, st);
-        case 2: return launch_type<GCfg<4, 4, 4, 2, 3, 4>>(a, cus, st);
-        case 3: return launch_type<GCfg<5, 4, 2, 4, 3, 4>>(a, cus, st);
-        case 4: return launch_type<GCfg<6, 4, 2, 4, 2, 4>>(a, cus, st);
-        case 5: return launch_type<GCfg<7, 4, 2, 4, 2, 8>>(a, cus, st);
+        case 2: return launch_type<GCfg<4, 4, 2, 4, 3, 4>>(a, cus, st);
+        case 3: return launch_type<GCfg<4, 4, 4, 2, 3, 4>>(a, cus, st);
+        case 4: return launch_type<GCfg<5, 4, 2, 4, 3, 4>>(a, cus, st);
+        case 5: return launch_type<GCfg<6, 4, 2, 4, 2, 4>>(a, cus, st);
+        case 6: return launch_type<GCfg<7, 4, 2, 4, 2, 8>>(a, cus, st);
         default: return launch_type<GCfg<8, 4, 2, 4, 2, 4>>(a, cus, st);
     }
 }

@@ -4,6 +4,18 @@ one, each rounded as the operator defines it.  So results are compared bit for
 bit, without a tolerance."""
 import torch
 
+# Sizes (rows, channels, K) for which a call on 256 CUs takes each of the tiles.
+TILES = {
+    "64x64": [(822, 282, 22), (1219, 1393, 69), (2000, 1000, 1500)],
+    "96x256": [(3124, 766, 227), (1203, 2773, 654)],
+    "128x256": [(2651, 2973, 36), (1296, 5610, 457)],
+    "256x128": [(2687, 2524, 125), (1882, 3533, 323)],
+    "160x256": [(4199, 2166, 35), (1162, 7279, 81), (1773, 5284, 161)],
+    "192x256": [(4291, 7989, 100), (1529, 7368, 371)],
+    "224x256": [(1602, 8023, 117), (1944, 6223, 314)],
+    "256x256": [(8293, 3748, 51), (4047, 4051, 247)],
+}
+
 
 def quantized(x):
     """(q int8, x_scale) of rows of any type."""

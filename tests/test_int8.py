@@ -5,6 +5,8 @@ import os
 import re
 import shutil
 import subprocess
+import sys
+import textwrap
 
 import pytest
 
@@ -152,3 +154,133 @@ def test_no_rows_and_workspaces():
     assert ws(w, stride=16, n=1 << 14) == 0
     r = rows(stride=16, n=1 << 14)
     assert lib.ter_hip_w8_mm(C.byref(w), C.byref(r), A, 1 << 23, L.T_F16, A, 1 << 30, None) == L.ERR_SHAPE
+
+
+# ---- what a call launches, over the HIP runtime without a device
+
+PRELUDE = """
+import ctypes as C, sys
+fake = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+fake.fake_log.restype = C.c_char_p
+fake.fake_fail.argtypes = [C.c_char_p]
+from ter_amd import _lib as L
+lib = C.CDLL(L.LIB_PATH)
+for name, res, args in L.SIGNATURES + L.INT8_SIGNATURES + L.SAMPLE_SIGNATURES:
+    f = getattr(lib, name)
+    f.restype, f.argtypes = res, args
+A = 1 << 20
+def log():
+    lines = fake.fake_log().decode().splitlines()
+    fake.fake_reset()
+    return lines
+def mm(M, N, K, xt=L.T_I8, yt=L.T_F16, stride=None):
+    w = L.W8()
+    assert lib.ter_hip_w8_init(C.byref(w), A, 1 << 60, K, N) == 0, lib.ter_hip_last_error()
+    x = L.Rows(A, A, stride or K, xt, M)
+    need = lib.ter_hip_w8_mm_ws(C.byref(w), C.byref(x))
+    return lib.ter_hip_w8_mm(C.byref(w), C.byref(x), A, N, yt, A if need else None, need, None)
+def draw(rows, V, ty=L.T_F16):
+    p = L.SampleParams()
+    p.temperature = p.top_p = 1.0
+    need = lib.ter_hip_sample_ws(rows, V)
+    return lib.ter_hip_sample(A, ty, V, rows, V, A, C.byref(p), A, None, A if need else None, need, None)
+def kernels():
+    # (device, blocks, threads, LDS, name) of the launches
+    return [l.split(None, 5)[1:] for l in log() if l.startswith("launch")]
+"""
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not installed")
+    so = str(tmp_path_factory.mktemp("fake") / "libfakehip.so")
+    subprocess.run([gxx, "-std=c++17", "-O1", "-shared", "-fPIC", "-Wall",
+                    os.path.join(ROOT, "tests", "c", "fake_hip.cpp"), "-o", so], check=True)
+
+    def run(body):
+        r = subprocess.run([sys.executable, "-c", PRELUDE + textwrap.dedent(body), so], cwd=ROOT, text=True,
+                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=120)
+        assert r.returncode == 0, r.stdout
+
+    return run
+
+
+def test_launches_of_a_product(fake):
+    fake("""
+    # one launch where rows are read in place or quantized by the product's kernel, else two
+    assert mm(1, 2560, 2560, L.T_F16) == 0
+    (k,) = kernels()
+    assert "int8_stream_kernel" in k[4], k
+    assert mm(4, 2560, 4096, L.T_F32) == 0 and len(kernels()) == 1
+    for M, K in ((5, 128), (4, 4100), (1, 16400)):
+        assert mm(M, 2560, K, L.T_BF16) == 0
+        q, k = kernels()
+        assert "rows8" in q[4] and "int8_stream_kernel" in k[4], (q, k)
+    assert mm(7, 100, 96) == 0 and len(kernels()) == 1
+    assert mm(7, 100, 96, stride=112) == 0 and len(kernels()) == 1
+    assert mm(7, 100, 96, stride=100) == 0
+    q, k = kernels()
+    assert "rows8_copy_kernel" in q[4]
+    assert mm(64, 100, 96) == 0 and "int8_stream_kernel" in kernels()[0][4]
+    assert mm(65, 100, 96) == 0 and "int8_gemm_kernel" in kernels()[0][4]
+    assert mm(0, 100, 96) == 0 and not kernels()
+    """)
+
+
+def test_every_tile_is_some_calls(fake):
+    """Each of the eight tiles is taken by the sizes that test_int8_gpu.py runs
+    for it; grids and LDS fit the GPU."""
+    from tests.int8_ref import TILES
+    fake(f"""
+    seen = set()
+    for tile, sizes in {TILES!r}.items():
+        for M, N, K in sizes:
+            assert mm(M, N, K, L.T_I8, L.T_I32) == 0, lib.ter_hip_last_error()
+            dev, blocks, threads, lds, name = kernels()[-1]
+            cfg = name[name.index("GCfg<") + 5:name.index(">")].split(", ")
+            mbw, sw, rw, cw = map(int, cfg[:4])
+            assert f"{{16 * mbw * rw}}x{{16 * sw * cw}}" == tile, (tile, M, N, K, name)
+            tiles = -(-M // (16 * mbw * rw)) * -(-N // (16 * sw * cw))
+            assert int(blocks) == min(tiles, 512 if tile == "64x64" else 256) * int(threads) or \\
+                int(blocks) == min(tiles, 512 if tile == "64x64" else 256), (blocks, tiles)
+            assert int(threads) == 64 * rw * cw and int(lds) <= 160 * 1024
+        seen.add(tile)
+    assert len(seen) == 8
+    """)
+
+
+def test_a_failed_launch_is_an_error(fake):
+    fake("""
+    for part, call in ((b"int8_stream", lambda: mm(3, 100, 96)), (b"int8_gemm", lambda: mm(300, 100, 96)),
+                       (b"rows8_quant", lambda: mm(30, 100, 96, L.T_F16)), (b"rows8_copy", lambda: mm(30, 100, 95))):
+        fake.fake_fail(part)
+        assert call() == L.ERR_HIP, part
+        assert lib.ter_hip_last_error()
+        fake.fake_fail(b"")
+        assert call() == 0
+    for part in (b"sample_max", b"sample_bins", b"sample_list", b"sample_finish"):
+        fake.fake_fail(part)
+        assert draw(2, 50000) == L.ERR_HIP
+        fake.fake_fail(b"")
+    fake.fake_fail(b"sample_rows")
+    assert draw(400, 50000) == L.ERR_HIP
+    """)
+
+
+def test_launches_of_a_draw(fake):
+    fake("""
+    # a row by slices where rows are few, by one workgroup where they are many or short
+    for rows, V, slices in ((1, 128256, 32), (1, 1 << 19, 64), (64, 128256, 8), (256, 128256, 2), (257, 128256, 1),
+                            (1, 4096, 1), (1, 4097, 2), (100000, 1000, 1)):
+        assert draw(rows, V) == 0, lib.ter_hip_last_error()
+        k = kernels()
+        need = lib.ter_hip_sample_ws(rows, V)
+        if slices == 1:
+            assert len(k) == 1 and "sample_rows_kernel" in k[0][4] and int(k[0][1]) == rows and need == 0, k
+        else:
+            assert [x[4].split("sample_")[1].split("_")[0] for x in k] == ["max", "bins", "list", "finish"], k
+            assert [int(x[1]) for x in k] == [rows * slices] * 3 + [rows], k
+            assert need % rows == 0 and need > 0
+    """)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ter_amd as T
-from tests.int8_ref import product, quantized, same
+from tests.int8_ref import TILES, product, quantized, same
 
 pytestmark = pytest.mark.gpu
 
@@ -71,6 +71,26 @@ def test_larger(cuda, m, n, k):
     want = want.to(torch.int32).float() * (xs[:, None] * ws)
     for dt in FLOATS:
         same(T.mm_int8(W, x, xs, dtype=dt), want.to(dt))
+
+
+@pytest.mark.parametrize("m,n,k", [s for sizes in TILES.values() for s in sizes])
+def test_every_tile(cuda, m, n, k):
+    """Sizes that do not fill the last tiles, in several rounds of the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    w = torch.randint(-128, 128, (n, k), generator=g, device="cuda", dtype=torch.int16).to(torch.int8)
+    wide = torch.randint(-128, 128, (m, k + 16), generator=g, device="cuda", dtype=torch.int16).to(torch.int8)
+    x = wide[:, :k]
+    xs, ws = (torch.rand(i, generator=g, device="cuda") * 0.01 + 1e-5 for i in (m, n))
+    W = T.PackedInt8.from_int8(w, ws)
+    want = (x.double() @ w.double().t().contiguous()).to(torch.int32)
+    y = torch.full((m + 1, n + 8), -7, dtype=torch.int32, device="cuda")
+    T.mm_int8(W, x, out=y[:m, :n])
+    assert torch.equal(y[:m, :n], want)
+    assert (y[m:] == -7).all() and (y[:, n:] == -7).all()
+    y = torch.full((m + 1, n + 8), -7, dtype=torch.bfloat16, device="cuda")
+    T.mm_int8(W, x, xs, out=y[:m, :n])
+    assert torch.equal(y[:m, :n], (want.float() * (xs[:, None] * ws)).bfloat16())
+    assert (y[m:] == -7).all() and (y[:, n:] == -7).all()
 
 
 def test_the_largest_sums(cuda):

@@ -188,6 +188,38 @@ def test_far_apart_and_close_logits(cuda):
         check(x, u, **kw)
 
 
+@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("spread,v", [(1e-4, 3000), (1e-4, 20000), (3e-3, 20000), (0.0, 20000), (1e-5, 70000)])
+def test_a_cluster_far_below_the_largest(cuda, spread, v, m):
+    """One logit far above, all others within a bin or a part of one: of different
+    values, more than lists hold, and of equal ones."""
+    g = torch.Generator().manual_seed(v)
+    x = -12.0 + torch.randn(m, v, generator=g) * spread
+    x[:, 77] = 0.0
+    u = spread_u(m)
+    for kw in (dict(), dict(top_k=v // 2), dict(top_p=0.9), dict(top_k=900, top_p=0.95), dict(temperature=2.0, min_p=1e-3)):
+        if m > 2:
+            check(x[::60], u[::60], **kw)
+            whole = T.sample(x.cuda(), u.cuda(), **kw)
+            assert torch.equal(whole[::60], T.sample(x[::60].cuda(), u[::60].cuda(), **kw))
+        else:
+            check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("v", [4095, 4096, 4097, 8191, 12289, 20001])
+def test_vocabularies_around_a_slice(cuda, v, dt):
+    """The largest logit, the cuts and the token at the ends of slices."""
+    x, u = rows(v, 7, v, dt)
+    for r, i in enumerate((0, v - 1, v // 2, v // 2 - 1, (v + 1) // 2, 4095 % v, 4096 % v)):
+        x[r, i] = 9.0
+    check(x, u)
+    check(x, u, top_k=1)
+    check(x, u, top_k=1024)
+    check(x, u, top_k=1025, top_p=0.99)
+    check(x, torch.full((7,), 0.9999), top_p=0.9)
+
+
 @pytest.mark.parametrize("dt", FLOATS)
 @pytest.mark.parametrize("pad,off", [(1, 0), (5, 3), (8, 8), (13, 1)])
 def test_rows_of_wider_ones(cuda, dt, pad, off):
