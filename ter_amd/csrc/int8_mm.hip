@@ -187,16 +187,22 @@ hipError_t launch(const Int8MmArgs& a, hipStream_t st) {
 }
 
 // Strips of a workgroup and waves that split K: enough waves for the GPU where
-// there are few channels, few joins where there are many.
+// there are few channels, few joins where there are many.  Measured (us; a
+// call's host time is 7.3): 16 x 6912 x 2560 rows, K, channels 7.5 with 8 or 16
+// waves; 32 x 2560 x 6912 8.4 with one strip and 8 waves, 7.3 with two and 4;
+// 64 x 2048 x 8192 10.4 and 7.2; 48 x 6912 x 2560 13.8 and 14.8; 16 x 2048 x
+// 128256 41.5 and 38.8.
 template <int MB, int XT>
 hipError_t launch_rows(const Int8MmArgs& a, hipStream_t st) {
-    constexpr int D = MB == 4 ? 3 : 4;
     const int strips = 2 * i8_pairs(a.N);
-    if constexpr (MB < 4) {
-        if (strips <= 256) return launch<MB, 1, 16, MB == 2 ? 3 : 4, XT>(a, st);
+    if constexpr (MB == 1) {
+        if (strips <= 256) return launch<1, 1, 16, 4, XT>(a, st);
+        if (strips <= 1024) return launch<1, 1, 8, 4, XT>(a, st);
+        return launch<1, 2, 4, 4, XT>(a, st);
+    } else {
+        if (strips <= 256) return launch<MB, 1, 8, 2, XT>(a, st);
+        return launch<MB, 2, 4, 2, XT>(a, st);
     }
-    if (strips <= 1024) return launch<MB, 1, 8, D, XT>(a, st);
-    return launch<MB, 2, 4, MB == 4 ? 2 : D, XT>(a, st);
 }
 
 }  // namespace
@@ -205,8 +211,11 @@ hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st) {
     if (a.x_type == TER_HIP_T_F16) return launch_rows<1, TER_HIP_T_F16>(a, st);
     if (a.x_type == TER_HIP_T_BF16) return launch_rows<1, TER_HIP_T_BF16>(a, st);
     if (a.x_type == TER_HIP_T_F32) return launch_rows<1, TER_HIP_T_F32>(a, st);
-    if (a.M > 64) return launch_int8_gemm(a, st);
     if (a.M <= 16) return launch_rows<1, TER_HIP_T_I8>(a, st);
+    // From 17 rows on and many channels the rows' reads by every workgroup weigh
+    // more than the tiles' way over LDS: 32 x 2560 x 128256 78.6 us here, 62.1 in
+    // tiles; 64 rows 111 and 70.  At 64 x 2048 x 8192 7.2 and 7.9.
+    if (a.M > 64 || i8_pairs(a.N) > 300) return launch_int8_gemm(a, st);
     if (a.M <= 32) return launch_rows<2, TER_HIP_T_I8>(a, st);
     return launch_rows<4, TER_HIP_T_I8>(a, st);
 }

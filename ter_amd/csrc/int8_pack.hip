@@ -146,19 +146,24 @@ __global__ __launch_bounds__(256) void w8_quantize_kernel(const void* __restrict
 __global__ __launch_bounds__(256) void w8_pack_kernel(const int8_t* __restrict__ q, long long stride,
                                                       const float* __restrict__ src_scale, int K, int N, int Ku,
                                                       uint8_t* __restrict__ tiles, float* __restrict__ scale,
-                                                      long long total) {
+                                                      bool vec, long long total) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256ll * gridDim.x) {
         const int n = (int)(i / (8 * Ku)), c = (int)(i % (8 * Ku));
         if (c == 0) gptr(scale)[n] = n < N ? gptr(src_scale)[n] : 0.f;
         const int8_t* row = q + (long long)n * stride;
-        u32x4 v;
-        for (int j = 0; j < 4; ++j) {
-            unsigned d = 0;
-            for (int b = 0; b < 4; ++b) {
-                const int k = c * 16 + 4 * j + b;
-                if (n < N && k < K) d |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+        u32x4 v = {};
+        if (n >= N || c * 16 >= K) {
+        } else if (vec && c * 16 + 16 <= K) {
+            v = *reinterpret_cast<const TER_GLOBAL u32x4*>(gptr(row) + c * 16);
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                unsigned d = 0;
+                for (int b = 0; b < 4; ++b) {
+                    const int k = c * 16 + 4 * j + b;
+                    if (k < K) d |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+                }
+                v[j] = d;
             }
-            v[j] = d;
         }
         *reinterpret_cast<TER_GLOBAL u32x4*>(gptr(tiles) + chunk_at(n, c, Ku)) = v;
     }
@@ -210,7 +215,7 @@ hipError_t launch_w8_pack(const int8_t* q, long long stride, const float* scale,
     const int Ku = i8_units(K);
     const long long n = (long long)i8_pairs(N) * 32 * 8 * Ku;
     hipLaunchKernelGGL(w8_pack_kernel, dim3(grid_of(n)), dim3(256), 0, st, q, stride, scale, K, N, Ku, tiles, out_scale,
-                       n);
+                       reinterpret_cast<uintptr_t>(q) % 16 == 0 && stride % 16 == 0, n);
     return hipGetLastError();
 }
 
