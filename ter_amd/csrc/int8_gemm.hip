@@ -43,11 +43,18 @@ struct GCfg {
 // loads of the next stage; the waits are explicit instead.  (Also for the
 // scalar registers, which a buffer load reads five wait states or more after a
 // lane read wrote them.)
-__device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned soff, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :
-                 : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory", "m0");
+// once: read by nobody else, so not kept in the caches.
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned soff, unsigned lds, bool once = false) {
+    if (once)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                     :
+                     : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :
+                     : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+                     : "memory", "m0");
 }
 
 __device__ __forceinline__ u32x4 resource(const void* p, unsigned bytes) {
@@ -106,7 +113,9 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         const int run = wave * C::WL + i;  // strip run / 2, k-tile run % 2
         wo[i] = (unsigned)((run >> 1) * a.Ku * 2048 + (run & 1) * 1024 + lane * 16);
     }
-    // what is loaded: unit iu of tile it
+    // what is loaded: unit iu of tile it.  Weights that one tile needs pass the
+    // caches by: 96 x 2560 x 128256 75.1 -> 66.3 us (8192 x 2560 x 6912, where
+    // they are needed again, 134 -> 161).
     int it = blockIdx.x, iu = 0, place = 0;
     u32x4 xr, wr;
     auto aim = [&] {
@@ -129,7 +138,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         else if (i >= C::XL + C::WL)
             if (more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
         if (i >= C::XL && i < C::XL + C::WL)
-            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024);
+            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, mt == 1);
         if (i == RUNS - 1) {
             place = place + 1 == C::NST ? 0 : place + 1;
             if (++iu == a.Ku) {
