@@ -27,6 +27,12 @@ __host__ __device__ inline int i8_units(int K) { return (K + kI8Unit - 1) / kI8U
 __host__ __device__ inline int i8_pairs(int N) { return (N + 31) / 32; }  // of strips
 inline size_t i8_tile_bytes(int K, int N) { return (size_t)i8_pairs(N) * i8_units(K) * 4096; }
 
+// Weights that are read by one workgroup each pass the caches by where they are
+// a good part of the memory-side cache or more (128 MiB of 256): by the next call
+// they would be gone.  Smaller ones may still be there (16 x 8192 x 8192 12.5
+// against 13.5 us, called again and again).
+inline bool i8_past_caches(int N, int Ku) { return (long long)N * Ku * kI8Unit >= 1ll << 27; }
+
 struct Int8MmArgs {
     const uint8_t* w;     // tiles
     const float* ws;      // [32 pairs] (zero behind N)

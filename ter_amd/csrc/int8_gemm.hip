@@ -94,7 +94,7 @@ __device__ __forceinline__ void wait_unit(int behind, bool more) {
 }
 
 template <class C, int YT>
-__global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int mt, int nt) {
+__global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int mt, int nt, bool once) {
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
@@ -113,8 +113,8 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         const int run = wave * C::WL + i;  // strip run / 2, k-tile run % 2
         wo[i] = (unsigned)((run >> 1) * a.Ku * 2048 + (run & 1) * 1024 + lane * 16);
     }
-    // what is loaded: unit iu of tile it.  Weights that one tile needs pass the
-    // caches by: 96 x 2560 x 128256 75.1 -> 66.3 us (8192 x 2560 x 6912, where
+    // what is loaded: unit iu of tile it.  Large weights that one tile needs pass
+    // the caches by: 96 x 2560 x 128256 75.1 -> 66.3 us (8192 x 2560 x 6912, where
     // they are needed again, 134 -> 161).
     int it = blockIdx.x, iu = 0, place = 0;
     u32x4 xr, wr;
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         else if (i >= C::XL + C::WL)
             if (more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
         if (i >= C::XL && i < C::XL + C::WL)
-            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, mt == 1);
+            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, once);
         if (i == RUNS - 1) {
             place = place + 1 == C::NST ? 0 : place + 1;
             if (++iu == a.Ku) {
@@ -243,7 +243,8 @@ hipError_t launch(const Int8MmArgs& a, int cus, hipStream_t st) {
     const int mt = (a.M + C::BM - 1) / C::BM, nt = (a.N + C::BN - 1) / C::BN;
     const int fit = kLdsMax / C::LDS > 1 ? 2 : 1;
     const int grid = mt * nt < cus * fit ? mt * nt : cus * fit;
-    hipLaunchKernelGGL((int8_gemm_kernel<C, YT>), dim3(grid), dim3(C::THREADS), C::LDS, st, a, mt, nt);
+    hipLaunchKernelGGL((int8_gemm_kernel<C, YT>), dim3(grid), dim3(C::THREADS), C::LDS, st, a, mt, nt,
+                       mt == 1 && i8_past_caches(a.N, a.Ku));
     return hipGetLastError();
 }
 

@@ -35,6 +35,8 @@ SIZES = [
     (33, 100, 640), (64, 128, 256), (65, 129, 272), (127, 255, 512), (128, 256, 1024), (129, 257, 1040), (5, 2560, 2560),
     (1, 640, 2560), (7, 512, 2048), (257, 515, 387), (300, 1000, 2048), (1, 4099, 6912), (513, 769, 144), (1000, 31, 80),
     (1, 3, 20000), (19, 70, 9000),
+    # few rows by so many channels that tiles take them
+    (17, 9601, 128), (33, 10007, 200), (64, 9700, 130),
 ]
 
 
@@ -59,7 +61,9 @@ def test_rows_quantized_within_the_call(cuda, m, n, k, dt):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (8, 2560, 2560), (40, 6912, 2560), (200, 2048, 8192), (700, 2560, 640),
-                                   (2050, 1030, 1031), (4096, 512, 2048)])
+                                   (2050, 1030, 1031), (4096, 512, 2048),
+                                   # weights of 128 MiB and more pass the caches by
+                                   (1, 131103, 1024), (9, 131103, 1024), (30, 131103, 1024), (100, 131103, 1024)])
 def test_larger(cuda, m, n, k):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
     w = torch.randint(-128, 128, (n, k), generator=g, device="cuda", dtype=torch.int16).to(torch.int8)
