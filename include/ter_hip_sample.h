@@ -23,7 +23,8 @@
  * is below 2^-45 of the largest is never drawn.
  *
  *   - temperature 0 (or, read on the device, not above 0) takes the largest
- *     logit, whatever top_k, top_p, min_p and u;
+ *     logit, whatever top_k, top_p, min_p and u; one above 0 and below 2^-120
+ *     counts as 2^-120;
  *   - top_k 0 (or below, or V and more) keeps all; so do top_p 1 (and, on the
  *     device, more or NaN) and min_p 0 (below or NaN; above 1 counts as 1);
  *   - u is in [0, 1); on the device others count as the nearest in it, NaN as 0;

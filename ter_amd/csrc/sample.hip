@@ -98,7 +98,8 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
     const float q = a.p.min_p_dev ? gptr(a.p.min_p_dev)[row] : a.p.min_p;
     const float u = gptr(a.u)[row];
     Settings s;
-    s.T = t > 0.f ? (double)t : 0.0;
+    // (not below 2^-120: the bins of one below 2^-121 are past binary32)
+    s.T = t > 0.f ? (double)__builtin_fmaxf(t, 0x1p-120f) : 0.0;
     s.k = k > 0 && k < a.V ? k : a.V;
     s.p = p < 1.f ? p : 1.f;  // (NaN: 1)
     s.least = q > 0.f ? (u64)__builtin_ceil((double)__builtin_fminf(q, 1.f) * kOne) : 0;

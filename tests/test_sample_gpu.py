@@ -189,6 +189,24 @@ def test_far_apart_and_close_logits(cuda):
 
 
 @pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("t", [1e-37, 1e-38, 1e-40, 2.0 ** -149])
+def test_temperatures_near_zero(cuda, t, m):
+    """Those below 2^-120 count as it: logits within a few times that of each
+    other, up to thousands of times the temperature given, and ordinary ones."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(m, 4500, generator=g) * 1e-36
+    x[1::2] *= 1e3
+    x[1::4] *= 1e33
+    x[0, :50] -= 1e-35
+    temps = torch.full((m,), t)
+    for kw in (dict(), dict(top_k=700, top_p=0.9), dict(top_k=2000, min_p=1e-4)):
+        want = check(x, u := torch.rand(m, generator=g), temperature=2.0 ** -120, **kw)
+        for temperature in (t, temps.cuda()):
+            got = T.sample(x.cuda(), u.cuda(), temperature=temperature, **kw)
+            assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("m", [2, 300])
 @pytest.mark.parametrize("spread,v", [(1e-4, 3000), (1e-4, 20000), (3e-3, 20000), (0.0, 20000), (1e-5, 70000)])
 def test_a_cluster_far_below_the_largest(cuda, spread, v, m):
     """One logit far above, all others within a bin or a part of one: of different
