@@ -182,30 +182,37 @@ __global__ __launch_bounds__(256) void w8_unpack_kernel(const uint8_t* __restric
 
 inline unsigned grid_of(long long n) { return (unsigned)(n < (1ll << 30) ? (n + 255) / 256 : 1 << 22); }
 
+// (a launch has fewer than 2^32 threads)
 template <int TYPE, int T, int NC>
-void launch_rows_as(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
-                    hipStream_t st) {
-    constexpr int EL = (int)sizeof(typename Elem<TYPE>::T);
-    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (stride * EL % 16 == 0 || M == 1);
-    if (vec)
-        hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, true>), dim3(M), dim3(T), 0, st, x, stride, K, q, ldq, scale);
-    else
-        hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, false>), dim3(M), dim3(T), 0, st, x, stride, K, q, ldq, scale);
+hipError_t launch_rows_as(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                          hipStream_t st) {
+    typedef typename Elem<TYPE>::T E;
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (stride * (int)sizeof(E) % 16 == 0 || M == 1);
+    constexpr int kRows = 1 << 21;
+    for (int m = 0; m < M; m += kRows) {
+        const dim3 grid(M - m < kRows ? M - m : kRows);
+        const E* rows = static_cast<const E*>(x) + m * stride;
+        if (vec)
+            hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, true>), grid, dim3(T), 0, st, rows, stride, K, q + m * ldq,
+                               ldq, scale + m);
+        else
+            hipLaunchKernelGGL((rows8_quant_kernel<TYPE, T, NC, false>), grid, dim3(T), 0, st, rows, stride, K, q + m * ldq,
+                               ldq, scale + m);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <int TYPE>
-void launch_rows_quant(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
-                       hipStream_t st) {
-    if (ldq <= 2048)
-        launch_rows_as<TYPE, 256, 1>(x, stride, M, K, q, ldq, scale, st);
-    else if (ldq <= 4096)
-        launch_rows_as<TYPE, 512, 1>(x, stride, M, K, q, ldq, scale, st);
-    else if (ldq <= 8192)
-        launch_rows_as<TYPE, 1024, 1>(x, stride, M, K, q, ldq, scale, st);
-    else if (ldq <= 16384)
-        launch_rows_as<TYPE, 1024, 2>(x, stride, M, K, q, ldq, scale, st);
-    else
-        hipLaunchKernelGGL(rows8_long_kernel<TYPE>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+hipError_t launch_rows_quant(const void* x, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
+                             hipStream_t st) {
+    if (ldq <= 2048) return launch_rows_as<TYPE, 256, 1>(x, stride, M, K, q, ldq, scale, st);
+    if (ldq <= 4096) return launch_rows_as<TYPE, 512, 1>(x, stride, M, K, q, ldq, scale, st);
+    if (ldq <= 8192) return launch_rows_as<TYPE, 1024, 1>(x, stride, M, K, q, ldq, scale, st);
+    if (ldq <= 16384) return launch_rows_as<TYPE, 1024, 2>(x, stride, M, K, q, ldq, scale, st);
+    hipLaunchKernelGGL(rows8_long_kernel<TYPE>, dim3(M), dim3(256), 0, st, x, stride, K, q, ldq, scale);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -245,18 +252,13 @@ hipError_t launch_w8_unpack(const uint8_t* tiles, const float* scale, int8_t* q,
 
 hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
                         hipStream_t st) {
-    if (type == TER_HIP_T_I8) {
-        const int chunks = (int)(ldq / 16);
-        const long long n = (long long)M * chunks;
-        hipLaunchKernelGGL(rows8_copy_kernel, dim3(grid_of(n)), dim3(256), 0, st, static_cast<const int8_t*>(x), stride,
-                           K, q, ldq, chunks, n);
-    } else if (type == TER_HIP_T_F16) {
-        launch_rows_quant<TER_HIP_T_F16>(x, stride, M, K, q, ldq, scale, st);
-    } else if (type == TER_HIP_T_BF16) {
-        launch_rows_quant<TER_HIP_T_BF16>(x, stride, M, K, q, ldq, scale, st);
-    } else {
-        launch_rows_quant<TER_HIP_T_F32>(x, stride, M, K, q, ldq, scale, st);
-    }
+    if (type == TER_HIP_T_F16) return launch_rows_quant<TER_HIP_T_F16>(x, stride, M, K, q, ldq, scale, st);
+    if (type == TER_HIP_T_BF16) return launch_rows_quant<TER_HIP_T_BF16>(x, stride, M, K, q, ldq, scale, st);
+    if (type == TER_HIP_T_F32) return launch_rows_quant<TER_HIP_T_F32>(x, stride, M, K, q, ldq, scale, st);
+    const int chunks = (int)(ldq / 16);
+    const long long n = (long long)M * chunks;
+    hipLaunchKernelGGL(rows8_copy_kernel, dim3(grid_of(n)), dim3(256), 0, st, static_cast<const int8_t*>(x), stride, K, q,
+                       ldq, chunks, n);
     return hipGetLastError();
 }
 

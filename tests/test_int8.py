@@ -251,6 +251,18 @@ def test_every_tile_is_some_calls(fake):
     """)
 
 
+def test_rows_of_many_launches(fake):
+    """Rows quantized: no launch of 2^32 threads or more."""
+    fake("""
+    for M, K, launches in ((1 << 21, 8000, 1), ((1 << 21) + 1, 5000, 2), (1 << 23, 16384, 4), (1 << 23, 600, 4),
+                           (1 << 23, 16385, 1)):
+        assert mm(M, 64, K, L.T_BF16) == 0, lib.ter_hip_last_error()
+        k = [x for x in kernels() if "rows8" in x[4]]
+        assert len(k) == launches and sum(int(x[1]) for x in k) == M, k
+        assert all(int(x[1]) * int(x[2]) < 1 << 32 for x in k), k
+    """)
+
+
 def test_a_failed_launch_is_an_error(fake):
     fake("""
     for part, call in ((b"int8_stream", lambda: mm(3, 100, 96)), (b"int8_gemm", lambda: mm(300, 100, 96)),
