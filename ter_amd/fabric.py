@@ -794,7 +794,7 @@ def _launch_on(device: int, name: str, stream, *args):
         L.check(rc, name)
 
 
-def _empty_on(device: int, stream, shape, dtype):
+def _empty_on(device, stream, shape, dtype):
     """A tensor of the allocator of the stream (or graph) that will use it."""
     torch = _torch()
     if stream is not None:
@@ -809,13 +809,13 @@ class PackedInt8:
     (ter_hip_w8_*).  Beside PackedTrits, for what is not ternary: a head, an
     embedding, a projection."""
 
-    def __init__(self, K: int, N: int, device=None):
+    def __init__(self, K: int, N: int, device=None, stream=None):
         torch = _torch()
         self.K, self.N = int(K), int(N)
         nbytes = L.lib().ter_hip_w8_bytes(self.K, self.N) if 0 < self.K < 1 << 31 and 0 < self.N < 1 << 31 else 0
         if nbytes == 0:
             raise ValueError(f"bad shape K={K} N={N}")
-        self.buf = torch.empty(nbytes, dtype=torch.uint8, device="cuda" if device is None else device)
+        self.buf = _empty_on("cuda" if device is None else device, stream, nbytes, torch.uint8)
         self.w8 = L.W8()
         L.check(L.lib().ter_hip_w8_init(C.byref(self.w8), self.buf.data_ptr(), nbytes, self.K, self.N),
                 "ter_hip_w8_init")
@@ -829,7 +829,7 @@ class PackedInt8:
         st = _matrix(q, "q")
         _type_of(q.dtype, (L.T_I8,), "q")
         _vector(scale, "scale", torch.float32, q.shape[0], q.get_device())
-        w = cls(q.shape[1], q.shape[0], device=q.device)
+        w = cls(q.shape[1], q.shape[0], q.device, stream)
         _launch_on(w._dev, "ter_hip_w8_pack", stream, w._ref, q.data_ptr(), st, scale.data_ptr())
         return w
 
@@ -839,7 +839,7 @@ class PackedInt8:
         magnitude (the steps of quant_int8)."""
         st = _matrix(w, "w")
         ty = _type_of(w.dtype, (L.T_F16, L.T_BF16, L.T_F32), "w")
-        p = cls(w.shape[1], w.shape[0], device=w.device)
+        p = cls(w.shape[1], w.shape[0], w.device, stream)
         _launch_on(p._dev, "ter_hip_w8_quantize", stream, p._ref, w.data_ptr(), ty, st)
         return p
 
@@ -922,7 +922,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
                 raise ValueError("top_k must be a whole number >= 0")
             p.top_k = min(int(v), (1 << 31) - 1)
         else:
-            setattr(p, name, v)
+            setattr(p, name, float(v))
     if out is None:
         out = _empty_on(dev, stream, (M,), torch.int32)
     else:

@@ -207,6 +207,26 @@ def test_no_rows(cuda):
     assert y.shape == (0, 20) and y.dtype == torch.float16
 
 
+def test_weights_filled_on_another_stream(cuda):
+    """Their memory is that stream's, not what the current one still writes."""
+    g = gen(12)
+    q, ws = ints(g, 3000, 2000).cuda(), scales(g, 3000).cuda()
+    w = q.float()
+    st = torch.cuda.Stream()
+    n = T.PackedInt8(2000, 3000).buf.numel()
+    torch.cuda.synchronize()
+    for fill in (lambda s: T.PackedInt8.from_int8(q, ws, stream=s), lambda s: T.PackedInt8.quantize(w, stream=s)):
+        want = [t.cpu() for t in fill(None).to_int8()]
+        busy = torch.empty(n, dtype=torch.uint8, device="cuda")
+        for _ in range(200):
+            busy.fill_(7)
+        del busy
+        W = fill(st.cuda_stream)
+        torch.cuda.synchronize()
+        for a, b in zip(W.to_int8(), want):
+            assert torch.equal(a.cpu(), b)
+
+
 def test_another_stream(cuda):
     """Given as a handle: the call's workspace comes from that stream's memory."""
     g = gen(2)
