@@ -296,3 +296,13 @@ def test_launches_of_a_draw(fake):
             assert [int(x[1]) for x in k] == [rows * slices] * 3 + [rows], k
             assert need % rows == 0 and need > 0
     """)
+
+
+def test_wait_states_around_the_asm_loads(tmp_path):
+    """The loads to LDS of the product in tiles are inline asm: no buffer load
+    within five wait states of the lane read that wrote one of its registers."""
+    from tests import test_paged_waits as waits
+    code = waits.kernels(tmp_path, "int8_gemm_kernel")
+    assert len(code) >= 32
+    for name, kernel in code.items():
+        assert not kernel.faults(), name

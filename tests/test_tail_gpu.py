@@ -90,3 +90,35 @@ def test_behind_the_paged_attention(cuda):
         assert torch.equal(logits, again) and torch.equal(token, t)
         x = logits.double().cpu().numpy()
         assert token.tolist() == [draw(x[b], u[b].item(), 0.8, 50, 0.95)[0] for b in range(n)]
+
+
+def test_two_tails_at_once(cuda):
+    """Two graphs on two streams, each with its own workspaces, beside eager
+    calls on a third."""
+    h, v = 1030, 20011
+    g = torch.Generator(device="cuda").manual_seed(11)
+    W = T.PackedInt8.quantize(torch.randn(v, h, generator=g, device="cuda"))
+    parts = []
+    for m in (70, 20):
+        x, u = torch.randn(m, h, generator=g, device="cuda").half(), torch.rand(m, generator=g, device="cuda")
+
+        def step(x=x, u=u):
+            return T.sample(T.mm_int8(W, x), u, temperature=0.9, top_p=0.95)
+
+        want = step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            token = step()
+        parts.append((graph, token, want, step, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, token, _, _, st in parts:
+            with torch.cuda.stream(st):
+                token.fill_(-2)
+                for _ in range(4):
+                    graph.replay()
+        eager = [step() for _, _, _, step, _ in parts]
+        torch.cuda.synchronize()
+        for (_, token, want, _, _), e in zip(parts, eager):
+            assert torch.equal(token, want) and torch.equal(e, want)
