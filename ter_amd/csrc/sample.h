@@ -30,8 +30,9 @@ static_assert(sizeof(SampleRow) % 16 == 0, "");
 // workspace then).
 inline int sample_slices(int rows, int V) {
     const int want = (V + 4095) / 4096, fit = 512 / (rows > 0 ? rows : 1);
-    const int n = want < fit ? want : fit;
-    return n < kSlices ? n : kSlices;
+    int n = want < fit ? want : fit;
+    n = n < kSlices ? n : kSlices;
+    return n > 1 ? n : 1;
 }
 
 struct SampleArgs {

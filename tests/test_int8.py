@@ -179,9 +179,9 @@ def mm(M, N, K, xt=L.T_I8, yt=L.T_F16, stride=None):
     x = L.Rows(A, A, stride or K, xt, M)
     need = lib.ter_hip_w8_mm_ws(C.byref(w), C.byref(x))
     return lib.ter_hip_w8_mm(C.byref(w), C.byref(x), A, N, yt, A if need else None, need, None)
-def draw(rows, V, ty=L.T_F16):
+def draw(rows, V, ty=L.T_F16, temperature=1.0, top_k=0, dev=None):
     p = L.SampleParams()
-    p.temperature = p.top_p = 1.0
+    p.temperature, p.top_p, p.top_k, p.temperature_dev = temperature, 1.0, top_k, dev
     need = lib.ter_hip_sample_ws(rows, V)
     return lib.ter_hip_sample(A, ty, V, rows, V, A, C.byref(p), A, None, A if need else None, need, None)
 def kernels():
@@ -295,6 +295,24 @@ def test_launches_of_a_draw(fake):
             assert [x[4].split("sample_")[1].split("_")[0] for x in k] == ["max", "bins", "list", "finish"], k
             assert [int(x[1]) for x in k] == [rows * slices] * 3 + [rows], k
             assert need % rows == 0 and need > 0
+    """)
+
+
+def test_launches_that_take_the_largest(fake):
+    fake("""
+    # temperature 0 or top_k 1 on the host: a row's slices and their join; read on the device: the usual way
+    for kw in (dict(temperature=0.0), dict(top_k=1), dict(top_k=1, dev=A)):
+        assert draw(2, 128256, **kw) == 0
+        a, b = kernels()
+        assert "sample_largest_kernel" in a[4] and int(a[1]) == 64 and "largest_join" in b[4] and int(b[1]) == 2, (a, b)
+        assert draw(300, 128256, **kw) == 0
+        (a,) = kernels()
+        assert "sample_largest_kernel" in a[4] and int(a[1]) == 300, a
+    assert draw(2, 128256, temperature=0.0, dev=A) == 0 and len(kernels()) == 4
+    for part in (b"sample_largest_kernel", b"largest_join"):
+        fake.fake_fail(part)
+        assert draw(2, 50000, temperature=0.0) == L.ERR_HIP
+        fake.fake_fail(b"")
     """)
 
 

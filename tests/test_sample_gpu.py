@@ -188,6 +188,37 @@ def test_far_apart_and_close_logits(cuda):
         check(x, u, **kw)
 
 
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("m,v,pad", [(1, 1, 0), (9, 70, 3), (3, 4097, 1), (2, 128256, 0), (300, 9001, 5), (700, 64, 0)])
+def test_largest_of_every_row(cuda, m, v, pad, dt):
+    """Temperature 0 and top_k 1 on the host, which go a way of their own, as on
+    the device: of equal logits the lower index, rows masked or infinite."""
+    g = torch.Generator().manual_seed(m + v)
+    x = (torch.randn(m, v + pad, generator=g) * 2).round().to(dt)
+    x[m // 2, : v // 2] = float("nan")
+    x[m // 3, pad:] = -float("inf")
+    x[m - 1, v // 3:] = 1e4
+    if m > 4:
+        x[3, 1::7] = float("inf")
+        x[4, pad:] = float("nan")
+        x[5] = -0.0
+        x[5, ::2] = 0.0
+        x[6] = torch.finfo(dt).min
+        x[7] = torch.finfo(dt).max
+        x[7, v // 2:] = float("inf")
+    u = torch.rand(m, generator=g)
+    part = x[:, pad:]
+    want = check(part[:8], u[:8], temperature=0.0)
+    on_device = T.sample(x.cuda()[:, pad:], u.cuda(), temperature=torch.zeros(m, device="cuda")).cpu()
+    assert torch.equal(on_device[:8], want)
+    for kw in (dict(temperature=0.0), dict(temperature=0.0, top_p=0.5, min_p=0.2, top_k=v), dict(top_k=1),
+               dict(top_k=1, temperature=torch.full((m,), 1.5, device="cuda"), top_p=0.1)):
+        p = torch.full((m,), -1.0, device="cuda")
+        t = T.sample(x.cuda()[:, pad:], u.cuda(), prob_out=p, **kw).cpu()
+        assert torch.equal(t, on_device)
+        assert torch.equal(p.cpu(), (on_device >= 0).float())
+
+
 @pytest.mark.parametrize("m", [2, 300])
 @pytest.mark.parametrize("t", [1e-37, 1e-38, 1e-40, 2.0 ** -149])
 def test_temperatures_near_zero(cuda, t, m):
