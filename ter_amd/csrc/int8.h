@@ -44,7 +44,14 @@ struct Int8MmArgs {
     int y_type;
     int x_type;           // TER_HIP_T_I8, or rows quantized by the product's kernel: x, ldx and Kx are those of its elements
     int vec;              // such rows are 16-byte aligned
+    int* sums;            // [parts][M][i8_sums_stride(N)] where tiles take a part of K each (parts > 1)
+    int parts;
 };
+
+// Parts of K that the tiles of a call take (1: all of it), by sizes alone, and
+// the stride of their sums.
+int i8_parts(int M, int N, int Ku);
+__host__ __device__ inline int i8_sums_stride(int N) { return (N + 7) / 8 * 8; }
 
 // Rows that the product's kernel quantizes itself: a team of waves holds one
 // in registers, at most kI8Chunks of 8 values a lane where 4 waves work
@@ -67,6 +74,8 @@ hipError_t launch_w8_unpack(const uint8_t* tiles, const float* scale, int8_t* q,
 // scales [M] for types other than TER_HIP_T_I8.
 hipError_t launch_rows8(const void* x, int type, long long stride, int M, int K, int8_t* q, long long ldq, float* scale,
                         hipStream_t st);
+// Whether a call is computed in tiles.
+inline bool i8_in_tiles(int M, int N) { return M > 64 || (M > 16 && i8_pairs(N) > 300); }
 hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st);
 hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st);  // many rows
 

@@ -65,9 +65,23 @@ bool quant_within(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
 
 size_t row_bytes(const ter_hip_w8_t* w) { return (size_t)i8_units(w->K) * kI8Unit; }
 
-size_t ws_bytes_of(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
+// Of the workspace: the rows in 8 bits, and their scales.
+size_t rows_bytes_of(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
     if (x->n == 0 || in_place(w, x) || quant_within(w, x)) return 0;
     return (size_t)x->n * (row_bytes(w) + 4);
+}
+
+int parts_of(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
+    return i8_in_tiles(x->n, w->N) ? i8_parts(x->n, w->N, i8_units(w->K)) : 1;
+}
+
+// Behind them the sums of parts of K.
+size_t sums_at(const ter_hip_w8_t* w, const ter_hip_rows_t* x) { return (rows_bytes_of(w, x) + 15) / 16 * 16; }
+
+size_t ws_bytes_of(const ter_hip_w8_t* w, const ter_hip_rows_t* x) {
+    const int parts = parts_of(w, x);
+    if (parts == 1) return rows_bytes_of(w, x);
+    return sums_at(w, x) + (size_t)parts * x->n * i8_sums_stride(w->N) * 4;
 }
 
 }  // namespace
@@ -164,6 +178,8 @@ int ter_hip_w8_mm(const ter_hip_w8_t* w, const ter_hip_rows_t* x, void* y, int64
     a.Ku = i8_units(w->K);
     a.y_type = y_type;
     a.x_type = TER_HIP_T_I8;
+    a.parts = parts_of(w, x);
+    if (a.parts > 1) a.sums = reinterpret_cast<int*>(static_cast<char*>(ws) + sums_at(w, x));
     if (quant_within(w, x)) {
         a.x = static_cast<const int8_t*>(x->data);
         a.ldx = x->stride;

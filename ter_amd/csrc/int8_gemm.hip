@@ -93,8 +93,10 @@ __device__ __forceinline__ void wait_unit(int behind, bool more) {
     }
 }
 
-template <class C, int YT>
-__global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int mt, int nt, bool once) {
+// SPLIT: a tile is computed by a.parts workgroups, `per` units of K each, whose
+// bare sums int8_join_kernel joins; the grid is all of them.
+template <class C, int YT, bool SPLIT>
+__global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int mt, int nt, bool once, int per) {
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
@@ -116,7 +118,9 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     // what is loaded: unit iu of tile it.  Large weights that one tile needs pass
     // the caches by: 96 x 2560 x 128256 75.1 -> 66.3 us (8192 x 2560 x 6912, where
     // they are needed again, 134 -> 161).
-    int it = blockIdx.x, iu = 0, place = 0;
+    const int tiles = mt * nt, part = SPLIT ? (int)blockIdx.x / tiles : 0, tile0 = (int)blockIdx.x - part * tiles;
+    const int first = SPLIT ? part * per : 0, last = SPLIT && first + per < a.Ku ? first + per : a.Ku;
+    int it = tile0, iu = first, place = 0;
     u32x4 xr, wr;
     auto aim = [&] {
         int tm, tn;
@@ -128,7 +132,6 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         wr = resource(a.w + (long long)s0 * a.Ku * 2048,
                       (unsigned)((strips < C::BN / 16 ? strips : C::BN / 16) * a.Ku * 2048));
     };
-    const int tiles = mt * nt;
     constexpr int RUNS = C::XL + (C::XR != 0) + C::WL;
     auto issue = [&](int i) {  // load i of the next unit, to its place
         if (it >= tiles) return;
@@ -141,8 +144,8 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
             load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, once);
         if (i == RUNS - 1) {
             place = place + 1 == C::NST ? 0 : place + 1;
-            if (++iu == a.Ku) {
-                iu = 0;
+            if (++iu == last) {
+                iu = first;
                 it += gridDim.x;
                 if (it < tiles) aim();
             }
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     for (int k = 0; k < C::NST; ++k)
 #pragma unroll
         for (int i = 0; i < RUNS; ++i) issue(i);
-    int left = ((tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * a.Ku;  // units, the one at hand included
+    int left = SPLIT ? last - first : ((tiles - 1 - tile0) / (int)gridDim.x + 1) * a.Ku;  // units, the one at hand included
     wait_unit<C, C::NST - 1>(left - 1, more);
     barrier();
     int cur = 0;
@@ -182,9 +185,13 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     for (int q = 0; q < kAhead; ++q) x[q] = read_x(lds, q);
     constexpr int kSlots = C::SPREAD < STEPS ? C::SPREAD : STEPS - 1;
     bool loading = false;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    if (SPLIT) {
+        a.ldy = i8_sums_stride(a.N);
+        a.y = reinterpret_cast<char*>(a.sums + (long long)part * a.M * a.ldy);
+    }
+    for (int tile = tile0; tile < tiles; tile += gridDim.x) {
         i32x4 acc[C::MBW][C::SW] = {};
-        for (int u = 0; u < a.Ku; ++u) {
+        for (int u = first; u < last; ++u) {
             const unsigned char* st = lds + cur * C::STAGE;
             cur = cur + 1 == C::NST ? 0 : cur + 1;
             const unsigned char* next = lds + cur * C::STAGE;
@@ -235,16 +242,56 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     }
 }
 
+// Eight results of one row a thread: the parts' sums, scaled.
+template <int YT>
+__global__ __launch_bounds__(256) void int8_join_kernel(Int8MmArgs a) {
+    const int stride = i8_sums_stride(a.N), chunks = stride / 8;
+    const int i = blockIdx.x * 256 + threadIdx.x, m = i / chunks, n = (i - m * chunks) * 8;
+    if (m >= a.M) return;
+    i32x4 s[2] = {};
+    for (int p = 0; p < a.parts; ++p) {
+        const TER_GLOBAL i32x4* from = reinterpret_cast<const TER_GLOBAL i32x4*>(gptr(a.sums) + ((long long)p * a.M + m) * stride + n);
+        s[0] += from[0];
+        s[1] += from[1];
+    }
+    float ws[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) ws[c] = YT == TER_HIP_T_I32 ? 0.f : gptr(a.ws)[n + c];
+    const int v[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
+    store_run<YT, 8>(a.y, (long long)m * a.ldy + n, a.N - n, v, YT == TER_HIP_T_I32 ? 0.f : gptr(a.xs)[m], ws, wide_rows(a));
+}
+
 template <class C, int YT>
 hipError_t launch(const Int8MmArgs& a, int cus, hipStream_t st) {
     static LdsLimit limit;
-    const hipError_t e = limit.allow(C::LDS, {reinterpret_cast<const void*>(&int8_gemm_kernel<C, YT>)});
+    const hipError_t e = limit.allow(C::LDS, {reinterpret_cast<const void*>(&int8_gemm_kernel<C, YT, false>)});
     if (e != hipSuccess) return e;
     const int mt = (a.M + C::BM - 1) / C::BM, nt = (a.N + C::BN - 1) / C::BN;
     const int fit = kLdsMax / C::LDS > 1 ? 2 : 1;
     const int grid = mt * nt < cus * fit ? mt * nt : cus * fit;
-    hipLaunchKernelGGL((int8_gemm_kernel<C, YT>), dim3(grid), dim3(C::THREADS), C::LDS, st, a, mt, nt,
-                       mt == 1 && i8_past_caches(a.N, a.Ku));
+    hipLaunchKernelGGL((int8_gemm_kernel<C, YT, false>), dim3(grid), dim3(C::THREADS), C::LDS, st, a, mt, nt,
+                       mt == 1 && i8_past_caches(a.N, a.Ku), 0);
+    return hipGetLastError();
+}
+
+using Small = GCfg<2, 2, 2, 2, 5, 4>;
+
+hipError_t launch_parts(const Int8MmArgs& a, hipStream_t st) {
+    static LdsLimit limit;
+    const auto kernel = &int8_gemm_kernel<Small, TER_HIP_T_I32, true>;
+    hipError_t e = limit.allow(Small::LDS, {reinterpret_cast<const void*>(kernel)});
+    if (e != hipSuccess) return e;
+    const int mt = (a.M + Small::BM - 1) / Small::BM, nt = (a.N + Small::BN - 1) / Small::BN;
+    hipLaunchKernelGGL(kernel, dim3(mt * nt * a.parts), dim3(Small::THREADS), Small::LDS, st, a, mt, nt, false,
+                       (a.Ku + a.parts - 1) / a.parts);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    const dim3 grid((a.M * (i8_sums_stride(a.N) / 8) + 255) / 256), block(256);
+    switch (a.y_type) {
+        case TER_HIP_T_F16: hipLaunchKernelGGL(int8_join_kernel<TER_HIP_T_F16>, grid, block, 0, st, a); break;
+        case TER_HIP_T_BF16: hipLaunchKernelGGL(int8_join_kernel<TER_HIP_T_BF16>, grid, block, 0, st, a); break;
+        case TER_HIP_T_F32: hipLaunchKernelGGL(int8_join_kernel<TER_HIP_T_F32>, grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL(int8_join_kernel<TER_HIP_T_I32>, grid, block, 0, st, a); break;
+    }
     return hipGetLastError();
 }
 
@@ -276,28 +323,59 @@ constexpr Variant kVariants[] = {
     {256, 128, 1, 0.90f, 0.90f, 4.5f}, {160, 256, 1, 1.10f, 1.10f, 5.f}, {192, 256, 1, 1.21f, 1.21f, 6.f},
     {224, 256, 1, 1.37f, 1.37f, 7.f},  {256, 256, 1, 1.59f, 1.59f, 8.f},
 };
+
+// The variant of the least estimate, and that estimate.
+int best_variant(int M, int N, int Ku, int cus, float* us) {
+    int best = 0;
+    for (int i = 0; i < (int)(sizeof(kVariants) / sizeof(kVariants[0])); ++i) {
+        const Variant& v = kVariants[i];
+        const long long tiles = (long long)((M + v.bm - 1) / v.bm) * ((N + v.bn - 1) / v.bn);
+        const long long rounds = (tiles + (long long)cus * v.fit - 1) / ((long long)cus * v.fit);
+        const float t = (float)rounds * ((float)Ku * (tiles <= cus ? v.few : v.unit) + v.tile);
+        if (i == 0 || t < *us) {
+            *us = t;
+            best = i;
+        }
+    }
+    return best;
+}
 }  // namespace
 
+// Few tiles of a long K leave most of the GPU idle: parts of it then, as many
+// workgroups as fit at once, and their sums joined by one launch more, whose host
+// time counts too (us, rows x channels x K, all of K and parts): 380 x 512 x 8192
+// 24.6 and 13.7, 128 x 2560 x 6912 20.8 and 14.8, 300 x 2560 x 16384 44.3 and
+// 32.8, 256 x 2560 x 6912 21.3 and 16.8; 128 x 640 x 2560 9.6 and 13.3: not in parts.
+int i8_parts(int M, int N, int Ku) {
+    constexpr int kCus = 256;
+    constexpr float kJoin = 5.f, kJoinBytes = 1.f / 3e6f;  // us a launch, us a byte of sums
+    float least;
+    best_variant(M, N, Ku, kCus, &least);
+    const long long tiles = (long long)((M + 63) / 64) * ((N + 63) / 64);
+    int best = 1;
+    for (int parts = 2; parts <= 8 && parts * tiles <= 2 * kCus && parts * 4 <= Ku; ++parts) {
+        const int per = (Ku + parts - 1) / parts;
+        if (per * (parts - 1) >= Ku) continue;  // (each part has units)
+        const float us = (float)per * (parts * tiles <= kCus ? kVariants[0].few : kVariants[0].unit) + kVariants[0].tile +
+                         kJoin + kJoinBytes * 4.f * (float)parts * (float)M * (float)N;
+        if (us < least) {
+            least = us;
+            best = parts;
+        }
+    }
+    return best;
+}
+
 hipError_t launch_int8_gemm(const Int8MmArgs& a, hipStream_t st) {
+    if (a.parts > 1) return launch_parts(a, st);
     int dev = 0;
     const hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
     const int cus = device_cu_count(dev);
     if (cus <= 0) return hipErrorInvalidDevice;
-    int best = 0;
-    float least = 0.f;
-    for (int i = 0; i < (int)(sizeof(kVariants) / sizeof(kVariants[0])); ++i) {
-        const Variant& v = kVariants[i];
-        const long long tiles = (long long)((a.M + v.bm - 1) / v.bm) * ((a.N + v.bn - 1) / v.bn);
-        const long long rounds = (tiles + (long long)cus * v.fit - 1) / ((long long)cus * v.fit);
-        const float us = (float)rounds * ((float)a.Ku * (tiles <= cus ? v.few : v.unit) + v.tile);
-        if (i == 0 || us < least) {
-            least = us;
-            best = i;
-        }
-    }
-    switch (best) {
-        case 0: return launch_type<GCfg<2, 2, 2, 2, 5, 4>>(a, cus, st);
+    float us;
+    switch (best_variant(a.M, a.N, a.Ku, cus, &us)) {
+        case 0: return launch_type<Small>(a, cus, st);
         case 1: return launch_type<GCfg<3, 4, 2, 4, 3, 8>>(a, cus, st);
         case 2: return launch_type<GCfg<4, 4, 2, 4, 3, 4>>(a, cus, st);
         case 3: return launch_type<GCfg<4, 4, 4, 2, 3, 4>>(a, cus, st);

@@ -215,11 +215,11 @@ hipError_t launch_int8_mm(const Int8MmArgs& a, hipStream_t st) {
     if (a.x_type == TER_HIP_T_F16) return launch_rows<1, TER_HIP_T_F16>(a, st);
     if (a.x_type == TER_HIP_T_BF16) return launch_rows<1, TER_HIP_T_BF16>(a, st);
     if (a.x_type == TER_HIP_T_F32) return launch_rows<1, TER_HIP_T_F32>(a, st);
-    if (a.M <= 16) return launch_rows<1, TER_HIP_T_I8>(a, st);
     // From 17 rows on and many channels the rows' reads by every workgroup weigh
     // more than the tiles' way over LDS: 32 x 2560 x 128256 78.6 us here, 62.1 in
     // tiles; 64 rows 111 and 70.  At 64 x 2048 x 8192 7.2 and 7.9.
-    if (a.M > 64 || i8_pairs(a.N) > 300) return launch_int8_gemm(a, st);
+    if (i8_in_tiles(a.M, a.N)) return launch_int8_gemm(a, st);
+    if (a.M <= 16) return launch_rows<1, TER_HIP_T_I8>(a, st);
     if (a.M <= 32) return launch_rows<2, TER_HIP_T_I8>(a, st);
     return launch_rows<4, TER_HIP_T_I8>(a, st);
 }

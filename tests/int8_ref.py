@@ -48,3 +48,5 @@ def same(a, b):
     bad = (x != y).nonzero()
     assert len(bad) == 0, f"{len(bad)} of {x.numel()} differ, first at {bad[0].tolist()}: " \
                           f"{a.cpu()[tuple(bad[0])]} against {b.cpu()[tuple(bad[0])]}"
+# few tiles of a long K, computed by parts of it
+PARTS = [(380, 512, 8192), (65, 33, 9000), (209, 1282, 8192), (128, 2560, 6912), (70, 1003, 4097), (500, 40, 20000)]

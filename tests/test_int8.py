@@ -251,6 +251,32 @@ def test_every_tile_is_some_calls(fake):
     """)
 
 
+def test_parts_of_a_long_k(fake):
+    """Few tiles of a long K: by parts that have units each and fit the GPU at
+    once, joined by one more launch; their sums in the workspace."""
+    from tests.int8_ref import PARTS
+    fake(f"""
+    for M, N, K in {PARTS!r}:
+        assert mm(M, N, K, L.T_I8, L.T_BF16) == 0, lib.ter_hip_last_error()
+        *_, p, j = kernels()
+        assert "int8_gemm_kernel" in p[4] and "true>" in p[4] and "join" in j[4], (p, j)
+        tiles = -(-M // 64) * -(-N // 64)
+        parts, rest = divmod(int(p[1]), tiles)
+        units = -(-K // 128)
+        assert rest == 0 and 2 <= parts <= 8 and int(p[1]) <= 512, p
+        assert -(-units // parts) * (parts - 1) < units
+        assert int(j[1]) * 256 * 8 >= M * N
+        w = L.W8()
+        assert lib.ter_hip_w8_init(C.byref(w), A, 1 << 60, K, N) == 0
+        x = L.Rows(A, A, K, L.T_I8, M)
+        rows = 0 if K % 16 == 0 else -(-M * (units * 128 + 4) // 16) * 16
+        assert lib.ter_hip_w8_mm_ws(C.byref(w), C.byref(x)) == rows + parts * M * -(-N // 8) * 32
+    assert mm(380, 512, 1024) == 0 and len(kernels()) == 1
+    fake.fake_fail(b"int8_join")
+    assert mm(380, 512, 8192) == L.ERR_HIP
+    """)
+
+
 def test_rows_of_many_launches(fake):
     """Rows quantized: no launch of 2^32 threads or more."""
     fake("""

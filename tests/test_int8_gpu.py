@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ter_amd as T
-from tests.int8_ref import TILES, product, quantized, same
+from tests.int8_ref import PARTS, TILES, product, quantized, same
 
 pytestmark = pytest.mark.gpu
 
@@ -77,7 +77,7 @@ def test_larger(cuda, m, n, k):
         same(T.mm_int8(W, x, xs, dtype=dt), want.to(dt))
 
 
-@pytest.mark.parametrize("m,n,k", [s for sizes in TILES.values() for s in sizes])
+@pytest.mark.parametrize("m,n,k", [s for sizes in TILES.values() for s in sizes] + PARTS)
 def test_every_tile(cuda, m, n, k):
     """Sizes that do not fill the last tiles, in several rounds of the GPU."""
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
