@@ -89,7 +89,8 @@ __global__ __launch_bounds__(256) void rows8_long_kernel(const void* __restrict_
     }
 }
 
-// Integer rows at any alignment to aligned ones, 16 bytes a thread.
+// Integer rows at any alignment to aligned ones, 16 bytes a thread, from the aligned
+// words that hold them where those lie within the row.
 __global__ __launch_bounds__(256) void rows8_copy_kernel(const int8_t* __restrict__ x, long long stride, int K,
                                                          int8_t* __restrict__ q, long long ldq, int chunks,
                                                          long long total) {
@@ -97,14 +98,22 @@ __global__ __launch_bounds__(256) void rows8_copy_kernel(const int8_t* __restric
         const long long m = i / chunks;
         const int k0 = (int)(i - m * chunks) * 16;
         const int8_t* row = x + m * stride;
+        const int off = (int)(reinterpret_cast<uintptr_t>(row + k0) & 3);
         u32x4 v;
-        for (int j = 0; j < 4; ++j) {
-            unsigned d = 0;
-            for (int b = 0; b < 4; ++b) {
-                const int k = k0 + 4 * j + b;
-                if (k < K) d |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+        if (k0 >= off && k0 - off + 20 <= K) {
+            const TER_GLOBAL unsigned* w = reinterpret_cast<const TER_GLOBAL unsigned*>(gptr(row) + (k0 - off));
+            const unsigned d[5] = {w[0], w[1], w[2], w[3], w[4]};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_alignbyte(d[j + 1], d[j], (unsigned)off);
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                unsigned e = 0;
+                for (int b = 0; b < 4; ++b) {
+                    const int k = k0 + 4 * j + b;
+                    if (k < K) e |= (unsigned)(uint8_t)gptr(row)[k] << (8 * b);
+                }
+                v[j] = e;
             }
-            v[j] = d;
         }
         *reinterpret_cast<TER_GLOBAL u32x4*>(gptr(q) + m * ldq + k0) = v;
     }
