@@ -16,6 +16,13 @@
 //
 // Rows behind the last and values behind K are zeros by the buffer's range, or
 // meet the zeros that pad the weights.
+//
+// Measured: 8192 x 8192 x 8192 395 to 412 us, 2.67 to 2.79 P op/s (the library's
+// product 464); 8192 x 2560 x 6912 127 to 142 us by the machine, 2.0 to 2.3 (177).
+// Of a unit's 1.59 us in the largest tile the products alone are 1.03, the loads
+// alone 1.02: LDS serves both, and the barrier's wait is not all hidden.  Products
+// of 32 x 32 x 32 instead of 16 x 16 x 64 (8192 cubed 475 against 441 us then)
+// and 4 waves of 128 x 128 instead of 8 were slower.
 #include "common.h"
 #include "int8.h"
 #include "int8_store.h"
