@@ -80,7 +80,7 @@ __device__ __forceinline__ void quantize_rows(const Int8MmArgs& a, unsigned char
 }
 
 // XT: the type of rows that the workgroup quantizes itself, or TER_HIP_T_I8.
-// Such rows are few and short (quant_chunks): every workgroup does it again,
+// Such rows are few and short (i8_quant_within): every workgroup does it again,
 // under its first loads of weights, which is less than another launch takes.
 template <int MB, int S, int KS, int D, int YT, int XT, bool PAST>
 __global__ __launch_bounds__(64 * KS) void int8_stream_kernel(Int8MmArgs a, int groups) {
@@ -112,7 +112,8 @@ __global__ __launch_bounds__(64 * KS) void int8_stream_kernel(Int8MmArgs a, int 
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 // (the end of a strip is not the end of the range)
-                w[d][t][s] = load16(wr, u < a.Ku ? lane * 16 : 0x7FFFFFFFu, (unsigned)((s * a.Ku + (u < a.Ku ? u : 0)) * 2048 + t * 1024), PAST);
+                w[d][t][s] = load16(wr, u < a.Ku ? lane * 16 : 0x7FFFFFFFu,
+                                    (unsigned)((s * a.Ku + (u < a.Ku ? u : 0)) * 2048 + t * 1024), PAST);
             if constexpr (!kQuant) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i) x[d][t][i] = load16(xr, xo[i], (unsigned)(u * 128 + t * 64));

@@ -810,7 +810,8 @@ __device__ __forceinline__ u64 lane_of(u64 v, int i) {
 
 // The places among the spots that a wave's lanes hold (`here`: this lane has
 // one), each kept sum exact: the sum of all kept, and where u lies.
-__device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, u64 weight, bool here, const Runs& r, u64* target) {
+__device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, u64 weight, bool here, const Runs& r,
+                                       u64* target) {
     auto pick = [&](bool mine, u64 v) -> u64 {
         const u64 b = __ballot(mine);
         if (!b) return 0;
@@ -837,8 +838,8 @@ __device__ __forceinline__ u64 kept_of(const Settings& s, int V, const Spot& z, 
 
 // k <= kFew elements, lane i of the first wave with l; b: its bin, whose sums in
 // front are z's.
-__device__ __forceinline__ bool finish_lanes(const SampleArgs& a, int row, const Settings& s, const Weights& w, const Runs& q,
-                                             int k, u64 l, float x, u64 e, int b, Spot z) {
+__device__ __forceinline__ bool finish_lanes(const SampleArgs& a, int row, const Settings& s, const Weights& w,
+                                             const Runs& q, int k, u64 l, float x, u64 e, int b, Spot z) {
     const bool here = (int)(threadIdx.x & 63) < k;
     // (lanes from k on hold the largest entry: behind all.  Eight at a time: one
     // wave works here, and one by one each waits for the last.)
@@ -862,8 +863,8 @@ __device__ __forceinline__ bool finish_lanes(const SampleArgs& a, int row, const
 
 // The second list, if it has few elements.
 template <int NT, typename B>
-__device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w, const Runs& q,
-                           int k, Lds<NT>& sh) {
+__device__ __forceinline__ bool finish_few(const SampleArgs& a, int row, const Settings& s, const B& bin, const Weights& w,
+                                           const Runs& q, int k, Lds<NT>& sh) {
     if (threadIdx.x < 64) {
         const bool here = (int)threadIdx.x < k;
         const u64 l = here ? sh.second[threadIdx.x] : ~0ull;

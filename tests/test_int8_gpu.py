@@ -267,3 +267,36 @@ def test_captured_and_replayed(cuda, m):
         torch.cuda.synchronize()
         same(y, product(*quantized(new), w, ws, torch.float16))
         T.mm_int8(W, x[:1])  # eager work between
+
+
+@pytest.mark.parametrize("m,n,k", PARTS[:4])
+def test_parts_of_k_in_graphs(cuda, m, n, k):
+    """Rows quantized and parts' sums in one workspace: two graphs on two streams
+    at once, replayed with new rows, beside eager calls."""
+    g = gen(m)
+    W, w, ws = weights(g, n, k)
+    parts = []
+    for dt in (torch.float16, torch.float32):
+        x = torch.randn(m, k, generator=g).to(dt).cuda()
+        T.mm_int8(W, x, dtype=torch.bfloat16)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = T.mm_int8(W, x, dtype=torch.bfloat16)
+        parts.append((graph, x, y, torch.cuda.Stream()))
+    for _ in range(3):
+        want = []
+        for _, x, y, _ in parts:
+            new = torch.randn(m, k, generator=g).to(x.dtype)
+            x.copy_(new)
+            y.fill_(7)
+            want.append(product(*quantized(new), w, ws, torch.bfloat16))
+        torch.cuda.synchronize()
+        for graph, _, _, st in parts:
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = [T.mm_int8(W, x, dtype=torch.bfloat16) for _, x, _, _ in parts]
+        torch.cuda.synchronize()
+        for (_, _, y, _), e, want_y in zip(parts, eager, want):
+            same(y, want_y)
+            same(e, want_y)
