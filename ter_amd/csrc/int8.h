@@ -18,11 +18,11 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "int8_rows.h"
 #include "ter_hip_int8.h"
 
 namespace terhip {
 
-constexpr int kI8Unit = 128;  // K is padded to this
 __host__ __device__ inline int i8_units(int K) { return (K + kI8Unit - 1) / kI8Unit; }
 __host__ __device__ inline int i8_pairs(int N) { return (N + 31) / 32; }  // of strips
 inline size_t i8_tile_bytes(int K, int N) { return (size_t)i8_pairs(N) * i8_units(K) * 4096; }

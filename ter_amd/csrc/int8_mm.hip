@@ -93,17 +93,14 @@ __global__ __launch_bounds__(64 * KS) void int8_stream_kernel(Int8MmArgs a, int 
     const int j = lane & 15, g = lane >> 4;
     const int nb = blockIdx.x % groups, m0 = blockIdx.x / groups * (16 * MB);
     const int rows = a.M - m0 < 16 * MB ? a.M - m0 : 16 * MB;
-    // units past the last are past the range: zeros
+    // units past the last are past the range by the vector offset: zeros
     const __amdgpu_buffer_rsrc_t wr = resource(a.w + (long long)nb * S * a.Ku * 2048, (unsigned)(S * a.Ku * 2048));
     const __amdgpu_buffer_rsrc_t xr =
-        resource(a.x + (kQuant ? 0 : (long long)m0 * a.ldx), kQuant ? 0u : (unsigned)((rows - 1) * (int)a.ldx + a.Kx));
+        resource(a.x + (kQuant ? 0 : (long long)m0 * a.ldx), kQuant ? 0u : i8_rows_size(rows, (int)a.ldx, a.Kx));
     const int ldl = a.Ku * 128 + 16;
     unsigned xo[MB];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const int m = 16 * i + j;  // (rows behind the last: the last one's loads, whose sums nobody stores)
-        xo[i] = (unsigned)((m < rows ? m : rows - 1) * (kQuant ? ldl : (int)a.ldx) + g * 16);
-    }
+    for (int i = 0; i < MB; ++i) xo[i] = i8_stream_lane(16 * i + j, g, rows, kQuant ? ldl : (int)a.ldx);
     i32x4 acc[MB][S] = {};
     i32x4 w[D][2][S], x[kQuant ? 1 : D][2][MB];
     auto load = [&](int d, int u) {
@@ -116,7 +113,7 @@ __global__ __launch_bounds__(64 * KS) void int8_stream_kernel(Int8MmArgs a, int 
                                     (unsigned)((s * a.Ku + (u < a.Ku ? u : 0)) * 2048 + t * 1024), PAST);
             if constexpr (!kQuant) {
 #pragma unroll
-                for (int i = 0; i < MB; ++i) x[d][t][i] = load16(xr, xo[i], (unsigned)(u * 128 + t * 64));
+                for (int i = 0; i < MB; ++i) x[d][t][i] = load16(xr, i8_rows_at(xo[i], u, t), 0);
             }
         }
     };
@@ -129,7 +126,7 @@ __global__ __launch_bounds__(64 * KS) void int8_stream_kernel(Int8MmArgs a, int 
             if constexpr (kQuant) {
                 const int u = u0 + d * KS < a.Ku ? u0 + d * KS : a.Ku - 1;  // (past the last the weights are zeros)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) x[0][t][0] = *reinterpret_cast<const i32x4*>(rows8 + xo[0] + u * 128 + t * 64);
+                for (int t = 0; t < 2; ++t) x[0][t][0] = *reinterpret_cast<const i32x4*>(rows8 + i8_rows_at(xo[0], u, t));
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
