@@ -14,8 +14,11 @@
 // chunk fall on 16 different positions of 256 bytes, 8 of them on 8 of 128.
 // A load's lanes cover whole 128-byte lines of 8 rows in any case.
 //
-// Rows behind the last and values behind K are zeros by the buffer's range, or
-// meet the zeros that pad the weights.
+// Rows behind the last, and the last row's values behind K, are zeros by the
+// buffer's range, which covers a load's vector offset and not its scalar one: a
+// row's whole offset is in the former (int8_rows.h).  Other rows' values behind K
+// meet the zeros that pad the weights, whose unit is the scalar offset: behind the
+// last strip the vector offset alone is out of range.
 //
 // Measured: 8192 x 8192 x 8192 395 to 412 us, 2.67 to 2.79 P op/s (the library's
 // product 464); 8192 x 2560 x 6912 127 to 142 us by the machine, 2.0 to 2.3 (177).
@@ -50,8 +53,15 @@ struct GCfg {
 // loads of the next stage; the waits are explicit instead.  (Also for the
 // scalar registers, which a buffer load reads five wait states or more after a
 // lane read wrote them.)
+__device__ __forceinline__ void load_rows(u32x4 rsrc, unsigned voff, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rsrc)
+                 : "memory", "m0");
+}
+
 // once: read by nobody else, so not kept in the caches.
-__device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned voff, unsigned soff, unsigned lds, bool once = false) {
+__device__ __forceinline__ void load_weights(u32x4 rsrc, unsigned voff, unsigned soff, unsigned lds, bool once) {
     if (once)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
                      :
@@ -83,8 +93,6 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-__device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ (row >> 3 & 1); }
-
 // Until the loads of the units behind the next one are all that is in flight.
 template <class C, int BEHIND>
 __device__ __forceinline__ void wait_unit(int behind, bool more) {
@@ -113,10 +121,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     const int run0 = wave * C::XL + (more ? wave : C::XR);
     unsigned xo[C::XL + 1], wo[C::WL];
 #pragma unroll
-    for (int i = 0; i < C::XL + (C::XR != 0); ++i) {
-        const int row = (run0 + i) * 8 + (lane >> 3);
-        xo[i] = (unsigned)(row * (int)a.ldx + ((lane & 7) ^ swizzle(row)) * 16);
-    }
+    for (int i = 0; i < C::XL + (C::XR != 0); ++i) xo[i] = i8_tile_lane((run0 + i) * 8 + (lane >> 3), lane, (int)a.ldx);
 #pragma unroll
     for (int i = 0; i < C::WL; ++i) {
         const int run = wave * C::WL + i;  // strip run / 2, k-tile run % 2
@@ -135,7 +140,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         const int m0 = tm * C::BM, s0 = tn * (C::BN / 16);
         const int rows = a.M - m0 < C::BM ? a.M - m0 : C::BM;
         const int strips = 2 * i8_pairs(a.N) - s0;
-        xr = resource(a.x + (long long)m0 * a.ldx, (unsigned)((rows - 1) * (int)a.ldx + a.Kx));
+        xr = resource(a.x + (long long)m0 * a.ldx, i8_rows_size(rows, (int)a.ldx, a.Kx));
         wr = resource(a.w + (long long)s0 * a.Ku * 2048,
                       (unsigned)((strips < C::BN / 16 ? strips : C::BN / 16) * a.Ku * 2048));
     };
@@ -144,11 +149,11 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
         if (it >= tiles) return;
         const unsigned at = base + place * C::STAGE;
         if (i < C::XL)
-            load_to_lds(xr, xo[i], iu * 128, at + (run0 + i) * 1024);
+            load_rows(xr, i8_rows_at(xo[i], iu, 0), at + (run0 + i) * 1024);
         else if (i >= C::XL + C::WL)
-            if (more) load_to_lds(xr, xo[C::XL], iu * 128, at + (run0 + C::XL) * 1024);
+            if (more) load_rows(xr, i8_rows_at(xo[C::XL], iu, 0), at + (run0 + C::XL) * 1024);
         if (i >= C::XL && i < C::XL + C::WL)
-            load_to_lds(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, once);
+            load_weights(wr, wo[i - C::XL], iu * 2048, at + C::XB + (wave * C::WL + i - C::XL) * 1024, once);
         if (i == RUNS - 1) {
             place = place + 1 == C::NST ? 0 : place + 1;
             if (++iu == last) {
@@ -162,7 +167,7 @@ __global__ __launch_bounds__(C::THREADS) void int8_gemm_kernel(Int8MmArgs a, int
     const int xat = (rw * C::MBW * 16 + j) * 128, wat = C::XB + cw * C::SW * 2048 + lane * 16;
     auto read_x = [&](const unsigned char* st, int q) {  // step q of a stage: k-tile q / MBW, row block q % MBW
         // (rows 16 apart have the same swizzle)
-        return *reinterpret_cast<const i32x4*>(st + xat + q % C::MBW * 2048 + ((q / C::MBW * 4 + g) ^ swizzle(j)) * 16);
+        return *reinterpret_cast<const i32x4*>(st + xat + q % C::MBW * 2048 + ((q / C::MBW * 4 + g) ^ i8_swizzle(j)) * 16);
     };
     auto read_w = [&](const unsigned char* st, int t, int s) {
         return *reinterpret_cast<const i32x4*>(st + wat + s * 2048 + t * 1024);

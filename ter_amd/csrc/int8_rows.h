@@ -33,4 +33,11 @@ TER_I8_HD unsigned i8_stream_lane(int m, int g, int rows, int ldx) {
     return (unsigned)((m < rows ? m : rows - 1) * ldx + g * 16);
 }
 
+// Tiles: row `row` of a tile, 128 bytes of which 8 lanes load, each the chunk of 16
+// that belongs at its place in LDS.
+TER_I8_HD int i8_swizzle(int row) { return (row & 7) ^ (row >> 3 & 1); }
+TER_I8_HD unsigned i8_tile_lane(int row, int lane, int ldx) {
+    return (unsigned)(row * ldx + ((lane & 7) ^ i8_swizzle(row)) * 16);
+}
+
 }  // namespace terhip

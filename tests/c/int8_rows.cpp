@@ -3,6 +3,7 @@
 // rows, or its vector offset, all that the hardware checks, is at or behind the size.
 //
 // int8_rows stream: rows by 16, 32 and 64 of a wave, units past the last among them.
+// int8_rows tiles: rows by the tiles' 64 to 256, whole units of the last rows.
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -38,6 +39,24 @@ static void stream(int M, int K, int ldx) {
                 }
 }
 
+static void tiles(int M, int BM, int K, int ldx) {
+    const int units = (K + kI8Unit - 1) / kI8Unit;
+    for (int m0 = 0; m0 < M; m0 += BM) {
+        const int rows = M - m0 < BM ? M - m0 : BM;
+        const long long size = (long long)(rows - 1) * ldx + K;
+        const unsigned checked = i8_rows_size(rows, ldx, K);
+        for (int u = 0; u < units; ++u)
+            for (int run = 0; run < BM / 8; ++run)
+                for (int lane = 0; lane < 64; ++lane) {
+                    // (the lane's place in LDS is chunk lane % 8 of the row)
+                    const int row = run * 8 + lane / 8, chunk = (lane % 8) ^ i8_swizzle(row), k = u * kI8Unit + chunk * 16;
+                    const unsigned v = i8_rows_at(i8_tile_lane(row, lane, ldx), u, 0);
+                    load(v, size, checked, row < rows && k < K, "tiles", rows, K, u);
+                    if (row < rows && k < K && v != (unsigned)(row * ldx + k)) ++bad;
+                }
+    }
+}
+
 int main(int argc, char** argv) {
     if (argc < 2) return 2;
     if (!strcmp(argv[1], "stream")) {
@@ -48,6 +67,12 @@ int main(int argc, char** argv) {
                     stream(M, K, K + pad);
                 }
         for (int M : {1, 16, 64}) stream(M, 131056, 1 << 22);
+    } else if (!strcmp(argv[1], "tiles")) {
+        for (int BM : {64, 96, 128, 160, 192, 224, 256})
+            for (int M : {17, 64, 65, 66, 97, 200, 256, 257})
+                for (int K = 16; K <= 9000; K += K < 700 ? 16 : 1616 + 16)
+                    for (int pad : {0, 16, 4096}) tiles(M, BM, K, K + pad);
+        tiles(257, 256, 131056, 1 << 22);
     } else {
         return 2;
     }

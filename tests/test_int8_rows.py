@@ -54,3 +54,22 @@ def test_loads_of_few_rows_have_no_scalar_offset(tmp_path):
         assert with_one > 0, name
         # (rows of floating types come through LDS)
         assert without * strips == (with_one * blocks if rows == 3 else 0), (name, without, with_one)
+
+
+def test_tiles_are_read_within(walk):
+    walk("tiles")
+
+
+def test_loads_of_tiles_have_no_scalar_offset(tmp_path):
+    """The same of a tile's loads: 8 rows each, or half a strip of weights."""
+    found = waits.kernels(tmp_path, "int8_gemm_kernel")
+    assert len(found) >= 32
+    for name, kernel in found.items():
+        mbw, sw, rw, cw = map(int, re.findall(r"Li(\d+)E", name)[:4])
+        without, with_one = offsets(kernel)
+        # (weights twice: past the caches and through them; rows that the waves do not share evenly: one run more)
+        waves = rw * cw
+        runs, strips = 2 * mbw * rw, 2 * sw * cw
+        assert with_one * waves % (2 * strips) == 0, (name, with_one)
+        times = with_one * waves // (2 * strips)
+        assert times > 0 and without == times * -(-runs // waves), (name, without, with_one)
