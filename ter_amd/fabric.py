@@ -770,6 +770,14 @@ def _matrix(t, name: str, device: Optional[int] = None, width: Optional[int] = N
     return st[0] if s[0] > 1 else max(s[1], 1)
 
 
+def _int32(n: int, what: str) -> int:
+    """A size that the C-ABI takes in 32 bits, where ctypes would drop the others;
+    whether it is in range is checked behind the boundary."""
+    if n >= 1 << 31:
+        raise ValueError(f"{n} {what} are too many")
+    return n
+
+
 def _vector(t, name: str, dtype, n: int, device: int):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda or t.get_device() != device:
@@ -864,7 +872,7 @@ def mm_int8(W: PackedInt8, x, x_scale=None, dtype=None, out=None, stream=None):
     dev = W._dev
     xs = _matrix(x, "x", dev, W.K)
     xt = _type_of(x.dtype, (L.T_F16, L.T_BF16, L.T_F32, L.T_I8), "x")
-    M = x.shape[0]
+    M = _int32(x.shape[0], "rows")
     if out is not None:
         if dtype is not None and dtype != out.dtype:
             raise TypeError(f"out is {out.dtype}, not {dtype}")
