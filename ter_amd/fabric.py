@@ -918,7 +918,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     st = _matrix(logits, "logits")
     ty = _type_of(logits.dtype, (L.T_F16, L.T_BF16, L.T_F32), "logits")
     dev = logits.get_device()
-    M, V = logits.shape
+    M, V = _int32(logits.shape[0], "rows"), _int32(logits.shape[1], "logits of a row")
     _vector(u, "u", torch.float32, M, dev)
     p = L.SampleParams()
     for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),

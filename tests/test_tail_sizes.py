@@ -47,3 +47,14 @@ def test_rows_of_a_product(reached, m, dt):
     few = [Shape((5,), torch.float32)] * (dt == torch.int8)
     with pytest.raises(reached):
         T.mm_int8(W, Shape((5, 1), dt), *few)
+
+
+@pytest.mark.parametrize("dt", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("m,v", [(1 << 31, 1), ((1 << 32) + 5, 1), (1, 1 << 31), (3, (1 << 32) + 1000)])
+def test_rows_and_vocabulary_of_a_draw(reached, m, v, dt):
+    u, token = Shape((m,), torch.float32), Shape((m,), torch.int32)
+    for kw in (dict(), dict(out=token, prob_out=u)):
+        with pytest.raises(ValueError, match="too many"):
+            T.sample(Shape((m, v), dt), u, **kw)
+    with pytest.raises(reached):
+        T.sample(Shape((5, 1000), dt), Shape((5,), torch.float32))
