@@ -30,6 +30,11 @@
  *   - u is in [0, 1); on the device others count as the nearest in it, NaN as 0;
  *   - logits that are -infinity or NaN are never drawn; +infinity counts as the
  *     largest finite binary32; a row with nothing to draw gives token -1, prob 0.
+ *
+ * Thousands of logits next to each other where a cut or the draw falls (a row of
+ * zeros), and infinite ones, are slow: milliseconds for a row of 128256, and the
+ * call takes as long.  Rows that only fill up a batch are best given temperature
+ * 0 on the device, or logits of -infinity, which are settled at once.
  */
 #ifndef TER_HIP_SAMPLE_H
 #define TER_HIP_SAMPLE_H

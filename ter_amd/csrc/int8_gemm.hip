@@ -21,7 +21,7 @@
 // last strip the vector offset alone is out of range.
 //
 // Measured: 8192 x 8192 x 8192 395 to 412 us, 2.67 to 2.79 P op/s (the library's
-// product 464); 8192 x 2560 x 6912 127 to 142 us by the machine, 2.0 to 2.3 (177).
+// product 464); 8192 x 2560 x 6912 127 to 150 us by the machine, 1.9 to 2.3 (177).
 // Of a unit's 1.59 us in the largest tile the products alone are 1.03, the loads
 // alone 1.02: LDS serves both, and the barrier's wait is not all hidden.  Products
 // of 32 x 32 x 32 instead of 16 x 16 x 64 (8192 cubed 475 against 441 us then)
@@ -356,8 +356,10 @@ int best_variant(int M, int N, int Ku, int cus, float* us) {
 // Few tiles of a long K leave most of the GPU idle: parts of it then, as many
 // workgroups as fit at once, and their sums joined by one launch more, whose host
 // time counts too (us, rows x channels x K, all of K and parts): 380 x 512 x 8192
-// 24.6 and 13.7, 128 x 2560 x 6912 20.8 and 14.8, 300 x 2560 x 16384 44.3 and
-// 32.8, 256 x 2560 x 6912 21.3 and 16.8; 128 x 640 x 2560 9.6 and 13.3: not in parts.
+// 24.6 and 13.3, 128 x 2560 x 6912 20.8 and 14.7, 300 x 2560 x 16384 44.3 and
+// 31.9, 256 x 2560 x 6912 21.3 and 16.1; 128 x 640 x 2560 9.6 and 13.3: not in parts.
+// The parts are those of a whole GPU's 256 CUs, so that the workspace is one size on
+// every device; on a partition of one they are more than fit at once.
 int i8_parts(int M, int N, int Ku) {
     constexpr int kCus = 256;
     constexpr float kJoin = 5.f, kJoinBytes = 1.f / 3e6f;  // us a launch, us a byte of sums

@@ -9,11 +9,11 @@
 // read the same ones.  The waves' sums are joined in LDS, each wave joining
 // and storing a part of the results.
 //
-// Measured: 1 x 2048 x 128256 (rows, K, channels) 38.8 us, 6.8 TB/s, what a pure
-// read reaches on this card; 16 x 2560 x 128256 62 us, 5.3 TB/s and every
-// workgroup's read of the rows; 23 x 6912 x 2560 8.8 us, 2.0 TB/s: there 160
-// workgroups wait for 54 units in turn, 8 waves each.  One token of 2560 x 2560
-// takes 5.4 us, of which the weights' bytes are 1.
+// Measured: 1 x 2048 x 128256 (rows, K, channels) 38.8 to 39.5 us, 6.7 to 6.8 TB/s
+// (a pure read of as many bytes 39.2 to 40.4); 16 x 2560 x 128256 62 us, 5.3 TB/s
+// and every workgroup's read of the rows; 23 x 6912 x 2560 8.8 to 9.1 us, 2.0 TB/s:
+// 160 workgroups of 8 waves, a wave with two units in flight of the 7 it takes in
+// turn.  One token of 2560 x 2560 takes 5.4 us, of which the weights' bytes are 1.
 #include "common.h"
 #include "int8.h"
 #include "int8_quant.h"

@@ -15,6 +15,12 @@
 // 12.8 + 15.0; 256 rows fp16, top_p 0.92: 12.5 (5.2 TB/s) + 29.3 + 22.2 + 13.5, the
 // histogram by its 26 vector instructions an element (a weight in binary64 among
 // them) and the list by its own 12, not by the 65 MB read.
+//
+// A row whose places lie among more than 8192 elements of one bin (equal logits,
+// as zeros in 16 bits) or that has an infinite logit is searched by one
+// workgroup, and the call waits for it: 64 x 128256 fp16, top_k 50, top_p 0.95, 31 us
+// become 2770 with one row of zeros, of atomics that meet in one place, and 770
+// with one infinity; of 32000 tokens 28, 715 and 215.
 #include "common.h"
 #include "sample.h"
 
@@ -278,7 +284,7 @@ struct Row {
 };
 
 // One row by one workgroup: a search through the row's values for each cut and
-// for the draw.  Right for every row; the general path.
+// for the draw, four passes each.  Right for every row; the general path.
 template <int TYPE, int NT>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, int row, const double* table, Shared<NT>& sh) {
     Row<TYPE, NT> x{gptr(reinterpret_cast<const typename Logit<TYPE>::T*>(a.logits + (long long)row * a.stride)), a.V};
